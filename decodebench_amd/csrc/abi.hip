@@ -463,3 +463,203 @@ int db_tune_get(const char* key, int* value) {
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------- the paged KV cache
+namespace {
+
+// Rows of D elements at the strides given, all of them 16-byte aligned.
+int check_cache(const char* fn, const db_paged_cache* c, int dtype) {
+  if (!c || !c->k || !c->v) return fail(DB_ERR_INVALID, "%s: null cache", fn);
+  if (dtype != DB_DTYPE_F16 && dtype != DB_DTYPE_BF16)
+    return fail(DB_ERR_INVALID, "%s: unknown activation dtype %d", fn, dtype);
+  const bool fp8 = c->dtype == DB_DTYPE_FP8_E4M3;
+  if (!fp8 && c->dtype != dtype)
+    return fail(DB_ERR_INVALID, "%s: the cache must have the activations' type or e4m3", fn);
+  if (fp8 && (!c->k_scale || !c->v_scale))
+    return fail(DB_ERR_INVALID, "%s: an e4m3 cache needs an fp32 scale per KV head", fn);
+  if (!fp8 && (c->k_scale || c->v_scale))
+    return fail(DB_ERR_INVALID, "%s: a 16-bit cache takes no scales", fn);
+  if (c->pages < 1 || c->page_size < 1 || c->Hkv < 1 || c->D < 1)
+    return fail(DB_ERR_INVALID, "%s: need pages, page_size, Hkv and D >= 1 (got %d %d %d %d)", fn,
+                c->pages, c->page_size, c->Hkv, c->D);
+  const long long strides[] = {c->k_page_stride, c->k_head_stride, c->k_token_stride,
+                               c->v_page_stride, c->v_head_stride, c->v_token_stride};
+  for (long long s : strides)
+    if (s < 0 || s % (fp8 ? 16 : 8) != 0)
+      return fail(DB_ERR_INVALID, "%s: cache strides must keep rows 16-byte aligned", fn);
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (fp8 && (!aligned4(c->k_scale) || !aligned4(c->v_scale)))
+    return fail(DB_ERR_INVALID, "%s: scale vectors must be 4-byte aligned", fn);
+  return DB_OK;
+}
+
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+dbk::PagedCall paged_bounds(int T, int Hq, int Hkv, int D, int R, int max_new) {
+  dbk::PagedCall c = {};
+  c.T = T;
+  c.R = R;
+  c.Hq = Hq;
+  c.max_new = max_new;
+  c.cache.Hkv = Hkv;
+  c.cache.D = D;
+  return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int db_paged_plan(const int* past, const int* fresh, int* table, long long table_stride,
+                  int width, const int* free_pages, int free_count, const int* free_start,
+                  int page_size, int R, int T, int* q_start, int* kv_len, int* position,
+                  long long* slot, int* free_next, void* stream) {
+  const char* fn = "db_paged_plan";
+  if (R < 0 || T < 0 || free_count < 0)
+    return fail(DB_ERR_INVALID, "%s: need R, T, free_count >= 0 (got %d %d %d)", fn, R, T,
+                free_count);
+  if (width < 1 || page_size < 1 || table_stride < width)
+    return fail(DB_ERR_INVALID,
+                "%s: need width >= 1, page_size >= 1 and table rows of at least width entries "
+                "(got %d %d %lld)",
+                fn, width, page_size, table_stride);
+  if (!q_start || !free_next || (R > 0 && (!past || !fresh || !table || !kv_len)) ||
+      (T > 0 && (!position || !slot)) || (free_count > 0 && !free_pages))
+    return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  const void* words[] = {past, fresh, table, free_pages, free_start, q_start, kv_len, position,
+                         free_next};
+  for (const void* p : words)
+    if (!aligned4(p)) return fail(DB_ERR_INVALID, "%s: tensors must be 4-byte aligned", fn);
+  if (!aligned8(slot)) return fail(DB_ERR_INVALID, "%s: slot must be 8-byte aligned", fn);
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  if (err) return hip_status((hipError_t)err, fn);
+  const dbk::PlanCall c = {past, fresh, table, free_pages, free_start, table_stride, free_count,
+                           width, page_size, R, T, q_start, kv_len, position, slot, free_next};
+  return hip_status(dbk::launch_paged_plan(c, cus, (hipStream_t)stream), fn);
+}
+
+int db_rope_append(const void* qkv, long long qkv_stride, const int* position, int n_axes,
+                   const unsigned char* axis_of_pair, const long long* slot,
+                   const float* inv_freq, int rot, int interleaved,
+                   const db_paged_cache* cache, void* q, int T, int Hq, int dtype,
+                   void* stream) {
+  const char* fn = "db_rope_append";
+  const int rc = check_cache(fn, cache, dtype);
+  if (rc) return rc;
+  const int D = cache->D;
+  if (T < 0 || Hq < 1) return fail(DB_ERR_INVALID, "%s: need T >= 0, Hq >= 1", fn);
+  if (D % 16 != 0 || D > 256)
+    return fail(DB_ERR_INVALID, "%s: D=%d must be a multiple of 16 up to 256", fn, D);
+  if (rot < 16 || rot % 16 != 0 || rot > D)
+    return fail(DB_ERR_INVALID, "%s: rot=%d must be a multiple of 16 up to D=%d", fn, rot, D);
+  if (n_axes < 1 || n_axes > 4)
+    return fail(DB_ERR_INVALID, "%s: n_axes=%d outside [1, 4]", fn, n_axes);
+  if ((long long)Hq + 2ll * cache->Hkv > (1 << 16))
+    return fail(DB_ERR_INVALID, "%s: too many heads", fn);
+  if (qkv_stride < ((long long)Hq + 2ll * cache->Hkv) * D || qkv_stride % 8 != 0)
+    return fail(DB_ERR_INVALID, "%s: qkv rows must hold (Hq + 2 Hkv) D elements and be 16-byte "
+                "aligned", fn);
+  if (T == 0) return ok();
+  if (!qkv || !position || !slot || !inv_freq || !q)
+    return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(qkv) || !aligned16(q))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (!aligned4(position) || !aligned4(inv_freq) || !aligned8(slot))
+    return fail(DB_ERR_INVALID, "%s: position, inv_freq and slot must be aligned to their type",
+                fn);
+  dbk::RopeCall c = {};
+  for (int i = 0; axis_of_pair && i < rot / 2; ++i) {
+    if (axis_of_pair[i] >= n_axes)
+      return fail(DB_ERR_INVALID, "%s: pair %d turns with axis %d of %d", fn, i, axis_of_pair[i],
+                  n_axes);
+    c.axes[i / 16] |= (unsigned)axis_of_pair[i] << (2 * (i % 16));
+  }
+  c.qkv = qkv;
+  c.position = position;
+  c.slot = slot;
+  c.freq = inv_freq;
+  c.q = q;
+  c.cache = *cache;
+  c.qkv_row = qkv_stride;
+  c.T = T;
+  c.Hq = Hq;
+  c.rot = rot;
+  c.interleaved = interleaved ? 1 : 0;
+  c.bf16 = dtype == DB_DTYPE_BF16;
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  if (err) return hip_status((hipError_t)err, fn);
+  return hip_status(dbk::launch_rope_append(c, cus, (hipStream_t)stream), fn);
+}
+
+size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new) {
+  if (T < 1 || R < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128) || max_new < 0)
+    return 0;
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  if (err) return 0;
+  return dbk::paged_workspace_bytes(paged_bounds(T, Hq, Hkv, D, R, max_new), cus);
+}
+
+int db_paged_attention(const void* q, long long q_token_stride, long long q_head_stride,
+                       void* o, const db_paged_cache* cache, const int* table,
+                       long long table_stride, int width, const int* q_start,
+                       const int* kv_len, int T, int R, int Hq, int max_new, float scale,
+                       int causal, int window, int dtype, void* ws, size_t ws_bytes,
+                       void* stream) {
+  const char* fn = "db_paged_attention";
+  const int rc = check_cache(fn, cache, dtype);
+  if (rc) return rc;
+  const int D = cache->D;
+  if (D != 64 && D != 128)
+    return fail(DB_ERR_INVALID, "%s: head_dim D=%d, only 64 and 128 are supported", fn, D);
+  if (T < 0 || R < 0 || Hq < 1 || max_new < 0)
+    return fail(DB_ERR_INVALID, "%s: need T, R, max_new >= 0 and Hq >= 1", fn);
+  if (Hq % cache->Hkv != 0)
+    return fail(DB_ERR_INVALID, "%s: Hq=%d is not a multiple of Hkv=%d", fn, Hq, cache->Hkv);
+  if ((long long)T * Hq >= (1ll << 31) || (long long)R * cache->Hkv >= (1ll << 24))
+    return fail(DB_ERR_INVALID, "%s: T * Hq or R * Hkv is too large", fn);
+  if (!(scale > 0.0f) || !isfinite(scale))
+    return fail(DB_ERR_INVALID, "%s: scale must be finite and > 0", fn);
+  if (window < 0 || (window > 0 && !causal))
+    return fail(DB_ERR_INVALID, "%s: window must be >= 0, and a window needs causal", fn);
+  if (width < 1 || table_stride < 0)
+    return fail(DB_ERR_INVALID, "%s: need table rows of width >= 1 entries, a stride >= 0", fn);
+  if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride % 8 || q_head_stride % 8)
+    return fail(DB_ERR_INVALID, "%s: q strides must keep rows 16-byte aligned", fn);
+  if (T == 0 || R == 0) return ok();
+  if (!q || !o || !table || !q_start || !kv_len)
+    return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(q) || !aligned16(o))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (!aligned4(table) || !aligned4(q_start) || !aligned4(kv_len))
+    return fail(DB_ERR_INVALID, "%s: tables and lengths must be 4-byte aligned", fn);
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(DB_ERR_INVALID, "%s: needs a workspace, 256-byte aligned", fn);
+  dbk::PagedCall c = paged_bounds(T, Hq, cache->Hkv, D, R, max_new);
+  c.q = q;
+  c.o = o;
+  c.table = table;
+  c.q_start = q_start;
+  c.kv_len = kv_len;
+  c.cache = *cache;
+  c.q_token = q_token_stride;
+  c.q_head = q_head_stride;
+  c.table_row = table_stride;
+  c.width = width;
+  c.causal = causal ? 1 : 0;
+  c.window = window;
+  c.scale = scale;
+  c.bf16 = dtype == DB_DTYPE_BF16;
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  if (err) return hip_status((hipError_t)err, fn);
+  const size_t need = dbk::paged_workspace_bytes(c, cus);
+  if (ws_bytes < need)
+    return fail(DB_ERR_INVALID, "%s: workspace %zu bytes < %zu required", fn, ws_bytes, need);
+  return hip_status(dbk::launch_paged_attention(c, cus, ws, (hipStream_t)stream), fn);
+}
+
+}  // extern "C"

@@ -131,6 +131,53 @@ constexpr size_t kF4ScratchBytes = DB_F4_SCRATCH_BYTES;
 // device with hipGetSymbolAddress).
 hipError_t f4_scratch_address(void** out);
 
+// A step over a paged KV cache: the arguments of the three entry points as the
+// kernels take them (checked by the caller).
+struct PlanCall {
+  const int* past;       // [R] tokens of each request in the cache
+  const int* fresh;      // [R] tokens of this step
+  int* table;            // [R, width], rows table_row apart; taken pages are entered
+  const int* free_pages; // [free_count]
+  const int* free_start; // [1] or null: where the step's pages begin
+  long long table_row;
+  int free_count, width, page, R, T;
+  int* q_start;          // [R + 1]
+  int* kv_len;           // [R]
+  int* position;         // [T]
+  long long* slot;       // [T]
+  int* free_next;        // [1]
+};
+hipError_t launch_paged_plan(const PlanCall& c, int cu_count, hipStream_t stream);
+
+struct RopeCall {
+  const void* qkv;         // [T, (Hq + 2 Hkv) D], rows qkv_row elements apart
+  const int* position;     // [axes, T]
+  const long long* slot;   // [T]
+  const float* freq;       // [rot / 2]
+  void* q;                 // [T, Hq, D]
+  db_paged_cache cache;
+  long long qkv_row;
+  int T, Hq, rot, interleaved;
+  bool bf16;
+  unsigned axes[8];        // axis of pair i: bits 2 (i % 16) of word i / 16
+};
+hipError_t launch_rope_append(const RopeCall& c, int cu_count, hipStream_t stream);
+
+struct PagedCall {
+  const void* q;        // [T, Hq, D]
+  void* o;              // [T, Hq, D]
+  const int* table;     // [R, width]
+  const int* q_start;   // [R + 1]
+  const int* kv_len;    // [R]
+  db_paged_cache cache;
+  long long q_token, q_head, table_row;
+  int T, R, Hq, width, max_new, causal, window;
+  float scale;
+  bool bf16;
+};
+size_t paged_workspace_bytes(const PagedCall& c, int cu_count);
+hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream);
+
 // Read-only streaming probe (stream_probe.hip): `bytes` (a multiple of
 // kb_per_wave KB, kb_per_wave in {4, 8, 16}) read once, kb_per_wave KB per
 // wave; sink needs bytes / 16 words and is written only when the folded

@@ -1,0 +1,333 @@
+// paged_attn.h -- what the two kernels of paged attention share: arguments,
+// the assignment of work to workgroups, element types, page lookup, records.
+//
+// paged_attention computes, for the new tokens i = 0 .. n_r - 1 of every
+// request r (packed one request after another, q_start[r] the first row) and
+// every query head h,
+//   o[i, h] = sum_j softmax_j(scale q[i, h] . K[j, h / G]) V[j, h / G]
+// over the keys j of the request that token i sees: j < len_r, with `causal`
+// j <= pos_i = len_r - n_r + i, with a window j > pos_i - window, and only
+// keys whose page is in the cache.  A row that sees nothing is zero.
+//
+// Rows: the n_r G (token, query head) pairs of a (request, KV head) are the
+// rows of one product, row x = token x / G, head x % G, so that K and V are
+// read once for all of them; a row tile is MT of them.
+//
+// Lengths live on the GPU, so the host launches a grid by its bounds and every
+// workgroup finds its own work: it reads the lengths of all requests, takes
+// the key tiles that one split may hold (C: all work over the workgroups that
+// the chip wants) and from a prefix sum over the requests' split counts the
+// (request, KV head, row tile, split) of its number.  This costs about a
+// microsecond per workgroup, once, and no launch, no table to keep in step
+// with the lengths and no read on the host.  The KV head is the fastest index:
+// workgroups i and i + 8 run on one XCD, so with 8 heads all row tiles and
+// splits of a head share one L2.
+//
+// A split writes its running maximum, exp-sum and unnormalised output as an
+// fp32 record; paged_merge joins the records of a row.  There are fewer
+// than 2 `target` records: only requests of more than C tiles split, into
+// fewer than 2 tmax / C parts, and C >= (all tiles) / target.
+#pragma once
+
+#include "db_device.h"
+#include "db_kernels.h"
+
+namespace dbk {
+
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+constexpr float kPagedNegInf = -__builtin_huge_valf();
+
+// ---------------------------------------------------------------- types
+// 16-bit element types of the activations (and of a cache of that type).
+struct ElemF16 {
+  typedef _Float16 type;
+  typedef h8 vec8;
+  typedef h4 vec4;
+  static constexpr unsigned kExp = 0x7C00u;  // exponent bits: all set in Inf and NaN
+  __device__ static f4 mfma16(vec8 a, vec8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static f4 mfma16k16(vec4 a, vec4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static f16v mfma32(vec8 a, vec8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  // four e4m3 values to two pairs (exact: all of them are fp16 numbers)
+  __device__ static u2 widen(unsigned w) {
+    u2 r;
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    return r;
+  }
+};
+struct ElemBF16 {
+  typedef __bf16 type;
+  typedef b8 vec8;
+  typedef b4 vec4;
+  static constexpr unsigned kExp = 0x7F80u;
+  __device__ static f4 mfma16(vec8 a, vec8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static f4 mfma16k16(vec4 a, vec4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a),
+                                                     __builtin_bit_cast(s4, b), c, 0, 0, 0);
+  }
+  __device__ static f16v mfma32(vec8 a, vec8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static u2 widen(unsigned w) {  // exact as well: three mantissa bits
+    u2 r;
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+    return r;
+  }
+};
+
+// Whether a pair of 16-bit values holds an Inf or NaN.
+template <class E>
+__device__ __forceinline__ bool pair_nonfinite(unsigned w) {
+  return (w & E::kExp) == E::kExp || ((w >> 16) & E::kExp) == E::kExp;
+}
+
+// ------------------------------------------------------------- arguments
+// Region of the workspace of one kernel.
+struct PagedRecords {
+  int* head;      // [0]: groups (row tiles whose rows were split) of this call
+  int* desc;      // [groups][8]: splits, first record, first token, first row, rows
+  float2* ml;     // [records][MT]    maximum (base 2) and exp-sum
+  float* opart;   // [records][MT][D] unnormalised output
+  int records, groups;  // room
+};
+
+struct PagedArgs {
+  const void* q;
+  void* o;
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int* table;
+  const int* q_start;
+  const int* kv_len;
+  long long q_token, q_head;      // strides in elements
+  long long kp, kh, kt, vp, vh, vt;
+  long long table_row;
+  int T, R, Hq, Hkv, G;
+  int pages, page, width;
+  unsigned page_magic, page_shift;  // key / page, see page_of()
+  int causal, window;
+  float scale_log2;
+  int part;        // 0: every request, 1: those of at most kDecodeRows rows, 2: the others
+  int target;      // workgroups wanted
+  int min_tiles;   // fewest key tiles of a split
+  PagedRecords rec;
+};
+
+constexpr int kDecodeRows = 16;  // rows of the decode kernel's tile
+constexpr int kChunkRows = 128;  // rows of the chunk kernel's tile
+constexpr int kDecodeKeys = 16;
+constexpr int kChunkKeys = 64;
+constexpr int kPagedThreads = 256;
+constexpr int kDescInts = 8;
+
+// key / page for 0 <= key < 2^31, with magic = ceil(2^(31 + s) / page), s =
+// ceil(log2 page) = shift + 1: the excess magic * page - 2^(31 + s) is less
+// than 2^s, so key * excess < 2^(31 + s) and the quotient is exact.
+__device__ __forceinline__ int page_of(const PagedArgs& a, int key) {
+  return a.page_magic ? (int)(__umulhi((unsigned)key, a.page_magic) >> a.page_shift) : key;
+}
+
+// ------------------------------------------------------------- schedule
+struct PagedRequest {
+  int tok0, n, len;   // first row of q, new tokens, tokens in all
+  int row_tiles, tiles;  // row tiles, most key tiles of any of them
+};
+
+struct PagedWork {
+  PagedRequest req;
+  int r, head, tile, split, splits;
+  int rec, group;  // first record and group of the row tile, -1 if it is not split
+};
+
+__device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// Keys a request has at most: its length and what the block table can hold.
+__device__ __forceinline__ int paged_limit(const PagedArgs& a, int len) {
+  const long long held = (long long)a.width * a.page;
+  return (int)min((long long)min(len, 0x7FFFF000), held);
+}
+
+template <int MT, int KT>
+__device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r) {
+  PagedRequest q = {0, 0, 0, 0, 0};
+  if (r >= a.R) return q;
+  q.tok0 = clamp_int(a.q_start[r], 0, a.T);
+  q.n = max(clamp_int(a.q_start[r + 1], 0, a.T) - q.tok0, 0);
+  q.len = max(a.kv_len[r], 0);
+  const long long rows = (long long)q.n * a.G;
+  if (a.part != 0 && (rows <= kDecodeRows) != (a.part == 1)) q.n = 0;
+  if (q.n == 0) return q;
+  q.row_tiles = (int)((rows + MT - 1) / MT);
+  long long keys = paged_limit(a, q.len);
+  // With a window a row tile of tokens i .. i + d sees at most window + d keys.
+  if (a.window > 0) keys = min(keys, (long long)a.window + (MT - 1) / a.G + 1 + KT);
+  q.tiles = (int)((keys + KT - 1) / KT);
+  return q;
+}
+
+struct PagedShared {
+  int wave_sums[kPagedThreads / kWave][3];
+  unsigned long long wave_work[kPagedThreads / kWave];
+  PagedWork found;
+  int hit;
+};
+
+// Walks the workgroup's numbers w = blockIdx.x, + gridDim.x, ... : next()
+// says whether there is another piece of work and leaves it in `work`
+// (uniform).  All threads of the workgroup call it together; it ends with a
+// barrier behind every read of the shared state, so the caller's LDS is free.
+template <int MT, int KT>
+struct PagedSchedule {
+  const PagedArgs& a;
+  PagedShared& sh;
+  int w, round, C;
+  int base[3];       // units, records, groups of the rounds before (per KV head)
+  PagedRequest mine;
+  int count[3], incl[3], sums[3];
+
+  __device__ PagedSchedule(const PagedArgs& args, PagedShared& s)
+      : a(args), sh(s), w(blockIdx.x), round(0), base{0, 0, 0} {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    unsigned long long total = 0;
+    for (int r = (a.R - 1) / kPagedThreads * kPagedThreads; r >= 0; r -= kPagedThreads) {
+      mine = paged_request<MT, KT>(a, r + threadIdx.x);
+      total += (unsigned long long)mine.row_tiles * mine.tiles;
+    }
+    for (int d = 1; d < kWave; d <<= 1) total += __shfl_xor(total, d);
+    if (lane == 0) sh.wave_work[wave] = total;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < kPagedThreads / kWave; ++i) total += sh.wave_work[i];
+    total *= a.Hkv;
+    const unsigned long long per = (total + a.target - 1) / a.target;
+    C = (int)min(max(per, (unsigned long long)a.min_tiles), 0x7FFFFFFFull);
+    scan();
+    if (blockIdx.x == 0) {  // the groups of the whole call, for the merge
+      int groups = sums[2];
+      for (int r = kPagedThreads; r < a.R; r += kPagedThreads) {
+        const PagedRequest q = paged_request<MT, KT>(a, r + threadIdx.x);
+        int g = splits_of(q) > 1 ? q.row_tiles : 0;
+        for (int d = 1; d < kWave; d <<= 1) g += __shfl_xor(g, d);
+        __syncthreads();
+        if (lane == 0) sh.wave_sums[wave][0] = g;
+        __syncthreads();
+        for (int i = 0; i < kPagedThreads / kWave; ++i) groups += sh.wave_sums[i][0];
+      }
+      if (threadIdx.x == 0) a.rec.head[0] = groups * a.Hkv;
+      __syncthreads();
+    }
+  }
+
+  __device__ int splits_of(const PagedRequest& q) const {
+    return q.row_tiles == 0 ? 0 : max(1, (q.tiles + C - 1) / C);
+  }
+
+  // Prefix sums over the requests of this round.
+  __device__ void scan() {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int s = splits_of(mine);
+    count[0] = mine.row_tiles * s;
+    count[1] = s > 1 ? count[0] : 0;
+    count[2] = s > 1 ? mine.row_tiles : 0;
+    for (int k = 0; k < 3; ++k) incl[k] = count[k];
+    for (int d = 1; d < kWave; d <<= 1)
+      for (int k = 0; k < 3; ++k) {
+        const int v = __shfl_up(incl[k], d);
+        if (lane >= d) incl[k] += v;
+      }
+    __syncthreads();
+    if (lane == kWave - 1)
+      for (int k = 0; k < 3; ++k) sh.wave_sums[wave][k] = incl[k];
+    __syncthreads();
+    for (int k = 0; k < 3; ++k) sums[k] = 0;
+    for (int i = 0; i < kPagedThreads / kWave; ++i)
+      for (int k = 0; k < 3; ++k) {
+        if (i < wave) incl[k] += sh.wave_sums[i][k];
+        sums[k] += sh.wave_sums[i][k];
+      }
+  }
+
+  __device__ bool next(PagedWork& work) {
+    const int unit = w / a.Hkv;
+    while (unit >= base[0] + sums[0]) {
+      for (int k = 0; k < 3; ++k) base[k] += sums[k];
+      ++round;
+      if ((long long)round * kPagedThreads >= a.R) return false;
+      mine = paged_request<MT, KT>(a, round * kPagedThreads + threadIdx.x);
+      scan();
+    }
+    const int at = unit - base[0] - (incl[0] - count[0]);
+    __syncthreads();
+    if (at >= 0 && at < count[0]) {
+      PagedWork f;
+      f.req = mine;
+      f.r = round * kPagedThreads + threadIdx.x;
+      f.head = w % a.Hkv;
+      f.splits = count[0] / mine.row_tiles;
+      f.tile = mine.row_tiles - 1 - at / f.splits;  // the longest first
+      f.split = at % f.splits;
+      const bool split = f.splits > 1;
+      f.rec = split ? (base[1] + incl[1] - count[1] + f.tile * f.splits) * a.Hkv + f.head : -1;
+      f.group = split ? (base[2] + incl[2] - count[2] + f.tile) * a.Hkv + f.head : -1;
+      sh.found = f;
+    }
+    __syncthreads();
+    work = sh.found;
+    w += gridDim.x;
+    return true;
+  }
+};
+
+// Keys that the rows of one row tile see between them, as key tiles
+// [first, last), and this split's share of them.
+template <int MT, int KT>
+__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedWork& wk, int& first,
+                                            int& last) {
+  const PagedRequest& q = wk.req;
+  const int limit = paged_limit(a, q.len);
+  const long long row0 = (long long)wk.tile * MT;
+  const int i0 = (int)(row0 / a.G);
+  const int i1 = (int)min((row0 + MT - 1) / a.G, (long long)q.n - 1);
+  const int past = q.len - q.n;
+  const int hi = a.causal ? min(limit, past + i1 + 1) : limit;
+  const int lo = a.window > 0 ? max(past + i0 - a.window + 1, 0) : 0;
+  int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
+  const int per = (t1 - t0 + wk.splits - 1) / wk.splits;
+  first = min(t0 + wk.split * per, t1);
+  last = min(first + per, t1);
+}
+
+__device__ __forceinline__ void paged_describe(const PagedArgs& a, const PagedWork& wk, int MT) {
+  if (wk.split != 0 || wk.group < 0 || wk.group >= a.rec.groups || threadIdx.x != 0) return;
+  int* d = a.rec.desc + (size_t)wk.group * kDescInts;
+  const long long left = (long long)wk.req.n * a.G - (long long)wk.tile * MT;
+  d[0] = wk.splits;
+  d[1] = wk.rec;
+  d[2] = wk.req.tok0;
+  d[3] = wk.tile * MT;
+  d[4] = (int)min(left, (long long)MT);
+}
+
+// e4m3 or 16-bit caches: the element type of the products E, of the cache C8.
+typedef void (*PagedFn)(PagedArgs);
+PagedFn paged_decode_fn(bool bf16, bool fp8, int D);
+
+}  // namespace dbk

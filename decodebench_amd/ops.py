@@ -28,6 +28,7 @@ import math
 import sys
 import threading
 from pathlib import Path
+from typing import NamedTuple
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libdecodebench_hip.so"
 FAST_PATH = Path(__file__).resolve().parent / "lib" / "_fastcall.so"
@@ -37,6 +38,7 @@ DB_ERR_INVALID = -1
 DB_ERR_UNSUPPORTED = -2
 DTYPE_F16 = 0
 DTYPE_FP8_E4M3 = 1
+DTYPE_BF16 = 2
 
 _lock = threading.Lock()
 _lib = None
@@ -47,6 +49,16 @@ _captured_ws: dict[tuple, object] = {}  # workspaces made under graph capture (k
 
 _p = C.c_void_p
 _i = C.c_int
+_ll = C.c_longlong
+
+
+class _PagedCache(C.Structure):
+    """``db_paged_cache`` of the C ABI."""
+
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p),
+                ("k_page_stride", _ll), ("k_head_stride", _ll), ("k_token_stride", _ll),
+                ("v_page_stride", _ll), ("v_head_stride", _ll), ("v_token_stride", _ll),
+                ("pages", _i), ("page_size", _i), ("Hkv", _i), ("D", _i), ("dtype", _i)]
 
 
 def load_library():
@@ -82,6 +94,14 @@ def load_library():
                                    C.c_float, _p]),
             "db_f4_splitkv_noalloc": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, C.c_float,
                                            _p]),
+            "db_paged_plan": (_i, [_p, _p, _p, _ll, _i, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p,
+                                   _p, _p]),
+            "db_rope_append": (_i, [_p, _ll, _p, _i, _p, _p, _p, _i, _i, C.POINTER(_PagedCache),
+                                    _p, _i, _i, _i, _p]),
+            "db_paged_attention_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i]),
+            "db_paged_attention": (_i, [_p, _ll, _ll, _p, C.POINTER(_PagedCache), _p, _ll, _i, _p,
+                                        _p, _i, _i, _i, _i, C.c_float, _i, _i, _i, _p,
+                                        C.c_size_t, _p]),
             "db_stream_read": (_i, [_p, C.c_size_t, _i, C.c_uint, _p, _p]),
             "db_stream_capture_id": (_i, [_p, C.POINTER(C.c_ulonglong)]),
             "db_tune": (_i, [C.c_char_p, _i]),
@@ -579,3 +599,239 @@ def f4_flashdecode_noalloc(q, K, V, scale: float | None = None, n_splits: int | 
     _launch(lib.db_f4_splitkv_noalloc, idx, "db_f4_splitkv_noalloc", q.data_ptr(), K.data_ptr(),
             V.data_ptr(), out.data_ptr(), B, Hq, Hkv, L, D, S, scale)
     return out
+
+
+# ------------------------------------------------ a step over a paged KV cache
+class PagedPlan(NamedTuple):
+    """What :func:`paged_plan` lays out for a step of T token rows and R requests."""
+
+    q_start: object    # int32 [R + 1]: request r has the rows q_start[r] .. q_start[r + 1] - 1
+    kv_len: object     # int32 [R]: tokens in the cache once the step's are appended
+    position: object   # int32 [T]
+    slot: object       # int64 [T]: page number * page_size + place in the page, -1: none
+    free_next: object  # int32 [1]: where in free_pages the next step's pages begin
+
+
+def _strided(t, name: str, dt, dim: int):
+    """Check a GPU tensor of ``dim`` dimensions whose last one is contiguous;
+    returns its GPU's index."""
+    torch = _torch or _torch_mod()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU device (got {t.device})")
+    if dt is not None and t.dtype != dt:
+        raise TypeError(f"{name} must be {dt} (got {t.dtype})")
+    if t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions (got {tuple(t.shape)})")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return t.get_device()
+
+
+def _one_gpu(idx: int, *named) -> None:
+    for other, name in named:
+        if other != idx:
+            raise ValueError(f"{name} is on cuda:{other}, expected cuda:{idx}")
+
+
+def _strides(t, n: int):
+    """The first n strides, 0 where there is one element and none counts."""
+    return [st if size > 1 else 0 for st, size in zip(t.stride()[:n], t.shape)]
+
+
+def _activation(t, name: str) -> int:
+    torch = _torch
+    if t.dtype == torch.float16:
+        return DTYPE_F16
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    raise TypeError(f"{name} must be torch.float16 or torch.bfloat16 (got {t.dtype})")
+
+
+def _paged_cache(K, V, k_scale, v_scale, act, idx: int):
+    """The cache [pages, Hkv, page_size, D] as the C ABI takes it: strided, of the
+    activations' type or e4m3 with one fp32 scale per KV head."""
+    torch = _torch
+    _one_gpu(idx, (_strided(K, "K", None, 4), "K"), (_strided(V, "V", None, 4), "V"))
+    if K.shape != V.shape or K.dtype != V.dtype:
+        raise ValueError(f"K {tuple(K.shape)} {K.dtype} and V {tuple(V.shape)} {V.dtype} must "
+                         "agree")
+    pages, Hkv, page, D = K.shape
+    c = _PagedCache(K.data_ptr(), V.data_ptr(), None, None, *_strides(K, 3), *_strides(V, 3),
+                    pages, page, Hkv, D, DTYPE_FP8_E4M3)
+    if K.dtype == torch.float8_e4m3fn:
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is None:
+                raise ValueError(f"an e4m3 cache needs {name}, an fp32 tensor of shape ({Hkv},)")
+            _one_gpu(idx, (_gpu_tensors((t, name, torch.float32)), name))
+            if tuple(t.shape) != (Hkv,):
+                raise ValueError(f"{name} must have shape ({Hkv},) (got {tuple(t.shape)})")
+        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        return c
+    if K.dtype != act:
+        raise TypeError(f"the cache must be {act} or torch.float8_e4m3fn (got {K.dtype})")
+    if k_scale is not None or v_scale is not None:
+        raise ValueError("a 16-bit cache takes no scales")
+    c.dtype = _activation(K, "K")
+    return c
+
+
+def _row_output(shape, dtype, idx: int, out):
+    torch = _torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", idx))
+    _one_gpu(idx, (_gpu_tensors((out, "out", dtype)), "out"))
+    if tuple(out.shape) != tuple(shape):
+        raise ValueError(f"out must have shape {tuple(shape)} (got {tuple(out.shape)})")
+    return out
+
+
+def paged_plan(past_len, new_len, block_table, free_pages, page_size: int, n_tokens: int,
+               free_start=None) -> PagedPlan:
+    """Lay out a step's tokens over a paged cache, on the GPU: rows, lengths,
+    positions and cache slots, and the pages that the requests need.
+
+    past_len [R] int32 tokens of each request in the cache, new_len [R] int32
+    tokens of this step, block_table [R, width] int32 (rows may be strided).
+    Pages are taken from ``free_pages`` [F] int32 from ``free_start`` on (an
+    int32 tensor [1]; None: 0), requests in order, and entered in
+    ``block_table`` in place.  ``n_tokens`` is T, the rows that the step has
+    room for: rows behind the last token get slot -1, tokens beyond them are
+    left out of ``kv_len``.  Where pages run out (``free_next`` > F) or a
+    request outgrows its table row, the tokens concerned get slot -1."""
+    torch = _torch or _torch_mod()
+    i32 = torch.int32
+    idx = _gpu_tensors((past_len, "past_len", i32), (new_len, "new_len", i32),
+                       (free_pages, "free_pages", i32),
+                       *(((free_start, "free_start", i32),) if free_start is not None else ()))
+    _one_gpu(idx, (_strided(block_table, "block_table", i32, 2), "block_table"))
+    R, width = block_table.shape
+    if past_len.shape != (R,) or new_len.shape != (R,):
+        raise ValueError(f"past_len {tuple(past_len.shape)} and new_len {tuple(new_len.shape)} "
+                         f"must have one entry for each of the {R} rows of block_table")
+    if free_pages.dim() != 1:
+        raise ValueError(f"free_pages must be [F] (got {tuple(free_pages.shape)})")
+    if free_start is not None and free_start.numel() != 1:
+        raise ValueError("free_start must have one element")
+    if R > 1 and block_table.stride(0) < width:
+        raise ValueError("block_table rows must not overlap")
+    T = int(n_tokens)
+    if T < 0:
+        raise ValueError(f"n_tokens must be >= 0 (got {T})")
+    dev = past_len.device
+    # one allocation: slot first, the only one of 8 bytes
+    rows = torch.empty(2 * T + T + 2 * R + 2, dtype=i32, device=dev)
+    slot, position = rows[:2 * T].view(torch.int64), rows[2 * T:3 * T]
+    q_start, kv_len = rows[3 * T:3 * T + R + 1], rows[3 * T + R + 1:3 * T + 2 * R + 1]
+    free_next = rows[3 * T + 2 * R + 1:]
+    _launch((_lib or load_library()).db_paged_plan, idx, "db_paged_plan", past_len.data_ptr(),
+            new_len.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), width), width,
+            free_pages.data_ptr(), free_pages.numel(),
+            None if free_start is None else free_start.data_ptr(), int(page_size), R, T,
+            q_start.data_ptr(), kv_len.data_ptr(), position.data_ptr(), slot.data_ptr(),
+            free_next.data_ptr())
+    return PagedPlan(q_start, kv_len, position, slot, free_next)
+
+
+def rope_append(qkv, position, slot, K, V, inv_freq, axes=None, interleaved: bool = False,
+                k_scale=None, v_scale=None, out=None):
+    """Rotary positions on the queries and keys of a projection, keys and
+    values into the pages of the cache.  Returns the turned queries [T,Hq,D].
+
+    qkv [T, (Hq + 2 Hkv) D] fp16 or bf16 (rows may be strided), query, key and
+    value heads side by side; K/V [pages, Hkv, page_size, D] of that type, or
+    float8_e4m3fn with fp32 ``k_scale``/``v_scale`` [Hkv] (any strides with
+    contiguous rows of D, so a [pages, page_size, Hkv, D] cache is passed as its
+    ``permute(0, 2, 1, 3)``); slot [T] int64 as :func:`paged_plan` gives it (a
+    slot outside the cache writes nothing; slots must differ).
+
+    Pair i of a head turns by ``position * inv_freq[i]`` (inv_freq fp32, rot/2
+    entries, rot <= D; elements past rot stay): elements i and i + rot/2, or
+    2i and 2i+1 where ``interleaved``.  position is int32 [T], or [A, T] for
+    tokens with A axes (time, height, width): ``axes`` then names the axis of
+    each pair, e.g. ``[0] * 16 + [1] * 24 + [2] * 24``."""
+    torch = _torch or _torch_mod()
+    idx = _strided(qkv, "qkv", None, 2)
+    dt = _activation(qkv, "qkv")
+    cache = _paged_cache(K, V, k_scale, v_scale, qkv.dtype, idx)
+    T, Hkv, D = qkv.shape[0], cache.Hkv, cache.D
+    Hq = qkv.shape[1] // D - 2 * Hkv if D else 0
+    if Hq < 1 or (Hq + 2 * Hkv) * D != qkv.shape[1]:
+        raise ValueError(f"qkv rows of {qkv.shape[1]} elements are not (Hq + 2 * {Hkv}) * {D}")
+    _one_gpu(idx, (_gpu_tensors((position, "position", torch.int32), (slot, "slot", torch.int64),
+                                (inv_freq, "inv_freq", torch.float32)), "position"))
+    n_axes = 1 if position.dim() == 1 else position.shape[0]
+    if position.dim() not in (1, 2) or position.shape[-1] != T or slot.shape != (T,):
+        raise ValueError(f"position {tuple(position.shape)} and slot {tuple(slot.shape)} must "
+                         f"have one entry for each of the {T} rows of qkv")
+    if inv_freq.dim() != 1:
+        raise ValueError(f"inv_freq must be [rot / 2] (got {tuple(inv_freq.shape)})")
+    axis_map = None
+    if axes is not None:
+        axis_map = bytes(axes)
+        if len(axis_map) != inv_freq.numel():
+            raise ValueError(f"axes has {len(axis_map)} entries for {inv_freq.numel()} pairs")
+    elif n_axes != 1:
+        raise ValueError("positions of several axes need axes, the axis of each pair")
+    q = _row_output((T, Hq, D), qkv.dtype, idx, out)
+    _launch((_lib or load_library()).db_rope_append, idx, "db_rope_append", qkv.data_ptr(),
+            qkv.stride(0) if T > 1 else qkv.shape[1], position.data_ptr(), n_axes, axis_map,
+            slot.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.numel(), bool(interleaved),
+            C.byref(cache), q.data_ptr(), T, Hq, dt)
+    return q
+
+
+def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None = None,
+                    causal: bool = True, window: int | None = None, max_new: int | None = None,
+                    k_scale=None, v_scale=None, out=None):
+    """Attention of each request's new tokens over its pages of the cache:
+    single tokens, drafts and chunks of a prompt alike.  Returns [T,Hq,D].
+
+    q [T,Hq,D] fp16 or bf16 (token and head strides free); K/V and their scales
+    as in :func:`rope_append`, D 64 or 128, Hq a multiple of Hkv; block_table
+    [R, width], q_start [R+1] and kv_len [R] int32 on the GPU.  Request r has
+    the rows q_start[r] .. q_start[r+1]-1, the last of its kv_len[r] tokens,
+    whose keys and values are in the cache already.  A token sees the keys up
+    to its own position (``causal``; all of its request otherwise), with
+    ``window`` only the last that many; a token that sees nothing gets zeros,
+    and what hidden keys and values hold never counts.  Rows that belong to no
+    request are not written.
+
+    ``max_new`` is the most new tokens a request has, where the caller knows it
+    (1 in a plain decode step): it spares the kernels that such a call does not
+    need, and nothing else."""
+    torch = _torch or _torch_mod()
+    idx = _strided(q, "q", None, 3)
+    dt = _activation(q, "q")
+    cache = _paged_cache(K, V, k_scale, v_scale, q.dtype, idx)
+    T, Hq, D = q.shape
+    if D != cache.D:
+        raise ValueError(f"q {tuple(q.shape)} and K {tuple(K.shape)} disagree on D")
+    i32 = torch.int32
+    _one_gpu(idx, (_strided(block_table, "block_table", i32, 2), "block_table"),
+             (_gpu_tensors((q_start, "q_start", i32), (kv_len, "kv_len", i32)), "q_start"))
+    R, width = block_table.shape
+    if q_start.shape != (R + 1,) or kv_len.shape != (R,):
+        raise ValueError(f"q_start {tuple(q_start.shape)} and kv_len {tuple(kv_len.shape)} must "
+                         f"have R + 1 and R entries for the {R} rows of block_table")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be >= 1 (got {window})")
+    if max_new is not None and max_new < 1:
+        raise ValueError(f"max_new must be >= 1 (got {max_new})")
+    scale = 1.0 / math.sqrt(D) if scale is None and D else float(scale or 0.0)
+    o = _row_output((T, Hq, D), q.dtype, idx, out)
+    lib = _lib or load_library()
+    most = min(int(max_new or T), T)
+    if torch.cuda.current_device() == idx:
+        nbytes = lib.db_paged_attention_workspace_bytes(T, Hq, cache.Hkv, D, R, most)
+    else:
+        with torch.cuda.device(idx):
+            nbytes = lib.db_paged_attention_workspace_bytes(T, Hq, cache.Hkv, D, R, most)
+    # Nothing in it outlives the call, so torch's allocator hands it out anew
+    # each time: per stream, and from a graph's own pool under capture.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _launch(lib.db_paged_attention, idx, "db_paged_attention", q.data_ptr(), *_strides(q, 2),
+            o.data_ptr(), C.byref(cache), block_table.data_ptr(), *_strides(block_table, 1), width, q_start.data_ptr(), kv_len.data_ptr(), T, R,
+            Hq, most, scale, bool(causal), int(window or 0), dt, ws.data_ptr(), nbytes)
+    return o

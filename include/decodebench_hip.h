@@ -47,6 +47,8 @@ extern "C" {
 /* Weight element types accepted by the GEMV entry points. */
 #define DB_DTYPE_F16 0
 #define DB_DTYPE_FP8_E4M3 1 /* OCP e4m3fn + per-output-row fp32 scale */
+/* Activations and caches of the paged entry points only. */
+#define DB_DTYPE_BF16 2
 
 /* ABI revision of this header (DB_ABI_VERSION). */
 int db_abi_version(void);
@@ -192,6 +194,91 @@ int db_f4_splitkv(const void* q, const void* k, const void* v, void* o,
 int db_f4_splitkv_noalloc(const void* q, const void* k, const void* v, void* o,
                           int B, int Hq, int Hkv, int L, int D, int S,
                           float scale, void* stream);
+
+/* ---- a serving step over a paged KV cache --------------------------------
+ * The cache is pages of page_size tokens; a request's tokens lie in the pages
+ * that its row of the block table names, token j in page table[j / page_size]
+ * at place j % page_size.  Three calls make a step: db_paged_plan lays out the
+ * step's tokens, db_rope_append turns queries and keys and writes keys and
+ * values into the cache, db_paged_attention attends over it.  Lengths, tables
+ * and slots stay on the GPU.  Wrong ones (lengths out of order, page numbers or
+ * slots outside the cache) lead to no access outside the tensors: such keys
+ * are not seen and such rows are not written.  No counterpart in the
+ * reference, whose cache is one dense [B, Hkv, L, D] tensor of equal lengths
+ * (src/decodebench/demos/llama_decode.py:110-116). */
+typedef struct db_paged_cache {
+  void* k;                /* element (page, head, token, d) at the strides below */
+  void* v;
+  const float* k_scale;   /* [Hkv], e4m3 only: value = scale[head] * e4m3, > 0 */
+  const float* v_scale;
+  long long k_page_stride, k_head_stride, k_token_stride; /* in elements; rows of */
+  long long v_page_stride, v_head_stride, v_token_stride; /* D are contiguous     */
+  int pages, page_size, Hkv, D;
+  int dtype;              /* DB_DTYPE_F16, DB_DTYPE_BF16 or DB_DTYPE_FP8_E4M3 */
+} db_paged_cache;
+
+/* Rows, lengths, positions and slots of a step's tokens, from the requests'
+ * lengths.  past [R] tokens in the cache and fresh [R] new tokens (negative
+ * ones count as 0); requests in order have the rows q_start[r] ..
+ * q_start[r + 1] - 1 of T, and tokens that T rows do not hold are left out.
+ *   kv_len [R]  = past + new tokens laid out
+ *   position [T], slot [T] = page number * page_size + place in the page
+ * A request's new pages are taken from free_pages[*free_start ...] (0 where
+ * free_start is NULL), requests in order, and entered in its row of `table`
+ * [R, width] (rows table_stride entries apart); *free_next is where the next
+ * step's pages begin.  More than free_count says that pages ran out: entries
+ * without a page get -1, tokens without one slot -1, as tokens past the
+ * table's width.  Rows behind the last token get position 0 and slot -1.
+ * Contract: R >= 0, T >= 0, width >= 1, page_size >= 1, free_count >= 0;
+ * outputs overlap no input. */
+int db_paged_plan(const int* past, const int* fresh, int* table, long long table_stride,
+                  int width, const int* free_pages, int free_count, const int* free_start,
+                  int page_size, int R, int T, int* q_start, int* kv_len, int* position,
+                  long long* slot, int* free_next, void* stream);
+
+/* Rotary positions, and the cache write.  A row of qkv [T, (Hq + 2 Hkv) D]
+ * (rows qkv_stride elements apart) is query, key and value heads.  Pair i < rot / 2 of a
+ * query or key head turns by position[axis(i), t] * inv_freq[i] (taken in 64
+ * bits): elements i and i + rot / 2, or 2 i and 2 i + 1 where `interleaved`;
+ * elements past rot stay as they are.  axis_of_pair [rot / 2] (host memory,
+ * values below n_axes; NULL: all 0) says which row of position [n_axes, T]
+ * turns a pair: time, height and width of image and video tokens.  Queries go
+ * to q [T, Hq, D], keys and values to the cache at slot[t] (values unturned);
+ * a slot outside the cache writes nothing.  Slots of one call must differ:
+ * what two tokens write to one slot is either's, 16 bytes at a time.
+ * e4m3: round(clamp(x / scale[head], -448, 448)).
+ * Contract: T >= 0, Hq >= 1, D a multiple of 16 up to 256, rot a multiple of
+ * 16 up to D, 1 <= n_axes <= 4, dtype DB_DTYPE_F16 or DB_DTYPE_BF16, a cache of
+ * that type or e4m3; qkv, q and cache rows 16-byte aligned. */
+int db_rope_append(const void* qkv, long long qkv_stride, const int* position, int n_axes,
+                   const unsigned char* axis_of_pair, const long long* slot,
+                   const float* inv_freq, int rot, int interleaved,
+                   const db_paged_cache* cache, void* q, int T, int Hq, int dtype,
+                   void* stream);
+
+/* Attention of each request's new tokens over its pages: rows q_start[r] ..
+ * q_start[r + 1] - 1 of q [T, Hq, D] (strides in elements) are the last tokens of
+ * request r's kv_len[r], which are in the cache already.
+ *   o[t, h] = sum_j softmax_j(scale q[t, h] . K[j, h / G]) V[j, h / G]
+ * over the keys j < kv_len[r] (table [R, width], rows table_stride entries
+ * apart, shared ones too); with `causal` those up to the token's own
+ * position, with window > 0 (causal only) the last `window` of these; keys
+ * whose page is not in the cache are not seen.  A token that sees nothing gets
+ * zeros; what a hidden key or value holds never counts, Inf and NaN included.
+ * Rows of o [T, Hq, D] (dense) that belong to no request stay as they are.
+ * max_new > 0 says how many new tokens a request has at most (0: T), which
+ * decides which kernels are launched; a call that breaks it is still right.
+ * Contract: T >= 0, R >= 0, Hq a multiple of Hkv, T * Hq < 2^31, D 64 or 128,
+ * scale finite and > 0, dtype as db_rope_append; q, o and cache rows 16-byte
+ * aligned; ws of db_paged_attention_workspace_bytes, 256-byte aligned, not
+ * shared by calls that overlap in time. */
+size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new);
+int db_paged_attention(const void* q, long long q_token_stride, long long q_head_stride,
+                       void* o, const db_paged_cache* cache, const int* table,
+                       long long table_stride, int width, const int* q_start,
+                       const int* kv_len, int T, int R, int Hq, int max_new, float scale,
+                       int causal, int window, int dtype, void* ws, size_t ws_bytes,
+                       void* stream);
 
 /* Capture state of `stream`: *capture_id is the id of the hipGraph capture
  * the stream is recording into (unique per capture), or 0 when it is not
