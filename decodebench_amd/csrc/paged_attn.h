@@ -133,7 +133,6 @@ struct PagedArgs {
 
 constexpr int kDecodeRows = 16;  // rows of the decode kernel's tile
 constexpr int kChunkRows = 128;  // rows of the chunk kernel's tile
-constexpr int kDecodeKeys = 16;
 constexpr int kChunkKeys = 64;
 constexpr int kPagedThreads = 256;
 constexpr int kDescInts = 8;
@@ -183,114 +182,115 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r)
   return q;
 }
 
-struct PagedShared {
-  int wave_sums[kPagedThreads / kWave][3];
-  unsigned long long wave_work[kPagedThreads / kWave];
-  PagedWork found;
-  int hit;
-};
+// Inclusive prefix sum over the 64 lanes (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) {
+  return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1);
+}
+
+// Max over lanes that differ in bit 5 (and in bit 4) of their number.  (The
+// results are copied out before the bit casts: a bit cast of a vector's
+// element reads its element 0 whatever the index.)
+__device__ __forceinline__ float max_xor32(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const unsigned x = r[0], y = r[1];
+  return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ __forceinline__ float max_xor16(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const unsigned x = r[0], y = r[1];
+  return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
 
 // Walks the workgroup's numbers w = blockIdx.x, + gridDim.x, ... : next()
-// says whether there is another piece of work and leaves it in `work`
-// (uniform).  All threads of the workgroup call it together; it ends with a
-// barrier behind every read of the shared state, so the caller's LDS is free.
+// says whether there is another piece of work and leaves it in `work`, in
+// scalar registers.  Every wave does the search for itself, a lane to a
+// request and 64 requests a round: no LDS, no barrier.
 template <int MT, int KT>
 struct PagedSchedule {
   const PagedArgs& a;
-  PagedShared& sh;
   int w, round, C;
-  int base[3];       // units, records, groups of the rounds before (per KV head)
-  PagedRequest mine;
-  int count[3], incl[3], sums[3];
+  int units0, recs0, groups0;  // of the rounds before (per KV head)
+  PagedRequest mine;           // this lane's request of the round
+  int splits, units, before, total;
 
-  __device__ PagedSchedule(const PagedArgs& args, PagedShared& s)
-      : a(args), sh(s), w(blockIdx.x), round(0), base{0, 0, 0} {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    unsigned long long total = 0;
-    for (int r = (a.R - 1) / kPagedThreads * kPagedThreads; r >= 0; r -= kPagedThreads) {
-      mine = paged_request<MT, KT>(a, r + threadIdx.x);
-      total += (unsigned long long)mine.row_tiles * mine.tiles;
+  __device__ explicit PagedSchedule(const PagedArgs& args)
+      : a(args), w(blockIdx.x), round(0), units0(0), recs0(0), groups0(0) {
+    const int lane = threadIdx.x & (kWave - 1);
+    float work = 0.0f;  // its rounding may move C by one tile in 2^24
+    for (int r = (a.R - 1) / kWave * kWave; r >= 0; r -= kWave) {
+      mine = paged_request<MT, KT>(a, r + lane);
+      work += (float)mine.row_tiles * (float)mine.tiles;
     }
-    for (int d = 1; d < kWave; d <<= 1) total += __shfl_xor(total, d);
-    if (lane == 0) sh.wave_work[wave] = total;
-    __syncthreads();
-    total = 0;
-    for (int i = 0; i < kPagedThreads / kWave; ++i) total += sh.wave_work[i];
-    total *= a.Hkv;
-    const unsigned long long per = (total + a.target - 1) / a.target;
-    C = (int)min(max(per, (unsigned long long)a.min_tiles), 0x7FFFFFFFull);
+    const float per = ceilf(wave_sum(work) * (float)a.Hkv / (float)a.target);
+    C = max(a.min_tiles, (int)fminf(per, 1073741824.0f));
     scan();
-    if (blockIdx.x == 0) {  // the groups of the whole call, for the merge
-      int groups = sums[2];
-      for (int r = kPagedThreads; r < a.R; r += kPagedThreads) {
-        const PagedRequest q = paged_request<MT, KT>(a, r + threadIdx.x);
-        int g = splits_of(q) > 1 ? q.row_tiles : 0;
-        for (int d = 1; d < kWave; d <<= 1) g += __shfl_xor(g, d);
-        __syncthreads();
-        if (lane == 0) sh.wave_sums[wave][0] = g;
-        __syncthreads();
-        for (int i = 0; i < kPagedThreads / kWave; ++i) groups += sh.wave_sums[i][0];
+    if (blockIdx.x == 0 && threadIdx.x < kWave) {  // the groups of the whole call, for the merge
+      int groups = splits > 1 ? mine.row_tiles : 0;
+      for (int r = kWave; r < a.R; r += kWave) {
+        const PagedRequest q = paged_request<MT, KT>(a, r + lane);
+        groups += splits_of(q) > 1 ? q.row_tiles : 0;
       }
-      if (threadIdx.x == 0) a.rec.head[0] = groups * a.Hkv;
-      __syncthreads();
+      groups = wave_total(groups) * a.Hkv;
+      if (lane == 0) a.rec.head[0] = groups;
     }
   }
 
   __device__ int splits_of(const PagedRequest& q) const {
     return q.row_tiles == 0 ? 0 : max(1, (q.tiles + C - 1) / C);
   }
-
-  // Prefix sums over the requests of this round.
   __device__ void scan() {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int s = splits_of(mine);
-    count[0] = mine.row_tiles * s;
-    count[1] = s > 1 ? count[0] : 0;
-    count[2] = s > 1 ? mine.row_tiles : 0;
-    for (int k = 0; k < 3; ++k) incl[k] = count[k];
-    for (int d = 1; d < kWave; d <<= 1)
-      for (int k = 0; k < 3; ++k) {
-        const int v = __shfl_up(incl[k], d);
-        if (lane >= d) incl[k] += v;
-      }
-    __syncthreads();
-    if (lane == kWave - 1)
-      for (int k = 0; k < 3; ++k) sh.wave_sums[wave][k] = incl[k];
-    __syncthreads();
-    for (int k = 0; k < 3; ++k) sums[k] = 0;
-    for (int i = 0; i < kPagedThreads / kWave; ++i)
-      for (int k = 0; k < 3; ++k) {
-        if (i < wave) incl[k] += sh.wave_sums[i][k];
-        sums[k] += sh.wave_sums[i][k];
-      }
+    splits = splits_of(mine);
+    units = mine.row_tiles * splits;
+    const int incl = wave_scan(units);
+    before = incl - units;
+    total = __builtin_amdgcn_readlane(incl, kWave - 1);
   }
 
   __device__ bool next(PagedWork& work) {
-    const int unit = w / a.Hkv;
-    while (unit >= base[0] + sums[0]) {
-      for (int k = 0; k < 3; ++k) base[k] += sums[k];
+    const int unit = w / a.Hkv, lane = threadIdx.x & (kWave - 1);
+    while (unit >= units0 + total) {
+      units0 += total;
+      recs0 += wave_total(splits > 1 ? units : 0);
+      groups0 += wave_total(splits > 1 ? mine.row_tiles : 0);
       ++round;
-      if ((long long)round * kPagedThreads >= a.R) return false;
-      mine = paged_request<MT, KT>(a, round * kPagedThreads + threadIdx.x);
+      if ((long long)round * kWave >= a.R) return false;
+      mine = paged_request<MT, KT>(a, round * kWave + lane);
       scan();
     }
-    const int at = unit - base[0] - (incl[0] - count[0]);
-    __syncthreads();
-    if (at >= 0 && at < count[0]) {
-      PagedWork f;
-      f.req = mine;
-      f.r = round * kPagedThreads + threadIdx.x;
-      f.head = w % a.Hkv;
-      f.splits = count[0] / mine.row_tiles;
-      f.tile = mine.row_tiles - 1 - at / f.splits;  // the longest first
-      f.split = at % f.splits;
-      const bool split = f.splits > 1;
-      f.rec = split ? (base[1] + incl[1] - count[1] + f.tile * f.splits) * a.Hkv + f.head : -1;
-      f.group = split ? (base[2] + incl[2] - count[2] + f.tile) * a.Hkv + f.head : -1;
-      sh.found = f;
+    const int at0 = unit - units0;
+    const unsigned long long hit = __ballot(at0 >= before && at0 - before < units);
+    const int who = __builtin_ctzll(hit);
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
+    work.req.tok0 = of(mine.tok0);
+    work.req.n = of(mine.n);
+    work.req.len = of(mine.len);
+    work.req.row_tiles = of(mine.row_tiles);
+    work.req.tiles = of(mine.tiles);
+    work.r = round * kWave + who;
+    work.head = w % a.Hkv;
+    work.splits = of(splits);
+    const int at = at0 - of(before);
+    work.tile = work.req.row_tiles - 1 - at / work.splits;  // the longest first
+    work.split = at % work.splits;
+    work.rec = work.group = -1;
+    if (work.splits > 1) {
+      const bool mine_before = lane < who && splits > 1;
+      work.rec = (recs0 + wave_total(mine_before ? units : 0) + work.tile * work.splits) * a.Hkv +
+                 work.head;
+      work.group =
+          (groups0 + wave_total(mine_before ? mine.row_tiles : 0) + work.tile) * a.Hkv + work.head;
     }
-    __syncthreads();
-    work = sh.found;
     w += gridDim.x;
     return true;
   }
@@ -328,6 +328,7 @@ __device__ __forceinline__ void paged_describe(const PagedArgs& a, const PagedWo
 
 // e4m3 or 16-bit caches: the element type of the products E, of the cache C8.
 typedef void (*PagedFn)(PagedArgs);
-PagedFn paged_decode_fn(bool bf16, bool fp8, int D);
+int paged_decode_min_tiles(bool fp8, int D);
+PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned);
 
 }  // namespace dbk

@@ -39,7 +39,6 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
   constexpr int KS = D + 8, VS = D + 16;           // row strides in LDS (elements)
   constexpr int QSTEPS = D / 16, NB = D / 32;
 
-  __shared__ PagedShared s_sched;
   __shared__ __align__(16) elem s_k[KT * KS];
   __shared__ __align__(16) elem s_v[KT * VS];
 
@@ -47,7 +46,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n32 = lane & 31, half = lane >> 5;
 
-  PagedSchedule<MT, KT> schedule(a, s_sched);
+  PagedSchedule<MT, KT> schedule(a);
   PagedWork wk;
   while (schedule.next(wk)) {
     const PagedRequest& rq = wk.req;
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[kb][i]);
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 32)) * scale;
+      tmax = max_xor32(tmax) * scale;
       const float m_new = fmaxf(m_run, tmax);
       const float m_use = m_new == kPagedNegInf ? 0.0f : m_new;
       const float alpha = fast_exp2(m_run - m_use);
@@ -294,19 +293,25 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
         if (half == 0) a.rec.ml[at] = make_float2(m_run, l);
       }
     }
+    __syncthreads();  // the tiles are read: the next piece may write them
   }
 }
 
 // Joins the records of split rows: o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
-// One wave a row; the groups' count and places come from the first kernel.
+// A workgroup a row, its four waves a quarter of the splits each, eight records
+// in flight a wave (a wave alone, one record after the other, took 45 us for
+// the 64 splits of one request of 8192 tokens); the groups' count and places
+// come from the first kernel.
 template <class E, int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge(PagedArgs a, int mt) {
   typedef typename E::type elem;
   constexpr int PER = D / kWave;  // elements a lane
+  constexpr int kAtOnce = 8;
+  __shared__ float s_acc[kWaves][D], s_m[kWaves], s_l[kWaves];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int total = min(a.rec.head[0], a.rec.groups) * mt;
-  for (int task = blockIdx.x * kWaves + wave; task < total; task += gridDim.x * kWaves) {
+  for (int task = blockIdx.x; task < total; task += gridDim.x) {
     const int group = task / mt, row = task % mt;
     const int* d = a.rec.desc + (size_t)group * kDescInts;
     const int splits = d[0], rec0 = d[1], head = rec0 % a.Hkv;
@@ -314,24 +319,61 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge(PagedArgs a, int mt
     float M = kPagedNegInf, L = 0.0f, acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const size_t at = (size_t)(rec0 + s * a.Hkv) * mt + row;
-      const float2 ml = a.rec.ml[at];
-      if (ml.y == 0.0f) continue;  // saw nothing
-      const float Mn = fmaxf(M, ml.x);
-      const float keep = M == kPagedNegInf ? 0.0f : fast_exp2(M - Mn), w = fast_exp2(ml.x - Mn);
-      const float* op = a.rec.opart + at * D + lane * PER;
-      L = L * keep + w * ml.y;
+    for (int s0 = wave; s0 < splits; s0 += kWaves * kAtOnce) {
+      float2 ml[kAtOnce];
+      float v[kAtOnce][PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] = acc[i] * keep + w * op[i];
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int s = min(s0 + j * kWaves, splits - 1);
+        const size_t at = (size_t)(rec0 + s * a.Hkv) * mt + row;
+        ml[j] = a.rec.ml[at];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[j][i] = a.rec.opart[at * D + lane * PER + i];
+      }
+      float Mn = M;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (s0 + j * kWaves >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
+        if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);
+      }
+      const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
+      L *= keep;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] *= keep;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (ml[j].y == 0.0f) continue;  // saw nothing
+        const float w = fast_exp2(ml[j].x - Mn);
+        L = fmaf(w, ml[j].y, L);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, v[j][i], acc[i]);
+      }
       M = Mn;
     }
-    const int xr = d[3] + row;
-    elem* op = static_cast<elem*>(a.o) +
-               ((size_t)(d[2] + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D + lane * PER;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) op[i] = (elem)(L == 0.0f ? 0.0f : acc[i] * inv);
+    for (int i = 0; i < PER; ++i) s_acc[wave][lane * PER + i] = acc[i];
+    if (lane == 0) {
+      s_m[wave] = M;
+      s_l[wave] = L;
+    }
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float Mt = kPagedNegInf, Lt = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        if (s_l[w] != 0.0f) Mt = fmaxf(Mt, s_m[w]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        if (s_l[w] == 0.0f) continue;
+        const float e = fast_exp2(s_m[w] - Mt);
+        Lt = fmaf(e, s_l[w], Lt);
+        o = fmaf(e, s_acc[w][threadIdx.x], o);
+      }
+      const int xr = d[3] + row;
+      static_cast<elem*>(a.o)[((size_t)(d[2] + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D +
+                              threadIdx.x] = (elem)(Lt == 0.0f ? 0.0f : o / Lt);
+    }
+    __syncthreads();
   }
 }
 
@@ -374,6 +416,13 @@ PagedRecords region(char* base, int target, int mt, int D) {
   r.opart = reinterpret_cast<float*>(base);
   (void)D;
   return r;
+}
+
+// Whether 16 keys from a multiple of 16 on always lie in one page, at offsets
+// from its first key that 32 bits hold.
+bool paged_aligned(const db_paged_cache& kv) {
+  constexpr long long kFar = 1 << 26;
+  return kv.page_size % 16 == 0 && kv.k_token_stride < kFar && kv.v_token_stride < kFar;
 }
 
 // Which kernels a call of these bounds needs.
@@ -450,12 +499,13 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
                        stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(1024), dim3(kPagedThreads), 0, stream, a, mt);
+    hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(2048), dim3(kPagedThreads), 0, stream, a, mt);
     return hipGetLastError();
   };
   hipError_t e = hipSuccess;
   if (decode)
-    e = run(paged_decode_fn(c.bf16, fp8, D), chunk ? 1 : 0, kDecodeRows, 8);
+    e = run(paged_decode_fn(c.bf16, fp8, D, paged_aligned(kv)), chunk ? 1 : 0, kDecodeRows,
+            paged_decode_min_tiles(fp8, D));
   if (e == hipSuccess && chunk)
     e = run(pick_chunk(c.bf16, fp8, D), decode ? 2 : 0, kChunkRows, 8);
   return e;

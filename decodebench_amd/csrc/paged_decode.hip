@@ -1,21 +1,28 @@
 // paged_decode.hip -- paged attention of few rows (single tokens, drafts).
 //
 // A workgroup of four waves owns one (request, KV head, row tile of 16 rows)
-// and one split of the keys; wave w takes the 16-key tiles w, w + 4, ... of
-// the split.  Bound by HBM: every key and value is read once per row tile, and
+// and one split of the keys; wave w takes the key tiles w, w + 4, ... of the
+// split.  Bound by HBM: every key and value is read once per row tile, and
 // rows beyond the few that a request has cost nothing but idle MFMA columns.
 //
+//  * A tile is 16 keys where K takes 4 KB of them, 32 (two sub-tiles of 16)
+//    where it takes less (e4m3, heads of 64), so that a tile's fixed work, its
+//    maximum and its rescale, is paid per 8 KB of cache.
 //  * Scores: v_mfma_f32_16x16x32, A = 16 keys straight from the cache to
 //    registers (lane (g4, n16) holds 16-byte chunks g4, g4 + 4, ... of key
 //    n16), B = the rows.  An e4m3 chunk is 16 elements, so its two halves are
 //    two MFMA steps; the rows are loaded in the same order.
-//  * Softmax with running maximum and sum, base 2, fp32, on the four keys that
-//    each lane holds.  Probabilities are rounded to the element type for the
-//    product and summed as rounded, so numerator and denominator agree.
-//  * P.V: O^T = V^T P^T on 16x16x16 MFMAs, V^T through the wave's copy of the
-//    tile in LDS and the transposing read ds_read_b64_tr_b16.
-//  * A lane looks up the page of key n16 of a tile (the lookups run one tile
-//    ahead of the loads); rows of V take theirs from that lane.
+//  * Softmax with running maximum and sum, base 2, fp32, on the keys that each
+//    lane holds.  Probabilities are rounded to the element type for the product
+//    and summed as rounded, so numerator and denominator agree.
+//  * P.V: O^T = V^T P^T on 16x16x16 (two sub-tiles: 16x16x32) MFMAs, V^T
+//    through the wave's copy of the tile in LDS and the transposing read
+//    ds_read_b64_tr_b16.
+//  * Pages of a multiple of 16 tokens (ALIGNED): a sub-tile lies in one page.
+//    Lane i works out where the wave's i-th sub-tile is, 64 of them at once,
+//    and a tile's addresses are two scalars read from its lane.  Any other
+//    page size: a lane looks up the page of its own key, one tile ahead of the
+//    loads, and rows of V take theirs from that lane.
 //  * Masked keys: scores by selection, so no Inf or NaN of a masked key counts;
 //    a tile that some row sees only in part is searched for an Inf or NaN
 //    among its values, and one that has any is added key by key.
@@ -26,26 +33,46 @@ namespace dbk {
 namespace {
 
 constexpr int kWaves = kPagedThreads / kWave;
-constexpr int MT = kDecodeRows, KT = kDecodeKeys;
+constexpr int MT = kDecodeRows;
 
-template <class E, bool FP8, int D>
-__global__ __launch_bounds__(kPagedThreads) void paged_decode(PagedArgs a) {
+constexpr float kHidden = -1.0f;  // no probability
+
+constexpr int decode_keys(bool fp8, int D) { return D * (fp8 ? 1 : 2) >= 256 ? 16 : 32; }
+
+// Orders a wave's LDS accesses (not its loads from memory) as written.
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+__device__ __forceinline__ long long lane_i64(long long v, int lane) {
+  const int lo = __builtin_amdgcn_readlane((int)v, lane);
+  const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+
+template <class E, bool FP8, int D, bool ALIGNED>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
   typedef typename E::type elem;
   typedef typename E::vec8 vec8;
   typedef typename E::vec4 vec4;
   constexpr int CB = FP8 ? 1 : 2;          // bytes of a cache element
+  constexpr int KT = decode_keys(FP8, D);  // keys of a tile
+  constexpr int NS = KT / 16;              // sub-tiles
   constexpr int NK = D * CB / 64;          // 16-byte loads of K a lane (16 keys, 4 lanes each)
   constexpr int STEPS = D / 32;            // MFMA steps of a score
   constexpr int LPR = D * CB / 16;         // lanes per row of V
   constexpr int RPI = kWave / LPR;         // rows of V a load instruction
-  constexpr int NV = KT / RPI;
+  constexpr int NV = 16 / RPI;
   constexpr int VS = D + 16;               // row stride of the V tile in LDS (elements)
   constexpr int NB = D / 16;
-  constexpr size_t kRegion = sizeof(float) * MT * D;
-  static_assert(kRegion >= sizeof(elem) * KT * VS, "a V tile fits the wave's outputs");
+  constexpr int kTilesHeld = kWave / NS;   // tiles whose places the lanes hold
+  constexpr size_t kOut = sizeof(float) * MT * D, kTile = sizeof(elem) * KT * VS;
+  constexpr size_t kRegion = kOut > kTile ? kOut : kTile;
 
-  __shared__ PagedShared s_sched;
   __shared__ __align__(16) char s_region[kWaves][kRegion];
+  __shared__ float s_p[kWaves][KT][16];  // probabilities of a tile added key by key
   __shared__ float s_m[MT][kWaves], s_l[MT][kWaves];
 
   const int lane = threadIdx.x & (kWave - 1);
@@ -53,33 +80,55 @@ __global__ __launch_bounds__(kPagedThreads) void paged_decode(PagedArgs a) {
   const int n16 = lane & 15, g4 = lane >> 4;
   elem* const vbuf = reinterpret_cast<elem*>(s_region[wave]);
 
-  PagedSchedule<MT, KT> schedule(a, s_sched);
+  PagedSchedule<MT, KT> schedule(a);
   PagedWork wk;
   while (schedule.next(wk)) {
     const PagedRequest& rq = wk.req;
     int t_begin, t_end;
     paged_range<MT, KT>(a, wk, t_begin, t_end);
-    t_begin = __builtin_amdgcn_readfirstlane(t_begin);
-    t_end = __builtin_amdgcn_readfirstlane(t_end);
     paged_describe(a, wk, MT);
-    const int limit = __builtin_amdgcn_readfirstlane(paged_limit(a, rq.len));
+    const int limit = paged_limit(a, rq.len);
+
+    const char* const kbase = static_cast<const char*>(a.k) + wk.head * a.kh * CB;
+    const char* const vbase = static_cast<const char*>(a.v) + wk.head * a.vh * CB;
+    const int* const trow = a.table + wk.r * a.table_row;
+    const int first = t_begin + wave;
+    const int nt = first < t_end ? (t_end - first + kWaves - 1) / kWaves : 0;
+    auto tile_of = [&](int k) { return first + kWaves * k; };
+
+    // ---- where the keys are ------------------------------------------------
+    // ALIGNED: byte offsets of the first key and value of this lane's sub-tile
+    // (of 64 from tile `held` on), and a bit per sub-tile that has a page.
+    // Otherwise: page of key n16 of a sub-tile, -1 where there is none.
+    long long koff = 0, voff = 0;
+    unsigned long long has = 0;
+    int held = 0;
+    auto hold = [&](int k) {
+      held = k;
+      const int kk = k + lane / NS;
+      const int key = kk < nt ? tile_of(kk) * KT + 16 * (lane % NS) : limit;
+      int p = -1, off = 0;
+      if (key < limit) {
+        const int at = page_of(a, key);
+        off = key - at * a.page;
+        p = trow[at];
+      }
+      const bool ok = (unsigned)p < (unsigned)a.pages;
+      koff = ok ? (p * a.kp + off * a.kt) * CB : 0;
+      voff = ok ? (p * a.vp + off * a.vt) * CB : 0;
+      has = __ballot(ok);
+    };
+    auto lookup = [&](int k, int u) {
+      const int key = tile_of(k) * KT + 16 * u + n16;
+      if (k >= nt || key >= limit) return -1;
+      const int p = trow[page_of(a, key)];
+      return (unsigned)p < (unsigned)a.pages ? p : -1;
+    };
 
     // This lane's row (column n16 of the products) and the keys it sees.
     const int rows = (int)min((long long)rq.n * a.G - (long long)wk.tile * MT, (long long)MT);
     const int x = wk.tile * MT + min(n16, rows - 1);
     const int token = x / a.G, qhead = wk.head * a.G + x % a.G;
-    const int pos = rq.len - rq.n + token;
-    const int khi = a.causal ? min(limit, pos + 1) : limit;
-    const int klo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-    // Keys that every row sees.
-    int all_lo = klo, all_hi = khi;
-    for (int d = 1; d < 16; d <<= 1) {
-      all_lo = max(all_lo, __shfl_xor(all_lo, d));
-      all_hi = min(all_hi, __shfl_xor(all_hi, d));
-    }
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-
     vec8 qop[STEPS];
     {
       const elem* qp = static_cast<const elem*>(a.q) + (rq.tok0 + token) * a.q_token +
@@ -90,118 +139,167 @@ __global__ __launch_bounds__(kPagedThreads) void paged_decode(PagedArgs a) {
         qop[t] = __builtin_bit_cast(vec8, ld16(qp + at));
       }
     }
+    if constexpr (ALIGNED) hold(0);
+    const int past = rq.len - rq.n;
+    const int khi = a.causal ? min(limit, past + token + 1) : limit;
+    const int klo = a.window > 0 ? max(past + token - a.window + 1, 0) : 0;
+    // Keys that every row sees: the first row's end, the last row's beginning.
+    const int i0 = wk.tile * MT / a.G, i1 = (wk.tile * MT + rows - 1) / a.G;
+    const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
+    const int all_lo = a.window > 0 ? max(past + i1 - a.window + 1, 0) : 0;
     const float scale = a.scale_log2 * (FP8 ? a.k_scale[wk.head] : 1.0f);
-    const char* const kbase = static_cast<const char*>(a.k) + wk.head * a.kh * CB;
-    const char* const vbase = static_cast<const char*>(a.v) + wk.head * a.vh * CB;
-    const int* const trow = a.table + wk.r * a.table_row;
-
-    const int first = t_begin + wave;
-    const int nt = first < t_end ? (t_end - first + kWaves - 1) / kWaves : 0;
-    auto tile_of = [&](int k) { return first + kWaves * k; };
-
-    // Page of key n16 of the wave's k-th tile, -1 where there is none.
-    auto lookup = [&](int k) {
-      const int key = tile_of(k) * KT + n16;
-      if (k >= nt || key >= limit) return -1;
-      const int p = trow[page_of(a, key)];
-      return (unsigned)p < (unsigned)a.pages ? p : -1;
-    };
 
     f4 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = kPagedNegInf, l_run = 0.0f;
 
-    // Absent keys read row 0 of page 0: valid memory, never counted.
-    auto load_tile = [&](u4 (&kt)[NK], u4 (&vt)[NV], int tile, int pg) {
-      {
-        const int key = tile * KT + n16;
-        const int off = pg < 0 ? 0 : key - page_of(a, key) * a.page;
-        const char* p = kbase + (max(pg, 0) * a.kp + off * a.kt) * CB;
+    const unsigned lane_k = (unsigned)(n16 * (int)a.kt * CB + g4 * 16);
+    const unsigned lane_v = (unsigned)((lane / LPR) * (int)a.vt * CB + (lane % LPR) * 16);
+    // Absent keys read rows of page 0: valid memory, never counted.
+    auto load_tile = [&](u4 (&kt)[NS][NK], u4 (&vt)[NS][NV], int k, const int (&pg)[NS]) {
+      if constexpr (ALIGNED) {
+        if (k >= held + kTilesHeld) hold(k);
 #pragma unroll
-        for (int t = 0; t < NK; ++t) kt[t] = ld_stream(p + (g4 + 4 * t) * 16);
-      }
+        for (int u = 0; u < NS; ++u) {
+          const int from = (k - held) * NS + u;
+          const char* kp = kbase + lane_i64(koff, from);
+          const char* vp = vbase + lane_i64(voff, from);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int row = j * RPI + lane / LPR, key = tile * KT + row;
-        const int pr = __shfl(pg, row);
-        const int off = pr < 0 ? 0 : key - page_of(a, key) * a.page;
-        vt[j] = ld_stream(vbase + (max(pr, 0) * a.vp + off * a.vt) * CB + (lane % LPR) * 16);
+          for (int t = 0; t < NK; ++t) kt[u][t] = ld_stream(kp + (lane_k + t * 64u));
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            vt[u][j] = ld_stream(vp + j * RPI * a.vt * CB + lane_v);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+          const int key0 = tile_of(k) * KT + 16 * u;
+          {
+            const int key = key0 + n16;
+            const int off = pg[u] < 0 ? 0 : key - page_of(a, key) * a.page;
+            const char* p = kbase + (max(pg[u], 0) * a.kp + off * a.kt) * CB;
+#pragma unroll
+            for (int t = 0; t < NK; ++t) kt[u][t] = ld_stream(p + (g4 + 4 * t) * 16);
+          }
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const int row = j * RPI + lane / LPR, key = key0 + row;
+            const int pr = __shfl(pg[u], row);
+            const int off = pr < 0 ? 0 : key - page_of(a, key) * a.page;
+            vt[u][j] =
+                ld_stream(vbase + (max(pr, 0) * a.vp + off * a.vt) * CB + (lane % LPR) * 16);
+          }
+        }
       }
     };
+    // Bits of the tile's keys that are in the cache.
+    auto present = [&](int k, const int (&pg)[NS]) {
+      unsigned there = 0;
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        if constexpr (ALIGNED)
+          there |= (has >> ((k - held) * NS + u)) & 1 ? 0xFFFFu << (16 * u) : 0u;
+        else
+          there |= ((unsigned)__ballot(pg[u] >= 0) & 0xFFFFu) << (16 * u);
+      }
+      return there;
+    };
 
-    auto compute_tile = [&](const u4 (&kt)[NK], u4 (&vt)[NV], int tile, int pg) {
-      const int key0 = tile * KT;
-      const unsigned there = (unsigned)__ballot(pg >= 0) & 0xFFFFu;
-      const bool partial = there != 0xFFFFu || key0 < all_lo || key0 + KT > all_hi;
+    auto compute_tile = [&](const u4 (&kt)[NS][NK], u4 (&vt)[NS][NV], int k, unsigned there) {
+      const int key0 = tile_of(k) * KT;
+      const bool partial =
+          there != (unsigned)((1ull << KT) - 1) || key0 < all_lo || key0 + KT > all_hi;
       bool odd = false;  // a partly seen tile with an Inf or NaN among its values
       if (partial) {
         bool bad = false;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (!((there >> (j * RPI + lane / LPR)) & 1)) vt[j] = u4{0, 0, 0, 0};
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if constexpr (FP8) {
-              const unsigned w = vt[j][c] & 0x7F7F7F7Fu;  // NaN: seven bits set (no Inf in e4m3)
-              bad = bad || (w & 0xFFu) == 0x7Fu || ((w >> 8) & 0xFFu) == 0x7Fu ||
-                    ((w >> 16) & 0xFFu) == 0x7Fu || (w >> 24) == 0x7Fu;
-            } else {
-              bad = bad || pair_nonfinite<E>(vt[j][c]);
+          for (int j = 0; j < NV; ++j) {
+            const int row = 16 * u + j * RPI + lane / LPR;
+            if (!((there >> row) & 1) || key0 + row >= limit) vt[u][j] = u4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if constexpr (FP8) {
+                const unsigned w = vt[u][j][c] & 0x7F7F7F7Fu;  // NaN: seven bits set (no Inf)
+                bad = bad || (w & 0xFFu) == 0x7Fu || ((w >> 8) & 0xFFu) == 0x7Fu ||
+                      ((w >> 16) & 0xFFu) == 0x7Fu || (w >> 24) == 0x7Fu;
+              } else {
+                bad = bad || pair_nonfinite<E>(vt[u][j][c]);
+              }
             }
           }
-        }
         odd = __any(bad);
       }
       // the tile's values, rows in key order
-      wave_lds_order();
+      lds_order();
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        elem* row = vbuf + (j * RPI + lane / LPR) * VS + (lane % LPR) * (16 / CB);
-        if constexpr (FP8) {
-          const u2 w0 = E::widen(vt[j][0]), w1 = E::widen(vt[j][1]);
-          const u2 w2 = E::widen(vt[j][2]), w3 = E::widen(vt[j][3]);
-          *reinterpret_cast<u4*>(row) = u4{w0[0], w0[1], w1[0], w1[1]};
-          *reinterpret_cast<u4*>(row + 8) = u4{w2[0], w2[1], w3[0], w3[1]};
-        } else {
-          *reinterpret_cast<u4*>(row) = vt[j];
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          elem* row = vbuf + (16 * u + j * RPI + lane / LPR) * VS + (lane % LPR) * (16 / CB);
+          const u4 v = vt[u][j];
+          if constexpr (FP8) {
+            const u2 w0 = E::widen(v[0]), w1 = E::widen(v[1]);
+            const u2 w2 = E::widen(v[2]), w3 = E::widen(v[3]);
+            *reinterpret_cast<u4*>(row) = u4{w0[0], w0[1], w1[0], w1[1]};
+            *reinterpret_cast<u4*>(row + 8) = u4{w2[0], w2[1], w3[0], w3[1]};
+          } else {
+            *reinterpret_cast<u4*>(row) = v;
+          }
         }
-      }
-      wave_lds_order();
+      lds_order();
 
-      // s[j]: score of key key0 + 4 g4 + j and row n16
-      f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      // s[4 u + j]: score of key key0 + 16 u + 4 g4 + j and row n16
+      float s[4 * NS];
 #pragma unroll
-      for (int t = 0; t < NK; ++t) {
-        if constexpr (FP8) {
-          const u2 w0 = E::widen(kt[t][0]), w1 = E::widen(kt[t][1]);
-          const u2 w2 = E::widen(kt[t][2]), w3 = E::widen(kt[t][3]);
-          acc = E::mfma16(__builtin_bit_cast(vec8, u4{w0[0], w0[1], w1[0], w1[1]}), qop[2 * t], acc);
-          acc = E::mfma16(__builtin_bit_cast(vec8, u4{w2[0], w2[1], w3[0], w3[1]}), qop[2 * t + 1],
-                          acc);
-        } else {
-          acc = E::mfma16(__builtin_bit_cast(vec8, kt[t]), qop[t], acc);
+      for (int u = 0; u < NS; ++u) {
+        f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < NK; ++t) {
+          const u4 c = kt[u][t];
+          if constexpr (FP8) {
+            const u2 w0 = E::widen(c[0]), w1 = E::widen(c[1]);
+            const u2 w2 = E::widen(c[2]), w3 = E::widen(c[3]);
+            acc = E::mfma16(__builtin_bit_cast(vec8, u4{w0[0], w0[1], w1[0], w1[1]}), qop[2 * t],
+                            acc);
+            acc = E::mfma16(__builtin_bit_cast(vec8, u4{w2[0], w2[1], w3[0], w3[1]}),
+                            qop[2 * t + 1], acc);
+          } else {
+            acc = E::mfma16(__builtin_bit_cast(vec8, c), qop[t], acc);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * u + j] = acc[j] * scale;
+      }
+      unsigned sees = ~0u;  // bit 4 u + j
+      if (partial) {
+        sees = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) {
+          const int kk = 16 * (i >> 2) + 4 * g4 + (i & 3);
+          const bool ok = key0 + kk >= klo && key0 + kk < khi && ((there >> kk) & 1);
+          sees |= ok ? 1u << i : 0u;
+          s[i] = ok ? s[i] : kPagedNegInf;
         }
       }
-      float s[4];
-      bool sees[4];
+      float tmax = s[0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = key0 + 4 * g4 + j;
-        sees[j] = key >= klo && key < khi && ((there >> (4 * g4 + j)) & 1);
-        s[j] = sees[j] ? acc[j] * scale : kPagedNegInf;
-      }
-      float tmax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+      for (int i = 1; i < 4 * NS; ++i) tmax = fmaxf(tmax, s[i]);
+      tmax = max_xor32(max_xor16(tmax));
       const float m_new = fmaxf(m_run, tmax);
       // A row that has seen nothing yet keeps -inf; its exponents use 0.
       const float m_use = m_new == kPagedNegInf ? 0.0f : m_new;
       const float alpha = fast_exp2(m_run - m_use);
-      vec4 pb;
+      elem pb[4 * NS];
+      float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pb[j] = (elem)fast_exp2(s[j] - m_use);
-      l_run = l_run * alpha + (((float)pb[0] + (float)pb[1]) + ((float)pb[2] + (float)pb[3]));
+      for (int i = 0; i < 4 * NS; ++i) {
+        pb[i] = (elem)fast_exp2(s[i] - m_use);
+        sum += (float)pb[i];
+      }
+      l_run = fmaf(l_run, alpha, sum);
       m_run = m_new;
       if (__any(alpha != 1.0f)) {
 #pragma unroll
@@ -209,54 +307,85 @@ __global__ __launch_bounds__(kPagedThreads) void paged_decode(PagedArgs a) {
       }
       if (odd) {
         // Key by key: only keys that the row sees are added.
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i)
+          s_p[wave][16 * (i >> 2) + 4 * g4 + (i & 3)][n16] =
+              (sees >> i) & 1 ? (float)pb[i] : kHidden;
+        lds_order();
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
+        for (int kk = 0; kk < KT; ++kk) {
+          const float p = s_p[wave][kk][n16];
+          if (p == kHidden) continue;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = __shfl((float)pb[j], 16 * g + n16);
-            const bool sp = __shfl((int)sees[j], 16 * g + n16) != 0;
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float v = (float)vbuf[(4 * g + j) * VS + 16 * b + 4 * g4 + i];
-                o[b][i] += sp ? p * v : 0.0f;
-              }
-          }
+            for (int c = 0; c < 4; ++c)
+              o[b][c] += p * (float)vbuf[kk * VS + 16 * b + 4 * g4 + c];
         }
+        return;
+      }
+      auto read_v = [&](int u, int b) {
+        return __builtin_bit_cast(
+            u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s4*)(
+                        vbuf + (16 * u + 4 * g4 + (n16 >> 2)) * VS + 16 * b + 4 * (n16 & 3))));
+      };
+      if constexpr (NS == 1) {
+        const vec4 p = {pb[0], pb[1], pb[2], pb[3]};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          o[b] = E::mfma16k16(__builtin_bit_cast(vec4, read_v(0, b)), p, o[b]);
       } else {
+        const vec8 p = {pb[0], pb[1], pb[2], pb[3], pb[4], pb[5], pb[6], pb[7]};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const vec4 va = __builtin_bit_cast(
-              vec4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s4*)(
-                            vbuf + (4 * g4 + (n16 >> 2)) * VS + 16 * b + 4 * (n16 & 3))));
-          o[b] = E::mfma16k16(va, pb, o[b]);
+          const u2 v0 = read_v(0, b), v1 = read_v(1, b);
+          o[b] = E::mfma16(__builtin_bit_cast(vec8, u4{v0[0], v0[1], v1[0], v1[1]}), p, o[b]);
         }
       }
     };
 
+    // ---- this wave's tiles, two register sets of one tile each ------------
     if (nt > 0) {
-      u4 ka[NK], va[NV], kb[NK], vb[NV];
-      int pa = lookup(0), pb = lookup(1);
-      load_tile(ka, va, tile_of(0), pa);
-      for (int k = 0; k < nt; k += 2) {
-        int pn = lookup(k + 2);
-        if (k + 1 < nt) load_tile(kb, vb, tile_of(k + 1), pb);
-        compute_tile(ka, va, tile_of(k), pa);
-        if (k + 1 >= nt) break;
-        pa = pn;
-        pn = lookup(k + 3);
-        if (k + 2 < nt) load_tile(ka, va, tile_of(k + 2), pa);
-        compute_tile(kb, vb, tile_of(k + 1), pb);
-        pb = pn;
+      u4 ka[NS][NK], va[NS][NV], kb[NS][NK], vb[NS][NV];
+      int pa[NS], pb[NS], pc[NS];
+      unsigned ta, tb;
+      auto find = [&](int k, int (&pg)[NS]) {
+        if constexpr (!ALIGNED)
+#pragma unroll
+          for (int u = 0; u < NS; ++u) pg[u] = lookup(k, u);
+      };
+      find(0, pa);
+      find(1, pb);
+      load_tile(ka, va, 0, pa);
+      ta = present(0, pa);
+      int k = 0;
+      for (; k + 3 <= nt; k += 2) {
+        find(k + 2, pc);
+        load_tile(kb, vb, k + 1, pb);
+        tb = present(k + 1, pb);
+        compute_tile(ka, va, k, ta);
+        find(k + 3, pb);
+        load_tile(ka, va, k + 2, pc);
+        ta = present(k + 2, pc);
+        compute_tile(kb, vb, k + 1, tb);
+      }
+      if (k + 1 < nt) {
+        load_tile(kb, vb, k + 1, pb);
+        tb = present(k + 1, pb);
+        // all of tile k + 1 is requested before tile k is waited for
+        __builtin_amdgcn_sched_barrier(0);
+        compute_tile(ka, va, k, ta);
+        compute_tile(kb, vb, k + 1, tb);
+      } else {
+        compute_tile(ka, va, k, ta);
       }
     }
 
     // ---- the waves' rows meet in LDS ---------------------------------------
     float l_tot = l_run + __shfl_xor(l_run, 16);
     l_tot += __shfl_xor(l_tot, 32);
-    wave_lds_order();
+    lds_order();
     float* const so = reinterpret_cast<float*>(s_region[wave]);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -299,19 +428,30 @@ __global__ __launch_bounds__(kPagedThreads) void paged_decode(PagedArgs a) {
         if (d4 == 0) a.rec.ml[at] = make_float2(M, lw);
       }
     }
+    __syncthreads();  // the region is read: the next piece may write it
   }
 }
 
 template <class E, bool FP8>
-PagedFn pick_size(int D) {
-  return D == 64 ? paged_decode<E, FP8, 64> : paged_decode<E, FP8, 128>;
+PagedFn pick_size(int D, bool aligned) {
+  if (D == 64)
+    return aligned ? paged_decode<E, FP8, 64, true> : paged_decode<E, FP8, 64, false>;
+  return aligned ? paged_decode<E, FP8, 128, true> : paged_decode<E, FP8, 128, false>;
 }
 
 }  // namespace
 
-PagedFn paged_decode_fn(bool bf16, bool fp8, int D) {
-  if (bf16) return fp8 ? pick_size<ElemBF16, true>(D) : pick_size<ElemBF16, false>(D);
-  return fp8 ? pick_size<ElemF16, true>(D) : pick_size<ElemF16, false>(D);
+// Two tiles a wave: fewer cost more in starts and merges than they spread.
+int paged_decode_min_tiles(bool fp8, int D) {
+  (void)fp8;
+  (void)D;
+  return 2 * kWaves;
+}
+
+PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned) {
+  if (bf16)
+    return fp8 ? pick_size<ElemBF16, true>(D, aligned) : pick_size<ElemBF16, false>(D, aligned);
+  return fp8 ? pick_size<ElemF16, true>(D, aligned) : pick_size<ElemF16, false>(D, aligned);
 }
 
 }  // namespace dbk

@@ -539,6 +539,14 @@ def test_attention_of_many_requests():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,L", [(64, 5000), (128, 4300)])
+def test_attention_of_long_splits(D, L):
+    """So many heads that a wave walks more tiles than its lanes hold places for."""
+    requests = [(1, L - 13 * r) for r in range(20)]
+    check_attention(make_step(requests, 32, 32, D, 16, torch.float16, torch.float16), max_new=1)
+
+
+@pytest.mark.gpu
 def test_attention_offsets_past_32_bits():
     """Pages behind 2^31 elements (and 2^32 bytes) of a long cache."""
     Hkv, page, D = 8, 64, 128
