@@ -132,7 +132,6 @@ struct PagedArgs {
 };
 
 constexpr int kDecodeRows = 16;  // rows of the decode kernel's tile
-constexpr int kChunkRows = 128;  // rows of the chunk kernel's tile
 constexpr int kChunkKeys = 64;
 constexpr int kPagedThreads = 256;
 constexpr int kDescInts = 8;

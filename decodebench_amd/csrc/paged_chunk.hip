@@ -1,10 +1,9 @@
-// paged_chunk.hip -- paged attention of many rows (chunks of a prompt), the
-// merge of split rows, and the launches of a call.
+// paged_chunk.hip -- paged attention of many rows: chunks of a prompt, drafts.
 //
-// A workgroup of four waves owns one (request, KV head, row tile of 128 rows)
-// and one split of the keys; wave w has rows 32 w .. 32 w + 31 and all four
-// share 64-key tiles of K and V in LDS.  Bound by the MFMAs and, beside them,
-// the softmax on the VALU.
+// A workgroup of NW waves owns one (request, KV head, row tile of 32 NW rows)
+// and one split of the keys; wave w has rows 32 w .. 32 w + 31 and all share
+// 64-key tiles of K and V in LDS.  Bound by the MFMAs and, beside them, the
+// softmax on the VALU.
 //
 //  * S^T = K Q^T on v_mfma_f32_32x32x16: a lane holds scores of one row (its
 //    column), 32 of the tile's 64 keys, the other half in lane ^ 32, so a
@@ -13,8 +12,17 @@
 //    accumulator registers 8 s .. 8 s + 7 of lane half h are keys 16 s + 4 h +
 //    0..3 and 16 s + 8 + 4 h + 0..3, and V^T is read from LDS in that order by
 //    two transposing reads (ds_read_b64_tr_b16) per operand.
-//  * The next tile's loads are in flight in registers while this one is
-//    computed.  Lane i of every wave looks up the page of key i of a tile.
+//  * Exponents are taken against a reference that moves only when a row's
+//    maximum leaves it by more than 2^12, to 2^8 below that maximum: the output
+//    is rescaled a few times a row instead of at most tiles, and small
+//    probabilities stay clear of fp16's subnormals.
+//  * Two tiles in LDS: while tile t is computed, tile t + 1 goes from registers
+//    to the other half and tile t + 2 is on its way to registers; one barrier a
+//    tile.
+//  * Pages of a multiple of 16 tokens (ALIGNED): lane 4 t + g holds where the
+//    g-th 16 keys of the t-th of 16 tiles are, and the table entries of the
+//    next 16 tiles, so an address is two scalars read from a lane.  Any other
+//    page size: lane i looks up the page of key i of a tile, one tile ahead.
 //  * A wave skips tiles that none of its rows sees, and masks only tiles that
 //    some row sees in part (as paged_decode, an Inf or NaN among such a tile's
 //    values is added key by key).
@@ -24,23 +32,40 @@ namespace dbk {
 
 namespace {
 
-constexpr int kWaves = kPagedThreads / kWave;
-constexpr int MT = kChunkRows, KT = kChunkKeys;
-constexpr int kRowsPerWave = MT / kWaves;
+constexpr int KT = kChunkKeys;
+constexpr int kHold = kWave / (KT / 16);  // tiles whose places the lanes hold
 
-template <class E, bool FP8, int D>
-__global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
+// Exponent references: a row's maximum may be kAbove over its reference, which
+// is set kBelow under the maximum.
+constexpr float kAbove = 12.0f, kBelow = 8.0f;
+
+__device__ __forceinline__ long long lane_i64(long long v, int lane) {
+  const int lo = __builtin_amdgcn_readlane((int)v, lane);
+  const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+
+// The lowest n of 64 bits (none below 0, all from 64 on).
+__device__ __forceinline__ unsigned long long below(int n) {
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
+template <class E, bool FP8, int D, bool ALIGNED, int NW>
+__global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(PagedArgs a) {
   typedef typename E::type elem;
   typedef typename E::vec8 vec8;
+  constexpr int MT = 32 * NW;
   constexpr int CB = FP8 ? 1 : 2;
-  constexpr int LPR = D * CB / 16;                 // threads per row of a tile
-  constexpr int RPI = kPagedThreads / LPR;         // rows a load instruction of the workgroup
-  constexpr int NL = KT / RPI;                     // loads of K (and of V) a thread
+  constexpr int RW = KT / NW;                      // rows of a tile that a wave loads
+  constexpr int LPR = D * CB / 16;                 // lanes per row
+  constexpr int RPI = kWave / LPR;                 // rows a load instruction
+  constexpr int NL = RW > RPI ? RW / RPI : 1;      // loads of K (and of V) a lane
   constexpr int KS = D + 8, VS = D + 16;           // row strides in LDS (elements)
   constexpr int QSTEPS = D / 16, NB = D / 32;
 
-  __shared__ __align__(16) elem s_k[KT * KS];
-  __shared__ __align__(16) elem s_v[KT * VS];
+  __shared__ __align__(16) elem s_k[2][KT * KS];
+  __shared__ __align__(16) elem s_v[2][KT * VS];
+  __shared__ int s_odd[2];  // tile + 1 of a tile with an Inf or NaN left out
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -48,38 +73,62 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
 
   PagedSchedule<MT, KT> schedule(a);
   PagedWork wk;
-  while (schedule.next(wk)) {
+  if (!schedule.next(wk)) return;
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  __syncthreads();
+  {
     const PagedRequest& rq = wk.req;
     int t_begin, t_end;
     paged_range<MT, KT>(a, wk, t_begin, t_end);
-    t_begin = __builtin_amdgcn_readfirstlane(t_begin);
-    t_end = __builtin_amdgcn_readfirstlane(t_end);
     paged_describe(a, wk, MT);
-    const int limit = __builtin_amdgcn_readfirstlane(paged_limit(a, rq.len));
+    const int limit = paged_limit(a, rq.len);
+
+    const char* const kbase = static_cast<const char*>(a.k) + wk.head * a.kh * CB;
+    const char* const vbase = static_cast<const char*>(a.v) + wk.head * a.vh * CB;
+    const int* const trow = a.table + wk.r * a.table_row;
+
+    // ---- where the keys are ------------------------------------------------
+    // ALIGNED: byte offsets of this lane's 16 keys and values (of the tiles
+    // held .. held + 15) and a bit for each that has a page; `ahead` is the
+    // table entry for the 16 tiles after these.
+    long long koff = 0, voff = 0;
+    unsigned long long has = 0;
+    int held = t_begin, ahead = -1;
+    auto entry = [&](int tile) {  // of this lane's 16 keys, 16 tiles from `tile` on
+      const int key = (tile + lane / 4) * KT + 16 * (lane % 4);
+      return tile + lane / 4 < t_end && key < limit ? trow[page_of(a, key)] : -1;
+    };
+    auto hold = [&](int tile) {
+      held = tile;
+      const int p = ahead;
+      ahead = entry(tile + kHold);
+      const int key = (tile + lane / 4) * KT + 16 * (lane % 4);
+      const bool ok = (unsigned)p < (unsigned)a.pages;
+      const int off = ok ? key - page_of(a, key) * a.page : 0;
+      koff = ok ? (p * a.kp + off * a.kt) * CB : 0;
+      voff = ok ? (p * a.vp + off * a.vt) * CB : 0;
+      has = __ballot(ok);
+    };
+    // Otherwise: page of key `lane` of a tile, -1 where there is none.
+    auto lookup = [&](int tile) {
+      const int key = tile * KT + lane;
+      if (tile >= t_end || key >= limit) return -1;
+      const int p = trow[page_of(a, key)];
+      return (unsigned)p < (unsigned)a.pages ? p : -1;
+    };
+    int pg = -1;
+    if constexpr (ALIGNED)
+      ahead = entry(t_begin);
+    else
+      pg = lookup(t_begin);
 
     // This lane's row and the keys it sees; rows past the last one see none.
     const long long left = (long long)rq.n * a.G - (long long)wk.tile * MT;
     const int rows = (int)min(left, (long long)MT);
-    const int lrow = wave * kRowsPerWave + n32;
+    const int lrow = wave * 32 + n32;
     const bool live = lrow < rows;
     const int x = wk.tile * MT + min(lrow, rows - 1);
     const int token = x / a.G, qhead = wk.head * a.G + x % a.G;
-    const int pos = rq.len - rq.n + token;
-    const int khi = !live ? 0 : a.causal ? min(limit, pos + 1) : limit;
-    const int klo = !live ? 0x7FFFFFFF : a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-    // Keys that every live row sees, and keys that any of them sees.
-    int all_lo = live ? klo : 0, all_hi = live ? khi : 0x7FFFFFFF, any_lo = klo, any_hi = khi;
-    for (int d = 1; d < 32; d <<= 1) {
-      all_lo = max(all_lo, __shfl_xor(all_lo, d));
-      all_hi = min(all_hi, __shfl_xor(all_hi, d));
-      any_lo = min(any_lo, __shfl_xor(any_lo, d));
-      any_hi = max(any_hi, __shfl_xor(any_hi, d));
-    }
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
-    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-
     vec8 qop[QSTEPS];
     {
       const elem* qp = static_cast<const elem*>(a.q) + (rq.tok0 + token) * a.q_token +
@@ -87,48 +136,108 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
 #pragma unroll
       for (int t = 0; t < QSTEPS; ++t) qop[t] = __builtin_bit_cast(vec8, ld16(qp + 16 * t));
     }
+    const int past = rq.len - rq.n;
+    const int khi = !live ? 0 : a.causal ? min(limit, past + token + 1) : limit;
+    const int klo = !live ? 0x7FFFFFFF : a.window > 0 ? max(past + token - a.window + 1, 0) : 0;
+    // Keys that every row of the workgroup sees (wg_), that every live row of
+    // the wave sees (all_) and that any of them sees (any_), from its first and
+    // last live row (none: nothing at all).
+    const int wg_hi = a.causal ? min(limit, past + (wk.tile * MT) / a.G + 1) : limit;
+    const int wg_lo =
+        a.window > 0 ? max(past + (wk.tile * MT + rows - 1) / a.G - a.window + 1, 0) : 0;
+    const bool any = wave * 32 < rows;
+    const int i0 = (wk.tile * MT + min(wave * 32, rows - 1)) / a.G;
+    const int i1 = (wk.tile * MT + min(wave * 32 + 31, rows - 1)) / a.G;
+    const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
+    const int any_hi = !any ? 0 : a.causal ? min(limit, past + i1 + 1) : limit;
+    const int all_lo = a.window > 0 ? max(past + i1 - a.window + 1, 0) : 0;
+    const int any_lo = a.window > 0 ? max(past + i0 - a.window + 1, 0) : 0;
     const float scale = a.scale_log2 * (FP8 ? a.k_scale[wk.head] : 1.0f);
-    const char* const kbase = static_cast<const char*>(a.k) + wk.head * a.kh * CB;
-    const char* const vbase = static_cast<const char*>(a.v) + wk.head * a.vh * CB;
-    const int* const trow = a.table + wk.r * a.table_row;
 
-    // Page of key `lane` of a tile, -1 where there is none.
-    auto lookup = [&](int tile) {
-      const int key = tile * KT + lane;
-      if (tile >= t_end || key >= limit) return -1;
-      const int p = trow[page_of(a, key)];
-      return (unsigned)p < (unsigned)a.pages ? p : -1;
-    };
-    // Absent keys read row 0 of page 0: valid memory, zero in LDS.
-    auto load_tile = [&](u4 (&kt)[NL], u4 (&vt)[NL], int tile, int pg) {
+    // ---- tiles to registers and to LDS -------------------------------------
+    const int row0 = wave * RW;  // of the tile, this wave's first
+    const int lrow_l = min(lane / LPR, RW - 1), lcol = (lane % LPR) * 16;
+    const unsigned lane_k = (unsigned)((row0 % 16 + lrow_l) * (int)a.kt * CB + lcol);
+    const unsigned lane_v = (unsigned)((row0 % 16 + lrow_l) * (int)a.vt * CB + lcol);
+    // Absent keys read rows of page 0: valid memory, zero in LDS.
+    auto load_tile = [&](u4 (&kt)[NL], u4 (&vt)[NL], int tile) {
+      if constexpr (ALIGNED) {
+        if (tile >= held + kHold) hold(tile);
 #pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const int row = j * RPI + threadIdx.x / LPR, key = tile * KT + row;
-        const int pr = __shfl(pg, row), page = max(pr, 0);
-        const int off = pr < 0 ? 0 : key - page_of(a, key) * a.page;
-        const int c = (threadIdx.x % LPR) * 16;
-        kt[j] = ld16(kbase + (page * a.kp + off * a.kt) * CB + c);
-        vt[j] = ld16(vbase + (page * a.vp + off * a.vt) * CB + c);
+        for (int j = 0; j < NL; ++j) {
+          const int g = (row0 + j * RPI) / 16;  // row0 % 16 + j RPI runs on from its group
+          const int in = (row0 % 16 + j * RPI) / 16 * 16;
+          const long long ko = lane_i64(koff, (tile - held) * 4 + g);
+          const long long vo = lane_i64(voff, (tile - held) * 4 + g);
+          kt[j] = ld16(kbase + ko + (j * RPI - in) * a.kt * CB + lane_k);
+          vt[j] = ld16(vbase + vo + (j * RPI - in) * a.vt * CB + lane_v);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          const int row = row0 + j * RPI + lrow_l, key = tile * KT + row;
+          const int pr = __shfl(pg, row), page = max(pr, 0);
+          const int off = pr < 0 ? 0 : key - page_of(a, key) * a.page;
+          kt[j] = ld16(kbase + (page * a.kp + off * a.kt) * CB + lcol);
+          vt[j] = ld16(vbase + (page * a.vp + off * a.vt) * CB + lcol);
+        }
       }
     };
-    auto store_row = [&](elem* to, u4 w) {
+    // Keys of a tile that are in the cache and below the request's end.
+    auto present = [&](int tile) -> unsigned long long {
+      if constexpr (ALIGNED) {
+        const unsigned b = (unsigned)(has >> ((tile - held) * 4)) & 15u;
+        unsigned long long there = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) there |= (b >> g) & 1 ? 0xFFFFull << (16 * g) : 0ull;
+        return there & below(limit - tile * KT);
+      } else {
+        return __ballot(pg >= 0);
+      }
+    };
+    // Widens a chunk of e4m3; otherwise the chunk itself.
+    auto widen = [&](u4 w, u4 (&to)[2 / CB]) {
       if constexpr (FP8) {
         const u2 w0 = E::widen(w[0]), w1 = E::widen(w[1]);
         const u2 w2 = E::widen(w[2]), w3 = E::widen(w[3]);
-        *reinterpret_cast<u4*>(to) = u4{w0[0], w0[1], w1[0], w1[1]};
-        *reinterpret_cast<u4*>(to + 8) = u4{w2[0], w2[1], w3[0], w3[1]};
+        to[0] = u4{w0[0], w0[1], w1[0], w1[1]};
+        to[1] = u4{w2[0], w2[1], w3[0], w3[1]};
       } else {
-        *reinterpret_cast<u4*>(to) = w;
+        to[0] = w;
       }
     };
-    auto store_tile = [&](const u4 (&kt)[NL], const u4 (&vt)[NL], unsigned long long there) {
+    // A tile to LDS: zeros for keys that are not there, and, in a tile that
+    // some row of the workgroup sees in part, for values that are Inf or NaN:
+    // a hidden key's probability is zero, but zero times those is not.
+    auto store_tile = [&](u4 (&kt)[NL], u4 (&vt)[NL], int tile, unsigned long long there, int buf) {
+      const bool partial = there != ~0ull || tile * KT < wg_lo || tile * KT + KT > wg_hi;
+      bool odd = false;
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
-        const int row = j * RPI + threadIdx.x / LPR, c = (threadIdx.x % LPR) * (16 / CB);
-        const bool ok = (there >> row) & 1;
-        store_row(s_k + row * KS + c, ok ? kt[j] : u4{0, 0, 0, 0});
-        store_row(s_v + row * VS + c, ok ? vt[j] : u4{0, 0, 0, 0});
+        const int row = row0 + j * RPI + lrow_l, c = (lane % LPR) * (16 / CB);
+        u4 kw[2 / CB], vw[2 / CB];
+        widen(kt[j], kw);
+        widen(vt[j], vw);
+        if (partial) {
+          const bool ok = (there >> row) & 1;
+#pragma unroll
+          for (int h = 0; h < 2 / CB; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const unsigned v = vw[h][i];
+              const bool lo = (v & E::kExp) == E::kExp, hi = ((v >> 16) & E::kExp) == E::kExp;
+              odd = odd || (ok && (lo || hi));
+              vw[h][i] = ok ? v & ((lo ? 0u : 0x0000FFFFu) | (hi ? 0u : 0xFFFF0000u)) : 0u;
+              kw[h][i] = ok ? kw[h][i] : 0u;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2 / CB; ++h) {
+          *reinterpret_cast<u4*>(s_k[buf] + row * KS + c + 8 * h) = kw[h];
+          *reinterpret_cast<u4*>(s_v[buf] + row * VS + c + 8 * h) = vw[h];
+        }
       }
+      if (odd) s_odd[buf] = tile + 1;
     };
 
     f16v o[NB];
@@ -136,11 +245,49 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-    float m_run = kPagedNegInf, l_run = 0.0f;  // l: of this lane's keys
+    float m_ref = kPagedNegInf, l_run = 0.0f;  // l: of this lane's keys
 
-    auto compute_tile = [&](int tile, unsigned long long there) {
+    // V^T of 16 keys (step t) and 32 dims (block b): the A operand.
+    auto read_v = [&](const elem* vb0, int t, int b) {
+      const elem* at = vb0 + 16 * t * VS + 32 * b;
+      const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                               (__attribute__((address_space(3))) s4*)(at)));
+      const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                               (__attribute__((address_space(3))) s4*)(at + 8 * VS)));
+      return u4{lo[0], lo[1], hi[0], hi[1]};
+    };
+
+    // Adds the Infs and NaNs that store_tile left out to the rows that see them
+    // (values read again from the cache; a rare path, kept small).
+    auto add_odd = [&](int key0, unsigned long long sees) {
+#pragma unroll 1
+      for (int kk = 0; kk < KT; ++kk) {
+        if (!__any((sees >> kk) & 1)) continue;  // also keys without a page
+        const int key = key0 + kk, at = page_of(a, key);
+        const char* row = vbase + (trow[at] * a.vp + (key - at * a.page) * a.vt) * CB;
+        const bool ok = (sees >> kk) & 1;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const char* four = row + (32 * b + 8 * c + 4 * half) * CB;
+            const u2 w = FP8 ? E::widen(*reinterpret_cast<const unsigned*>(four))
+                             : *reinterpret_cast<const u2*>(four);
+            const typename E::vec4 v = __builtin_bit_cast(typename E::vec4, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[b][4 * c + i] += ok && !__builtin_isfinite((float)v[i]) ? (float)v[i] : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+    };
+
+    auto compute_tile = [&](int tile, unsigned long long there, int buf) {
       const int key0 = tile * KT;
       if (key0 >= any_hi || key0 + KT <= any_lo) return;
+      const elem* const kb0 = s_k[buf] + n32 * KS + 8 * half;
+      const elem* const vb0 = s_v[buf] + (4 * half + ((lane & 15) >> 2)) * VS +
+                              16 * ((lane >> 4) & 1) + 4 * (lane & 3);
       f16v s[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
@@ -148,120 +295,89 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
         for (int t = 0; t < QSTEPS; ++t)
-          s[kb] = E::mfma32(__builtin_bit_cast(
-                                vec8, ld16(s_k + (32 * kb + n32) * KS + 16 * t + 8 * half)),
-                            qop[t], s[kb]);
+          s[kb] = E::mfma32(__builtin_bit_cast(vec8, ld16(kb0 + 32 * kb * KS + 16 * t)), qop[t],
+                            s[kb]);
       }
       const bool partial = there != ~0ull || key0 < all_lo || key0 + KT > all_hi;
-      unsigned sees[2] = {0xFFFFu, 0xFFFFu};  // bit i: register i of block kb counts
+      // Keys of the tile that this lane's row sees, a bit each.  (Bits tested at
+      // fixed places of words shifted by the lane's half: places that depend on
+      // the lane were hoisted out of the loop, 96 registers of them.)
+      unsigned long long sees = ~0ull;
       if (partial) {
+        sees = there & below(khi - key0) & ~below(klo - key0);
+        const unsigned w0 = (unsigned)sees >> (4 * half), w1 = (unsigned)(sees >> 32) >> (4 * half);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          sees[kb] = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int kk = 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
-            const bool ok = key0 + kk >= klo && key0 + kk < khi && ((there >> kk) & 1);
-            sees[kb] |= ok ? 1u << i : 0u;
-            s[kb][i] = ok ? s[kb][i] : kPagedNegInf;
-          }
+        for (int i = 0; i < 16; ++i) {
+          const unsigned bit = 1u << (8 * (i >> 2) + (i & 3));
+          s[0][i] = w0 & bit ? s[0][i] : kPagedNegInf;
+          s[1][i] = w1 & bit ? s[1][i] : kPagedNegInf;
         }
       }
-      float tmax = kPagedNegInf;
+      float tmax = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[kb][i]);
       tmax = max_xor32(tmax) * scale;
-      const float m_new = fmaxf(m_run, tmax);
-      const float m_use = m_new == kPagedNegInf ? 0.0f : m_new;
-      const float alpha = fast_exp2(m_run - m_use);
+      if (__any(tmax > m_ref + kAbove)) {
+        const float m_new = fmaxf(m_ref, tmax - kBelow);
+        const float alpha = m_ref == kPagedNegInf ? 0.0f : fast_exp2(m_ref - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] *= alpha;
+        m_ref = m_new;
+      }
+      // A row that has seen nothing yet keeps -inf; its exponents use 0.
+      const float m_use = m_ref == kPagedNegInf ? 0.0f : m_ref;
       vec8 p[4];
-      float sum = 0.0f;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const elem e = (elem)fast_exp2(fmaf(s[kb][i], scale, -m_use));
-          p[2 * kb + (i >> 3)][i & 7] = e;
-          sum += (float)e;
+          const float e = fast_exp2(fmaf(s[kb][i], scale, -m_use));
+          sum[i & 3] += e;
+          p[2 * kb + (i >> 3)][i & 7] = (elem)e;
         }
-      l_run = fmaf(l_run, alpha, sum);
-      m_run = m_new;
-      if (__any(alpha != 1.0f)) {
+      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) o[b] *= alpha;
-      }
-      if (partial) {
-        bool bad = false;
-        for (int i = lane; i < KT * D / 8; i += kWave) {
-          const u4 w = ld16(s_v + (i / (D / 8)) * VS + (i % (D / 8)) * 8);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) bad = bad || pair_nonfinite<E>(w[c]);
-        }
-        if (__any(bad)) {
-          // Key by key: only keys that the row sees are added.  Two keys of
-          // each half a step, the registers moving up by one pair a step.
-          u4 pr[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) pr[t] = __builtin_bit_cast(u4, p[t]);
-          unsigned bits = sees[0] | (sees[1] << 16);
-#pragma unroll 1
-          for (int step = 0; step < 16; ++step) {
-            const vec8 now = __builtin_bit_cast(vec8, pr[0]);
-            const int i0 = 2 * step;  // accumulator register of 32
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float pv = __shfl((float)now[e], n32 + 32 * h);
-                const bool sp = (__shfl((int)bits, n32 + 32 * h) >> e) & 1;
-                const int i = i0 + e;
-                const elem* row = s_v + (32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3)) * VS;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                  for (int c = 0; c < 16; ++c) {
-                    const float v = (float)row[32 * b + 8 * (c >> 2) + 4 * half + (c & 3)];
-                    o[b][c] += sp ? pv * v : 0.0f;
-                  }
-              }
-            }
-            bits >>= 2;
-            const u4 keep[4] = {pr[0], pr[1], pr[2], pr[3]};
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              pr[t] = u4{keep[t][1], keep[t][2], keep[t][3], t < 3 ? keep[t < 3 ? t + 1 : 3][0] : 0u};
-          }
-          return;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const elem* at = s_v + (16 * t + 4 * half + ((lane & 15) >> 2)) * VS + 32 * b +
-                           16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                             (__attribute__((address_space(3))) s4*)(at)));
-          u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                             (__attribute__((address_space(3))) s4*)(at + 8 * VS)));
-          o[b] = E::mfma32(__builtin_bit_cast(vec8, u4{lo[0], lo[1], hi[0], hi[1]}), p[t], o[b]);
-        }
-      }
+        for (int b = 0; b < NB; ++b)
+          o[b] = E::mfma32(__builtin_bit_cast(vec8, read_v(vb0, t, b)), p[t], o[b]);
+      if ((there != ~0ull || key0 < wg_lo || key0 + KT > wg_hi) && s_odd[buf] == tile + 1)
+        add_odd(key0, sees);
     };
 
-    u4 kt[NL], vt[NL];
-    int pg = lookup(t_begin);
-    if (t_begin < t_end) load_tile(kt, vt, t_begin, pg);
-    for (int tile = t_begin; tile < t_end; ++tile) {
-      const unsigned long long there = __ballot(pg >= 0);
-      pg = lookup(tile + 1);
-      __syncthreads();  // the previous tile is read
-      store_tile(kt, vt, there);
+    // Between barriers: tile t is read, tile t + 1 written, tile t + 2 loaded.
+    if (t_begin < t_end) {
+      u4 kt[NL], vt[NL];
+      if constexpr (ALIGNED) hold(t_begin);
+      load_tile(kt, vt, t_begin);
+      unsigned long long there = present(t_begin), next = 0;
+      store_tile(kt, vt, t_begin, there, 0);
+      if (t_begin + 1 < t_end) {
+        if constexpr (!ALIGNED) pg = lookup(t_begin + 1);
+        load_tile(kt, vt, t_begin + 1);
+        next = present(t_begin + 1);
+        if constexpr (!ALIGNED) pg = lookup(t_begin + 2);
+      }
       __syncthreads();
-      if (tile + 1 < t_end) load_tile(kt, vt, tile + 1, pg);
-      compute_tile(tile, there);
+      for (int tile = t_begin; tile < t_end; ++tile) {
+        const int buf = (tile - t_begin) & 1;
+        const unsigned long long now = there;
+        if (tile + 1 < t_end) {
+          there = next;
+          store_tile(kt, vt, tile + 1, there, buf ^ 1);
+          if (tile + 2 < t_end) {
+            load_tile(kt, vt, tile + 2);
+            next = present(tile + 2);
+            if constexpr (!ALIGNED) pg = lookup(tile + 3);
+          }
+        }
+        compute_tile(tile, now, buf);
+        __syncthreads();
+      }
     }
 
     // ---- outputs -----------------------------------------------------------
@@ -278,7 +394,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
           for (int c = 0; c < 4; ++c) {
             typename E::vec4 r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = (elem)(l == 0.0f ? 0.0f : o[b][4 * c + i] * inv);
+            for (int i = 0; i < 4; ++i) r[i] = (elem)(o[b][4 * c + i] * inv);
             *reinterpret_cast<typename E::vec4*>(op + 32 * b + 8 * c + 4 * half) = r;
           }
       } else if (rec < a.rec.records) {
@@ -290,10 +406,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<f4*>(op + 32 * b + 8 * c + 4 * half) =
                 f4{o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]} * vscale;
-        if (half == 0) a.rec.ml[at] = make_float2(m_run, l);
+        if (half == 0) a.rec.ml[at] = make_float2(m_ref, l);
       }
     }
-    __syncthreads();  // the tiles are read: the next piece may write them
   }
 }
 
@@ -304,6 +419,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_chunk(PagedArgs a) {
 // come from the first kernel.
 template <class E, int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge(PagedArgs a, int mt) {
+  constexpr int kWaves = kPagedThreads / kWave;
   typedef typename E::type elem;
   constexpr int PER = D / kWave;  // elements a lane
   constexpr int kAtOnce = 8;
@@ -377,14 +493,24 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge(PagedArgs a, int mt
   }
 }
 
-template <class E, bool FP8>
-PagedFn pick_size(int D) {
-  return D == 64 ? paged_chunk<E, FP8, 64> : paged_chunk<E, FP8, 128>;
+template <class E, bool FP8, int D, int NW>
+PagedFn pick_pages(bool aligned) {
+  return aligned ? paged_chunk<E, FP8, D, true, NW> : paged_chunk<E, FP8, D, false, NW>;
 }
-
-PagedFn pick_chunk(bool bf16, bool fp8, int D) {
-  if (bf16) return fp8 ? pick_size<ElemBF16, true>(D) : pick_size<ElemBF16, false>(D);
-  return fp8 ? pick_size<ElemF16, true>(D) : pick_size<ElemF16, false>(D);
+template <class E, bool FP8, int NW>
+PagedFn pick_size(int D, bool aligned) {
+  return D == 64 ? pick_pages<E, FP8, 64, NW>(aligned) : pick_pages<E, FP8, 128, NW>(aligned);
+}
+template <int NW>
+PagedFn pick_type(bool bf16, bool fp8, int D, bool aligned) {
+  if (bf16)
+    return fp8 ? pick_size<ElemBF16, true, NW>(D, aligned)
+               : pick_size<ElemBF16, false, NW>(D, aligned);
+  return fp8 ? pick_size<ElemF16, true, NW>(D, aligned)
+             : pick_size<ElemF16, false, NW>(D, aligned);
+}
+PagedFn pick_chunk(int waves, bool bf16, bool fp8, int D, bool aligned) {
+  return waves == 2 ? pick_type<2>(bf16, fp8, D, aligned) : pick_type<8>(bf16, fp8, D, aligned);
 }
 
 void (*pick_merge(bool bf16, int D))(PagedArgs, int) {
@@ -394,8 +520,23 @@ void (*pick_merge(bool bf16, int D))(PagedArgs, int) {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Workgroups wanted of each kernel: two a CU.
-int paged_target(int cu_count) { return 2 * cu_count; }
+// How a call of these bounds runs: the waves of the chunk kernel (0: none), and
+// the workgroups wanted of each kernel.
+struct PagedPlanned {
+  bool decode;
+  int chunk_waves, decode_target, chunk_target;
+};
+PagedPlanned planned(const PagedCall& c, int cu_count) {
+  const int most = c.max_new > 0 && c.max_new < c.T ? c.max_new : c.T;
+  const long long rows = (long long)most * (c.Hq / c.cache.Hkv);
+  PagedPlanned p;
+  p.chunk_waves = rows <= kDecodeRows ? 0 : rows <= 64 ? 2 : 8;
+  // one request: many rows, or few at most
+  p.decode = p.chunk_waves == 0 || c.R > 1;
+  p.decode_target = 2 * cu_count;
+  p.chunk_target = p.chunk_waves == 2 ? 2 * cu_count : cu_count;
+  return p;
+}
 
 size_t region_bytes(int target, int mt, int D) {
   const size_t records = 2 * (size_t)target, groups = (size_t)target;
@@ -403,7 +544,7 @@ size_t region_bytes(int target, int mt, int D) {
          round256(records * mt * sizeof(float2)) + round256(records * mt * D * sizeof(float));
 }
 
-PagedRecords region(char* base, int target, int mt, int D) {
+PagedRecords region(char* base, int target, int mt) {
   PagedRecords r;
   r.records = 2 * target;
   r.groups = target;
@@ -414,7 +555,6 @@ PagedRecords region(char* base, int target, int mt, int D) {
   r.ml = reinterpret_cast<float2*>(base);
   base += round256((size_t)r.records * mt * sizeof(float2));
   r.opart = reinterpret_cast<float*>(base);
-  (void)D;
   return r;
 }
 
@@ -425,28 +565,20 @@ bool paged_aligned(const db_paged_cache& kv) {
   return kv.page_size % 16 == 0 && kv.k_token_stride < kFar && kv.v_token_stride < kFar;
 }
 
-// Which kernels a call of these bounds needs.
-void kernels_of(const PagedCall& c, bool* decode, bool* chunk) {
-  const int most = c.max_new > 0 && c.max_new < c.T ? c.max_new : c.T;
-  *decode = true;
-  *chunk = (long long)most * (c.Hq / c.cache.Hkv) > kDecodeRows;
-  if (*chunk && c.R == 1) *decode = false;  // one request: many rows, or few at most
-}
-
 }  // namespace
 
 size_t paged_workspace_bytes(const PagedCall& c, int cu_count) {
-  bool decode, chunk;
-  kernels_of(c, &decode, &chunk);
-  const int target = paged_target(cu_count), D = c.cache.D;
-  return (decode ? region_bytes(target, kDecodeRows, D) : 0) +
-         (chunk ? region_bytes(target, kChunkRows, D) : 0);
+  const PagedPlanned p = planned(c, cu_count);
+  const int D = c.cache.D;
+  return (p.decode ? region_bytes(p.decode_target, kDecodeRows, D) : 0) +
+         (p.chunk_waves ? region_bytes(p.chunk_target, 32 * p.chunk_waves, D) : 0);
 }
 
 hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream) {
   const db_paged_cache& kv = c.cache;
   const bool fp8 = kv.dtype == DB_DTYPE_FP8_E4M3;
-  const int target = paged_target(cu_count), D = kv.D;
+  const int D = kv.D;
+  const PagedPlanned p = planned(c, cu_count);
   PagedArgs a;
   a.q = c.q;
   a.o = c.o;
@@ -482,32 +614,32 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
   a.causal = c.causal;
   a.window = c.window;
   a.scale_log2 = c.scale * 1.4426950408889634f;
-  a.target = target;
 
-  bool decode, chunk;
-  kernels_of(c, &decode, &chunk);
+  const bool aligned = paged_aligned(kv);
   char* base = static_cast<char*>(ws);
-  auto run = [&](PagedFn fn, int part, int mt, int min_tiles) {
+  auto run = [&](PagedFn fn, int part, int threads, int mt, int target, int min_tiles) {
     a.part = part;
+    a.target = target;
     a.min_tiles = min_tiles;
-    a.rec = region(base, target, mt, D);
+    a.rec = region(base, target, mt);
     base += region_bytes(target, mt, D);
     // Row tiles of every request at most, and the splits beyond one each.
     const long long tiles = (long long)c.T * a.G / mt + c.R;
     const long long grid = tiles * a.Hkv + target;
-    hipLaunchKernelGGL(fn, dim3((unsigned)(grid < 65536 ? grid : 65536)), dim3(kPagedThreads), 0,
+    hipLaunchKernelGGL(fn, dim3((unsigned)(grid < 65536 ? grid : 65536)), dim3(threads), 0,
                        stream, a);
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(2048), dim3(kPagedThreads), 0, stream, a, mt);
     return hipGetLastError();
   };
   hipError_t e = hipSuccess;
-  if (decode)
-    e = run(paged_decode_fn(c.bf16, fp8, D, paged_aligned(kv)), chunk ? 1 : 0, kDecodeRows,
-            paged_decode_min_tiles(fp8, D));
-  if (e == hipSuccess && chunk)
-    e = run(pick_chunk(c.bf16, fp8, D), decode ? 2 : 0, kChunkRows, 8);
+  if (p.decode)
+    e = run(paged_decode_fn(c.bf16, fp8, D, aligned), p.chunk_waves ? 1 : 0, kPagedThreads,
+            kDecodeRows, p.decode_target, paged_decode_min_tiles(fp8, D));
+  if (e == hipSuccess && p.chunk_waves)
+    e = run(pick_chunk(p.chunk_waves, c.bf16, fp8, D, aligned), p.decode ? 2 : 0,
+            p.chunk_waves * kWave, 32 * p.chunk_waves, p.chunk_target, 4);
   return e;
 }
 
