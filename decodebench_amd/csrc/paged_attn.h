@@ -25,8 +25,8 @@
 //
 // A split writes its running maximum, exp-sum and unnormalised output as an
 // fp32 record; paged_merge joins the records of a row.  There are fewer
-// than 2 `target` records: only requests of more than C tiles split, into
-// fewer than 2 tmax / C parts, and C >= (all tiles) / target.
+// than 2 `target` records: only requests of at least 1.5 C tiles split, into
+// at most 4/3 tmax / C parts, and C >= (all tiles) / target.
 #pragma once
 
 #include "db_device.h"
@@ -181,6 +181,12 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r)
   return q;
 }
 
+__device__ __forceinline__ long long lane_i64(long long v, int lane) {
+  const int lo = __builtin_amdgcn_readlane((int)v, lane);
+  const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+
 // Inclusive prefix sum over the 64 lanes (DPP row shifts and broadcasts).
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
@@ -211,10 +217,11 @@ __device__ __forceinline__ float max_xor16(float v) {
   return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
-// Walks the workgroup's numbers w = blockIdx.x, + gridDim.x, ... : next()
-// says whether there is another piece of work and leaves it in `work`, in
-// scalar registers.  Every wave does the search for itself, a lane to a
-// request and 64 requests a round: no LDS, no barrier.
+// Finds the piece of work of the workgroup's number: find() says whether there
+// is one and leaves it in `work`, in scalar registers.  Every wave does the
+// search for itself, a lane to a request and 64 requests a round: no LDS, no
+// barrier.  The host's grid holds every piece: a request has at most rows / MT
+// + 1 row tiles, and the splits beyond one each are at most all tiles / C.
 template <int MT, int KT>
 struct PagedSchedule {
   const PagedArgs& a;
@@ -246,7 +253,9 @@ struct PagedSchedule {
   }
 
   __device__ int splits_of(const PagedRequest& q) const {
-    return q.row_tiles == 0 ? 0 : max(1, (q.tiles + C - 1) / C);
+    // to the nearest: ceil would run 192 row tiles of 80 key tiles on 256 CUs
+    // (C = 60) as 384 halves, no sooner done and all of them to be merged
+    return q.row_tiles == 0 ? 0 : max(1, (int)((2ll * q.tiles + C) / (2ll * C)));
   }
   __device__ void scan() {
     splits = splits_of(mine);
@@ -256,7 +265,7 @@ struct PagedSchedule {
     total = __builtin_amdgcn_readlane(incl, kWave - 1);
   }
 
-  __device__ bool next(PagedWork& work) {
+  __device__ bool find(PagedWork& work) {
     const int unit = w / a.Hkv, lane = threadIdx.x & (kWave - 1);
     while (unit >= units0 + total) {
       units0 += total;
@@ -290,7 +299,6 @@ struct PagedSchedule {
       work.group =
           (groups0 + wave_total(mine_before ? mine.row_tiles : 0) + work.tile) * a.Hkv + work.head;
     }
-    w += gridDim.x;
     return true;
   }
 };
@@ -327,7 +335,7 @@ __device__ __forceinline__ void paged_describe(const PagedArgs& a, const PagedWo
 
 // e4m3 or 16-bit caches: the element type of the products E, of the cache C8.
 typedef void (*PagedFn)(PagedArgs);
-int paged_decode_min_tiles(bool fp8, int D);
+PagedFn paged_decode_merge_fn(bool bf16, int D);
 PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned);
 
 }  // namespace dbk

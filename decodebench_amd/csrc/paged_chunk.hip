@@ -39,12 +39,6 @@ constexpr int kHold = kWave / (KT / 16);  // tiles whose places the lanes hold
 // is set kBelow under the maximum.
 constexpr float kAbove = 12.0f, kBelow = 8.0f;
 
-__device__ __forceinline__ long long lane_i64(long long v, int lane) {
-  const int lo = __builtin_amdgcn_readlane((int)v, lane);
-  const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-  return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
-}
-
 // The lowest n of 64 bits (none below 0, all from 64 on).
 __device__ __forceinline__ unsigned long long below(int n) {
   return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
@@ -73,7 +67,7 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
 
   PagedSchedule<MT, KT> schedule(a);
   PagedWork wk;
-  if (!schedule.next(wk)) return;
+  if (!schedule.find(wk)) return;
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   __syncthreads();
   {
@@ -413,83 +407,98 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
 }
 
 // Joins the records of split rows: o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
-// A workgroup a row, its four waves a quarter of the splits each, eight records
-// in flight a wave (a wave alone, one record after the other, took 45 us for
-// the 64 splits of one request of 8192 tokens); the groups' count and places
-// come from the first kernel.
+// A workgroup of 16 waves has 16 rows of a row tile: a wave a row where there
+// are up to 8 splits, two or four waves a row where there are more, each with
+// its share of the splits and eight records in flight.  (A wave alone, one
+// record after another, took 45 us for the 64 splits of one request of 8192
+// tokens; four waves a row whatever the splits 47 us for 192 row tiles of 256
+// rows in two splits.)  The groups' count and places come from the first kernel.
+constexpr int kMergeWaves = 16;
+
 template <class E, int D>
-__global__ __launch_bounds__(kPagedThreads) void paged_merge(PagedArgs a, int mt) {
-  constexpr int kWaves = kPagedThreads / kWave;
+__global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, int mt) {
   typedef typename E::type elem;
   constexpr int PER = D / kWave;  // elements a lane
   constexpr int kAtOnce = 8;
-  __shared__ float s_acc[kWaves][D], s_m[kWaves], s_l[kWaves];
+  __shared__ float s_acc[kMergeWaves][D], s_m[kMergeWaves], s_l[kMergeWaves];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int total = min(a.rec.head[0], a.rec.groups) * mt;
+  const int parts = mt / kMergeWaves;
+  const int total = min(a.rec.head[0], a.rec.groups) * parts;
   for (int task = blockIdx.x; task < total; task += gridDim.x) {
-    const int group = task / mt, row = task % mt;
+    const int group = task / parts;
     const int* d = a.rec.desc + (size_t)group * kDescInts;
     const int splits = d[0], rec0 = d[1], head = rec0 % a.Hkv;
-    if (row >= d[4] || rec0 + (splits - 1) * a.Hkv >= a.rec.records) continue;
-    float M = kPagedNegInf, L = 0.0f, acc[PER];
+    if (rec0 + (splits - 1) * a.Hkv >= a.rec.records) continue;
+    const int first = task % parts * kMergeWaves, rows = min(d[4] - first, kMergeWaves);
+    const int share = splits <= 8 ? 1 : splits <= 16 ? 2 : 4;  // waves of a row
+    for (int r0 = 0; r0 < rows; r0 += kMergeWaves / share) {
+      const int sub = r0 + wave / share, row = first + min(sub, rows - 1);
+      float M = kPagedNegInf, L = 0.0f, acc[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-    for (int s0 = wave; s0 < splits; s0 += kWaves * kAtOnce) {
-      float2 ml[kAtOnce];
-      float v[kAtOnce][PER];
+      for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+      for (int s0 = wave % share; s0 < splits; s0 += share * kAtOnce) {
+        float2 ml[kAtOnce];
+        float v[kAtOnce][PER];
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const int s = min(s0 + j * kWaves, splits - 1);
-        const size_t at = (size_t)(rec0 + s * a.Hkv) * mt + row;
-        ml[j] = a.rec.ml[at];
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int s = min(s0 + j * share, splits - 1);
+          const size_t at = (size_t)(rec0 + s * a.Hkv) * mt + row;
+          ml[j] = a.rec.ml[at];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[j][i] = a.rec.opart[at * D + lane * PER + i];
+          for (int i = 0; i < PER; ++i) v[j][i] = a.rec.opart[at * D + lane * PER + i];
+        }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          if (s0 + j * share >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
+          if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);
+        }
+        const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
+        L *= keep;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] *= keep;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          if (ml[j].y == 0.0f) continue;  // saw nothing
+          const float w = fast_exp2(ml[j].x - Mn);
+          L = fmaf(w, ml[j].y, L);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, v[j][i], acc[i]);
+        }
+        M = Mn;
       }
-      float Mn = M;
+      if (share > 1) {  // the row's waves meet in the first one
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        if (s0 + j * kWaves >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
-        if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);
+        for (int i = 0; i < PER; ++i) s_acc[wave][lane * PER + i] = acc[i];
+        if (lane == 0) {
+          s_m[wave] = M;
+          s_l[wave] = L;
+        }
+        __syncthreads();
+        float Mt = kPagedNegInf, Lt = 0.0f;
+        for (int w = wave / share * share; w < wave / share * share + share; ++w)
+          if (s_l[w] != 0.0f) Mt = fmaxf(Mt, s_m[w]);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+        for (int w = wave / share * share; w < wave / share * share + share; ++w) {
+          if (s_l[w] == 0.0f) continue;
+          const float e = fast_exp2(s_m[w] - Mt);
+          Lt = fmaf(e, s_l[w], Lt);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[i] = fmaf(e, s_acc[w][lane * PER + i], acc[i]);
+        }
+        L = Lt;
+        __syncthreads();
       }
-      const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
-      L *= keep;
+      if (sub < rows && wave % share == 0) {
+        const int xr = d[3] + row;
+        elem* op = static_cast<elem*>(a.o) +
+                   ((size_t)(d[2] + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D + lane * PER;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] *= keep;
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        if (ml[j].y == 0.0f) continue;  // saw nothing
-        const float w = fast_exp2(ml[j].x - Mn);
-        L = fmaf(w, ml[j].y, L);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, v[j][i], acc[i]);
+        for (int i = 0; i < PER; ++i) op[i] = (elem)(L == 0.0f ? 0.0f : acc[i] / L);
       }
-      M = Mn;
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s_acc[wave][lane * PER + i] = acc[i];
-    if (lane == 0) {
-      s_m[wave] = M;
-      s_l[wave] = L;
-    }
-    __syncthreads();
-    if (threadIdx.x < D) {
-      float Mt = kPagedNegInf, Lt = 0.0f, o = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        if (s_l[w] != 0.0f) Mt = fmaxf(Mt, s_m[w]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        if (s_l[w] == 0.0f) continue;
-        const float e = fast_exp2(s_m[w] - Mt);
-        Lt = fmaf(e, s_l[w], Lt);
-        o = fmaf(e, s_acc[w][threadIdx.x], o);
-      }
-      const int xr = d[3] + row;
-      static_cast<elem*>(a.o)[((size_t)(d[2] + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D +
-                              threadIdx.x] = (elem)(Lt == 0.0f ? 0.0f : o / Lt);
-    }
-    __syncthreads();
   }
 }
 
@@ -525,37 +534,44 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 struct PagedPlanned {
   bool decode;
   int chunk_waves, decode_target, chunk_target;
+  int decode_items;  // row tiles of the decode kernel, of all KV heads, at most
 };
 PagedPlanned planned(const PagedCall& c, int cu_count) {
   const int most = c.max_new > 0 && c.max_new < c.T ? c.max_new : c.T;
   const long long rows = (long long)most * (c.Hq / c.cache.Hkv);
   PagedPlanned p;
   p.chunk_waves = rows <= kDecodeRows ? 0 : rows <= 64 ? 2 : 8;
-  // one request: many rows, or few at most
-  p.decode = p.chunk_waves == 0 || c.R > 1;
+  // Up to 64 rows a request, or one request: the chunk kernel takes them all.
+  p.decode = p.chunk_waves == 0 || (p.chunk_waves == 8 && c.R > 1);
   p.decode_target = 2 * cu_count;
   p.chunk_target = p.chunk_waves == 2 ? 2 * cu_count : cu_count;
+  const long long G = c.Hq / c.cache.Hkv;
+  p.decode_items = (int)(((long long)c.T * G / kDecodeRows + c.R) * c.cache.Hkv);
   return p;
 }
 
-size_t region_bytes(int target, int mt, int D) {
-  const size_t records = 2 * (size_t)target, groups = (size_t)target;
-  return 256 + round256(groups * kDescInts * sizeof(int)) +
-         round256(records * mt * sizeof(float2)) + round256(records * mt * D * sizeof(float));
-}
-
-PagedRecords region(char* base, int target, int mt) {
+// Room for records and descriptions of row tiles.
+PagedRecords region(char* base, int records, int groups, int mt, int D, size_t* bytes) {
   PagedRecords r;
-  r.records = 2 * target;
-  r.groups = target;
+  r.records = records;
+  r.groups = groups;
+  size_t at = 0;
   r.head = reinterpret_cast<int*>(base);
-  base += 256;
-  r.desc = reinterpret_cast<int*>(base);
-  base += round256((size_t)r.groups * kDescInts * sizeof(int));
-  r.ml = reinterpret_cast<float2*>(base);
-  base += round256((size_t)r.records * mt * sizeof(float2));
-  r.opart = reinterpret_cast<float*>(base);
+  at += 256;
+  r.desc = reinterpret_cast<int*>(base + at);
+  at += round256((size_t)groups * kDescInts * sizeof(int));
+  r.ml = reinterpret_cast<float2*>(base + at);
+  at += round256((size_t)records * mt * sizeof(float2));
+  r.opart = reinterpret_cast<float*>(base + at);
+  at += round256((size_t)records * mt * D * sizeof(float));
+  *bytes = at;
   return r;
+}
+PagedRecords decode_region(char* base, const PagedPlanned& p, int D, size_t* bytes) {
+  return region(base, 2 * p.decode_target, p.decode_items, kDecodeRows, D, bytes);
+}
+PagedRecords chunk_region(char* base, const PagedPlanned& p, int D, size_t* bytes) {
+  return region(base, 2 * p.chunk_target, p.chunk_target, 32 * p.chunk_waves, D, bytes);
 }
 
 // Whether 16 keys from a multiple of 16 on always lie in one page, at offsets
@@ -569,9 +585,10 @@ bool paged_aligned(const db_paged_cache& kv) {
 
 size_t paged_workspace_bytes(const PagedCall& c, int cu_count) {
   const PagedPlanned p = planned(c, cu_count);
-  const int D = c.cache.D;
-  return (p.decode ? region_bytes(p.decode_target, kDecodeRows, D) : 0) +
-         (p.chunk_waves ? region_bytes(p.chunk_target, 32 * p.chunk_waves, D) : 0);
+  size_t decode = 0, chunk = 0;
+  if (p.decode) decode_region(nullptr, p, c.cache.D, &decode);
+  if (p.chunk_waves) chunk_region(nullptr, p, c.cache.D, &chunk);
+  return decode + chunk;
 }
 
 hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream) {
@@ -617,30 +634,44 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
 
   const bool aligned = paged_aligned(kv);
   char* base = static_cast<char*>(ws);
-  auto run = [&](PagedFn fn, int part, int threads, int mt, int target, int min_tiles) {
-    a.part = part;
-    a.target = target;
-    a.min_tiles = min_tiles;
-    a.rec = region(base, target, mt);
-    base += region_bytes(target, mt, D);
-    // Row tiles of every request at most, and the splits beyond one each.
-    const long long tiles = (long long)c.T * a.G / mt + c.R;
-    const long long grid = tiles * a.Hkv + target;
-    hipLaunchKernelGGL(fn, dim3((unsigned)(grid < 65536 ? grid : 65536)), dim3(threads), 0,
-                       stream, a);
-    const hipError_t e = hipGetLastError();
+  size_t bytes = 0;
+  if (p.decode) {
+    a.part = p.chunk_waves ? 1 : 0;
+    a.target = p.decode_target;
+    a.min_tiles = 8;
+    a.rec = decode_region(base, p, D, &bytes);
+    base += bytes;
+    hipLaunchKernelGGL(paged_decode_fn(c.bf16, fp8, D, aligned), dim3(p.decode_target),
+                       dim3(kPagedThreads), 0, stream, a);
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(2048), dim3(kPagedThreads), 0, stream, a, mt);
-    return hipGetLastError();
-  };
-  hipError_t e = hipSuccess;
-  if (p.decode)
-    e = run(paged_decode_fn(c.bf16, fp8, D, aligned), p.chunk_waves ? 1 : 0, kPagedThreads,
-            kDecodeRows, p.decode_target, paged_decode_min_tiles(fp8, D));
-  if (e == hipSuccess && p.chunk_waves)
-    e = run(pick_chunk(p.chunk_waves, c.bf16, fp8, D, aligned), p.decode ? 2 : 0,
-            p.chunk_waves * kWave, 32 * p.chunk_waves, p.chunk_target, 4);
-  return e;
+    // An item a request and KV head and G rows each where the tokens are single;
+    // the merge walks what is beyond.
+    const long long items = (long long)c.R * a.Hkv;
+    const int merge_x = (int)(items < 4096 ? items : 4096), merge_y = a.G < 16 ? a.G : 16;
+    hipLaunchKernelGGL(paged_decode_merge_fn(c.bf16, D), dim3(merge_x, merge_y),
+                       dim3(kPagedThreads), 0, stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (p.chunk_waves) {
+    const int mt = 32 * p.chunk_waves;
+    a.part = p.decode ? 2 : 0;
+    a.target = p.chunk_target;
+    a.min_tiles = 4;
+    a.rec = chunk_region(base, p, D, &bytes);
+    // Row tiles of every request at most, and the splits beyond one each.
+    const long long grid = ((long long)c.T * a.G / mt + c.R) * a.Hkv + p.chunk_target;
+    hipLaunchKernelGGL(pick_chunk(p.chunk_waves, c.bf16, fp8, D, aligned), dim3((unsigned)grid),
+                       dim3(p.chunk_waves * kWave), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(2 * cu_count), dim3(kMergeWaves * kWave), 0,
+                       stream, a, mt);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace dbk

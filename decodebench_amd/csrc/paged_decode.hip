@@ -46,11 +46,110 @@ __device__ __forceinline__ void lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
-__device__ __forceinline__ long long lane_i64(long long v, int lane) {
-  const int lo = __builtin_amdgcn_readlane((int)v, lane);
-  const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-  return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+// ------------------------------------------------------------- schedule
+// All work of a call in one line: for each KV head, each request in order, each
+// row tile of it, its key tiles from the first that a row sees to the last.
+// The line is cut into `target` equal parts, a workgroup each, so that all of
+// them end together whatever the lengths are (splitting each request by itself
+// left 64 requests of 800 to 8000 tokens at 63% of the stream rate).  A part
+// holds the end of one item, whole items, and the beginning of another.
+struct DecodeRequest {
+  int tok0, n, len;
+  int t0, tiles;     // first key tile, and how many, of each row tile (none: one all the same)
+  int row_tiles;
+};
+
+template <int KT>
+__device__ __forceinline__ DecodeRequest decode_request(const PagedArgs& a, int r) {
+  DecodeRequest q = {0, 0, 0, 0, 0, 0};
+  if (r >= a.R) return q;
+  q.tok0 = clamp_int(a.q_start[r], 0, a.T);
+  q.n = max(clamp_int(a.q_start[r + 1], 0, a.T) - q.tok0, 0);
+  q.len = max(a.kv_len[r], 0);
+  const int rows = q.n * a.G;
+  if (a.part != 0 && rows > kDecodeRows) q.n = 0;
+  if (q.n == 0) return q;
+  q.row_tiles = (rows + MT - 1) / MT;
+  const int limit = paged_limit(a, q.len);
+  q.t0 = a.window > 0 ? min(max(q.len - q.n - a.window + 1, 0), limit) / KT : 0;
+  q.tiles = max((limit + KT - 1) / KT - q.t0, 1);
+  return q;
 }
+
+__device__ __forceinline__ long long wave_scan64(long long v) {
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int d = 1; d < kWave; d <<= 1) {
+    const long long u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// A position on the line, in scalar registers but for what each lane holds of
+// a request of the present 64 ones.  Every wave has its own: no LDS, no barrier.
+template <int KT>
+struct DecodeLine {
+  const PagedArgs& a;
+  DecodeRequest mine;
+  long long per_head;     // key tiles of one KV head
+  long long upto, all;    // of this round's requests up to this one, and in all
+  long long before;       // of the rounds before
+  int items_before, items_head;  // row tiles of the rounds before; of one KV head
+  int round;
+  long long at;           // within the KV head
+  int head;
+
+  __device__ explicit DecodeLine(const PagedArgs& args) : a(args) {
+    const int lane = threadIdx.x & (kWave - 1);
+    long long sum = 0;
+    int items = 0;
+    for (int r = (a.R - 1) / kWave * kWave; r >= 0; r -= kWave) {
+      mine = decode_request<KT>(a, r + lane);
+      sum += (long long)mine.row_tiles * mine.tiles;
+      items += mine.row_tiles;
+    }
+    if (a.R > kWave)
+      for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+    items_head = wave_total(items);
+    round = 0;
+    before = 0;
+    items_before = 0;
+    scan();
+    per_head = a.R > kWave ? lane_i64(sum, 0) : all;
+  }
+  __device__ void scan() {
+    upto = wave_scan64((long long)mine.row_tiles * mine.tiles);
+    all = lane_i64(upto, kWave - 1);
+  }
+  __device__ void to_round(int r) {
+    round = r;
+    mine = decode_request<KT>(a, r * kWave + (int)(threadIdx.x & (kWave - 1)));
+    scan();
+  }
+  // The item at `at`: its request (lane `who` of the round), row tile and the
+  // tile within it.  Positions only grow within a head.
+  __device__ void locate(int& who, int& row_tile, int& tile, int& item) {
+    if (at < before) {  // a new head
+      before = 0;
+      items_before = 0;
+      to_round(0);
+    }
+    while (at >= before + all) {
+      before += all;
+      items_before += wave_total(mine.row_tiles);
+      to_round(round + 1);
+    }
+    const long long in = at - before;
+    who = __builtin_ctzll(__ballot(in < upto));
+    const int tiles = __builtin_amdgcn_readlane(mine.tiles, who);
+    const int rts = __builtin_amdgcn_readlane(mine.row_tiles, who);
+    const long long off = in - (lane_i64(upto, who) - (long long)tiles * rts);
+    row_tile = rts == 1 ? 0 : (int)(off / tiles);
+    tile = (int)(off - (long long)row_tile * tiles);
+    const bool earlier = (int)(threadIdx.x & (kWave - 1)) < who;
+    item = head * items_head + items_before + wave_total(earlier ? mine.row_tiles : 0) + row_tile;
+  }
+};
 
 template <class E, bool FP8, int D, bool ALIGNED>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
@@ -80,18 +179,50 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
   const int n16 = lane & 15, g4 = lane >> 4;
   elem* const vbuf = reinterpret_cast<elem*>(s_region[wave]);
 
-  PagedSchedule<MT, KT> schedule(a);
-  PagedWork wk;
-  while (schedule.next(wk)) {
-    const PagedRequest& rq = wk.req;
-    int t_begin, t_end;
-    paged_range<MT, KT>(a, wk, t_begin, t_end);
-    paged_describe(a, wk, MT);
+  DecodeLine<KT> line(a);
+  // This workgroup's part [begin, end) of the line.
+  const long long total = line.per_head * a.Hkv;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.rec.head[0] = line.items_head * a.Hkv;
+  const long long per = max((total + a.target - 1) / a.target, (long long)a.min_tiles);
+  long long begin = per * blockIdx.x;
+  const long long end = min(begin + per, total);
+  if (begin >= end) return;
+  line.head = (int)(begin / line.per_head);
+  line.at = begin - line.per_head * line.head;
+  for (bool once = true; begin < end; once = false) {
+    if (!once) __syncthreads();  // the region is read: the next piece may write it
+    DecodeRequest rq;
+    int who, row_tile, tile_in, item;
+    line.locate(who, row_tile, tile_in, item);
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
+    rq.tok0 = of(line.mine.tok0);
+    rq.n = of(line.mine.n);
+    rq.len = of(line.mine.len);
+    rq.t0 = of(line.mine.t0);
+    rq.tiles = of(line.mine.tiles);
+    const int r = line.round * kWave + who, head = line.head;
+    const int take = (int)min(end - begin, (long long)(rq.tiles - tile_in));
     const int limit = paged_limit(a, rq.len);
+    const int t_begin = rq.t0 + tile_in, t_end = t_begin + take;
+    // Rows that other workgroups have keys of go to a record: of this
+    // workgroup's two the first if it goes on with an item, else the second.
+    const bool starts = tile_in == 0, whole = starts && take == rq.tiles;
+    const int rec = whole ? -1 : 2 * blockIdx.x + (starts ? 1 : 0);
+    const int rows = min(rq.n * a.G - row_tile * MT, MT);
+    if (starts && threadIdx.x == 0 && item < a.rec.groups) {
+      int* d = a.rec.desc + (size_t)item * kDescInts;
+      // the workgroup of the item's last tile
+      d[0] = whole ? 0 : (int)((begin + rq.tiles - 1) / per) - (int)blockIdx.x + 1;
+      d[1] = blockIdx.x;
+      d[2] = rq.tok0;
+      d[3] = row_tile * MT;
+      d[4] = rows;
+      d[5] = head;
+    }
 
-    const char* const kbase = static_cast<const char*>(a.k) + wk.head * a.kh * CB;
-    const char* const vbase = static_cast<const char*>(a.v) + wk.head * a.vh * CB;
-    const int* const trow = a.table + wk.r * a.table_row;
+    const char* const kbase = static_cast<const char*>(a.k) + head * a.kh * CB;
+    const char* const vbase = static_cast<const char*>(a.v) + head * a.vh * CB;
+    const int* const trow = a.table + r * a.table_row;
     const int first = t_begin + wave;
     const int nt = first < t_end ? (t_end - first + kWaves - 1) / kWaves : 0;
     auto tile_of = [&](int k) { return first + kWaves * k; };
@@ -126,9 +257,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
     };
 
     // This lane's row (column n16 of the products) and the keys it sees.
-    const int rows = (int)min((long long)rq.n * a.G - (long long)wk.tile * MT, (long long)MT);
-    const int x = wk.tile * MT + min(n16, rows - 1);
-    const int token = x / a.G, qhead = wk.head * a.G + x % a.G;
+    const int x = row_tile * MT + min(n16, rows - 1);
+    const int token = x / a.G, qhead = head * a.G + x % a.G;
     vec8 qop[STEPS];
     {
       const elem* qp = static_cast<const elem*>(a.q) + (rq.tok0 + token) * a.q_token +
@@ -144,10 +274,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
     const int khi = a.causal ? min(limit, past + token + 1) : limit;
     const int klo = a.window > 0 ? max(past + token - a.window + 1, 0) : 0;
     // Keys that every row sees: the first row's end, the last row's beginning.
-    const int i0 = wk.tile * MT / a.G, i1 = (wk.tile * MT + rows - 1) / a.G;
+    const int i0 = row_tile * MT / a.G, i1 = (row_tile * MT + rows - 1) / a.G;
     const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
     const int all_lo = a.window > 0 ? max(past + i1 - a.window + 1, 0) : 0;
-    const float scale = a.scale_log2 * (FP8 ? a.k_scale[wk.head] : 1.0f);
+    const float scale = a.scale_log2 * (FP8 ? a.k_scale[head] : 1.0f);
 
     f4 o[NB];
 #pragma unroll
@@ -395,8 +525,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
       s_l[lane][wave] = l_tot;
     }
     __syncthreads();
-    const float vscale = FP8 ? a.v_scale[wk.head] : 1.0f;
-    const int rec = wk.rec < 0 ? -1 : wk.rec + wk.split * a.Hkv;
+    const float vscale = FP8 ? a.v_scale[head] : 1.0f;
     for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kPagedThreads) {
       const int row = idx / (D / 4), d4 = idx % (D / 4);
       float M = kPagedNegInf;
@@ -414,9 +543,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
       }
       ow *= vscale;
       if (rec < 0) {
-        const int xr = wk.tile * MT + row;
+        const int xr = row_tile * MT + row;
         elem* op = static_cast<elem*>(a.o) +
-                   ((size_t)(rq.tok0 + xr / a.G) * a.Hq + wk.head * a.G + xr % a.G) * D + 4 * d4;
+                   ((size_t)(rq.tok0 + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D + 4 * d4;
         const float inv = lw == 0.0f ? 0.0f : 1.0f / lw;
         vec4 r;
 #pragma unroll
@@ -428,7 +557,86 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
         if (d4 == 0) a.rec.ml[at] = make_float2(M, lw);
       }
     }
-    __syncthreads();  // the region is read: the next piece may write it
+    begin += take;
+    line.at += take;
+    if (line.at >= line.per_head) {
+      line.at = 0;
+      ++line.head;
+    }
+  }
+}
+
+// Joins the records of a row that several workgroups had keys of:
+// o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.  A workgroup an item and
+// row; D / 4 threads take a record, 1024 / D records at once, eight of each
+// thread's in flight, so up to 64 (D = 128) splits cost one round trip.
+template <class E, int D>
+__global__ __launch_bounds__(kPagedThreads) void paged_decode_merge(PagedArgs a) {
+  typedef typename E::type elem;
+  constexpr int LPR = D / 4, GROUPS = kPagedThreads / LPR, AT_ONCE = 8;
+  __shared__ __align__(16) float s_acc[GROUPS][D];
+  __shared__ float s_m[GROUPS], s_l[GROUPS];
+  const int group = threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+  const int items = min(a.rec.head[0], a.rec.groups);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int* d = a.rec.desc + (size_t)item * kDescInts;
+    const int splits = d[0], wg = d[1];
+    if (splits < 2 || 2 * (wg + splits - 1) >= a.rec.records) continue;
+    for (int row = blockIdx.y; row < d[4]; row += gridDim.y) {
+      float M = kPagedNegInf, L = 0.0f;
+      f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s0 = group; s0 < splits; s0 += GROUPS * AT_ONCE) {
+        float2 ml[AT_ONCE];
+        f4 v[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          const int s = min(s0 + j * GROUPS, splits - 1);
+          const size_t at = (size_t)(2 * (wg + s) + (s == 0 ? 1 : 0)) * MT + row;
+          ml[j] = a.rec.ml[at];
+          v[j] = *reinterpret_cast<const f4*>(a.rec.opart + at * D + col);
+        }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          if (s0 + j * GROUPS >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
+          if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);  // else: saw nothing
+        }
+        const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
+        L *= keep;
+        acc *= keep;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          if (ml[j].y == 0.0f) continue;
+          const float w = fast_exp2(ml[j].x - Mn);
+          L = fmaf(w, ml[j].y, L);
+          acc += w * v[j];
+        }
+        M = Mn;
+      }
+      *reinterpret_cast<f4*>(&s_acc[group][col]) = acc;
+      if (col == 0) {
+        s_m[group] = M;
+        s_l[group] = L;
+      }
+      __syncthreads();
+      if (threadIdx.x < D) {
+        float Mt = kPagedNegInf, Lt = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          if (s_l[g] != 0.0f) Mt = fmaxf(Mt, s_m[g]);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          if (s_l[g] == 0.0f) continue;
+          const float e = fast_exp2(s_m[g] - Mt);
+          Lt = fmaf(e, s_l[g], Lt);
+          o = fmaf(e, s_acc[g][threadIdx.x], o);
+        }
+        const int xr = d[3] + row;
+        static_cast<elem*>(a.o)[((size_t)(d[2] + xr / a.G) * a.Hq + d[5] * a.G + xr % a.G) * D +
+            threadIdx.x] = (elem)(Lt == 0.0f ? 0.0f : o / Lt);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -441,11 +649,9 @@ PagedFn pick_size(int D, bool aligned) {
 
 }  // namespace
 
-// Two tiles a wave: fewer cost more in starts and merges than they spread.
-int paged_decode_min_tiles(bool fp8, int D) {
-  (void)fp8;
-  (void)D;
-  return 2 * kWaves;
+PagedFn paged_decode_merge_fn(bool bf16, int D) {
+  if (bf16) return D == 64 ? paged_decode_merge<ElemBF16, 64> : paged_decode_merge<ElemBF16, 128>;
+  return D == 64 ? paged_decode_merge<ElemF16, 64> : paged_decode_merge<ElemF16, 128>;
 }
 
 PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned) {
