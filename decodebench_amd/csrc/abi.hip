@@ -594,13 +594,19 @@ int db_rope_append(const void* qkv, long long qkv_stride, const int* position, i
   return hip_status(dbk::launch_rope_append(c, cus, (hipStream_t)stream), fn);
 }
 
-size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new) {
+size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new,
+                                          size_t* zeroed) {
+  if (zeroed) *zeroed = 0;
   if (T < 1 || R < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128) || max_new < 0)
     return 0;
   int err = 0;
   const int cus = dbk::device_cu_count(&err);
   if (err) return 0;
-  return dbk::paged_workspace_bytes(paged_bounds(T, Hq, Hkv, D, R, max_new), cus);
+  size_t zero = 0;
+  const size_t bytes =
+      dbk::paged_workspace_bytes(paged_bounds(T, Hq, Hkv, D, R, max_new), cus, &zero);
+  if (zeroed) *zeroed = zero;
+  return bytes;
 }
 
 int db_paged_attention(const void* q, long long q_token_stride, long long q_head_stride,
@@ -621,6 +627,11 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
     return fail(DB_ERR_INVALID, "%s: Hq=%d is not a multiple of Hkv=%d", fn, Hq, cache->Hkv);
   if ((long long)T * Hq >= (1ll << 31) || (long long)R * cache->Hkv >= (1ll << 24))
     return fail(DB_ERR_INVALID, "%s: T * Hq or R * Hkv is too large", fn);
+  // Key tiles that the work of a KV head may come to.
+  const long long G = Hq / cache->Hkv, held = (long long)width * cache->page_size / 16 + 1;
+  const long long most = max_new > 0 && max_new < T ? max_new : T;
+  if (held >= (1ll << 31) || (most * G <= 16 ? T * G / 16 + R : R) * held >= (1ll << 31))
+    return fail(DB_ERR_INVALID, "%s: R * width * page_size is too large", fn);
   if (!(scale > 0.0f) || !isfinite(scale))
     return fail(DB_ERR_INVALID, "%s: scale must be finite and > 0", fn);
   if (window < 0 || (window > 0 && !causal))
@@ -656,7 +667,8 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
   int err = 0;
   const int cus = dbk::device_cu_count(&err);
   if (err) return hip_status((hipError_t)err, fn);
-  const size_t need = dbk::paged_workspace_bytes(c, cus);
+  size_t zeroed = 0;
+  const size_t need = dbk::paged_workspace_bytes(c, cus, &zeroed);
   if (ws_bytes < need)
     return fail(DB_ERR_INVALID, "%s: workspace %zu bytes < %zu required", fn, ws_bytes, need);
   return hip_status(dbk::launch_paged_attention(c, cus, ws, (hipStream_t)stream), fn);

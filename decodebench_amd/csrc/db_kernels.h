@@ -175,7 +175,8 @@ struct PagedCall {
   float scale;
   bool bf16;
 };
-size_t paged_workspace_bytes(const PagedCall& c, int cu_count);
+// Bytes of workspace, the first *zeroed of them zero between calls.
+size_t paged_workspace_bytes(const PagedCall& c, int cu_count, size_t* zeroed);
 hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream);
 
 // Read-only streaming probe (stream_probe.hip): `bytes` (a multiple of

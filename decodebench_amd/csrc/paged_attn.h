@@ -100,8 +100,9 @@ __device__ __forceinline__ bool pair_nonfinite(unsigned w) {
 // ------------------------------------------------------------- arguments
 // Region of the workspace of one kernel.
 struct PagedRecords {
-  int* head;      // [0]: groups (row tiles whose rows were split) of this call
-  int* desc;      // [groups][8]: splits, first record, first token, first row, rows
+  int* tickets;   // decode: [workgroups][kTicketInts], zero between calls
+  int* head;      // chunk: [0]: groups (row tiles whose rows were split) of this call
+  int* desc;      // chunk: [groups][8]: splits, first record, first token, first row, rows
   float2* ml;     // [records][MT]    maximum (base 2) and exp-sum
   float* opart;   // [records][MT][D] unnormalised output
   int records, groups;  // room
@@ -135,6 +136,7 @@ constexpr int kDecodeRows = 16;  // rows of the decode kernel's tile
 constexpr int kChunkKeys = 64;
 constexpr int kPagedThreads = 256;
 constexpr int kDescInts = 8;
+constexpr int kTicketInts = 64;  // a 256-byte line each: 8 tickets in one cost 1.7 us of contention
 
 // key / page for 0 <= key < 2^31, with magic = ceil(2^(31 + s) / page), s =
 // ceil(log2 page) = shift + 1: the excess magic * page - 2^(31 + s) is less
@@ -185,6 +187,11 @@ __device__ __forceinline__ long long lane_i64(long long v, int lane) {
   const int lo = __builtin_amdgcn_readlane((int)v, lane);
   const int hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
   return (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+
+// The lowest n of 64 bits (none below 0, all from 64 on).
+__device__ __forceinline__ unsigned long long below(int n) {
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
 // Inclusive prefix sum over the 64 lanes (DPP row shifts and broadcasts).
@@ -335,7 +342,6 @@ __device__ __forceinline__ void paged_describe(const PagedArgs& a, const PagedWo
 
 // e4m3 or 16-bit caches: the element type of the products E, of the cache C8.
 typedef void (*PagedFn)(PagedArgs);
-PagedFn paged_decode_merge_fn(bool bf16, int D);
 PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned);
 
 }  // namespace dbk

@@ -24,8 +24,8 @@
 //    next 16 tiles, so an address is two scalars read from a lane.  Any other
 //    page size: lane i looks up the page of key i of a tile, one tile ahead.
 //  * A wave skips tiles that none of its rows sees, and masks only tiles that
-//    some row sees in part (as paged_decode, an Inf or NaN among such a tile's
-//    values is added key by key).
+//    some row sees in part (an Inf or NaN among such a tile's values as in
+//    paged_decode: left out of the product, added to the rows that see it).
 #include "paged_attn.h"
 
 namespace dbk {
@@ -38,11 +38,6 @@ constexpr int kHold = kWave / (KT / 16);  // tiles whose places the lanes hold
 // Exponent references: a row's maximum may be kAbove over its reference, which
 // is set kBelow under the maximum.
 constexpr float kAbove = 12.0f, kBelow = 8.0f;
-
-// The lowest n of 64 bits (none below 0, all from 64 on).
-__device__ __forceinline__ unsigned long long below(int n) {
-  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
-}
 
 template <class E, bool FP8, int D, bool ALIGNED, int NW>
 __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(PagedArgs a) {
@@ -533,8 +528,8 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // the workgroups wanted of each kernel.
 struct PagedPlanned {
   bool decode;
-  int chunk_waves, decode_target, chunk_target;
-  int decode_items;  // row tiles of the decode kernel, of all KV heads, at most
+  int chunk_waves, chunk_target;
+  int decode_groups;  // a whole number of parts for each KV head
 };
 PagedPlanned planned(const PagedCall& c, int cu_count) {
   const int most = c.max_new > 0 && c.max_new < c.T ? c.max_new : c.T;
@@ -543,35 +538,48 @@ PagedPlanned planned(const PagedCall& c, int cu_count) {
   p.chunk_waves = rows <= kDecodeRows ? 0 : rows <= 64 ? 2 : 8;
   // Up to 64 rows a request, or one request: the chunk kernel takes them all.
   p.decode = p.chunk_waves == 0 || (p.chunk_waves == 8 && c.R > 1);
-  p.decode_target = 2 * cu_count;
+  // Parts of a KV head's line: a workgroup a CU where requests are few (a line of
+  // 32 parts and one request: 13.4 against 16.1 us with 64, at 8192 tokens, 27.9
+  // against 30.4 at 32768), else two (256 requests of 500 tokens 72 against 84).
+  const int per_cu = 4ll * c.R * c.cache.Hkv <= cu_count ? 1 : 2;
+  p.decode_groups = max(1, per_cu * cu_count / c.cache.Hkv) * c.cache.Hkv;
   p.chunk_target = p.chunk_waves == 2 ? 2 * cu_count : cu_count;
-  const long long G = c.Hq / c.cache.Hkv;
-  p.decode_items = (int)(((long long)c.T * G / kDecodeRows + c.R) * c.cache.Hkv);
   return p;
 }
 
-// Room for records and descriptions of row tiles.
-PagedRecords region(char* base, int records, int groups, int mt, int D, size_t* bytes) {
-  PagedRecords r;
-  r.records = records;
-  r.groups = groups;
+// Workspace of a call: the decode kernel's tickets (zero between calls), its
+// records, then the chunk kernel's.
+struct PagedSpace {
+  PagedRecords decode, chunk;
+  size_t bytes;
+};
+PagedSpace layout(const PagedPlanned& p, int D, char* base) {
+  PagedSpace s = {};
   size_t at = 0;
-  r.head = reinterpret_cast<int*>(base);
-  at += 256;
-  r.desc = reinterpret_cast<int*>(base + at);
-  at += round256((size_t)groups * kDescInts * sizeof(int));
-  r.ml = reinterpret_cast<float2*>(base + at);
-  at += round256((size_t)records * mt * sizeof(float2));
-  r.opart = reinterpret_cast<float*>(base + at);
-  at += round256((size_t)records * mt * D * sizeof(float));
-  *bytes = at;
-  return r;
-}
-PagedRecords decode_region(char* base, const PagedPlanned& p, int D, size_t* bytes) {
-  return region(base, 2 * p.decode_target, p.decode_items, kDecodeRows, D, bytes);
-}
-PagedRecords chunk_region(char* base, const PagedPlanned& p, int D, size_t* bytes) {
-  return region(base, 2 * p.chunk_target, p.chunk_target, 32 * p.chunk_waves, D, bytes);
+  auto take = [&](size_t n) {
+    char* const here = base + at;
+    at += round256(n);
+    return here;
+  };
+  auto records = [&](PagedRecords& r, int count, int mt) {
+    r.records = count;
+    r.ml = reinterpret_cast<float2*>(take((size_t)count * mt * sizeof(float2)));
+    r.opart = reinterpret_cast<float*>(take((size_t)count * mt * D * sizeof(float)));
+  };
+  if (p.decode) {
+    s.decode.tickets =
+        reinterpret_cast<int*>(take((size_t)p.decode_groups * kTicketInts * sizeof(int)));
+    records(s.decode, 2 * p.decode_groups, kDecodeRows);
+  }
+  if (p.chunk_waves) {
+    s.chunk.groups = p.chunk_target;
+    s.chunk.head = reinterpret_cast<int*>(take(sizeof(int)));
+    s.chunk.desc =
+        reinterpret_cast<int*>(take((size_t)p.chunk_target * kDescInts * sizeof(int)));
+    records(s.chunk, 2 * p.chunk_target, 32 * p.chunk_waves);
+  }
+  s.bytes = at;
+  return s;
 }
 
 // Whether 16 keys from a multiple of 16 on always lie in one page, at offsets
@@ -583,12 +591,10 @@ bool paged_aligned(const db_paged_cache& kv) {
 
 }  // namespace
 
-size_t paged_workspace_bytes(const PagedCall& c, int cu_count) {
+size_t paged_workspace_bytes(const PagedCall& c, int cu_count, size_t* zeroed) {
   const PagedPlanned p = planned(c, cu_count);
-  size_t decode = 0, chunk = 0;
-  if (p.decode) decode_region(nullptr, p, c.cache.D, &decode);
-  if (p.chunk_waves) chunk_region(nullptr, p, c.cache.D, &chunk);
-  return decode + chunk;
+  *zeroed = p.decode ? (size_t)p.decode_groups * kTicketInts * sizeof(int) : 0;
+  return layout(p, c.cache.D, nullptr).bytes;
 }
 
 hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream) {
@@ -633,25 +639,14 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
   a.scale_log2 = c.scale * 1.4426950408889634f;
 
   const bool aligned = paged_aligned(kv);
-  char* base = static_cast<char*>(ws);
-  size_t bytes = 0;
+  const PagedSpace space = layout(p, D, static_cast<char*>(ws));
   if (p.decode) {
     a.part = p.chunk_waves ? 1 : 0;
-    a.target = p.decode_target;
     a.min_tiles = 8;
-    a.rec = decode_region(base, p, D, &bytes);
-    base += bytes;
-    hipLaunchKernelGGL(paged_decode_fn(c.bf16, fp8, D, aligned), dim3(p.decode_target),
+    a.rec = space.decode;
+    hipLaunchKernelGGL(paged_decode_fn(c.bf16, fp8, D, aligned), dim3(p.decode_groups),
                        dim3(kPagedThreads), 0, stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    // An item a request and KV head and G rows each where the tokens are single;
-    // the merge walks what is beyond.
-    const long long items = (long long)c.R * a.Hkv;
-    const int merge_x = (int)(items < 4096 ? items : 4096), merge_y = a.G < 16 ? a.G : 16;
-    hipLaunchKernelGGL(paged_decode_merge_fn(c.bf16, D), dim3(merge_x, merge_y),
-                       dim3(kPagedThreads), 0, stream, a);
-    e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   if (p.chunk_waves) {
@@ -659,7 +654,7 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
     a.part = p.decode ? 2 : 0;
     a.target = p.chunk_target;
     a.min_tiles = 4;
-    a.rec = chunk_region(base, p, D, &bytes);
+    a.rec = space.chunk;
     // Row tiles of every request at most, and the splits beyond one each.
     const long long grid = ((long long)c.T * a.G / mt + c.R) * a.Hkv + p.chunk_target;
     hipLaunchKernelGGL(pick_chunk(p.chunk_waves, c.bf16, fp8, D, aligned), dim3((unsigned)grid),

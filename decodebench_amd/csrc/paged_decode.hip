@@ -24,8 +24,9 @@
 //    page size: a lane looks up the page of its own key, one tile ahead of the
 //    loads, and rows of V take theirs from that lane.
 //  * Masked keys: scores by selection, so no Inf or NaN of a masked key counts;
-//    a tile that some row sees only in part is searched for an Inf or NaN
-//    among its values, and one that has any is added key by key.
+//    in a tile that some row sees only in part the values that are Inf or NaN
+//    are left out of the product (their probability may be zero, but zero times
+//    those is not) and added to the rows that do see them.
 #include "paged_attn.h"
 
 namespace dbk {
@@ -35,7 +36,8 @@ namespace {
 constexpr int kWaves = kPagedThreads / kWave;
 constexpr int MT = kDecodeRows;
 
-constexpr float kHidden = -1.0f;  // no probability
+constexpr int kSc1 = 16;         // cache policy of a buffer access: device scope
+constexpr int kVmcnt0 = 0x0F70;  // s_waitcnt vmcnt(0), the other counters left alone
 
 constexpr int decode_keys(bool fp8, int D) { return D * (fp8 ? 1 : 2) >= 256 ? 16 : 32; }
 
@@ -47,12 +49,14 @@ __device__ __forceinline__ void lds_order() {
 }
 
 // ------------------------------------------------------------- schedule
-// All work of a call in one line: for each KV head, each request in order, each
-// row tile of it, its key tiles from the first that a row sees to the last.
-// The line is cut into `target` equal parts, a workgroup each, so that all of
-// them end together whatever the lengths are (splitting each request by itself
-// left 64 requests of 800 to 8000 tokens at 63% of the stream rate).  A part
-// holds the end of one item, whole items, and the beginning of another.
+// The work of a KV head in one line: each request in order, each row tile of
+// it, its key tiles from the first that a row sees to the last.  The line is cut
+// into equal parts, a workgroup each, so that all of them end together whatever
+// the lengths are (splitting each request by itself left 64 requests of 800 to
+// 8000 tokens at 63% of the stream rate).  A part holds the end of one item,
+// whole items, and the beginning of another.  The workgroups of a part's KV
+// heads are neighbours, so the heads of a page, which lie side by side, are read
+// at about the same time.
 struct DecodeRequest {
   int tok0, n, len;
   int t0, tiles;     // first key tile, and how many, of each row tile (none: one all the same)
@@ -76,80 +80,133 @@ __device__ __forceinline__ DecodeRequest decode_request(const PagedArgs& a, int 
   return q;
 }
 
-__device__ __forceinline__ long long wave_scan64(long long v) {
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int d = 1; d < kWave; d <<= 1) {
-    const long long u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-
-// A position on the line, in scalar registers but for what each lane holds of
-// a request of the present 64 ones.  Every wave has its own: no LDS, no barrier.
+// The line of a KV head; what each lane holds is of a request of the present 64.
+// Every wave has its own: no LDS, no barrier.  (The host has checked that all
+// tiles of a line are fewer than 2^31.)
 template <int KT>
 struct DecodeLine {
   const PagedArgs& a;
   DecodeRequest mine;
-  long long per_head;     // key tiles of one KV head
-  long long upto, all;    // of this round's requests up to this one, and in all
-  long long before;       // of the rounds before
-  int items_before, items_head;  // row tiles of the rounds before; of one KV head
+  int length;      // key tiles in all
+  int upto, all;   // of this round's requests up to this one, and in all
+  int before;      // of the rounds before
   int round;
-  long long at;           // within the KV head
-  int head;
 
-  __device__ explicit DecodeLine(const PagedArgs& args) : a(args) {
+  __device__ explicit DecodeLine(const PagedArgs& args) : a(args), before(0), round(0) {
     const int lane = threadIdx.x & (kWave - 1);
-    long long sum = 0;
-    int items = 0;
-    for (int r = (a.R - 1) / kWave * kWave; r >= 0; r -= kWave) {
-      mine = decode_request<KT>(a, r + lane);
-      sum += (long long)mine.row_tiles * mine.tiles;
-      items += mine.row_tiles;
+    int sum = 0;
+    for (int r = (a.R - 1) / kWave * kWave; r > 0; r -= kWave) {
+      const DecodeRequest q = decode_request<KT>(a, r + lane);
+      sum += q.row_tiles * q.tiles;
     }
-    if (a.R > kWave)
-      for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
-    items_head = wave_total(items);
-    round = 0;
-    before = 0;
-    items_before = 0;
+    mine = decode_request<KT>(a, lane);
     scan();
-    per_head = a.R > kWave ? lane_i64(sum, 0) : all;
+    length = all + (a.R > kWave ? wave_total(sum) : 0);
   }
   __device__ void scan() {
-    upto = wave_scan64((long long)mine.row_tiles * mine.tiles);
-    all = lane_i64(upto, kWave - 1);
-  }
-  __device__ void to_round(int r) {
-    round = r;
-    mine = decode_request<KT>(a, r * kWave + (int)(threadIdx.x & (kWave - 1)));
-    scan();
+    upto = wave_scan(mine.row_tiles * mine.tiles);
+    all = __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   // The item at `at`: its request (lane `who` of the round), row tile and the
-  // tile within it.  Positions only grow within a head.
-  __device__ void locate(int& who, int& row_tile, int& tile, int& item) {
-    if (at < before) {  // a new head
-      before = 0;
-      items_before = 0;
-      to_round(0);
-    }
+  // tile within it.  Positions only grow.
+  __device__ void locate(int at, int& who, int& row_tile, int& tile) {
     while (at >= before + all) {
       before += all;
-      items_before += wave_total(mine.row_tiles);
-      to_round(round + 1);
+      ++round;
+      mine = decode_request<KT>(a, round * kWave + (int)(threadIdx.x & (kWave - 1)));
+      scan();
     }
-    const long long in = at - before;
+    const int in = at - before;
     who = __builtin_ctzll(__ballot(in < upto));
     const int tiles = __builtin_amdgcn_readlane(mine.tiles, who);
     const int rts = __builtin_amdgcn_readlane(mine.row_tiles, who);
-    const long long off = in - (lane_i64(upto, who) - (long long)tiles * rts);
-    row_tile = rts == 1 ? 0 : (int)(off / tiles);
-    tile = (int)(off - (long long)row_tile * tiles);
-    const bool earlier = (int)(threadIdx.x & (kWave - 1)) < who;
-    item = head * items_head + items_before + wave_total(earlier ? mine.row_tiles : 0) + row_tile;
+    const int off = in - (__builtin_amdgcn_readlane(upto, who) - tiles * rts);
+    row_tile = rts == 1 ? 0 : off / tiles;
+    tile = off - row_tile * tiles;
   }
 };
+
+// Joins the `splits` records of a row tile, the first in workgroup wg0's second
+// place, the others in the first places of wg0 + Hkv, + 2 Hkv, ...: a thread a
+// float4 of a row and a share of the records, sixteen of them in flight, then the
+// shares through LDS (`scratch`: 6 floats a thread).
+template <class E, int D>
+__device__ __forceinline__ void join_records(const PagedArgs& a, int tok0, int row_tile, int rows,
+                                             int head, int wg0, int splits, float* scratch) {
+  typedef typename E::vec4 vec4;
+  constexpr int AT_ONCE = 16;
+  const __amdgpu_buffer_rsrc_t r_ml = make_rsrc(a.rec.ml, a.rec.records * MT * 8);
+  const __amdgpu_buffer_rsrc_t r_op = make_rsrc(a.rec.opart, a.rec.records * MT * D * 4);
+  const int slots = rows * (D / 4);
+  const int shares = slots >= kPagedThreads ? 1 : kPagedThreads / slots;
+  for (int s_base = 0; s_base < slots; s_base += kPagedThreads / shares) {
+    const int share = threadIdx.x / min(slots, kPagedThreads);
+    const int slot = s_base + threadIdx.x % min(slots, kPagedThreads);
+    const bool on = share < shares && slot < slots;
+    const int row = slot / (D / 4), d4 = slot % (D / 4);
+    float M = kPagedNegInf, L = 0.0f;
+    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = share; on && s0 < splits; s0 += shares * AT_ONCE) {
+      float2 ml[AT_ONCE];
+      f4 v[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int s = min(s0 + j * shares, splits - 1);
+        const size_t at = (size_t)(2 * (wg0 + s * a.Hkv) + (s == 0 ? 1 : 0)) * MT + row;
+        ml[j] = __builtin_bit_cast(
+            float2, __builtin_amdgcn_raw_buffer_load_b64(r_ml, (int)at * 8, 0, kSc1));
+        v[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+                                          r_op, (int)(at * D + 4 * d4) * 4, 0, kSc1));
+      }
+      float Mn = M;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        if (s0 + j * shares >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
+        if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);  // else: saw nothing
+      }
+      const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
+      L *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        if (ml[j].y == 0.0f) continue;
+        const float w = fast_exp2(ml[j].x - Mn);
+        L = fmaf(w, ml[j].y, L);
+        acc += w * v[j];
+      }
+      M = Mn;
+    }
+    float* mine = scratch + threadIdx.x * 6;
+    mine[0] = M;
+    mine[1] = L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine[2 + i] = acc[i];
+    __syncthreads();
+    if (on && share == 0) {
+      float Mt = kPagedNegInf, Lt = 0.0f;
+      f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      const int step = 6 * min(slots, kPagedThreads);
+      for (int g = 0; g < shares; ++g)
+        if (mine[g * step + 1] != 0.0f) Mt = fmaxf(Mt, mine[g * step]);
+      for (int g = 0; g < shares; ++g) {
+        const float* c = mine + g * step;
+        if (c[1] == 0.0f) continue;
+        const float e = fast_exp2(c[0] - Mt);
+        Lt = fmaf(e, c[1], Lt);
+        o += e * f4{c[2], c[3], c[4], c[5]};
+      }
+      const int xr = row_tile * MT + row;
+      const float inv = Lt == 0.0f ? 0.0f : 1.0f / Lt;
+      vec4 r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = (typename E::type)(o[i] * inv);
+      *reinterpret_cast<vec4*>(static_cast<typename E::type*>(a.o) +
+                               ((size_t)(tok0 + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D +
+                               4 * d4) = r;
+    }
+    __syncthreads();
+  }
+}
 
 template <class E, bool FP8, int D, bool ALIGNED>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
@@ -171,37 +228,36 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
   constexpr size_t kRegion = kOut > kTile ? kOut : kTile;
 
   __shared__ __align__(16) char s_region[kWaves][kRegion];
-  __shared__ float s_p[kWaves][KT][16];  // probabilities of a tile added key by key
   __shared__ float s_m[MT][kWaves], s_l[MT][kWaves];
+  __shared__ int s_arrived;
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n16 = lane & 15, g4 = lane >> 4;
   elem* const vbuf = reinterpret_cast<elem*>(s_region[wave]);
 
+  const __amdgpu_buffer_rsrc_t r_ml = make_rsrc(a.rec.ml, a.rec.records * MT * 8);
+  const __amdgpu_buffer_rsrc_t r_op = make_rsrc(a.rec.opart, a.rec.records * MT * D * 4);
   DecodeLine<KT> line(a);
-  // This workgroup's part [begin, end) of the line.
-  const long long total = line.per_head * a.Hkv;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.rec.head[0] = line.items_head * a.Hkv;
-  const long long per = max((total + a.target - 1) / a.target, (long long)a.min_tiles);
-  long long begin = per * blockIdx.x;
-  const long long end = min(begin + per, total);
-  if (begin >= end) return;
-  line.head = (int)(begin / line.per_head);
-  line.at = begin - line.per_head * line.head;
+  // This workgroup's part [begin, end) of its KV head's line.
+  const int part = blockIdx.x / a.Hkv, head = blockIdx.x % a.Hkv;
+  const int parts = gridDim.x / a.Hkv;
+  const int per = max((line.length + parts - 1) / parts, a.min_tiles);
+  int begin = (int)min((long long)per * part, (long long)line.length);
+  const int end = (int)min((long long)begin + per, (long long)line.length);
   for (bool once = true; begin < end; once = false) {
     if (!once) __syncthreads();  // the region is read: the next piece may write it
     DecodeRequest rq;
-    int who, row_tile, tile_in, item;
-    line.locate(who, row_tile, tile_in, item);
+    int who, row_tile, tile_in;
+    line.locate(begin, who, row_tile, tile_in);
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
     rq.tok0 = of(line.mine.tok0);
     rq.n = of(line.mine.n);
     rq.len = of(line.mine.len);
     rq.t0 = of(line.mine.t0);
     rq.tiles = of(line.mine.tiles);
-    const int r = line.round * kWave + who, head = line.head;
-    const int take = (int)min(end - begin, (long long)(rq.tiles - tile_in));
+    const int r = line.round * kWave + who;
+    const int take = min(end - begin, rq.tiles - tile_in);
     const int limit = paged_limit(a, rq.len);
     const int t_begin = rq.t0 + tile_in, t_end = t_begin + take;
     // Rows that other workgroups have keys of go to a record: of this
@@ -209,16 +265,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
     const bool starts = tile_in == 0, whole = starts && take == rq.tiles;
     const int rec = whole ? -1 : 2 * blockIdx.x + (starts ? 1 : 0);
     const int rows = min(rq.n * a.G - row_tile * MT, MT);
-    if (starts && threadIdx.x == 0 && item < a.rec.groups) {
-      int* d = a.rec.desc + (size_t)item * kDescInts;
-      // the workgroup of the item's last tile
-      d[0] = whole ? 0 : (int)((begin + rq.tiles - 1) / per) - (int)blockIdx.x + 1;
-      d[1] = blockIdx.x;
-      d[2] = rq.tok0;
-      d[3] = row_tile * MT;
-      d[4] = rows;
-      d[5] = head;
-    }
 
     const char* const kbase = static_cast<const char*>(a.k) + head * a.kh * CB;
     const char* const vbase = static_cast<const char*>(a.v) + head * a.vh * CB;
@@ -336,31 +382,62 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
       return there;
     };
 
+    // Adds the Infs and NaNs that a partly seen tile left out to the rows that see
+    // them (values read again from the cache; a rare path, kept small).
+    auto add_odd = [&](int key0, unsigned sees) {
+#pragma unroll 1
+      for (int kk = 0; kk < KT; ++kk) {
+        const bool ok = (sees >> kk) & 1;
+        if (!__any(ok)) continue;  // also keys without a page
+        const int key = key0 + kk, at = page_of(a, key);
+        const char* row = vbase + (trow[at] * a.vp + (key - at * a.page) * a.vt) * CB;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const char* four = row + (16 * b + 4 * g4) * CB;
+          const u2 w = FP8 ? E::widen(*reinterpret_cast<const unsigned*>(four))
+                           : *reinterpret_cast<const u2*>(four);
+          const vec4 v = __builtin_bit_cast(vec4, w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            o[b][c] += ok && !__builtin_isfinite((float)v[c]) ? (float)v[c] : 0.0f;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+
     auto compute_tile = [&](const u4 (&kt)[NS][NK], u4 (&vt)[NS][NV], int k, unsigned there) {
       const int key0 = tile_of(k) * KT;
       const bool partial =
           there != (unsigned)((1ull << KT) - 1) || key0 < all_lo || key0 + KT > all_hi;
-      bool odd = false;  // a partly seen tile with an Inf or NaN among its values
+      bool odd = false;  // an Inf or NaN among the values of a partly seen tile, left out
+      unsigned sees = ~0u;   // bit 16 u + 4 g4 + j: this lane's row sees that key
       if (partial) {
-        bool bad = false;
+        const unsigned in = there & (unsigned)below(limit - key0);
+        sees = in & (unsigned)(below(khi - key0) & ~below(klo - key0));
+        const unsigned mine = in >> (lane / LPR);
 #pragma unroll
         for (int u = 0; u < NS; ++u)
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
-            const int row = 16 * u + j * RPI + lane / LPR;
-            if (!((there >> row) & 1) || key0 + row >= limit) vt[u][j] = u4{0, 0, 0, 0};
+            const bool ok = mine & (1u << (16 * u + j * RPI));
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
+              unsigned w = ok ? vt[u][j][c] : 0u;
               if constexpr (FP8) {
-                const unsigned w = vt[u][j][c] & 0x7F7F7F7Fu;  // NaN: seven bits set (no Inf)
-                bad = bad || (w & 0xFFu) == 0x7Fu || ((w >> 8) & 0xFFu) == 0x7Fu ||
-                      ((w >> 16) & 0xFFu) == 0x7Fu || (w >> 24) == 0x7Fu;
+                // NaN: the seven low bits of a byte set (there is no Inf); 0x80
+                // marks those bytes
+                const unsigned n = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                odd = odd || n != 0;
+                w &= ~(n | (n - (n >> 7)));
               } else {
-                bad = bad || pair_nonfinite<E>(vt[u][j][c]);
+                const bool lo = (w & E::kExp) == E::kExp, hi = ((w >> 16) & E::kExp) == E::kExp;
+                odd = odd || lo || hi;
+                w &= (lo ? 0u : 0x0000FFFFu) | (hi ? 0u : 0xFFFF0000u);
               }
+              vt[u][j][c] = w;
             }
           }
-        odd = __any(bad);
+        odd = __any(odd);
       }
       // the tile's values, rows in key order
       lds_order();
@@ -403,16 +480,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * u + j] = acc[j] * scale;
       }
-      unsigned sees = ~0u;  // bit 4 u + j
       if (partial) {
-        sees = 0;
+        const unsigned mine = sees >> (4 * g4);
 #pragma unroll
-        for (int i = 0; i < 4 * NS; ++i) {
-          const int kk = 16 * (i >> 2) + 4 * g4 + (i & 3);
-          const bool ok = key0 + kk >= klo && key0 + kk < khi && ((there >> kk) & 1);
-          sees |= ok ? 1u << i : 0u;
-          s[i] = ok ? s[i] : kPagedNegInf;
-        }
+        for (int i = 0; i < 4 * NS; ++i)
+          s[i] = mine & (1u << (16 * (i >> 2) + (i & 3))) ? s[i] : kPagedNegInf;
       }
       float tmax = s[0];
 #pragma unroll
@@ -435,25 +507,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] *= alpha;
       }
-      if (odd) {
-        // Key by key: only keys that the row sees are added.
-#pragma unroll
-        for (int i = 0; i < 4 * NS; ++i)
-          s_p[wave][16 * (i >> 2) + 4 * g4 + (i & 3)][n16] =
-              (sees >> i) & 1 ? (float)pb[i] : kHidden;
-        lds_order();
-#pragma unroll 1
-        for (int kk = 0; kk < KT; ++kk) {
-          const float p = s_p[wave][kk][n16];
-          if (p == kHidden) continue;
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              o[b][c] += p * (float)vbuf[kk * VS + 16 * b + 4 * g4 + c];
-        }
-        return;
-      }
       auto read_v = [&](int u, int b) {
         return __builtin_bit_cast(
             u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -473,6 +526,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
           o[b] = E::mfma16(__builtin_bit_cast(vec8, u4{v0[0], v0[1], v1[0], v1[1]}), p, o[b]);
         }
       }
+      if (odd) add_odd(key0, sees);
     };
 
     // ---- this wave's tiles, two register sets of one tile each ------------
@@ -553,90 +607,41 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
         *reinterpret_cast<vec4*>(op) = r;
       } else if (rec < a.rec.records) {
         const size_t at = (size_t)rec * MT + row;
-        *reinterpret_cast<f4*>(a.rec.opart + at * D + 4 * d4) = ow;
-        if (d4 == 0) a.rec.ml[at] = make_float2(M, lw);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, ow), r_op,
+                                               (int)(at * D + 4 * d4) * 4, 0, kSc1);
+        if (d4 == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, make_float2(M, lw)), r_ml,
+                                                (int)at * 8, 0, kSc1);
+      }
+    }
+    if (rec >= 0) {
+      // The last of the item's workgroups to arrive joins their records,
+      //   o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
+      // Its parts are first_part .. first_part + splits - 1; the ticket is that
+      // of the part that begins it (a part begins one such item at most).
+      const int item_begin = begin - tile_in;
+      const int first_part = item_begin / per;
+      const int splits = (item_begin + rq.tiles - 1) / per - first_part + 1;
+      const int wg0 = first_part * a.Hkv + head;
+      int* const ticket = a.rec.tickets + (size_t)wg0 * kTicketInts;
+      // Records are written through to memory and read from there (device
+      // scope, kSc1), since the item's workgroups run on any XCD; every thread's
+      // stores are done before the ticket is taken.  (Plain stores released and
+      // acquired by the ticket instead write back and invalidate whole L2s: one
+      // request of 8192 tokens took 28 us that way.)
+      __builtin_amdgcn_s_waitcnt(kVmcnt0);
+      __syncthreads();
+      if (threadIdx.x == 0)
+        s_arrived = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (s_arrived == splits - 1) {
+        if (threadIdx.x == 0)
+          __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        join_records<E, D>(a, rq.tok0, row_tile, rows, head, wg0, splits,
+             reinterpret_cast<float*>(&s_region[0][0]));
       }
     }
     begin += take;
-    line.at += take;
-    if (line.at >= line.per_head) {
-      line.at = 0;
-      ++line.head;
-    }
-  }
-}
-
-// Joins the records of a row that several workgroups had keys of:
-// o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.  A workgroup an item and
-// row; D / 4 threads take a record, 1024 / D records at once, eight of each
-// thread's in flight, so up to 64 (D = 128) splits cost one round trip.
-template <class E, int D>
-__global__ __launch_bounds__(kPagedThreads) void paged_decode_merge(PagedArgs a) {
-  typedef typename E::type elem;
-  constexpr int LPR = D / 4, GROUPS = kPagedThreads / LPR, AT_ONCE = 8;
-  __shared__ __align__(16) float s_acc[GROUPS][D];
-  __shared__ float s_m[GROUPS], s_l[GROUPS];
-  const int group = threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
-  const int items = min(a.rec.head[0], a.rec.groups);
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int* d = a.rec.desc + (size_t)item * kDescInts;
-    const int splits = d[0], wg = d[1];
-    if (splits < 2 || 2 * (wg + splits - 1) >= a.rec.records) continue;
-    for (int row = blockIdx.y; row < d[4]; row += gridDim.y) {
-      float M = kPagedNegInf, L = 0.0f;
-      f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int s0 = group; s0 < splits; s0 += GROUPS * AT_ONCE) {
-        float2 ml[AT_ONCE];
-        f4 v[AT_ONCE];
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-          const int s = min(s0 + j * GROUPS, splits - 1);
-          const size_t at = (size_t)(2 * (wg + s) + (s == 0 ? 1 : 0)) * MT + row;
-          ml[j] = a.rec.ml[at];
-          v[j] = *reinterpret_cast<const f4*>(a.rec.opart + at * D + col);
-        }
-        float Mn = M;
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-          if (s0 + j * GROUPS >= splits) ml[j] = make_float2(kPagedNegInf, 0.0f);
-          if (ml[j].y != 0.0f) Mn = fmaxf(Mn, ml[j].x);  // else: saw nothing
-        }
-        const float keep = L == 0.0f ? 0.0f : fast_exp2(M - Mn);
-        L *= keep;
-        acc *= keep;
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-          if (ml[j].y == 0.0f) continue;
-          const float w = fast_exp2(ml[j].x - Mn);
-          L = fmaf(w, ml[j].y, L);
-          acc += w * v[j];
-        }
-        M = Mn;
-      }
-      *reinterpret_cast<f4*>(&s_acc[group][col]) = acc;
-      if (col == 0) {
-        s_m[group] = M;
-        s_l[group] = L;
-      }
-      __syncthreads();
-      if (threadIdx.x < D) {
-        float Mt = kPagedNegInf, Lt = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-          if (s_l[g] != 0.0f) Mt = fmaxf(Mt, s_m[g]);
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          if (s_l[g] == 0.0f) continue;
-          const float e = fast_exp2(s_m[g] - Mt);
-          Lt = fmaf(e, s_l[g], Lt);
-          o = fmaf(e, s_acc[g][threadIdx.x], o);
-        }
-        const int xr = d[3] + row;
-        static_cast<elem*>(a.o)[((size_t)(d[2] + xr / a.G) * a.Hq + d[5] * a.G + xr % a.G) * D +
-            threadIdx.x] = (elem)(Lt == 0.0f ? 0.0f : o / Lt);
-      }
-      __syncthreads();
-    }
   }
 }
 
@@ -648,11 +653,6 @@ PagedFn pick_size(int D, bool aligned) {
 }
 
 }  // namespace
-
-PagedFn paged_decode_merge_fn(bool bf16, int D) {
-  if (bf16) return D == 64 ? paged_decode_merge<ElemBF16, 64> : paged_decode_merge<ElemBF16, 128>;
-  return D == 64 ? paged_decode_merge<ElemF16, 64> : paged_decode_merge<ElemF16, 128>;
-}
 
 PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned) {
   if (bf16)

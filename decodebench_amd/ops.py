@@ -27,6 +27,7 @@ import ctypes as C
 import math
 import sys
 import threading
+from contextlib import nullcontext
 from pathlib import Path
 from typing import NamedTuple
 
@@ -98,7 +99,8 @@ def load_library():
                                    _p, _p]),
             "db_rope_append": (_i, [_p, _ll, _p, _i, _p, _p, _p, _i, _i, C.POINTER(_PagedCache),
                                     _p, _i, _i, _i, _p]),
-            "db_paged_attention_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i]),
+            "db_paged_attention_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i,
+                                                               C.POINTER(C.c_size_t)]),
             "db_paged_attention": (_i, [_p, _ll, _ll, _p, C.POINTER(_PagedCache), _p, _ll, _i, _p,
                                         _p, _i, _i, _i, _i, C.c_float, _i, _i, _i, _p,
                                         C.c_size_t, _p]),
@@ -212,6 +214,12 @@ def _gpu_tensors(*items) -> int:
         elif d != idx:
             raise ValueError(f"{name} is on cuda:{d}, expected cuda:{idx} like {first}")
     return idx
+
+
+def _on_device(idx: int):
+    """Makes GPU ``idx`` current where it is not."""
+    torch = _torch
+    return nullcontext() if torch.cuda.current_device() == idx else torch.cuda.device(idx)
 
 
 def _launch(fn, idx: int, what: str, *args) -> None:
@@ -492,6 +500,14 @@ def f4_workspace(B: int, Hq: int, Hkv: int, L: int, D: int, S: int, device):
     nbytes = int(load_library().db_f4_workspace_bytes(B, Hq, Hkv, L, D, S))
     if nbytes == 0:
         return None
+    return _kept_workspace((), nbytes, nbytes, device)
+
+
+def _kept_workspace(kind: tuple, nbytes: int, zeroed: int, device):
+    """A workspace whose first ``zeroed`` bytes were zero when it was made, kept
+    as :func:`f4_workspace` says; ``kind`` tells those of other ops apart."""
+    import torch
+
     dev = torch.device(device)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     stream = torch.cuda.current_stream(idx).cuda_stream
@@ -499,21 +515,23 @@ def f4_workspace(B: int, Hq: int, Hkv: int, L: int, D: int, S: int, device):
         cid = C.c_ulonglong(0)
         _check(load_library().db_stream_capture_id(stream, C.byref(cid)),
                "db_stream_capture_id")
-        key = (idx, stream, cid.value, nbytes)
+        key = (*kind, idx, stream, cid.value, nbytes)
         cache = _captured_ws
     else:
-        key = (idx, stream, nbytes)
+        key = (*kind, idx, stream, nbytes)
         cache = _ws_cache
     ws = cache.get(key)
     if ws is None:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws[:zeroed].zero_()
         cache[key] = ws
     return ws
 
 
 def release_captured_workspaces() -> int:
-    """Drop the references to the F4 workspaces made under graph capture;
-    call it once every graph that recorded F4 calls has been destroyed.
+    """Drop the references to the workspaces of F4 and paged attention made
+    under graph capture; call it once every graph that recorded such calls has
+    been destroyed.
     Returns how many were released."""
     n = len(_captured_ws)
     _captured_ws.clear()
@@ -823,14 +841,16 @@ def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None =
     o = _row_output((T, Hq, D), q.dtype, idx, out)
     lib = _lib or load_library()
     most = min(int(max_new or T), T)
-    if torch.cuda.current_device() == idx:
-        nbytes = lib.db_paged_attention_workspace_bytes(T, Hq, cache.Hkv, D, R, most)
-    else:
-        with torch.cuda.device(idx):
-            nbytes = lib.db_paged_attention_workspace_bytes(T, Hq, cache.Hkv, D, R, most)
-    # Nothing in it outlives the call, so torch's allocator hands it out anew
-    # each time: per stream, and from a graph's own pool under capture.
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    with _on_device(idx):
+        zeroed = C.c_size_t(0)
+        nbytes = lib.db_paged_attention_workspace_bytes(T, Hq, cache.Hkv, D, R, most,
+                                                        C.byref(zeroed))
+        # Tickets that start at zero are kept as F4's are; otherwise nothing in the
+        # workspace outlives the call, and torch's allocator hands it out anew.
+        if zeroed.value:
+            ws = _kept_workspace(("paged",), nbytes, zeroed.value, idx)
+        else:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _launch(lib.db_paged_attention, idx, "db_paged_attention", q.data_ptr(), *_strides(q, 2),
             o.data_ptr(), C.byref(cache), block_table.data_ptr(), *_strides(block_table, 1), width, q_start.data_ptr(), kv_len.data_ptr(), T, R,
             Hq, most, scale, bool(causal), int(window or 0), dt, ws.data_ptr(), nbytes)

@@ -268,11 +268,14 @@ int db_rope_append(const void* qkv, long long qkv_stride, const int* position, i
  * Rows of o [T, Hq, D] (dense) that belong to no request stay as they are.
  * max_new > 0 says how many new tokens a request has at most (0: T), which
  * decides which kernels are launched; a call that breaks it is still right.
- * Contract: T >= 0, R >= 0, Hq a multiple of Hkv, T * Hq < 2^31, D 64 or 128,
+ * Contract: T >= 0, R >= 0, Hq a multiple of Hkv, T * Hq < 2^31, R * Hkv < 2^24,
+ * R * width * page_size below 2^34 or so, D 64 or 128,
  * scale finite and > 0, dtype as db_rope_append; q, o and cache rows 16-byte
  * aligned; ws of db_paged_attention_workspace_bytes, 256-byte aligned, not
- * shared by calls that overlap in time. */
-size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new);
+ * shared by calls that overlap in time.  Its first *zeroed bytes (zeroed may
+ * be NULL) must be zero at its first use; every call leaves them zero. */
+size_t db_paged_attention_workspace_bytes(int T, int Hq, int Hkv, int D, int R, int max_new,
+                                          size_t* zeroed);
 int db_paged_attention(const void* q, long long q_token_stride, long long q_head_stride,
                        void* o, const db_paged_cache* cache, const int* table,
                        long long table_stride, int width, const int* q_start,

@@ -808,7 +808,7 @@ def test_paged_workspace_of_refused_calls_is_none(lib):
     f = lib.db_paged_attention_workspace_bytes
     for bad in ((0, 32, 8, 128, 1, 1), (1, 30, 8, 128, 1, 1), (1, 32, 8, 96, 1, 1),
                 (1, 32, 8, 128, 0, 1), (1, 32, 8, 128, 1, -1)):
-        assert f(*bad) == 0
+        assert f(*bad, None) == 0
 
 
 def test_paged_wrappers_refuse_cpu_tensors():
