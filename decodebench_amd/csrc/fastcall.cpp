@@ -40,11 +40,15 @@ struct Abi {
   decltype(&db_stream_capture_id) capture_id;
   decltype(&db_gemv_workspace_bytes) gemv_workspace_bytes;
   decltype(&db_gemv_ws) gemv_ws;
+  decltype(&db_paged_plan) paged_plan;
+  decltype(&db_rope_append) rope_append;
+  decltype(&db_paged_attention_workspace_bytes) paged_workspace_bytes;
+  decltype(&db_paged_attention) paged_attention;
 } abi;
 
 PyObject* raw_stream = nullptr;  // device index -> current stream's handle
 PyObject* get_device = nullptr;  // () -> current device
-PyObject* workspaces = nullptr;  // dict (device, stream, bytes) -> tensor
+PyObject* workspaces = nullptr;  // dict ([kind,] device, stream, bytes) -> tensor
 PyObject* cu_counts = nullptr;   // dict device -> compute units
 
 const at::Tensor* tensor(PyObject* o) {
@@ -273,12 +277,255 @@ PyObject* f4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------ a step over a paged KV cache
+// A GPU tensor of the type and number of dimensions, its last one contiguous.
+bool strided(const at::Tensor* t, at::ScalarType type, int64_t dim, int idx) {
+  return t && t->is_cuda() && t->scalar_type() == type && t->dim() == dim &&
+         (idx < 0 || t->get_device() == idx) && (t->size(dim - 1) <= 1 || t->stride(dim - 1) == 1);
+}
+
+// Whether the sizes fit the C ABI's ints.
+bool ints(const at::Tensor* t) {
+  for (const int64_t n : t->sizes())
+    if (n > INT_MAX) return false;
+  return true;
+}
+
+long long stride_of(const at::Tensor* t, int64_t d) { return t->size(d) > 1 ? t->stride(d) : 0; }
+
+int activation(at::ScalarType t) {
+  return t == at::kHalf ? DB_DTYPE_F16 : t == at::kBFloat16 ? DB_DTYPE_BF16 : -1;
+}
+
+bool paged_cache(PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso, at::ScalarType act,
+                 int idx, db_paged_cache* c) {
+  const at::Tensor *k = tensor(ko), *v = tensor(vo);
+  if (!k) return false;
+  const at::ScalarType type = k->scalar_type();
+  if (!strided(k, type, 4, idx) || !strided(v, type, 4, idx) || k->sizes() != v->sizes() ||
+      !ints(k))
+    return false;
+  *c = {};
+  if (type == at::kFloat8_e4m3fn) {
+    const at::Tensor *ks = tensor(kso), *vs = tensor(vso);
+    for (const at::Tensor* s : {ks, vs})
+      if (!plain(s, at::kFloat, idx) || s->dim() != 1 || s->size(0) != k->size(1)) return false;
+    c->k_scale = static_cast<const float*>(ks->data_ptr());
+    c->v_scale = static_cast<const float*>(vs->data_ptr());
+    c->dtype = DB_DTYPE_FP8_E4M3;
+  } else {
+    if (type != act || kso != Py_None || vso != Py_None) return false;
+    c->dtype = activation(type);
+  }
+  c->k = k->data_ptr();
+  c->v = v->data_ptr();
+  c->k_page_stride = stride_of(k, 0);
+  c->k_head_stride = stride_of(k, 1);
+  c->k_token_stride = stride_of(k, 2);
+  c->v_page_stride = stride_of(v, 0);
+  c->v_head_stride = stride_of(v, 1);
+  c->v_token_stride = stride_of(v, 2);
+  c->pages = (int)k->size(0);
+  c->Hkv = (int)k->size(1);
+  c->page_size = (int)k->size(2);
+  c->D = (int)k->size(3);
+  return true;
+}
+
+at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, int idx) {
+  return at::empty(sizes, at::TensorOptions().dtype(type).device(
+                              at::Device(at::kCUDA, (c10::DeviceIndex)idx)));
+}
+
+bool integer(PyObject* o, long* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  *v = PyLong_AsLong(o);
+  if (*v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return *v >= 0 && *v <= INT_MAX;
+}
+
+// (past_len, new_len, block_table, free_pages, page_size, n_tokens, free_start or None):
+// (q_start, kv_len, position, slot, free_next)
+PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  const at::Tensor *past = tensor(a[0]), *fresh = tensor(a[1]), *table = tensor(a[2]),
+                   *pages = tensor(a[3]);
+  long page = 0, T = 0;
+  if (!plain(past, at::kInt, -1) || !integer(a[4], &page) || !integer(a[5], &T)) Py_RETURN_NONE;
+  const int idx = past->get_device();
+  if (!plain(fresh, at::kInt, idx) || !plain(pages, at::kInt, idx) ||
+      !strided(table, at::kInt, 2, idx) || !ints(table) || pages->dim() != 1 || !ints(pages))
+    Py_RETURN_NONE;
+  const int64_t R = table->size(0), width = table->size(1);
+  if (past->dim() != 1 || past->size(0) != R || fresh->dim() != 1 || fresh->size(0) != R ||
+      (R > 1 && table->stride(0) < width))
+    Py_RETURN_NONE;
+  const int* start = nullptr;
+  if (a[6] != Py_None) {
+    const at::Tensor* t = tensor(a[6]);
+    if (!plain(t, at::kInt, idx) || t->numel() != 1) Py_RETURN_NONE;
+    start = static_cast<const int*>(t->data_ptr());
+  }
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  at::Tensor out[5] = {empty_on({R + 1}, at::kInt, idx), empty_on({R}, at::kInt, idx),
+                       empty_on({T}, at::kInt, idx), empty_on({T}, at::kLong, idx),
+                       empty_on({1}, at::kInt, idx)};
+  const int *pp = static_cast<const int*>(past->data_ptr()),
+            *np = static_cast<const int*>(fresh->data_ptr()),
+            *fp = static_cast<const int*>(pages->data_ptr());
+  int* tp = static_cast<int*>(table->data_ptr());
+  const long long row = R > 1 ? table->stride(0) : width;
+  const int count = (int)pages->numel();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.paged_plan(pp, np, tp, row, (int)width, fp, count, start, (int)page, (int)R, (int)T,
+                      static_cast<int*>(out[0].data_ptr()), static_cast<int*>(out[1].data_ptr()),
+                      static_cast<int*>(out[2].data_ptr()),
+                      static_cast<long long*>(out[3].data_ptr()),
+                      static_cast<int*>(out[4].data_ptr()), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(5);
+  if (!result) return nullptr;
+  for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(out[i]));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// (qkv, position, slot, K, V, inv_freq, axes as bytes or None, interleaved, k_scale, v_scale)
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) Py_RETURN_NONE;
+  const at::Tensor *qkv = tensor(a[0]), *pos = tensor(a[1]), *slot = tensor(a[2]),
+                   *freq = tensor(a[5]);
+  if (!qkv || activation(qkv->scalar_type()) < 0 || !PyBool_Check(a[7])) Py_RETURN_NONE;
+  const at::ScalarType type = qkv->scalar_type();
+  if (!strided(qkv, type, 2, -1) || !ints(qkv)) Py_RETURN_NONE;
+  const int idx = qkv->get_device();
+  db_paged_cache cache;
+  if (!paged_cache(a[3], a[4], a[8], a[9], type, idx, &cache) || cache.D < 1) Py_RETURN_NONE;
+  const int64_t T = qkv->size(0), Hq = qkv->size(1) / cache.D - 2ll * cache.Hkv;
+  if (Hq < 1 || (Hq + 2ll * cache.Hkv) * cache.D != qkv->size(1) || !plain(pos, at::kInt, idx) ||
+      !plain(slot, at::kLong, idx) || !plain(freq, at::kFloat, idx) || pos->dim() < 1 ||
+      pos->dim() > 2 || pos->size(pos->dim() - 1) != T || slot->dim() != 1 || slot->size(0) != T ||
+      freq->dim() != 1 || freq->size(0) > 128)
+    Py_RETURN_NONE;
+  const int64_t axes = pos->dim() == 1 ? 1 : pos->size(0);
+  if (axes < 1 || axes > 4) Py_RETURN_NONE;
+  const unsigned char* map = nullptr;
+  if (a[6] != Py_None) {
+    if (!PyBytes_CheckExact(a[6]) || PyBytes_GET_SIZE(a[6]) != freq->size(0)) Py_RETURN_NONE;
+    map = reinterpret_cast<const unsigned char*>(PyBytes_AS_STRING(a[6]));
+  } else if (axes != 1) {
+    Py_RETURN_NONE;
+  }
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  at::Tensor q = empty_on({T, Hq, cache.D}, type, idx);
+  const void* xp = qkv->data_ptr();
+  const long long row = T > 1 ? qkv->stride(0) : qkv->size(1);
+  const int* pp = static_cast<const int*>(pos->data_ptr());
+  const long long* sp = static_cast<const long long*>(slot->data_ptr());
+  const float* fp = static_cast<const float*>(freq->data_ptr());
+  const int rot = 2 * (int)freq->size(0), inter = a[7] == Py_True;
+  void* qp = q.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.rope_append(xp, row, pp, (int)axes, map, sp, fp, rot, inter, &cache, qp, (int)T,
+                       (int)Hq, activation(type), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(q);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, K, V, block_table, q_start, kv_len, scale or None, causal, window or None,
+//  max_new or None, k_scale, v_scale): with a workspace that needs tickets outside
+// capture only, and already in the cache.
+PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(a[0]), *table = tensor(a[3]), *start = tensor(a[4]),
+                   *len = tensor(a[5]);
+  if (!q || activation(q->scalar_type()) < 0 || !PyBool_Check(a[7])) Py_RETURN_NONE;
+  const at::ScalarType type = q->scalar_type();
+  if (!strided(q, type, 3, -1) || !ints(q)) Py_RETURN_NONE;
+  const int idx = q->get_device();
+  db_paged_cache cache;
+  if (!paged_cache(a[1], a[2], a[10], a[11], type, idx, &cache)) Py_RETURN_NONE;
+  const int64_t T = q->size(0), Hq = q->size(1), D = q->size(2);
+  if (D != cache.D || D < 1 || !strided(table, at::kInt, 2, idx) || !ints(table) ||
+      !plain(start, at::kInt, idx) || !plain(len, at::kInt, idx))
+    Py_RETURN_NONE;
+  const int64_t R = table->size(0), width = table->size(1);
+  if (start->dim() != 1 || start->size(0) != R + 1 || len->dim() != 1 || len->size(0) != R)
+    Py_RETURN_NONE;
+  double scale = 1.0 / std::sqrt((double)D);
+  long window = 0, most = T;
+  if ((a[6] != Py_None && !number(a[6], &scale)) ||
+      (a[8] != Py_None && (!integer(a[8], &window) || window < 1)) ||
+      (a[9] != Py_None && (!integer(a[9], &most) || most < 1)))
+    Py_RETURN_NONE;
+  if (most > T) most = T;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  size_t zeroed = 0;
+  const size_t bytes = abi.paged_workspace_bytes((int)T, (int)Hq, cache.Hkv, (int)D, (int)R,
+                                                 (int)most, &zeroed);
+  if (bytes == 0) Py_RETURN_NONE;
+  at::Tensor ws;  // keeps the workspace alive through the call
+  if (zeroed > 0) {
+    unsigned long long capture = 0;
+    if (abi.capture_id(stream, &capture) != DB_OK || capture != 0) Py_RETURN_NONE;
+    PyObject* key = Py_BuildValue("(siKn)", "paged", idx, (unsigned long long)(uintptr_t)stream,
+                                  (Py_ssize_t)bytes);
+    PyObject* hit = key ? PyDict_GetItemWithError(workspaces, key) : nullptr;  // borrowed
+    Py_XDECREF(key);
+    const at::Tensor* t = hit ? tensor(hit) : nullptr;
+    if (!t) {
+      if (PyErr_Occurred()) return nullptr;
+      Py_RETURN_NONE;
+    }
+    ws = *t;
+  } else {
+    ws = empty_on({(int64_t)bytes}, at::kByte, idx);
+  }
+  at::Tensor o = empty_on({T, Hq, D}, type, idx);
+  const void* qp = q->data_ptr();
+  const long long qt = stride_of(q, 0), qh = stride_of(q, 1), row = stride_of(table, 0);
+  const int *tp = static_cast<const int*>(table->data_ptr()),
+            *sp = static_cast<const int*>(start->data_ptr()),
+            *lp = static_cast<const int*>(len->data_ptr());
+  void *op = o.data_ptr(), *wp = ws.data_ptr();
+  const int causal = a[7] == Py_True;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.paged_attention(qp, qt, qh, op, &cache, tp, row, (int)width, sp, lp, (int)T, (int)R,
+                           (int)Hq, (int)most, (float)scale, causal, (int)window,
+                           activation(type), wp, bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
 // (entry point addresses, raw_stream, get_device, workspaces, cu_counts)
 PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long p[10];
+  unsigned long long p[14];
   PyObject *rs, *gd, *ws, *cu;
-  if (!PyArg_ParseTuple(args, "(KKKKKKKKKK)OOO!O!", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6],
-                        &p[7], &p[8], &p[9], &rs, &gd, &PyDict_Type, &ws, &PyDict_Type, &cu))
+  if (!PyArg_ParseTuple(args, "(KKKKKKKKKKKKKK)OOO!O!", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6],
+                        &p[7], &p[8], &p[9], &p[10], &p[11], &p[12], &p[13], &rs, &gd, &PyDict_Type, &ws, &PyDict_Type, &cu))
     return nullptr;
   abi.f1 = reinterpret_cast<decltype(abi.f1)>((uintptr_t)p[0]);
   abi.f2 = reinterpret_cast<decltype(abi.f2)>((uintptr_t)p[1]);
@@ -290,6 +537,11 @@ PyObject* init(PyObject*, PyObject* args) {
   abi.capture_id = reinterpret_cast<decltype(abi.capture_id)>((uintptr_t)p[7]);
   abi.gemv_workspace_bytes = reinterpret_cast<decltype(abi.gemv_workspace_bytes)>((uintptr_t)p[8]);
   abi.gemv_ws = reinterpret_cast<decltype(abi.gemv_ws)>((uintptr_t)p[9]);
+  abi.paged_plan = reinterpret_cast<decltype(abi.paged_plan)>((uintptr_t)p[10]);
+  abi.rope_append = reinterpret_cast<decltype(abi.rope_append)>((uintptr_t)p[11]);
+  abi.paged_workspace_bytes =
+      reinterpret_cast<decltype(abi.paged_workspace_bytes)>((uintptr_t)p[12]);
+  abi.paged_attention = reinterpret_cast<decltype(abi.paged_attention)>((uintptr_t)p[13]);
   Py_INCREF(rs);
   Py_INCREF(gd);
   Py_INCREF(ws);
@@ -313,6 +565,9 @@ PyMethodDef methods[] = {
     {"f2", fast<f2>(), METH_FASTCALL, nullptr},
     {"f2n", fast<f2n>(), METH_FASTCALL, nullptr},
     {"f4", fast<f4>(), METH_FASTCALL, nullptr},
+    {"plan", fast<plan>(), METH_FASTCALL, nullptr},
+    {"rope", fast<rope>(), METH_FASTCALL, nullptr},
+    {"paged", fast<paged>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -151,7 +151,8 @@ def _load_fast(lib) -> None:
     entry = tuple(C.cast(getattr(lib, name), C.c_void_p).value for name in (
         "db_f1_rmsnorm_gemv", "db_f2_gateup_swiglu", "db_f2_rmsnorm_gateup_swiglu", "db_gemv",
         "db_f4_default_splits", "db_f4_workspace_bytes", "db_f4_splitkv",
-        "db_stream_capture_id", "db_gemv_workspace_bytes", "db_gemv_ws"))
+        "db_stream_capture_id", "db_gemv_workspace_bytes", "db_gemv_ws", "db_paged_plan",
+        "db_rope_append", "db_paged_attention_workspace_bytes", "db_paged_attention"))
     mod.init(entry, _raw_stream, get_device, _ws_cache, _cu_cache)
     _fast = mod
 
@@ -718,6 +719,10 @@ def paged_plan(past_len, new_len, block_table, free_pages, page_size: int, n_tok
     room for: rows behind the last token get slot -1, tokens beyond them are
     left out of ``kv_len``.  Where pages run out (``free_next`` > F) or a
     request outgrows its table row, the tokens concerned get slot -1."""
+    if _fast is not None:
+        p = _fast.plan(past_len, new_len, block_table, free_pages, page_size, n_tokens, free_start)
+        if p is not None:
+            return PagedPlan(*p)
     torch = _torch or _torch_mod()
     i32 = torch.int32
     idx = _gpu_tensors((past_len, "past_len", i32), (new_len, "new_len", i32),
@@ -738,11 +743,11 @@ def paged_plan(past_len, new_len, block_table, free_pages, page_size: int, n_tok
     if T < 0:
         raise ValueError(f"n_tokens must be >= 0 (got {T})")
     dev = past_len.device
-    # one allocation: slot first, the only one of 8 bytes
-    rows = torch.empty(2 * T + T + 2 * R + 2, dtype=i32, device=dev)
-    slot, position = rows[:2 * T].view(torch.int64), rows[2 * T:3 * T]
-    q_start, kv_len = rows[3 * T:3 * T + R + 1], rows[3 * T + R + 1:3 * T + 2 * R + 1]
-    free_next = rows[3 * T + 2 * R + 1:]
+    q_start = torch.empty(R + 1, dtype=i32, device=dev)
+    kv_len = torch.empty(R, dtype=i32, device=dev)
+    position = torch.empty(T, dtype=i32, device=dev)
+    slot = torch.empty(T, dtype=torch.int64, device=dev)
+    free_next = torch.empty(1, dtype=i32, device=dev)
     _launch((_lib or load_library()).db_paged_plan, idx, "db_paged_plan", past_len.data_ptr(),
             new_len.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), width), width,
             free_pages.data_ptr(), free_pages.numel(),
@@ -769,6 +774,12 @@ def rope_append(qkv, position, slot, K, V, inv_freq, axes=None, interleaved: boo
     2i and 2i+1 where ``interleaved``.  position is int32 [T], or [A, T] for
     tokens with A axes (time, height, width): ``axes`` then names the axis of
     each pair, e.g. ``[0] * 16 + [1] * 24 + [2] * 24``."""
+    axis_map = None if axes is None else bytes(axes)
+    if out is None and _fast is not None:
+        q = _fast.rope(qkv, position, slot, K, V, inv_freq, axis_map, interleaved, k_scale,
+                       v_scale)
+        if q is not None:
+            return q
     torch = _torch or _torch_mod()
     idx = _strided(qkv, "qkv", None, 2)
     dt = _activation(qkv, "qkv")
@@ -785,9 +796,7 @@ def rope_append(qkv, position, slot, K, V, inv_freq, axes=None, interleaved: boo
                          f"have one entry for each of the {T} rows of qkv")
     if inv_freq.dim() != 1:
         raise ValueError(f"inv_freq must be [rot / 2] (got {tuple(inv_freq.shape)})")
-    axis_map = None
-    if axes is not None:
-        axis_map = bytes(axes)
+    if axis_map is not None:
         if len(axis_map) != inv_freq.numel():
             raise ValueError(f"axes has {len(axis_map)} entries for {inv_freq.numel()} pairs")
     elif n_axes != 1:
@@ -819,6 +828,11 @@ def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None =
     ``max_new`` is the most new tokens a request has, where the caller knows it
     (1 in a plain decode step): it spares the kernels that such a call does not
     need, and nothing else."""
+    if out is None and _fast is not None:
+        o = _fast.paged(q, K, V, block_table, q_start, kv_len, scale, causal, window, max_new,
+                        k_scale, v_scale)
+        if o is not None:
+            return o
     torch = _torch or _torch_mod()
     idx = _strided(q, "q", None, 3)
     dt = _activation(q, "q")

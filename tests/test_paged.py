@@ -717,6 +717,52 @@ def test_calls_at_once_on_two_streams():
         assert all(torch.equal(o, w) for o in outs)
 
 
+@pytest.mark.gpu
+def test_native_call_path_and_python_steps_agree(monkeypatch):
+    """The native call path takes these calls, and the Python steps give the same."""
+    freq = (10000.0 ** (-torch.arange(0, 64, 2) / 64)).to(DEV)
+
+    def step(fp8, wide):
+        gen = torch.Generator().manual_seed(7)
+        K, V, ks, vs = cache_pair(gen, 40, 2, 16, 64, FP8 if fp8 else torch.bfloat16, "tokens")
+        table = torch.full((3, 9), -1, dtype=torch.int32, device=DEV)[:, :8]
+        free = torch.arange(40, dtype=torch.int32, device=DEV)
+        p = ops.paged_plan(ints([0, 0, 0]), ints([30, 1, wide]), table, free, 16, 31 + wide,
+                           free_start=ints([2]))
+        qkv = torch.randn(31 + wide, 8 * 64, generator=gen).bfloat16().to(DEV)
+        q = ops.rope_append(qkv, torch.stack([p.position, p.position + 3]), p.slot, K, V, freq,
+                            axes=[0] * 10 + [1] * 22, interleaved=fp8, k_scale=ks, v_scale=vs)
+        o = [ops.paged_attention(q, K, V, table, p.q_start, p.kv_len, k_scale=ks, v_scale=vs, **kw)
+             for kw in ({}, dict(max_new=30, window=9), dict(causal=False, scale=0.2),
+                        dict(max_new=1))]
+        return [*p, q, K.view(torch.uint8) if fp8 else K, V.view(torch.uint8) if fp8 else V, *o]
+
+    assert ops._fast is not None
+    for fp8, wide in ((False, 1), (True, 70)):
+        step(fp8, wide)                                  # makes the workspaces
+        calls = []
+        with monkeypatch.context() as m:
+            class Watch:
+                def __getattr__(self, name):
+                    fn = getattr(fast, name)
+
+                    def call(*args):
+                        r = fn(*args)
+                        calls.append((name, r is not None))
+                        return r
+                    return call
+
+            fast = ops._fast
+            m.setattr(ops, "_fast", Watch())
+            native = step(fp8, wide)
+        assert len(calls) == 6 and all(took for _, took in calls), calls
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_fast", None)
+            steps = step(fp8, wide)
+        for a, b in zip(native, steps):
+            assert a.dtype == b.dtype and torch.equal(a, b)
+
+
 # ------------------------------------------------------------------- refusals
 P = 0x10000  # a fake, aligned device address: never dereferenced
 
