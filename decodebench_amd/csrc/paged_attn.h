@@ -25,8 +25,8 @@
 //
 // A split writes its running maximum, exp-sum and unnormalised output as an
 // fp32 record; paged_merge joins the records of a row.  There are fewer
-// than 2 `target` records: only requests of at least 1.5 C tiles split, into
-// at most 4/3 tmax / C parts, and C >= (all tiles) / target.
+// than 2 `target` records: only requests of at least 1.75 C tiles split, into
+// at most 8/7 tmax / C parts, and C >= (all tiles) / target.
 #pragma once
 
 #include "db_device.h"
@@ -260,9 +260,9 @@ struct PagedSchedule {
   }
 
   __device__ int splits_of(const PagedRequest& q) const {
-    // to the nearest: ceil would run 192 row tiles of 80 key tiles on 256 CUs
-    // (C = 60) as 384 halves, no sooner done and all of them to be merged
-    return q.row_tiles == 0 ? 0 : max(1, (int)((2ll * q.tiles + C) / (2ll * C)));
+    // Two splits only for work worth nearly two parts: halves of 192 row tiles of 80
+    // key tiles on 256 CUs (C = 60) are no sooner done, and cost a merge.
+    return q.row_tiles == 0 ? 0 : max(1, (int)((4ll * q.tiles + C) / (4ll * C)));
   }
   __device__ void scan() {
     splits = splits_of(mine);

@@ -49,7 +49,9 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
   constexpr int LPR = D * CB / 16;                 // lanes per row
   constexpr int RPI = kWave / LPR;                 // rows a load instruction
   constexpr int NL = RW > RPI ? RW / RPI : 1;      // loads of K (and of V) a lane
-  constexpr int KS = D + 8, VS = D + 16;           // row strides in LDS (elements)
+  // Row strides in LDS (elements): 16 rows of a K read, and the four rows of 64
+  // bytes that half a wave takes in a transposing read of V, lie in different banks.
+  constexpr int KS = D + 8, VS = D + 32;
   constexpr int QSTEPS = D / 16, NB = D / 32;
 
   __shared__ __align__(16) elem s_k[2][KT * KS];
@@ -410,6 +412,52 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
 // rows in two splits.)  The groups' count and places come from the first kernel.
 constexpr int kMergeWaves = 16;
 
+// Rows row .. row + ROWS - 1 (below `end`) of a row tile of up to SPLITS splits, by
+// one wave with all their records in flight.
+template <class E, int D, int ROWS, int SPLITS>
+__device__ __forceinline__ void merge_rows(const PagedArgs& a, const int* d, int mt, int row,
+                                           int end, int splits, int rec0, int head) {
+  constexpr int PER = D / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  float2 ml[ROWS][SPLITS];
+  float v[ROWS][SPLITS][PER];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int s = 0; s < SPLITS; ++s) {
+      const size_t at = (size_t)(rec0 + min(s, splits - 1) * a.Hkv) * mt + min(row + r, end - 1);
+      ml[r][s] = a.rec.ml[at];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[r][s][i] = a.rec.opart[at * D + lane * PER + i];
+    }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    float M = kPagedNegInf, L = 0.0f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < SPLITS; ++s)
+      if (s < splits && ml[r][s].y != 0.0f) M = fmaxf(M, ml[r][s].x);  // else: saw nothing
+#pragma unroll
+    for (int s = 0; s < SPLITS; ++s) {
+      if (s >= splits || ml[r][s].y == 0.0f) continue;
+      const float w = fast_exp2(ml[r][s].x - M);
+      L = fmaf(w, ml[r][s].y, L);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, v[r][s][i], acc[i]);
+    }
+    if (row + r < end) {
+      const int xr = d[3] + row + r;
+      typename E::type* op =
+          static_cast<typename E::type*>(a.o) +
+          ((size_t)(d[2] + xr / a.G) * a.Hq + head * a.G + xr % a.G) * D + lane * PER;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        op[i] = (typename E::type)(L == 0.0f ? 0.0f : acc[i] / L);
+    }
+  }
+}
+
 template <class E, int D>
 __global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, int mt) {
   typedef typename E::type elem;
@@ -418,14 +466,26 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, 
   __shared__ float s_acc[kMergeWaves][D], s_m[kMergeWaves], s_l[kMergeWaves];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int parts = mt / kMergeWaves;
-  const int total = min(a.rec.head[0], a.rec.groups) * parts;
+  // Rows of a workgroup's piece: 64 where that makes a piece for each workgroup.
+  const int groups = min(a.rec.head[0], a.rec.groups);
+  const int part = groups * (mt / 64) >= (int)gridDim.x ? 64 : 16;
+  const int parts = mt / part, total = groups * parts;
   for (int task = blockIdx.x; task < total; task += gridDim.x) {
     const int group = task / parts;
     const int* d = a.rec.desc + (size_t)group * kDescInts;
     const int splits = d[0], rec0 = d[1], head = rec0 % a.Hkv;
     if (rec0 + (splits - 1) * a.Hkv >= a.rec.records) continue;
-    const int first = task % parts * kMergeWaves, rows = min(d[4] - first, kMergeWaves);
+    const int first = task % parts * part, rows = min(d[4] - first, part);
+    if (splits <= 2) {
+      for (int r0 = wave * 4; r0 < rows; r0 += 4 * kMergeWaves)
+        merge_rows<E, D, 4, 2>(a, d, mt, first + r0, first + rows, splits, rec0, head);
+      continue;
+    }
+    if (splits <= 4) {
+      for (int r0 = wave * 2; r0 < rows; r0 += 2 * kMergeWaves)
+        merge_rows<E, D, 2, 4>(a, d, mt, first + r0, first + rows, splits, rec0, head);
+      continue;
+    }
     const int share = splits <= 8 ? 1 : splits <= 16 ? 2 : 4;  // waves of a row
     for (int r0 = 0; r0 < rows; r0 += kMergeWaves / share) {
       const int sub = r0 + wave / share, row = first + min(sub, rows - 1);
