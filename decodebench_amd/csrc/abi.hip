@@ -494,6 +494,8 @@ int check_cache(const char* fn, const db_paged_cache* c, int dtype) {
   return DB_OK;
 }
 
+constexpr int kMostRows = 1 << 30;  // of a plan: its row numbers stay within an int
+
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 dbk::PagedCall paged_bounds(int T, int Hq, int Hkv, int D, int R, int max_new) {
@@ -524,6 +526,8 @@ int db_paged_plan(const int* past, const int* fresh, int* table, long long table
                 "%s: need width >= 1, page_size >= 1 and table rows of at least width entries "
                 "(got %d %d %lld)",
                 fn, width, page_size, table_stride);
+  if (R > kMostRows || T > kMostRows || free_count > kMostRows)
+    return fail(DB_ERR_INVALID, "%s: R, T or free_count above %d", fn, kMostRows);
   if (!q_start || !free_next || (R > 0 && (!past || !fresh || !table || !kv_len)) ||
       (T > 0 && (!position || !slot)) || (free_count > 0 && !free_pages))
     return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
@@ -561,6 +565,12 @@ int db_rope_append(const void* qkv, long long qkv_stride, const int* position, i
   if (qkv_stride < ((long long)Hq + 2ll * cache->Hkv) * D || qkv_stride % 8 != 0)
     return fail(DB_ERR_INVALID, "%s: qkv rows must hold (Hq + 2 Hkv) D elements and be 16-byte "
                 "aligned", fn);
+  if (T >= 1 << 26) return fail(DB_ERR_INVALID, "%s: T=%d must be below 2^26", fn, T);
+  const db_paged_cache& kv = *cache;
+  if ((kv.pages > 1 && (!kv.k_page_stride || !kv.v_page_stride)) ||
+      (kv.Hkv > 1 && (!kv.k_head_stride || !kv.v_head_stride)) ||
+      (kv.page_size > 1 && (!kv.k_token_stride || !kv.v_token_stride)))
+    return fail(DB_ERR_INVALID, "%s: the cache is written, its rows must not share memory", fn);
   if (T == 0) return ok();
   if (!qkv || !position || !slot || !inv_freq || !q)
     return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
@@ -625,12 +635,12 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
     return fail(DB_ERR_INVALID, "%s: need T, R, max_new >= 0 and Hq >= 1", fn);
   if (Hq % cache->Hkv != 0)
     return fail(DB_ERR_INVALID, "%s: Hq=%d is not a multiple of Hkv=%d", fn, Hq, cache->Hkv);
-  if ((long long)T * Hq >= (1ll << 31) || (long long)R * cache->Hkv >= (1ll << 24))
+  if ((long long)T * Hq >= (1ll << 30) || (long long)R * cache->Hkv >= (1ll << 22))
     return fail(DB_ERR_INVALID, "%s: T * Hq or R * Hkv is too large", fn);
   // Key tiles that the work of a KV head may come to.
   const long long G = Hq / cache->Hkv, held = (long long)width * cache->page_size / 16 + 1;
   const long long most = max_new > 0 && max_new < T ? max_new : T;
-  if (held >= (1ll << 31) || (most * G <= 16 ? T * G / 16 + R : R) * held >= (1ll << 31))
+  if (held >= (1ll << 30) || (most * G <= 16 ? T * G / 16 + R : R) * held >= (1ll << 30))
     return fail(DB_ERR_INVALID, "%s: R * width * page_size is too large", fn);
   if (!(scale > 0.0f) || !isfinite(scale))
     return fail(DB_ERR_INVALID, "%s: scale must be finite and > 0", fn);

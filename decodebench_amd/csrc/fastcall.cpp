@@ -500,7 +500,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (zeroed > 0) {
     unsigned long long capture = 0;
     if (abi.capture_id(stream, &capture) != DB_OK || capture != 0) Py_RETURN_NONE;
-    PyObject* key = Py_BuildValue("(siKn)", "paged", idx, (unsigned long long)(uintptr_t)stream,
+    PyObject* key = Py_BuildValue("(sKiKn)", "paged", (unsigned long long)zeroed, idx, (unsigned long long)(uintptr_t)stream,
                                   (Py_ssize_t)bytes);
     PyObject* hit = key ? PyDict_GetItemWithError(workspaces, key) : nullptr;  // borrowed
     Py_XDECREF(key);

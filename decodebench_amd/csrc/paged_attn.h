@@ -165,6 +165,11 @@ __device__ __forceinline__ int paged_limit(const PagedArgs& a, int len) {
   return (int)min((long long)min(len, 0x7FFFF000), held);
 }
 
+// The first key that a token at `pos` sees (a window may be as long as an int holds).
+__device__ __forceinline__ int first_seen(const PagedArgs& a, int pos) {
+  return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
 template <int MT, int KT>
 __device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r) {
   PagedRequest q = {0, 0, 0, 0, 0};
@@ -285,6 +290,7 @@ struct PagedSchedule {
     }
     const int at0 = unit - units0;
     const unsigned long long hit = __ballot(at0 >= before && at0 - before < units);
+    if (!hit) return false;  // sums out of range: q_start is not ascending
     const int who = __builtin_ctzll(hit);
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
     work.req.tok0 = of(mine.tok0);
@@ -322,7 +328,7 @@ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedWork&
   const int i1 = (int)min((row0 + MT - 1) / a.G, (long long)q.n - 1);
   const int past = q.len - q.n;
   const int hi = a.causal ? min(limit, past + i1 + 1) : limit;
-  const int lo = a.window > 0 ? max(past + i0 - a.window + 1, 0) : 0;
+  const int lo = first_seen(a, past + i0);
   int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
   const int per = (t1 - t0 + wk.splits - 1) / wk.splits;
   first = min(t0 + wk.split * per, t1);

@@ -129,20 +129,19 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
     }
     const int past = rq.len - rq.n;
     const int khi = !live ? 0 : a.causal ? min(limit, past + token + 1) : limit;
-    const int klo = !live ? 0x7FFFFFFF : a.window > 0 ? max(past + token - a.window + 1, 0) : 0;
+    const int klo = !live ? 0x7FFFFFFF : first_seen(a, past + token);
     // Keys that every row of the workgroup sees (wg_), that every live row of
     // the wave sees (all_) and that any of them sees (any_), from its first and
     // last live row (none: nothing at all).
     const int wg_hi = a.causal ? min(limit, past + (wk.tile * MT) / a.G + 1) : limit;
-    const int wg_lo =
-        a.window > 0 ? max(past + (wk.tile * MT + rows - 1) / a.G - a.window + 1, 0) : 0;
+    const int wg_lo = first_seen(a, past + (wk.tile * MT + rows - 1) / a.G);
     const bool any = wave * 32 < rows;
     const int i0 = (wk.tile * MT + min(wave * 32, rows - 1)) / a.G;
     const int i1 = (wk.tile * MT + min(wave * 32 + 31, rows - 1)) / a.G;
     const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
     const int any_hi = !any ? 0 : a.causal ? min(limit, past + i1 + 1) : limit;
-    const int all_lo = a.window > 0 ? max(past + i1 - a.window + 1, 0) : 0;
-    const int any_lo = a.window > 0 ? max(past + i0 - a.window + 1, 0) : 0;
+    const int all_lo = first_seen(a, past + i1);
+    const int any_lo = first_seen(a, past + i0);
     const float scale = a.scale_log2 * (FP8 ? a.k_scale[wk.head] : 1.0f);
 
     // ---- tiles to registers and to LDS -------------------------------------

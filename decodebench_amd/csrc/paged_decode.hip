@@ -75,7 +75,7 @@ __device__ __forceinline__ DecodeRequest decode_request(const PagedArgs& a, int 
   if (q.n == 0) return q;
   q.row_tiles = (rows + MT - 1) / MT;
   const int limit = paged_limit(a, q.len);
-  q.t0 = a.window > 0 ? min(max(q.len - q.n - a.window + 1, 0), limit) / KT : 0;
+  q.t0 = min(first_seen(a, q.len - q.n), limit) / KT;
   q.tiles = max((limit + KT - 1) / KT - q.t0, 1);
   return q;
 }
@@ -108,21 +108,27 @@ struct DecodeLine {
     all = __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   // The item at `at`: its request (lane `who` of the round), row tile and the
-  // tile within it.  Positions only grow.
-  __device__ void locate(int at, int& who, int& row_tile, int& tile) {
+  // tile within it.  Positions only grow.  False where the sums went out of range
+  // (a q_start that is not ascending counts rows more than once).
+  __device__ bool locate(int at, int& who, int& row_tile, int& tile) {
     while (at >= before + all) {
+      if ((round + 1) * kWave >= a.R) return false;
       before += all;
       ++round;
       mine = decode_request<KT>(a, round * kWave + (int)(threadIdx.x & (kWave - 1)));
       scan();
     }
     const int in = at - before;
-    who = __builtin_ctzll(__ballot(in < upto));
+    const unsigned long long hit = __ballot(in < upto);
+    if (!hit) return false;
+    who = __builtin_ctzll(hit);
     const int tiles = __builtin_amdgcn_readlane(mine.tiles, who);
     const int rts = __builtin_amdgcn_readlane(mine.row_tiles, who);
     const int off = in - (__builtin_amdgcn_readlane(upto, who) - tiles * rts);
+    if (off < 0 || off >= tiles * rts) return false;
     row_tile = rts == 1 ? 0 : off / tiles;
     tile = off - row_tile * tiles;
+    return true;
   }
 };
 
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
     if (!once) __syncthreads();  // the region is read: the next piece may write it
     DecodeRequest rq;
     int who, row_tile, tile_in;
-    line.locate(begin, who, row_tile, tile_in);
+    if (!line.locate(begin, who, row_tile, tile_in)) break;
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
     rq.tok0 = of(line.mine.tok0);
     rq.n = of(line.mine.n);
@@ -318,11 +324,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
     if constexpr (ALIGNED) hold(0);
     const int past = rq.len - rq.n;
     const int khi = a.causal ? min(limit, past + token + 1) : limit;
-    const int klo = a.window > 0 ? max(past + token - a.window + 1, 0) : 0;
+    const int klo = first_seen(a, past + token);
     // Keys that every row sees: the first row's end, the last row's beginning.
     const int i0 = row_tile * MT / a.G, i1 = (row_tile * MT + rows - 1) / a.G;
     const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
-    const int all_lo = a.window > 0 ? max(past + i1 - a.window + 1, 0) : 0;
+    const int all_lo = first_seen(a, past + i1);
     const float scale = a.scale_log2 * (FP8 ? a.k_scale[head] : 1.0f);
 
     f4 o[NB];

@@ -631,6 +631,9 @@ class PagedPlan(NamedTuple):
     free_next: object  # int32 [1]: where in free_pages the next step's pages begin
 
 
+_INT_MAX = 2 ** 31 - 1  # the C ABI's sizes are ints
+
+
 def _strided(t, name: str, dt, dim: int):
     """Check a GPU tensor of ``dim`` dimensions whose last one is contiguous;
     returns its GPU's index."""
@@ -645,6 +648,8 @@ def _strided(t, name: str, dt, dim: int):
         raise ValueError(f"{name} must have {dim} dimensions (got {tuple(t.shape)})")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
+    if max(t.shape) > _INT_MAX:
+        raise ValueError(f"{name} {tuple(t.shape)} has a dimension of 2^31 or more")
     return t.get_device()
 
 
@@ -739,9 +744,13 @@ def paged_plan(past_len, new_len, block_table, free_pages, page_size: int, n_tok
         raise ValueError("free_start must have one element")
     if R > 1 and block_table.stride(0) < width:
         raise ValueError("block_table rows must not overlap")
-    T = int(n_tokens)
-    if T < 0:
-        raise ValueError(f"n_tokens must be >= 0 (got {T})")
+    T, page = int(n_tokens), int(page_size)
+    if not 0 <= T <= _INT_MAX:
+        raise ValueError(f"n_tokens must be >= 0 and below 2^31 (got {T})")
+    if not 1 <= page <= _INT_MAX:
+        raise ValueError(f"page_size must be >= 1 and below 2^31 (got {page})")
+    if free_pages.numel() > _INT_MAX:
+        raise ValueError(f"free_pages has {free_pages.numel()} entries, 2^31 or more")
     dev = past_len.device
     q_start = torch.empty(R + 1, dtype=i32, device=dev)
     kv_len = torch.empty(R, dtype=i32, device=dev)
@@ -751,7 +760,7 @@ def paged_plan(past_len, new_len, block_table, free_pages, page_size: int, n_tok
     _launch((_lib or load_library()).db_paged_plan, idx, "db_paged_plan", past_len.data_ptr(),
             new_len.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), width), width,
             free_pages.data_ptr(), free_pages.numel(),
-            None if free_start is None else free_start.data_ptr(), int(page_size), R, T,
+            None if free_start is None else free_start.data_ptr(), page, R, T,
             q_start.data_ptr(), kv_len.data_ptr(), position.data_ptr(), slot.data_ptr(),
             free_next.data_ptr())
     return PagedPlan(q_start, kv_len, position, slot, free_next)
@@ -862,10 +871,11 @@ def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None =
         # Tickets that start at zero are kept as F4's are; otherwise nothing in the
         # workspace outlives the call, and torch's allocator hands it out anew.
         if zeroed.value:
-            ws = _kept_workspace(("paged",), nbytes, zeroed.value, idx)
+            ws = _kept_workspace(("paged", zeroed.value), nbytes, zeroed.value, idx)
         else:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _launch(lib.db_paged_attention, idx, "db_paged_attention", q.data_ptr(), *_strides(q, 2),
-            o.data_ptr(), C.byref(cache), block_table.data_ptr(), *_strides(block_table, 1), width, q_start.data_ptr(), kv_len.data_ptr(), T, R,
-            Hq, most, scale, bool(causal), int(window or 0), dt, ws.data_ptr(), nbytes)
+            o.data_ptr(), C.byref(cache), block_table.data_ptr(), *_strides(block_table, 1), width,
+            q_start.data_ptr(), kv_len.data_ptr(), T, R, Hq, most, scale, bool(causal),
+            min(int(window or 0), _INT_MAX), dt, ws.data_ptr(), nbytes)
     return o

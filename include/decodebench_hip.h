@@ -229,7 +229,7 @@ typedef struct db_paged_cache {
  * step's pages begin.  More than free_count says that pages ran out: entries
  * without a page get -1, tokens without one slot -1, as tokens past the
  * table's width.  Rows behind the last token get position 0 and slot -1.
- * Contract: R >= 0, T >= 0, width >= 1, page_size >= 1, free_count >= 0;
+ * Contract: R, T and free_count in [0, 2^30], width >= 1, page_size >= 1;
  * outputs overlap no input. */
 int db_paged_plan(const int* past, const int* fresh, int* table, long long table_stride,
                   int width, const int* free_pages, int free_count, const int* free_start,
@@ -247,9 +247,10 @@ int db_paged_plan(const int* past, const int* fresh, int* table, long long table
  * a slot outside the cache writes nothing.  Slots of one call must differ:
  * what two tokens write to one slot is either's, 16 bytes at a time.
  * e4m3: round(clamp(x / scale[head], -448, 448)).
- * Contract: T >= 0, Hq >= 1, D a multiple of 16 up to 256, rot a multiple of
+ * Contract: 0 <= T < 2^26, Hq >= 1, D a multiple of 16 up to 256, rot a multiple of
  * 16 up to D, 1 <= n_axes <= 4, dtype DB_DTYPE_F16 or DB_DTYPE_BF16, a cache of
- * that type or e4m3; qkv, q and cache rows 16-byte aligned. */
+ * that type or e4m3 whose rows do not share memory; qkv, q and cache rows
+ * 16-byte aligned. */
 int db_rope_append(const void* qkv, long long qkv_stride, const int* position, int n_axes,
                    const unsigned char* axis_of_pair, const long long* slot,
                    const float* inv_freq, int rot, int interleaved,
@@ -268,9 +269,9 @@ int db_rope_append(const void* qkv, long long qkv_stride, const int* position, i
  * Rows of o [T, Hq, D] (dense) that belong to no request stay as they are.
  * max_new > 0 says how many new tokens a request has at most (0: T), which
  * decides which kernels are launched; a call that breaks it is still right.
- * Contract: T >= 0, R >= 0, Hq a multiple of Hkv, T * Hq < 2^31, R * Hkv < 2^24,
- * R * width * page_size below 2^34 or so, D 64 or 128,
- * scale finite and > 0, dtype as db_rope_append; q, o and cache rows 16-byte
+ * Contract: T >= 0, R >= 0, Hq a multiple of Hkv, T * Hq < 2^30, R * Hkv < 2^22,
+ * N * (width * page_size / 16 + 1) < 2^30, where N is R, or R + T * G / 16 if
+ * max_new * G <= 16; q_start ascending, D 64 or 128, scale finite and > 0, dtype as db_rope_append; q, o and cache rows 16-byte
  * aligned; ws of db_paged_attention_workspace_bytes, 256-byte aligned, not
  * shared by calls that overlap in time.  Its first *zeroed bytes (zeroed may
  * be NULL) must be zero at its first use; every call leaves them zero. */

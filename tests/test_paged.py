@@ -590,6 +590,61 @@ def test_attention_is_the_same_every_time():
         assert torch.equal(ops.paged_attention(**s), first)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_of_the_longest_window(n, page):
+    """A window of 2^31 - 1 hides nothing, also where a request has more new
+    tokens than its length, so that the first of them lie before its start."""
+    s = make_step([(n, 90), (n, 60)], 4, 2, 64, page, torch.float16, torch.float16)
+    s["kv_len"] = ints([max(1, n - 3), 60])
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 40):
+        check_attention(s, window=window, want=attention_reference(
+            s["q"], s["K"], s["V"], s["block_table"], s["q_start"], s["kv_len"], 1 / 8.0, True, None,
+            None, None), max_new=n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 128), (torch.bfloat16, 64)])
+@pytest.mark.parametrize("n,L", [
+    # rows of 3 heads over one KV head: a tile of 64, or one and a bit of 256; 4 to
+    # over 100 tiles of 64 keys
+    (20, 300), (20, 700), (20, 1100), (20, 2600), (20, 7000), (90, 500), (90, 1000), (90, 2200),
+    (90, 4000), (90, 7000)])
+def test_attention_of_split_chunks(n, L, dtype, D):
+    """Rows joined from 1 to over 16 splits, some of which see nothing."""
+    s = make_step([(n, L)], 3, 1, D, 16, dtype, dtype)
+    check_attention(s)
+    check_attention(s, window=400)
+
+
+@pytest.mark.gpu
+def test_attention_of_other_heads_in_a_workspace_as_large():
+    """Calls whose workspaces have one size and tickets of different numbers."""
+    few = make_step([(1, 3000), (1, 2500)], 17, 17, 128, 16, torch.float16, torch.float16)
+    many = make_step([(1, 200 + 9 * r) for r in range(8)], 33, 33, 64, 16, torch.float16,
+                     torch.float16)
+    a, b = ops.paged_attention(**few, max_new=1), ops.paged_attention(**many, max_new=1)
+    for _ in range(3):
+        assert torch.equal(check_attention(few, max_new=1), a)
+        assert torch.equal(check_attention(many, max_new=1), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_attention_of_rows_in_no_order(max_new):
+    """A q_start that goes back or past the rows: requests without rows, and the
+    others' rows as they should be."""
+    s = make_step([(4, 50), (0, 40), (5, 60), (1, 20)], 4, 2, 64, 16, torch.float16, torch.float16)
+    want = attention_reference(s["q"], s["K"], s["V"], s["block_table"], s["q_start"],
+                               s["kv_len"], 1 / 8.0, True, None, None, None)
+    s["out"] = torch.full_like(s["q"], 7.0)
+    s["q_start"] = ints([0, 4, -9, 2 ** 31 - 1, -2 ** 31])
+    assert ops.paged_attention(**s, max_new=max_new).isfinite().all()
+    s["q_start"] = ints([-5, 4, 4, 9, 2 ** 31 - 1])      # the same rows once clamped
+    check_attention(s, want=want, max_new=max_new)
+
+
 # -------------------------------------------------------------- a whole step
 def run_step(state, freq, Hq):
     p = ops.paged_plan(state["past"], state["new"], state["table"], state["free"], 16,
@@ -850,6 +905,32 @@ def test_attention_contract_errors(lib):
     assert call(cache=a_cache(D=96)) == -1 and "64 and 128" in last(lib)
 
 
+def test_paged_calls_too_large_are_refused(lib):
+    """Sizes whose tiles, rows or grids an int could not count."""
+    far = 2 ** 27
+    cache = a_cache(k_page_stride=16384, v_page_stride=16384)
+    for T, R, Hq, most, width in (
+            (4, 8, 32, 1, far), (4, 64, 32, 1, far // 8), (4, 8, 32, 0, far),   # key tiles of all
+            (2 ** 24, 1, 32, 1, 256), (4, 1, 32, 1, 2 ** 30),                   # ... row tiles too
+            (2 ** 25, 4, 32, 0, 8), (4, 2 ** 19, 32, 1, 8)):                    # rows, requests
+        assert lib.db_paged_attention(P, 4096, 128, P, C.byref(cache), P, width, width, P, P, T, R,
+                                      Hq, most, 0.1, 1, 0, 0, P, 1 << 40, None) == -1, (T, R, width)
+        assert "too large" in last(lib)
+    for T, R, count in ((2 ** 30 + 1, 2, 9), (4, 2 ** 30 + 1, 9), (4, 2, 2 ** 30 + 1)):
+        assert lib.db_paged_plan(P, P, P, 8, 8, P, count, None, 16, R, T, P, P, P, P, P, None) == -1
+        assert "above" in last(lib)
+    assert lib.db_rope_append(P, 48 * 128, P, 1, None, P, P, 128, 0, C.byref(a_cache()), P, 2 ** 26,
+                              32, 0, None) == -1 and "2^26" in last(lib)
+
+
+def test_rope_append_refuses_a_cache_whose_rows_share_memory(lib):
+    for bad in ("k_page_stride", "v_page_stride", "k_head_stride", "v_head_stride",
+                "k_token_stride", "v_token_stride"):
+        assert lib.db_rope_append(P, 48 * 128, P, 1, None, P, P, 128, 0,
+                                  C.byref(a_cache(**{bad: 0})), P, 3, 32, 0, None) == -1, bad
+        assert "share memory" in last(lib)
+
+
 def test_paged_workspace_of_refused_calls_is_none(lib):
     f = lib.db_paged_attention_workspace_bytes
     for bad in ((0, 32, 8, 128, 1, 1), (1, 30, 8, 128, 1, 1), (1, 32, 8, 96, 1, 1),
@@ -912,6 +993,7 @@ def test_paged_wrappers_refuse():
     for exc, kw in (
             (ValueError, dict(past_len=ints([1]))), (TypeError, dict(new_len=ints([1, 1]).long())),
             (ValueError, dict(page_size=0)), (ValueError, dict(n_tokens=-1)),
+            (ValueError, dict(page_size=2 ** 32 + 16)), (ValueError, dict(n_tokens=2 ** 32 + 2)),
             (ValueError, dict(block_table=table[:1].expand(2, 2))),
             (ValueError, dict(block_table=table.t())),
             (ValueError, dict(free_pages=table)), (ValueError, dict(free_start=ints([0, 1])))):
