@@ -403,7 +403,7 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
 }
 
 // Joins the records of split rows: o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
-// A workgroup of 16 waves has 16 rows of a row tile: a wave a row where there
+// A workgroup of 16 waves has up to 64 rows of a row tile: a wave a row where there
 // are up to 8 splits, two or four waves a row where there are more, each with
 // its share of the splits and eight records in flight.  (A wave alone, one
 // record after another, took 45 us for the 64 splits of one request of 8192
@@ -465,9 +465,12 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, 
   __shared__ float s_acc[kMergeWaves][D], s_m[kMergeWaves], s_l[kMergeWaves];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // Rows of a workgroup's piece: 64 where that makes a piece for each workgroup.
+  // Rows of a workgroup's piece: 64 where that makes a piece for each workgroup, 16
+  // where it does for half of them, else 4, which a workgroup joins at once however
+  // many the splits (20 rows of 8 heads in 31 splits: 17 us in pieces of 16).
   const int groups = min(a.rec.head[0], a.rec.groups);
-  const int part = groups * (mt / 64) >= (int)gridDim.x ? 64 : 16;
+  const int grid = (int)gridDim.x;
+  const int part = groups * (mt / 64) >= grid ? 64 : 2 * groups * (mt / 16) >= grid ? 16 : 4;
   const int parts = mt / part, total = groups * parts;
   for (int task = blockIdx.x; task < total; task += gridDim.x) {
     const int group = task / parts;
