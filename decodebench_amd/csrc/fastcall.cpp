@@ -536,8 +536,9 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* init(PyObject*, PyObject* args) {
   unsigned long long p[14];
   PyObject *rs, *gd, *ws, *cu;
-  if (!PyArg_ParseTuple(args, "(KKKKKKKKKKKKKK)OOO!O!", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6],
-                        &p[7], &p[8], &p[9], &p[10], &p[11], &p[12], &p[13], &rs, &gd, &PyDict_Type, &ws, &PyDict_Type, &cu))
+  if (!PyArg_ParseTuple(args, "(KKKKKKKKKKKKKK)OOO!O!", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5],
+                        &p[6], &p[7], &p[8], &p[9], &p[10], &p[11], &p[12], &p[13], &rs, &gd,
+                        &PyDict_Type, &ws, &PyDict_Type, &cu))
     return nullptr;
   abi.f1 = reinterpret_cast<decltype(abi.f1)>((uintptr_t)p[0]);
   abi.f2 = reinterpret_cast<decltype(abi.f2)>((uintptr_t)p[1]);

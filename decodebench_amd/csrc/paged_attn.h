@@ -1,5 +1,5 @@
 // paged_attn.h -- what the two kernels of paged attention share: arguments,
-// the assignment of work to workgroups, element types, page lookup, records.
+// element types, page lookup, records; and how the chunk kernel finds its work.
 //
 // paged_attention computes, for the new tokens i = 0 .. n_r - 1 of every
 // request r (packed one request after another, q_start[r] the first row) and
@@ -11,22 +11,20 @@
 //
 // Rows: the n_r G (token, query head) pairs of a (request, KV head) are the
 // rows of one product, row x = token x / G, head x % G, so that K and V are
-// read once for all of them; a row tile is MT of them.
+// read once for all of them; a row tile is MT of them (16 in paged_decode, 64
+// or 256 in paged_chunk).
 //
 // Lengths live on the GPU, so the host launches a grid by its bounds and every
-// workgroup finds its own work: it reads the lengths of all requests, takes
-// the key tiles that one split may hold (C: all work over the workgroups that
-// the chip wants) and from a prefix sum over the requests' split counts the
-// (request, KV head, row tile, split) of its number.  This costs about a
-// microsecond per workgroup, once, and no launch, no table to keep in step
-// with the lengths and no read on the host.  The KV head is the fastest index:
-// workgroups i and i + 8 run on one XCD, so with 8 heads all row tiles and
-// splits of a head share one L2.
+// workgroup finds its own work from the lengths of all requests.  This costs
+// about a microsecond per workgroup, once, and no launch, no table to keep in
+// step with the lengths and no read on the host.  The KV head is the fastest
+// index: workgroups i and i + 8 run on one XCD, so with 8 heads all row tiles
+// and splits of a head share one L2.
 //
-// A split writes its running maximum, exp-sum and unnormalised output as an
-// fp32 record; paged_merge joins the records of a row.  There are fewer
-// than 2 `target` records: only requests of at least 1.75 C tiles split, into
-// at most 8/7 tmax / C parts, and C >= (all tiles) / target.
+// Where a row's keys are split, each part writes its running maximum, exp-sum
+// and unnormalised output as an fp32 record.  paged_decode cuts the work into
+// equal parts (two records a workgroup at most) and joins the records in the
+// same launch; paged_chunk splits whole row tiles and paged_merge joins them.
 #pragma once
 
 #include "db_device.h"
@@ -127,8 +125,8 @@ struct PagedArgs {
   int causal, window;
   float scale_log2;
   int part;        // 0: every request, 1: those of at most kDecodeRows rows, 2: the others
-  int target;      // workgroups wanted
-  int min_tiles;   // fewest key tiles of a split
+  int target;      // chunk: workgroups wanted
+  int min_tiles;   // fewest key tiles of a split or part
   PagedRecords rec;
 };
 
@@ -229,11 +227,16 @@ __device__ __forceinline__ float max_xor16(float v) {
   return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
-// Finds the piece of work of the workgroup's number: find() says whether there
-// is one and leaves it in `work`, in scalar registers.  Every wave does the
-// search for itself, a lane to a request and 64 requests a round: no LDS, no
-// barrier.  The host's grid holds every piece: a request has at most rows / MT
-// + 1 row tiles, and the splits beyond one each are at most all tiles / C.
+// The chunk kernel's search for the piece of work of the workgroup's number:
+// find() says whether there is one and leaves it in `work`, in scalar registers.
+// C is the key tiles that one split may hold, all work over the workgroups that
+// the chip wants; a prefix sum over the requests' split counts gives the
+// (request, KV head, row tile, split).  Every wave does the search for itself, a
+// lane to a request and 64 requests a round: no LDS, no barrier.  The host's grid
+// holds every piece: a request has at most rows / MT + 1 row tiles, and the
+// splits beyond one each are at most all tiles / C.  There are fewer than 2
+// `target` records: only requests of at least 1.75 C tiles split, into at most
+// 8/7 tmax / C parts, and C >= (all tiles) / target.
 template <int MT, int KT>
 struct PagedSchedule {
   const PagedArgs& a;
@@ -346,7 +349,6 @@ __device__ __forceinline__ void paged_describe(const PagedArgs& a, const PagedWo
   d[4] = (int)min(left, (long long)MT);
 }
 
-// e4m3 or 16-bit caches: the element type of the products E, of the cache C8.
 typedef void (*PagedFn)(PagedArgs);
 PagedFn paged_decode_fn(bool bf16, bool fp8, int D, bool aligned);
 

@@ -1,9 +1,12 @@
 // paged_decode.hip -- paged attention of few rows (single tokens, drafts).
 //
-// A workgroup of four waves owns one (request, KV head, row tile of 16 rows)
-// and one split of the keys; wave w takes the key tiles w, w + 4, ... of the
-// split.  Bound by HBM: every key and value is read once per row tile, and
-// rows beyond the few that a request has cost nothing but idle MFMA columns.
+// A workgroup of four waves owns an equal part of a KV head's work (see
+// DecodeLine): keys of one (request, row tile of 16 rows) after another; wave w
+// takes the key tiles w, w + 4, ... of each.  Bound by HBM: every key and value
+// is read once per row tile, and rows beyond the few that a request has cost
+// nothing but idle MFMA columns.  64 requests of 800 to 8000 tokens (8 heads of
+// 128, 1.15 GB of cache): 0.21 ms, 5.5 TB/s, where a plain read reaches 7.1; equal
+// lengths in a [pages, heads, page, D] cache reach 6.1 to 6.5.
 //
 //  * A tile is 16 keys where K takes 4 KB of them, 32 (two sub-tiles of 16)
 //    where it takes less (e4m3, heads of 64), so that a tile's fixed work, its
@@ -644,7 +647,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_decode(PagedArgs a) {
         if (threadIdx.x == 0)
           __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         join_records<E, D>(a, rq.tok0, row_tile, rows, head, wg0, splits,
-             reinterpret_cast<float*>(&s_region[0][0]));
+                           reinterpret_cast<float*>(&s_region[0][0]));
       }
     }
     begin += take;

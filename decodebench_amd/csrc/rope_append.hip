@@ -18,8 +18,6 @@
 // Measured on MI355X, 8192 tokens of 32 + 2 x 8 heads of 128 in bf16 (201 MB):
 // 34 us, 5.9 TB/s, where a copy of as many bytes reaches 4.8; with a place worked
 // out anew for each token and one token's loads in flight 45 us.
-#include "db_device.h"
-#include "db_kernels.h"
 #include "paged_attn.h"
 
 namespace dbk {

@@ -2,7 +2,8 @@
 
 Each op takes torch tensors on the GPU, allocates its output with
 ``torch.empty`` and launches one kernel (two where K is split over workgroups
-or an F4 merge takes a launch of its own) on ``torch.cuda.current_stream()``
+or an F4 merge takes a launch of its own, up to three for paged attention) on
+``torch.cuda.current_stream()``
 through the C ABI declared in ``include/decodebench_hip.h``.  No op allocates
 inside the library, synchronises, or reads device memory on the host, so the
 ops work as ``Sequence`` stages, inside a ``profile(fused=...)`` callable, and
