@@ -45,11 +45,12 @@ constexpr int kHold = kWave / (KT / 16);  // tiles whose places the lanes hold
 // is set kBelow under the maximum.
 constexpr float kAbove = 12.0f, kBelow = 8.0f;
 
-template <class E, bool FP8, int D, bool ALIGNED, int NW>
-__global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(PagedArgs a) {
+template <class E, bool FP8, int D, bool ALIGNED, int NW, int KP>
+__global__ __launch_bounds__(NW * kWave, 2) void paged_chunk(PagedArgs a) {
   typedef typename E::type elem;
   typedef typename E::vec8 vec8;
-  constexpr int MT = 32 * NW;
+  constexpr int MT = 32 * NW / KP;
+  constexpr int WK = KT / KP;                      // keys of a tile that a wave takes
   constexpr int CB = FP8 ? 1 : 2;
   constexpr int RW = KT / NW;                      // rows of a tile that a wave loads
   constexpr int LPR = D * CB / 16;                 // lanes per row
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n32 = lane & 31, half = lane >> 5;
+  const int block = wave % (NW / KP), kpart = wave / (NW / KP) * WK;  // rows and keys of the wave
 
   PagedSchedule<MT, KT> schedule(a);
   PagedWork wk;
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
     // This lane's row and the keys it sees; rows past the last one see none.
     const long long left = (long long)rq.n * a.G - (long long)wk.tile * MT;
     const int rows = (int)min(left, (long long)MT);
-    const int lrow = wave * 32 + n32;
+    const int lrow = block * 32 + n32;
     const bool live = lrow < rows;
     const int x = wk.tile * MT + min(lrow, rows - 1);
     const int token = x / a.G, qhead = wk.head * a.G + x % a.G;
@@ -141,9 +143,9 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
     // last live row (none: nothing at all).
     const int wg_hi = a.causal ? min(limit, past + (wk.tile * MT) / a.G + 1) : limit;
     const int wg_lo = first_seen(a, past + (wk.tile * MT + rows - 1) / a.G);
-    const bool any = wave * 32 < rows;
-    const int i0 = (wk.tile * MT + min(wave * 32, rows - 1)) / a.G;
-    const int i1 = (wk.tile * MT + min(wave * 32 + 31, rows - 1)) / a.G;
+    const bool any = block * 32 < rows;
+    const int i0 = (wk.tile * MT + min(block * 32, rows - 1)) / a.G;
+    const int i1 = (wk.tile * MT + min(block * 32 + 31, rows - 1)) / a.G;
     const int all_hi = a.causal ? min(limit, past + i0 + 1) : limit;
     const int any_hi = !any ? 0 : a.causal ? min(limit, past + i1 + 1) : limit;
     const int all_lo = first_seen(a, past + i1);
@@ -279,14 +281,14 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
     };
 
     auto compute_tile = [&](int tile, unsigned long long there, int buf) {
-      const int key0 = tile * KT;
-      if (key0 >= any_hi || key0 + KT <= any_lo) return;
-      const elem* const kb0 = s_k[buf] + n32 * KS + 8 * half;
-      const elem* const vb0 = s_v[buf] + (4 * half + ((lane & 15) >> 2)) * VS +
+      const int key0 = tile * KT, lo = key0 + kpart, hi = lo + WK;  // lo .. hi - 1: the wave's
+      if (lo >= any_hi || hi <= any_lo) return;
+      const elem* const kb0 = s_k[buf] + (kpart + n32) * KS + 8 * half;
+      const elem* const vb0 = s_v[buf] + (kpart + 4 * half + ((lane & 15) >> 2)) * VS +
                               16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      f16v s[2];
+      f16v s[WK / 32];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < WK / 32; ++kb) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
@@ -294,24 +296,24 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
           s[kb] = E::mfma32(__builtin_bit_cast(vec8, ld16(kb0 + 32 * kb * KS + 16 * t)), qop[t],
                             s[kb]);
       }
-      const bool partial = there != ~0ull || key0 < all_lo || key0 + KT > all_hi;
       // Keys of the tile that this lane's row sees, a bit each.  (Bits tested at
       // fixed places of words shifted by the lane's half: places that depend on
       // the lane were hoisted out of the loop, 96 registers of them.)
-      unsigned long long sees = ~0ull;
-      if (partial) {
-        sees = there & below(khi - key0) & ~below(klo - key0);
-        const unsigned w0 = (unsigned)sees >> (4 * half), w1 = (unsigned)(sees >> 32) >> (4 * half);
+      const unsigned long long mine = below(WK) << kpart;
+      unsigned long long sees = mine;
+      if ((there & mine) != mine || lo < all_lo || hi > all_hi) {
+        sees = there & mine & below(khi - key0) & ~below(klo - key0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const unsigned bit = 1u << (8 * (i >> 2) + (i & 3));
-          s[0][i] = w0 & bit ? s[0][i] : kPagedNegInf;
-          s[1][i] = w1 & bit ? s[1][i] : kPagedNegInf;
+        for (int kb = 0; kb < WK / 32; ++kb) {
+          const unsigned w = (unsigned)(sees >> (kpart + 32 * kb)) >> (4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[kb][i] = w & (1u << (8 * (i >> 2) + (i & 3))) ? s[kb][i] : kPagedNegInf;
         }
       }
       float tmax = s[0][0];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < WK / 32; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[kb][i]);
       tmax = max_xor32(tmax) * scale;
@@ -325,10 +327,13 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
       }
       // A row that has seen nothing yet keeps -inf; its exponents use 0.
       const float m_use = m_ref == kPagedNegInf ? 0.0f : m_ref;
-      vec8 p[4];
+      // Probabilities are rounded to the element type for the product with V, half
+      // a step each that the product averages over a row's keys; their sum is of
+      // the fp32 values.
+      vec8 p[WK / 16];
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < WK / 32; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float e = fast_exp2(fmaf(s[kb][i], scale, -m_use));
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
         }
       l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < WK / 16; ++t)
 #pragma unroll
         for (int b = 0; b < NB; ++b)
           o[b] = E::mfma32(__builtin_bit_cast(vec8, read_v(vb0, t, b)), p[t], o[b]);
@@ -377,7 +382,40 @@ __global__ __launch_bounds__(NW * kWave, NW >= 4 ? 2 : 1) void paged_chunk(Paged
     }
 
     // ---- outputs -----------------------------------------------------------
-    const float l = l_run + __shfl_xor(l_run, 32);
+    float l = l_run + __shfl_xor(l_run, 32);
+    if constexpr (KP == 2) {  // the other keys' waves hand over what they have, through LDS
+      constexpr int OS = D + 4;  // floats; rows in different banks
+      static_assert(sizeof(s_k) >= sizeof(float) * MT * OS, "the keys' tiles hold the outputs");
+      float* const so = reinterpret_cast<float*>(s_k) + (block * 32 + n32) * OS + 4 * half;
+      float2* const sml = reinterpret_cast<float2*>(s_v) + block * 32 + n32;
+      if (kpart != 0) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<f4*>(so + 32 * b + 8 * c) =
+                f4{o[b][4 * c], o[b][4 * c + 1], o[b][4 * c + 2], o[b][4 * c + 3]};
+        if (half == 0) *sml = make_float2(m_ref, l);
+      }
+      __syncthreads();
+      if (kpart != 0) return;
+      const float2 ml = *sml;
+      if (ml.y != 0.0f) {  // else: saw nothing
+        const float m_new = l != 0.0f ? fmaxf(m_ref, ml.x) : ml.x;
+        const float w0 = l != 0.0f ? fast_exp2(m_ref - m_new) : 0.0f, w1 = fast_exp2(ml.x - m_new);
+        l = fmaf(l, w0, ml.y * w1);
+        m_ref = m_new;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const f4 v = *reinterpret_cast<const f4*>(so + 32 * b + 8 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[b][4 * c + i] = fmaf(o[b][4 * c + i], w0, v[i] * w1);
+          }
+      }
+    }
     const float vscale = FP8 ? a.v_scale[wk.head] : 1.0f;
     const int rec = wk.rec < 0 ? -1 : wk.rec + wk.split * a.Hkv;
     if (live) {
@@ -567,7 +605,8 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, 
 
 template <class E, bool FP8, int D, int NW>
 PagedFn pick_pages(bool aligned) {
-  return aligned ? paged_chunk<E, FP8, D, true, NW> : paged_chunk<E, FP8, D, false, NW>;
+  constexpr int KP = NW == 4 ? 2 : 1;
+  return aligned ? paged_chunk<E, FP8, D, true, NW, KP> : paged_chunk<E, FP8, D, false, NW, KP>;
 }
 template <class E, bool FP8, int NW>
 PagedFn pick_size(int D, bool aligned) {
@@ -581,8 +620,8 @@ PagedFn pick_type(bool bf16, bool fp8, int D, bool aligned) {
   return fp8 ? pick_size<ElemF16, true, NW>(D, aligned)
              : pick_size<ElemF16, false, NW>(D, aligned);
 }
-PagedFn pick_chunk(int waves, bool bf16, bool fp8, int D, bool aligned) {
-  return waves == 2 ? pick_type<2>(bf16, fp8, D, aligned) : pick_type<8>(bf16, fp8, D, aligned);
+PagedFn pick_chunk(int rows, bool bf16, bool fp8, int D, bool aligned) {
+  return rows == 64 ? pick_type<4>(bf16, fp8, D, aligned) : pick_type<8>(bf16, fp8, D, aligned);
 }
 
 void (*pick_merge(bool bf16, int D))(PagedArgs, int) {
@@ -592,26 +631,26 @@ void (*pick_merge(bool bf16, int D))(PagedArgs, int) {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// How a call of these bounds runs: the waves of the chunk kernel (0: none), and
+// How a call of these bounds runs: the rows of the chunk kernel's tile (0: none), and
 // the workgroups wanted of each kernel.
 struct PagedPlanned {
   bool decode;
-  int chunk_waves, chunk_target;
+  int chunk_rows, chunk_target;
   int decode_groups;  // a whole number of parts for each KV head
 };
 PagedPlanned planned(const PagedCall& c, int cu_count) {
   const int most = c.max_new > 0 && c.max_new < c.T ? c.max_new : c.T;
   const long long rows = (long long)most * (c.Hq / c.cache.Hkv);
   PagedPlanned p;
-  p.chunk_waves = rows <= kDecodeRows ? 0 : rows <= 64 ? 2 : 8;
+  p.chunk_rows = rows <= kDecodeRows ? 0 : rows <= 64 ? 64 : 256;
   // Up to 64 rows a request, or one request: the chunk kernel takes them all.
-  p.decode = p.chunk_waves == 0 || (p.chunk_waves == 8 && c.R > 1);
+  p.decode = p.chunk_rows == 0 || (p.chunk_rows == 256 && c.R > 1);
   // Parts of a KV head's line: a workgroup a CU where requests are few (a line of
   // 32 parts and one request: 13.4 against 16.1 us with 64, at 8192 tokens, 27.9
   // against 30.4 at 32768), else two (256 requests of 500 tokens 72 against 84).
   const int per_cu = 4ll * c.R * c.cache.Hkv <= cu_count ? 1 : 2;
   p.decode_groups = max(1, per_cu * cu_count / c.cache.Hkv) * c.cache.Hkv;
-  p.chunk_target = p.chunk_waves == 2 ? 2 * cu_count : cu_count;
+  p.chunk_target = p.chunk_rows == 64 ? 2 * cu_count : cu_count;
   return p;
 }
 
@@ -639,12 +678,12 @@ PagedSpace layout(const PagedPlanned& p, int D, char* base) {
         reinterpret_cast<int*>(take((size_t)p.decode_groups * kTicketInts * sizeof(int)));
     records(s.decode, 2 * p.decode_groups, kDecodeRows);
   }
-  if (p.chunk_waves) {
+  if (p.chunk_rows) {
     s.chunk.groups = p.chunk_target;
     s.chunk.head = reinterpret_cast<int*>(take(sizeof(int)));
     s.chunk.desc =
         reinterpret_cast<int*>(take((size_t)p.chunk_target * kDescInts * sizeof(int)));
-    records(s.chunk, 2 * p.chunk_target, 32 * p.chunk_waves);
+    records(s.chunk, 2 * p.chunk_target, p.chunk_rows);
   }
   s.bytes = at;
   return s;
@@ -709,7 +748,7 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
   const bool aligned = paged_aligned(kv);
   const PagedSpace space = layout(p, D, static_cast<char*>(ws));
   if (p.decode) {
-    a.part = p.chunk_waves ? 1 : 0;
+    a.part = p.chunk_rows ? 1 : 0;
     a.min_tiles = 8;
     a.rec = space.decode;
     hipLaunchKernelGGL(paged_decode_fn(c.bf16, fp8, D, aligned), dim3(p.decode_groups),
@@ -717,16 +756,16 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (p.chunk_waves) {
-    const int mt = 32 * p.chunk_waves;
+  if (p.chunk_rows) {
+    const int mt = p.chunk_rows;
     a.part = p.decode ? 2 : 0;
     a.target = p.chunk_target;
     a.min_tiles = 4;
     a.rec = space.chunk;
     // Row tiles of every request at most, and the splits beyond one each.
     const long long grid = ((long long)c.T * a.G / mt + c.R) * a.Hkv + p.chunk_target;
-    hipLaunchKernelGGL(pick_chunk(p.chunk_waves, c.bf16, fp8, D, aligned), dim3((unsigned)grid),
-                       dim3(p.chunk_waves * kWave), 0, stream, a);
+    hipLaunchKernelGGL(pick_chunk(mt, c.bf16, fp8, D, aligned), dim3((unsigned)grid),
+                       dim3((mt == 64 ? 4 : 8) * kWave), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(pick_merge(c.bf16, D), dim3(2 * cu_count), dim3(kMergeWaves * kWave), 0,
