@@ -1,8 +1,12 @@
 // paged_chunk.hip -- paged attention of many rows: chunks of a prompt, drafts.
 //
-// A workgroup of NW waves owns one (request, KV head, row tile of 32 NW rows)
-// and one split of the keys; wave w has rows 32 w .. 32 w + 31 and all share
-// 64-key tiles of K and V in LDS.  A tile of 256 rows of 128 takes a CU about
+// A workgroup owns one (request, KV head, row tile) and one split of the keys; its
+// waves have 32 rows each and share 64-key tiles of K and V in LDS.  Row tiles
+// have 256 rows (eight waves) or, where no request has more, 64: four waves then,
+// two (KP) to each 32 rows, each with half of every tile's keys, joined through
+// LDS at the end (with one wave to 32 rows 16 drafts of 5 tokens took 17.9 us
+// instead of 15.6).  Two such workgroups fit a CU, so the registers of a wave are
+// held to 256 (300 of them and one workgroup a CU: 16.6).  A tile of 256 rows of 128 takes a CU about
 // 4200 clocks, in which each SIMD has 2050 of MFMAs and 1900 of softmax, and the
 // LDS 2300 (256 KB of operands for the eight waves, 32 KB written).  2048 tokens
 // of 32 heads of 128, the last of 8192: 0.28 ms, 0.86 PFLOP/s, where a large
@@ -643,7 +647,9 @@ PagedPlanned planned(const PagedCall& c, int cu_count) {
   const long long rows = (long long)most * (c.Hq / c.cache.Hkv);
   PagedPlanned p;
   p.chunk_rows = rows <= kDecodeRows ? 0 : rows <= 64 ? 64 : 256;
-  // Up to 64 rows a request, or one request: the chunk kernel takes them all.
+  // Up to 64 rows a request, or one request: the chunk kernel takes them all (16
+  // drafts of 5 tokens at 4000, 4 heads a KV head: 58.7 us, on the decode kernel 81;
+  // where 8 heads fill the decode kernel's row tiles, 15.8 and 14.0).
   p.decode = p.chunk_rows == 0 || (p.chunk_rows == 256 && c.R > 1);
   // Parts of a KV head's line: a workgroup a CU where requests are few (a line of
   // 32 parts and one request: 13.4 against 16.1 us with 64, at 8192 tokens, 27.9

@@ -590,6 +590,27 @@ def test_attention_is_the_same_every_time():
         assert torch.equal(ops.paged_attention(**s), first)
 
 
+DRAFTS = [(20, 20), (12, 300), (5, 37), (1, 64), (0, 9), (20, 333), (11, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [None, 1, 31, 33, 100])
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype,cache", [
+    (6, 2, 128, 16, torch.float16, torch.float16), (3, 1, 64, 24, torch.bfloat16, torch.bfloat16),
+    (6, 2, 64, 32, torch.bfloat16, FP8), (3, 1, 128, 20, torch.float16, FP8)])
+def test_attention_of_drafts(window, Hq, Hkv, D, page, dtype, cache):
+    """Up to 60 rows a request: the keys of a tile are shared by two waves, and of
+    some tiles one of the two sees nothing."""
+    s = make_step(DRAFTS, Hq, Hkv, D, page, dtype, cache)
+    check_attention(s, window=window, max_new=20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, FP8])
+def test_attention_of_drafts_hidden_inf_and_nan(dtype):
+    test_attention_hidden_inf_and_nan(dtype, 20)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 5, 40])
 @pytest.mark.parametrize("page", [16, 24])
