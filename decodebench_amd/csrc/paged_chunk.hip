@@ -755,7 +755,7 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
   const PagedSpace space = layout(p, D, static_cast<char*>(ws));
   if (p.decode) {
     a.part = p.chunk_rows ? 1 : 0;
-    a.min_tiles = 8;
+    a.min_tiles = 8;  // two a wave: shorter parts cost more to join than they save
     a.rec = space.decode;
     hipLaunchKernelGGL(paged_decode_fn(c.bf16, fp8, D, aligned), dim3(p.decode_groups),
                        dim3(kPagedThreads), 0, stream, a);
