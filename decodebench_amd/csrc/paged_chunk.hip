@@ -36,6 +36,8 @@
 //  * A wave skips tiles that none of its rows sees, and masks only tiles that
 //    some row sees in part (an Inf or NaN among such a tile's values as in
 //    paged_decode: left out of the product, added to the rows that see it).
+#include <mutex>
+
 #include "paged_attn.h"
 
 namespace dbk {
@@ -753,6 +755,11 @@ hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hi
 
   const bool aligned = paged_aligned(kv);
   const PagedSpace space = layout(p, D, static_cast<char*>(ws));
+  // Calls of several host threads on one stream may share a workspace that one keeps
+  // from call to call: a call's launches must then stand together on the stream, or
+  // another's chunk kernel would overwrite records that are not joined yet.
+  static std::mutex together;
+  const std::lock_guard<std::mutex> hold(together);
   if (p.decode) {
     a.part = p.chunk_rows ? 1 : 0;
     a.min_tiles = 8;  // two a wave: shorter parts cost more to join than they save

@@ -91,8 +91,8 @@ struct DecodeLine {
   const PagedArgs& a;
   DecodeRequest mine;
   int length;      // key tiles in all
-  int upto, all;   // of this round's requests up to this one, and in all
-  int before;      // of the rounds before
+  int upto, all;   // of the present 64 requests up to this one, and in all
+  int before;      // of the requests before them
   int round;
 
   __device__ explicit DecodeLine(const PagedArgs& args) : a(args), before(0), round(0) {

@@ -794,6 +794,31 @@ def test_calls_at_once_on_two_streams():
 
 
 @pytest.mark.gpu
+def test_calls_of_threads_on_one_stream():
+    """Threads that share a stream share its kept workspace; a call of three
+    launches (single tokens, split chunks, their join) is not torn apart."""
+    import threading
+
+    steps = [make_step([(1, 900), (90, 4000 + 700 * i), (1, 70)], 6, 2, 128, 16, torch.float16,
+                       torch.float16, seed=i) for i in range(4)]
+    want = [check_attention(s) for s in steps]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        for _ in range(60):
+            got = ops.paged_attention(**steps[i])
+            if _ % 10 == 9 and not torch.equal(got, want[i]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not bad
+
+
+@pytest.mark.gpu
 def test_native_call_path_and_python_steps_agree(monkeypatch):
     """The native call path takes these calls, and the Python steps give the same."""
     freq = (10000.0 ** (-torch.arange(0, 64, 2) / 64)).to(DEV)
