@@ -640,6 +640,16 @@ def test_attention_of_split_chunks(n, L, dtype, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 30, 500])
+def test_attention_of_one_request_and_many_rows_of_nobody(n):
+    """Rows enough to fill the chip, most of them behind the request's last."""
+    s = make_step([(n, 3000)], 8, 8, 64, 16, torch.float16, torch.float16, extra=9000 - n)
+    s["out"] = torch.full_like(s["q"], 7.0)
+    got = check_attention(s)
+    assert (got[n:] == 7.0).all()
+
+
+@pytest.mark.gpu
 def test_attention_of_other_heads_in_a_workspace_as_large():
     """Calls whose workspaces have one size and tickets of different numbers."""
     few = make_step([(1, 3000), (1, 2500)], 17, 17, 128, 16, torch.float16, torch.float16)
