@@ -147,6 +147,7 @@ __device__ __forceinline__ int page_of(const PagedArgs& a, int key) {
 struct PagedRequest {
   int tok0, n, len;   // first row of q, new tokens, tokens in all
   int row_tiles, tiles;  // row tiles, most key tiles of any of them
+  bool back;             // q_start goes back from this request to the next
 };
 
 struct PagedWork {
@@ -168,13 +169,61 @@ __device__ __forceinline__ int first_seen(const PagedArgs& a, int pos) {
   return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
 }
 
+// Inclusive prefix sum over the 64 lanes (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+// The same with the maximum, of values that are not negative.
+__device__ __forceinline__ int wave_max_scan(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return v;
+}
+
+// Rows of q and length of this lane's request `r`, of 64 requests in lane order.
+// `upto` kInOrder: as q_start says.  Else the rows go from the furthest that a q_start up
+// to its own says to the furthest up to the next one's, and `upto` is the end of
+// the requests before these 64 (0 at first), which becomes theirs: no row belongs to
+// two requests and at most T count, which grid, records and tickets are sized by.
+// A kernel takes q_start at its word first and, if it goes back anywhere, starts again.
+// (A scan in every call: drafts 16.1 us instead of 15.8, 256 requests of one token with
+// no max_new 105 instead of 102.)
+constexpr int kInOrder = -1;
+struct PagedRows {
+  int tok0, n, len;
+};
+__device__ __forceinline__ PagedRows paged_rows(const PagedArgs& a, int r, int& upto) {
+  if (r >= a.R && upto == kInOrder) return {0, 0, 0};
+  const int at = min(r, a.R - 1);
+  int start = clamp_int(a.q_start[at], 0, a.T), end = clamp_int(a.q_start[at + 1], 0, a.T);
+  const int len = max(a.kv_len[at], 0);
+  if (upto != kInOrder) {
+    const int first = max(upto, __builtin_amdgcn_readfirstlane(start));
+    end = max(first, wave_max_scan(end));
+    start = __builtin_amdgcn_update_dpp(first, end, 0x138, 0xf, 0xf, false);  // wave_shr:1
+    upto = __builtin_amdgcn_readlane(end, kWave - 1);
+  }
+  return {start, end - start, len};
+}
+
 template <int MT, int KT>
-__device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r) {
-  PagedRequest q = {0, 0, 0, 0, 0};
-  if (r >= a.R) return q;
-  q.tok0 = clamp_int(a.q_start[r], 0, a.T);
-  q.n = max(clamp_int(a.q_start[r + 1], 0, a.T) - q.tok0, 0);
-  q.len = max(a.kv_len[r], 0);
+__device__ __forceinline__ PagedRequest paged_request(const PagedArgs& a, int r, int& upto) {
+  PagedRequest q = {0, 0, 0, 0, 0, false};
+  const PagedRows own = paged_rows(a, r, upto);
+  q.tok0 = own.tok0;
+  q.back = own.n < 0;
+  q.n = max(own.n, 0);
+  q.len = own.len;
   const long long rows = (long long)q.n * a.G;
   if (a.part != 0 && (rows <= kDecodeRows) != (a.part == 1)) q.n = 0;
   if (q.n == 0) return q;
@@ -197,16 +246,6 @@ __device__ __forceinline__ unsigned long long below(int n) {
   return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
-// Inclusive prefix sum over the 64 lanes (DPP row shifts and broadcasts).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return v;
-}
 __device__ __forceinline__ int wave_total(int v) {
   return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1);
 }
@@ -233,8 +272,9 @@ __device__ __forceinline__ float max_xor16(float v) {
 // the chip wants; a prefix sum over the requests' split counts gives the
 // (request, KV head, row tile, split).  Every wave does the search for itself, a
 // lane to a request and 64 requests a round: no LDS, no barrier.  The host's grid
-// holds every piece: a request has at most rows / MT + 1 row tiles, and the
-// splits beyond one each are at most all tiles / C.  There are fewer than 2
+// holds every piece, so every group that is counted for the merge is described: the
+// requests have at most T rows between them and one row tile each that is not full,
+// and the splits beyond one each are at most all tiles / C.  There are fewer than 2
 // `target` records: only requests of at least 1.75 C tiles split, into at most
 // 8/7 tmax / C parts, and C >= (all tiles) / target.
 template <int MT, int KT>
@@ -243,23 +283,36 @@ struct PagedSchedule {
   int w, round, C;
   int units0, recs0, groups0;  // of the rounds before (per KV head)
   PagedRequest mine;           // this lane's request of the round
+  int upto;                    // where the round's rows end, or kInOrder
   int splits, units, before, total;
 
   __device__ explicit PagedSchedule(const PagedArgs& args)
       : a(args), w(blockIdx.x), round(0), units0(0), recs0(0), groups0(0) {
     const int lane = threadIdx.x & (kWave - 1);
-    float work = 0.0f;  // its rounding may move C by one tile in 2^24
-    for (int r = (a.R - 1) / kWave * kWave; r >= 0; r -= kWave) {
-      mine = paged_request<MT, KT>(a, r + lane);
-      work += (float)mine.row_tiles * (float)mine.tiles;
+    float work;  // its rounding may move C by one tile in 2^24
+    for (int begin = kInOrder;; begin = 0) {
+      bool back = false;
+      int far = begin;
+      work = 0.0f;
+      for (int r = 0; r < a.R; r += kWave) {
+        const PagedRequest q = paged_request<MT, KT>(a, r + lane, far);
+        if (r == 0) {
+          mine = q;
+          upto = far;
+        }
+        work += (float)q.row_tiles * (float)q.tiles;
+        back = back || q.back;
+      }
+      if (!__any(back)) break;  // (none goes back after a scan)
     }
     const float per = ceilf(wave_sum(work) * (float)a.Hkv / (float)a.target);
     C = max(a.min_tiles, (int)fminf(per, 1073741824.0f));
     scan();
     if (blockIdx.x == 0 && threadIdx.x < kWave) {  // the groups of the whole call, for the merge
       int groups = splits > 1 ? mine.row_tiles : 0;
+      int far = upto;
       for (int r = kWave; r < a.R; r += kWave) {
-        const PagedRequest q = paged_request<MT, KT>(a, r + lane);
+        const PagedRequest q = paged_request<MT, KT>(a, r + lane, far);
         groups += splits_of(q) > 1 ? q.row_tiles : 0;
       }
       groups = wave_total(groups) * a.Hkv;
@@ -288,12 +341,12 @@ struct PagedSchedule {
       groups0 += wave_total(splits > 1 ? mine.row_tiles : 0);
       ++round;
       if ((long long)round * kWave >= a.R) return false;
-      mine = paged_request<MT, KT>(a, round * kWave + lane);
+      mine = paged_request<MT, KT>(a, round * kWave + lane, upto);
       scan();
     }
     const int at0 = unit - units0;
     const unsigned long long hit = __ballot(at0 >= before && at0 - before < units);
-    if (!hit) return false;  // sums out of range: q_start is not ascending
+    if (!hit) return false;  // another stream changes the lengths meanwhile
     const int who = __builtin_ctzll(hit);
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
     work.req.tok0 = of(mine.tok0);

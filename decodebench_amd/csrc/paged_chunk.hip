@@ -526,7 +526,12 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void paged_merge(PagedArgs a, 
     const int group = task / parts;
     const int* d = a.rec.desc + (size_t)group * kDescInts;
     const int splits = d[0], rec0 = d[1], head = rec0 % a.Hkv;
-    if (rec0 + (splits - 1) * a.Hkv >= a.rec.records) continue;
+    // Nothing outside the records and o, also if another stream has changed the
+    // lengths since the groups were counted and this one was not described.
+    if (splits < 2 || rec0 < 0 || rec0 + (splits - 1ll) * a.Hkv >= a.rec.records || d[2] < 0 ||
+        d[3] < 0 || d[4] < 1 || d[4] > mt ||
+        (long long)d[2] * a.G + d[3] + d[4] > (long long)a.T * a.G)
+      continue;
     const int first = task % parts * part, rows = min(d[4] - first, part);
     if (splits <= 2) {
       for (int r0 = wave * 4; r0 < rows; r0 += 4 * kMergeWaves)

@@ -203,7 +203,8 @@ int db_f4_splitkv_noalloc(const void* q, const void* k, const void* v, void* o,
  * values into the cache, db_paged_attention attends over it.  Lengths, tables
  * and slots stay on the GPU.  Wrong ones (lengths out of order, page numbers or
  * slots outside the cache) lead to no access outside the tensors: such keys
- * are not seen and such rows are not written.  No counterpart in the
+ * are not seen and such rows are not written, and a row that several requests
+ * name is the first one's.  No counterpart in the
  * reference, whose cache is one dense [B, Hkv, L, D] tensor of equal lengths
  * (src/decodebench/demos/llama_decode.py:110-116). */
 typedef struct db_paged_cache {

@@ -676,6 +676,136 @@ def test_attention_of_rows_in_no_order(max_new):
     check_attention(s, want=want, max_new=max_new)
 
 
+# ------------------------------------------------------- rows counted twice
+# How paged_attention sizes a call from T and R alone, and what its kernels then
+# find in q_start: a model on the CPU, for 256 compute units.  `own_rows` is their
+# rule, `said_rows` what q_start says taken at its word, where rows that two
+# requests name count twice.
+def own_rows(q_start, T):
+    ends = []
+    for x in q_start:
+        ends.append(max([min(max(x, 0), T), *ends[-1:]]))
+    return [b - a for a, b in zip(ends, ends[1:])]
+
+
+def said_rows(q_start, T):
+    at = [min(max(x, 0), T) for x in q_start]
+    return [max(b - a, 0) for a, b in zip(at, at[1:])]
+
+
+def chunk_schedule(rows, lens, T, G, Hkv, mt=256, cus=256):
+    """Pieces of work against the grid, split row tiles of pieces in the grid against
+    those counted for the join, and the room for them and for their records."""
+    target = 2 * cus if mt == 64 else cus
+    tiles = [(-(-n * G // mt) if n * G > (16 if mt == 256 else 0) else 0, -(-max(L, 0) // 64))
+             for n, L in zip(rows, lens)]
+    C = max(4, -(-sum(a * b for a, b in tiles) * Hkv // target))
+    splits = [max(1, (4 * b + C) // (4 * C)) if a else 0 for a, b in tiles]
+    units = sum(a * k for (a, _), k in zip(tiles, splits)) * Hkv
+    grid = (T * G // mt + len(rows)) * Hkv + target
+    counted = sum(a for (a, _), k in zip(tiles, splits) if k > 1) * Hkv
+    described, at = 0, 0
+    for (a, _), k in zip(tiles, splits):
+        for _ in range(a):
+            described += sum(1 for h in range(Hkv) if at * Hkv + h < grid) if k > 1 else 0
+            at += k
+    records = sum(a * k for (a, _), k in zip(tiles, splits) if k > 1) * Hkv
+    return dict(units=units, grid=grid, counted=counted, described=described, records=records,
+                room=target)
+
+
+def orders():
+    """(q_start, lengths, T, G, Hkv, whether they need more than the grid has): rows
+    that many requests name, the longest request last."""
+    yield [0, 640] * 21, [64] * 40 + [32768], 640, 4, 1, True
+    yield [0, 640] * 21, [64] * 40 + [32768], 640, 4, 8, True
+    yield [0, 4096] * 50 + [0, 300], [64] * 100 + [32768], 4096, 4, 8, True
+    yield [0, 300] + [100, 300] * 19 + [250, 640], [64] * 40 + [8000], 640, 4, 1, False
+
+
+def test_rows_counted_twice_would_not_fit_the_grid():
+    for q_start, lens, T, G, Hkv, too_many in orders():
+        said = chunk_schedule(said_rows(q_start, T), lens, T, G, Hkv)
+        assert (said["units"] > said["grid"]) is too_many
+        assert (said["described"] < said["counted"]) is too_many
+        own = chunk_schedule(own_rows(q_start, T), lens, T, G, Hkv)
+        assert own["units"] <= own["grid"] and own["described"] == own["counted"]
+
+
+def test_rows_counted_once_fit_the_grid():
+    gen = torch.Generator().manual_seed(8)
+
+    def below(n):
+        return int(torch.randint(0, n, (1,), generator=gen))
+
+    for turn in range(400):
+        T, R, G, Hkv = 1 + below(5000), 1 + below(150), 1 + below(8), 1 + below(16)
+        top = (2 ** below(12) + 2) * 64
+        lens = [below(top) for _ in range(R)]
+        q_start = [below(3 * T) - T for _ in range(R + 1)]
+        if turn % 3 == 0:
+            q_start.sort()
+        for mt in (64, 256):
+            s = chunk_schedule(own_rows(q_start, T), lens, T, G, Hkv, mt)
+            assert s["units"] <= s["grid"] and s["described"] == s["counted"]
+            assert s["counted"] <= s["room"] and s["records"] <= 2 * s["room"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_start", [
+    [0, 640] * 21, [0, 300] + [100, 300] * 19 + [250, 640],
+    [0, 2 ** 31 - 1, -2 ** 31] * 13 + [5, 100, 2 ** 31 - 1]])
+def test_attention_of_rows_that_many_requests_name(q_start):
+    """Each row is the first request's that names it, and nothing around the output is
+    written, also after calls of more rows whose splits stand in the workspace."""
+    before = make_step([(3, 70), (900, 3000)], 4, 1, 64, 16, torch.float16, torch.float16)
+    first = check_attention(before)
+    s = make_step([(0, 64)] * 40 + [(0, 8000)], 4, 1, 64, 16, torch.float16, torch.float16,
+                  extra=640)
+    starts = [0]
+    for n in own_rows(q_start, 640):
+        starts.append(starts[-1] + n)
+    want = attention_reference(s["q"], s["K"], s["V"], s["block_table"], ints(starts),
+                               s["kv_len"], 1 / 8.0, True, None, None, None)
+    around = torch.full((640 + 2 * 512, 4, 64), 7.0, dtype=torch.float16, device=DEV)
+    s.update(q_start=ints(q_start), out=around[512:-512])
+    for max_new in (None, 16, 1):
+        around.fill_(7.0)
+        check_attention(s, want=want, max_new=max_new)
+        assert (around[:512] == 7.0).all() and (around[-512:] == 7.0).all()
+    assert torch.equal(check_attention(before), first)
+
+
+def test_lines_of_rows_counted_twice_would_pass_an_int():
+    """The decode kernel's line of work: what the host bounds it by, and the tiles of
+    16 keys of 2048 requests that name the same 4096 rows."""
+    T, R, G, L, width = 4096, 4096, 4, 16384, 1024
+    q_start = [0] + [0, T] * (R // 2)
+    line = {rule: sum(-(-n * G // 16) * (L // 16) for n in rule(q_start, T))
+            for rule in (said_rows, own_rows)}
+    assert line[said_rows] >= 2 ** 31
+    assert line[own_rows] <= (T * G // 16 + R) * (width + 1) < 2 ** 30
+
+
+@pytest.mark.gpu
+def test_attention_of_single_tokens_after_rows_that_many_requests_name():
+    """Thousands of requests that name the same rows leave the kept workspace as
+    they found it: calls that share it stay right."""
+    T, R, G = 4096, 4096, 4
+    fine = make_step([(1, 700 + 40 * r) for r in range(70)], G, 1, 64, 16, torch.float16,
+                     torch.float16)
+    first = check_attention(fine, max_new=1)
+    s = make_step([(T, 8)], G, 1, 64, 16, torch.float16, torch.float16)
+    table = torch.zeros(1, 1024, dtype=torch.int32, device=DEV)
+    table[0, 0] = s["block_table"][0, 0]
+    o, size = attention_reference(s["q"], s["K"], s["V"], table[:, :1], s["q_start"], s["kv_len"],
+                                  1 / 8.0, True, None, None, None)
+    s.update(block_table=table.expand(R, 1024), q_start=ints([0] + [T, 0] * (R // 2 - 1) + [T, T]),
+             kv_len=ints([8] + [16384] * (R - 1)))
+    check_attention(s, want=(o, size), max_new=1)
+    assert torch.equal(check_attention(fine, max_new=1), first)
+
+
 # -------------------------------------------------------------- a whole step
 def run_step(state, freq, Hq):
     p = ops.paged_plan(state["past"], state["new"], state["table"], state["free"], 16,
