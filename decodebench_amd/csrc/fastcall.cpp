@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -337,14 +338,13 @@ at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, int idx) {
                               at::Device(at::kCUDA, (c10::DeviceIndex)idx)));
 }
 
-// `n` elements of `type` in the storage of the int32 tensor `all`, from its
-// element `from` on.
-at::Tensor part_of(const at::Tensor& all, int64_t from, int64_t n, at::ScalarType type) {
-  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-      c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
-  t.unsafeGetTensorImpl()->set_storage_offset(from * 4 / (int64_t)c10::elementSize(type));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-  return t;
+// The same for `n` elements, on the current device, from the allocator of `like`'s
+// storage where it names one: at::empty without its dispatch.
+at::Tensor empty_like_of(const at::Tensor* like, int64_t n, at::ScalarType type, int idx) {
+  c10::Allocator* const from = like->storage().allocator();
+  if (!from) return empty_on({n}, type, idx);
+  return at::Tensor(at::detail::empty_generic(
+      {n}, from, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
 }
 
 bool integer(PyObject* o, long* v) {
@@ -384,11 +384,12 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int found = stream_of(idx, &stream);
   if (found < 0) return nullptr;
   if (found == 0) Py_RETURN_NONE;
-  // One allocation; slot, the only one of 8 bytes, first.  (Five took 3 us more.)
-  const at::Tensor all = empty_on({3 * (int64_t)T + 2 * R + 2}, at::kInt, idx);
-  at::Tensor out[5] = {part_of(all, 3 * T, R + 1, at::kInt), part_of(all, 3 * T + R + 1, R, at::kInt),
-                       part_of(all, 2 * T, T, at::kInt), part_of(all, 0, T, at::kLong),
-                       part_of(all, 3 * T + 2 * R + 1, 1, at::kInt)};
+  // Storage of its own for each: torch saves no two types of one storage, and with a
+  // part of one all of it.
+  at::Tensor out[5] = {
+      empty_like_of(past, R + 1, at::kInt, idx), empty_like_of(past, R, at::kInt, idx),
+      empty_like_of(past, T, at::kInt, idx), empty_like_of(past, T, at::kLong, idx),
+      empty_like_of(past, 1, at::kInt, idx)};
   const int *pp = static_cast<const int*>(past->data_ptr()),
             *np = static_cast<const int*>(fresh->data_ptr()),
             *fp = static_cast<const int*>(pages->data_ptr());

@@ -139,6 +139,33 @@ def test_plan_keeps_entries_without_a_page():
     check_plan([5, 20], [2, 3], 16, 5, [8, 9], width=3, table=[[-1, -1, -1], [4, -1, -1]])
 
 
+@pytest.mark.gpu
+def test_a_plan_is_saved_and_loaded(monkeypatch):
+    """A plan's tensors are saved together, and alone as what they hold, on the native
+    call path as on the Python one."""
+    import io
+
+    table = ints([[7, -1, -1], [9, 8, -1]])
+    args = (ints([3, 20]), ints([40, 2]), table, ints([4, 5, 6]), 16, 1000)
+
+    def saved(what):
+        out = io.BytesIO()
+        torch.save(what, out)
+        out.seek(0)
+        return torch.load(out, weights_only=True), len(out.getvalue())
+
+    ops.load_library()
+    assert ops._fast is not None
+    sizes = []
+    for fast in (ops._fast, None):
+        monkeypatch.setattr(ops, "_fast", fast)
+        p = ops.paged_plan(*args)
+        for got, w in zip(saved(tuple(p))[0], p):
+            assert got.dtype == w.dtype and torch.equal(got, w)
+        sizes.append(saved(p.kv_len)[1])
+    assert sizes[0] == sizes[1]
+
+
 # ----------------------------------------------------------------- rope_append
 def cache_pair(gen, pages, Hkv, page, D, dtype, layout="heads", dev=DEV):
     def one():
