@@ -89,12 +89,6 @@ struct ElemBF16 {
   }
 };
 
-// Whether a pair of 16-bit values holds an Inf or NaN.
-template <class E>
-__device__ __forceinline__ bool pair_nonfinite(unsigned w) {
-  return (w & E::kExp) == E::kExp || ((w >> 16) & E::kExp) == E::kExp;
-}
-
 // ------------------------------------------------------------- arguments
 // Region of the workspace of one kernel.
 struct PagedRecords {
