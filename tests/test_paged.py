@@ -703,6 +703,43 @@ def test_attention_of_rows_in_no_order(max_new):
     check_attention(s, want=want, max_new=max_new)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,D,page", [
+    (torch.float16, torch.float16, 128, 16), (torch.bfloat16, torch.bfloat16, 64, 24),
+    (torch.bfloat16, FP8, 128, 32)])
+def test_attention_of_prompts_from_nothing(dtype, cache, D, page):
+    """No past: the row tiles of a request see anything from one tile of keys to all."""
+    check_attention(make_step([(900, 900)], 8, 2, D, page, dtype, cache))
+    check_attention(make_step([(330, 330), (1, 1), (515, 515), (64, 64)], 8, 2, D, page, dtype,
+                              cache), max_new=515)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [None, 1, 3])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [7, 64, 300])
+def test_attention_of_many_heads_over_one(G, D, max_new):
+    """A token's rows fill a row tile, or several."""
+    s = make_step([(1, 200), (3, 90), (2, 33), (0, 4)], G, 1, D, 16, torch.bfloat16, FP8)
+    check_attention(s, max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("max_new", [None, 1, 8])
+def test_attention_of_a_row_of_q_that_is_not_finite(bad, max_new):
+    """It shows in its own row and head and nowhere else."""
+    for requests in ([(1, 300), (1, 40), (1, 700)], [(20, 300), (1, 40), (30, 70)],
+                     [(2, 300), (3, 40)]):
+        s = make_step(requests, 8, 2, 64, 16, torch.float16, torch.float16)
+        o, size = attention_reference(s["q"], s["K"], s["V"], s["block_table"], s["q_start"],
+                                      s["kv_len"], 1 / 8.0, True, None, None, None)
+        s["q"][-1, 3] = bad
+        o[-1, 3] = math.nan
+        got = check_attention(s, want=(o, size), max_new=max_new)
+        assert got[-1, 3].isnan().all()
+
+
 # ------------------------------------------------------- rows counted twice
 # How paged_attention sizes a call from T and R alone, and what its kernels then
 # find in q_start: a model on the CPU, for 256 compute units.  `own_rows` is their
