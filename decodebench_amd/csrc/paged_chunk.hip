@@ -10,7 +10,8 @@
 // 4200 clocks, in which each SIMD has 2050 of MFMAs and 1900 of softmax, and the
 // LDS 2300 (256 KB of operands for the eight waves, 32 KB written).  2048 tokens
 // of 32 heads of 128, the last of 8192: 0.28 ms, 0.86 PFLOP/s, where a large
-// library matrix product reaches 1.13.  Two schedules that run the MFMAs beside
+// library matrix product reaches 1.13; 12% of that is CUs whose row tiles see
+// fewer keys than the longest (2048 tokens from nothing, where half is: 73 us).  Two schedules that run the MFMAs beside
 // the softmax (the waves of a SIMD half a tile apart; a wave's own scores, softmax
 // and values woven together) took 2% less for twice the code; 64 rows a wave,
 // which halve the LDS reads, spill registers and took 1.6 times as long.

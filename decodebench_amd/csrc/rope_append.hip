@@ -16,7 +16,7 @@
 // (8 pairs of a head, or 8 values) for all the tokens, so that what it has to
 // work out about the place is shared and four tokens' loads are in flight.
 // Measured on MI355X, 8192 tokens of 32 + 2 x 8 heads of 128 in bf16 (201 MB):
-// 34 us, 5.9 TB/s, where a copy of as many bytes reaches 4.8; with a place worked
+// 35.5 us, 5.7 TB/s, where a copy of as many bytes reaches 4.8; with a place worked
 // out anew for each token and one token's loads in flight 45 us.
 #include "paged_attn.h"
 

@@ -777,7 +777,8 @@ def rope_append(qkv, position, slot, K, V, inv_freq, axes=None, interleaved: boo
     float8_e4m3fn with fp32 ``k_scale``/``v_scale`` [Hkv] (any strides with
     contiguous rows of D, so a [pages, page_size, Hkv, D] cache is passed as its
     ``permute(0, 2, 1, 3)``); slot [T] int64 as :func:`paged_plan` gives it (a
-    slot outside the cache writes nothing; slots must differ).
+    slot outside the cache writes nothing; slots must differ).  D is a multiple of
+    16 up to 256 (:func:`paged_attention` reads caches of D 64 and 128).
 
     Pair i of a head turns by ``position * inv_freq[i]`` (inv_freq fp32, rot/2
     entries, rot <= D; elements past rot stay): elements i and i + rot/2, or
@@ -833,11 +834,13 @@ def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None =
     to its own position (``causal``; all of its request otherwise), with
     ``window`` only the last that many; a token that sees nothing gets zeros,
     and what hidden keys and values hold never counts.  Rows that belong to no
-    request are not written.
+    request are not written; q_start ascends, and where it does not, a row is the
+    first request's that names it.
 
     ``max_new`` is the most new tokens a request has, where the caller knows it
     (1 in a plain decode step): it spares the kernels that such a call does not
-    need, and nothing else."""
+    need (256 requests of one token and 500 keys: 71 us instead of 102), and
+    nothing else."""
     if out is None and _fast is not None:
         o = _fast.paged(q, K, V, block_table, q_start, kv_len, scale, causal, window, max_new,
                         k_scale, v_scale)
