@@ -338,13 +338,13 @@ at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, int idx) {
                               at::Device(at::kCUDA, (c10::DeviceIndex)idx)));
 }
 
-// The same for `n` elements, on the current device, from the allocator of `like`'s
-// storage where it names one: at::empty without its dispatch.
-at::Tensor empty_like_of(const at::Tensor* like, int64_t n, at::ScalarType type, int idx) {
-  c10::Allocator* const from = like->storage().allocator();
-  if (!from) return empty_on({n}, type, idx);
+// The same for `n` elements on the current device, without at::empty's dispatch: from
+// torch's allocator, as the storage of an empty tensor names it.
+at::Tensor empty_here(int64_t n, at::ScalarType type, int idx) {
+  static c10::Allocator* const allocator = empty_on({0}, type, idx).storage().allocator();
+  if (!allocator) return empty_on({n}, type, idx);
   return at::Tensor(at::detail::empty_generic(
-      {n}, from, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
+      {n}, allocator, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
 }
 
 bool integer(PyObject* o, long* v) {
@@ -387,9 +387,8 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // Storage of its own for each: torch saves no two types of one storage, and with a
   // part of one all of it.
   at::Tensor out[5] = {
-      empty_like_of(past, R + 1, at::kInt, idx), empty_like_of(past, R, at::kInt, idx),
-      empty_like_of(past, T, at::kInt, idx), empty_like_of(past, T, at::kLong, idx),
-      empty_like_of(past, 1, at::kInt, idx)};
+      empty_here(R + 1, at::kInt, idx), empty_here(R, at::kInt, idx), empty_here(T, at::kInt, idx),
+      empty_here(T, at::kLong, idx), empty_here(1, at::kInt, idx)};
   const int *pp = static_cast<const int*>(past->data_ptr()),
             *np = static_cast<const int*>(fresh->data_ptr()),
             *fp = static_cast<const int*>(pages->data_ptr());

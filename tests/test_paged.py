@@ -166,6 +166,18 @@ def test_a_plan_is_saved_and_loaded(monkeypatch):
     assert sizes[0] == sizes[1]
 
 
+@pytest.mark.gpu
+def test_a_plan_of_lengths_in_memory_of_another_owner():
+    """Inputs whose storage no allocator of torch's made."""
+    args = [ints([3, 20]), ints([40, 2]), ints([[7, -1, -1], [9, 8, -1]]), ints([4, 5, 6])]
+    want = ops.paged_plan(*args, 16, 50)
+    args[2] = ints([[7, -1, -1], [9, 8, -1]])
+    got = ops.paged_plan(*(torch.from_dlpack(x) for x in args), 16, 50)
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+    assert args[2].tolist() == [[7, 4, 5], [9, 8, -1]]
+
+
 # ----------------------------------------------------------------- rope_append
 def cache_pair(gen, pages, Hkv, page, D, dtype, layout="heads", dev=DEV):
     def one():
