@@ -685,3 +685,270 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
 }
 
 }  // extern "C"
+
+// ------------------------------------- block-scaled e4m3, mixture of experts
+namespace {
+
+constexpr int kMostSize = 1 << 22;   // of the tokens, rows and columns of a product
+constexpr int kMostTokens = 1 << 20; // of a mixture-of-experts layer
+constexpr long long kMostOffset = 1ll << 29;  // elements that a kernel's 32-bit offsets reach
+
+size_t blocks128(int n) { return ((size_t)n + 127) / 128; }
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+bool is16bit(int dtype) { return dtype == DB_DTYPE_F16 || dtype == DB_DTYPE_BF16; }
+
+int check_workspace(const char* fn, const void* ws, size_t bytes, size_t need) {
+  if (need == 0) return DB_OK;
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(DB_ERR_INVALID, "%s: needs a workspace, 256-byte aligned", fn);
+  if (bytes < need)
+    return fail(DB_ERR_INVALID, "%s: workspace %zu bytes < %zu required", fn, bytes, need);
+  return DB_OK;
+}
+
+// Bytes of the activations that a call quantises first, and their scales.
+size_t quantized_bytes(int T, int K) {
+  return round256((size_t)T * K) + round256((size_t)T * blocks128(K) * sizeof(float));
+}
+
+int check_route(const char* fn, const void* x, long long x_stride, const void* router, int T,
+                int H, int E, int k, int dtype) {
+  if (!is16bit(dtype)) return fail(DB_ERR_INVALID, "%s: unknown activation dtype %d", fn, dtype);
+  if (H < 8 || H % 8 != 0 || H >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: H=%d must be a multiple of 8 below 2^22", fn, H);
+  if (E < 1 || E > 1024) return fail(DB_ERR_INVALID, "%s: E=%d outside [1, 1024]", fn, E);
+  if (k < 1 || k > E || k > 64)
+    return fail(DB_ERR_INVALID, "%s: k=%d outside [1, min(E, 64)]", fn, k);
+  if (T < 0 || T >= kMostTokens)
+    return fail(DB_ERR_INVALID, "%s: T=%d must be >= 0 and below 2^20", fn, T);
+  if (x_stride < H || x_stride % 8 != 0)
+    return fail(DB_ERR_INVALID, "%s: x rows must hold H elements and be 16-byte aligned", fn);
+  if (T == 0) return DB_OK;
+  if (!x || !router) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(x) || !aligned16(router))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  return DB_OK;
+}
+
+int check_moe(const char* fn, const db_moe* m, const void* x, long long x_stride, const void* y,
+              int T, int k) {
+  if (!m) return fail(DB_ERR_INVALID, "%s: null weights", fn);
+  if (!is16bit(m->dtype))
+    return fail(DB_ERR_INVALID, "%s: unknown activation dtype %d", fn, m->dtype);
+  const bool fp8 = m->w_dtype == DB_DTYPE_FP8_E4M3;
+  if (!fp8 && m->w_dtype != m->dtype)
+    return fail(DB_ERR_INVALID, "%s: the weights must have the activations' type or e4m3", fn);
+  if (m->E < 1 || m->E > 1024)
+    return fail(DB_ERR_INVALID, "%s: E=%d outside [1, 1024]", fn, m->E);
+  const int step = fp8 ? 16 : 8;
+  if (m->H < step || m->I < step || m->H % step || m->I % step || m->H >= kMostSize ||
+      m->I >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: H=%d and I=%d must be multiples of %d below 2^22", fn, m->H,
+                m->I, step);
+  if (k < 1 || k > 64) return fail(DB_ERR_INVALID, "%s: k=%d outside [1, 64]", fn, k);
+  if (T < 0 || T >= kMostTokens)
+    return fail(DB_ERR_INVALID, "%s: T=%d must be >= 0 and below 2^20", fn, T);
+  if (x_stride < m->H || x_stride % 8 != 0)
+    return fail(DB_ERR_INVALID, "%s: x rows must hold H elements and be 16-byte aligned", fn);
+  const long long pairs = (long long)T * k;
+  if (x_stride >= kMostOffset || T * x_stride >= kMostOffset || pairs * m->I >= kMostOffset ||
+      pairs * m->H >= kMostOffset)
+    return fail(DB_ERR_INVALID, "%s: T=%d tokens are too many for one call", fn, T);
+  if (fp8 ? !m->sg || !m->su || !m->sd : m->sg || m->su || m->sd)
+    return fail(DB_ERR_INVALID, fp8 ? "%s: e4m3 weights need a scale for each block"
+                                    : "%s: 16-bit weights take no scales", fn);
+  if (!aligned4(m->sg) || !aligned4(m->su) || !aligned4(m->sd))
+    return fail(DB_ERR_INVALID, "%s: scales must be 4-byte aligned", fn);
+  if (T == 0) return DB_OK;
+  if (!x || !y || !m->wg || !m->wu || !m->wd)
+    return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(x) || !aligned16(y) || !aligned16(m->wg) || !aligned16(m->wu) ||
+      !aligned16(m->wd))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  return DB_OK;
+}
+
+dbk::MoeExpertsCall experts_call(const void* x, long long x_stride, const int* experts,
+                                 const float* weights, const db_moe& m, void* y, int T, int k) {
+  dbk::MoeExpertsCall c = {};
+  c.x = x;
+  c.x_row = x_stride;
+  c.experts = experts;
+  c.weights = weights;
+  c.y = y;
+  c.w = m;
+  c.T = T;
+  c.k = k;
+  c.bf16 = m.dtype == DB_DTYPE_BF16;
+  return c;
+}
+
+// The parts of a layer's workspace: what the router gives, then what each half needs.
+struct LayerSpace {
+  size_t experts, weights, rest, bytes;
+};
+LayerSpace layer_space(const db_moe& m, int T, int k) {
+  const size_t pairs = (size_t)T * k;
+  LayerSpace s;
+  s.experts = 0;
+  s.weights = round256(pairs * sizeof(int));
+  s.rest = s.weights + round256(pairs * sizeof(float));
+  s.bytes = s.rest + db_moe_route_workspace_bytes(T, m.E) + db_moe_experts_workspace_bytes(&m, T, k);
+  return s;
+}
+
+}  // namespace
+
+extern "C" {
+
+int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
+                       long long scale_t, long long scale_b, int T, int K, int dtype,
+                       void* stream) {
+  const char* fn = "db_quantize_blocks";
+  if (!is16bit(dtype)) return fail(DB_ERR_INVALID, "%s: unknown activation dtype %d", fn, dtype);
+  if (T < 0 || T >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: T=%d must be >= 0 and below 2^22", fn, T);
+  if (K < 16 || K % 16 != 0 || K >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: K=%d must be a multiple of 16 below 2^22", fn, K);
+  if (x_stride < K || x_stride % 8 != 0)
+    return fail(DB_ERR_INVALID, "%s: x rows must hold K elements and be 16-byte aligned", fn);
+  if (scale_t < 0 || scale_b < 0 || (T > 1 && !scale_t) || (T > 0 && K > 128 && !scale_b))
+    return fail(DB_ERR_INVALID, "%s: scales must not share memory", fn);
+  if (T == 0) return ok();
+  if (!x || !q || !scale) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(x) || !aligned16(q))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (!aligned4(scale)) return fail(DB_ERR_INVALID, "%s: scales must be 4-byte aligned", fn);
+  const dbk::QuantCall c = {x, q, scale, x_stride, scale_t, scale_b, T, K, dtype == DB_DTYPE_BF16};
+  return hip_status(dbk::launch_quantize_blocks(c, (hipStream_t)stream), fn);
+}
+
+size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype) {
+  if (T < 1 || K < 1 || N < 1 || T >= kMostSize || K >= kMostSize || N >= kMostSize) return 0;
+  return is16bit(x_dtype) ? quantized_bytes(T, K) : 0;
+}
+
+int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long long xs_t,
+                   long long xs_b, const void* W, const float* w_scale, void* y, int T, int K,
+                   int N, int x_dtype, int y_dtype, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "db_gemm_blocks";
+  if (!is16bit(y_dtype)) return fail(DB_ERR_INVALID, "%s: unknown output dtype %d", fn, y_dtype);
+  const bool fp8 = x_dtype == DB_DTYPE_FP8_E4M3;
+  if (!fp8 && x_dtype != y_dtype)
+    return fail(DB_ERR_INVALID, "%s: x must be e4m3 or have the output's type", fn);
+  if (T < 0 || T >= kMostSize || N < 1 || N >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: need T >= 0 and N >= 1 below 2^22 (got %d %d)", fn, T, N);
+  if (K < 16 || K % 16 != 0 || K >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: K=%d must be a multiple of 16 below 2^22", fn, K);
+  if (x_stride < K || x_stride % (fp8 ? 16 : 8) != 0 || x_stride >= kMostOffset / 64)
+    return fail(DB_ERR_INVALID, "%s: x rows must hold K elements, be 16-byte aligned and less "
+                "than 2^23 elements apart", fn);
+  if (fp8 ? !x_scale : x_scale != nullptr)
+    return fail(DB_ERR_INVALID, fp8 ? "%s: e4m3 activations need a scale for each block"
+                                    : "%s: 16-bit activations take no scales", fn);
+  if (xs_t < 0 || xs_b < 0) return fail(DB_ERR_INVALID, "%s: strides must be >= 0", fn);
+  if (T == 0) return ok();
+  if (!x || !W || !w_scale || !y) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned16(x) || !aligned16(W) || !aligned16(y))
+    return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (!aligned4(x_scale) || !aligned4(w_scale))
+    return fail(DB_ERR_INVALID, "%s: scales must be 4-byte aligned", fn);
+  const int rc =
+      check_workspace(fn, ws, ws_bytes, db_gemm_blocks_workspace_bytes(T, K, N, x_dtype));
+  if (rc) return rc;
+  dbk::GemmBlocksCall c = {x, x_scale, W, w_scale, y, x_stride, xs_t, xs_b, T, K, N,
+                           y_dtype == DB_DTYPE_BF16};
+  if (!fp8) {
+    char* const q = static_cast<char*>(ws);
+    float* const scale = reinterpret_cast<float*>(q + round256((size_t)T * K));
+    const dbk::QuantCall quant = {x, q, scale, x_stride, 1, T, T, K, c.bf16};
+    const hipError_t e = dbk::launch_quantize_blocks(quant, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_status(e, fn);
+    c.x = q;
+    c.x_scale = scale;
+    c.x_row = K;
+    c.xs_t = 1;
+    c.xs_b = T;
+  }
+  return hip_status(dbk::launch_gemm_blocks(c, (hipStream_t)stream), fn);
+}
+
+size_t db_moe_route_workspace_bytes(int T, int E) {
+  if (T < 1 || T >= kMostTokens || E < 1 || E > 1024) return 0;
+  return round256((size_t)T * E * sizeof(double));
+}
+
+int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts, float* weights,
+                 int T, int H, int E, int k, int renormalize, int dtype, void* ws,
+                 size_t ws_bytes, void* stream) {
+  const char* fn = "db_moe_route";
+  int rc = check_route(fn, x, x_stride, Wr, T, H, E, k, dtype);
+  if (rc) return rc;
+  if (T == 0) return ok();
+  if (!experts || !weights) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned4(experts) || !aligned4(weights))
+    return fail(DB_ERR_INVALID, "%s: experts and weights must be 4-byte aligned", fn);
+  rc = check_workspace(fn, ws, ws_bytes, db_moe_route_workspace_bytes(T, E));
+  if (rc) return rc;
+  const dbk::MoeRouteCall c = {x, Wr, experts, weights, static_cast<double*>(ws), x_stride, T, H,
+                               E, k, renormalize != 0, dtype == DB_DTYPE_BF16};
+  return hip_status(dbk::launch_moe_route(c, (hipStream_t)stream), fn);
+}
+
+size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k) {
+  if (!m || T < 1 || T >= kMostTokens || k < 1 || k > 64 || m->E < 1 || m->E > 1024 || m->H < 1 ||
+      m->I < 1 || m->H >= kMostSize || m->I >= kMostSize)
+    return 0;
+  dbk::MoeExpertsCall c = experts_call(nullptr, 0, nullptr, nullptr, *m, nullptr, T, k);
+  return dbk::moe_experts_workspace(c, nullptr);
+}
+
+int db_moe_experts(const void* x, long long x_stride, const int* experts, const float* weights,
+                   const db_moe* m, void* y, int T, int k, void* ws, size_t ws_bytes,
+                   void* stream) {
+  const char* fn = "db_moe_experts";
+  int rc = check_moe(fn, m, x, x_stride, y, T, k);
+  if (rc) return rc;
+  if (T == 0) return ok();
+  if (!experts || !weights) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!aligned4(experts) || !aligned4(weights))
+    return fail(DB_ERR_INVALID, "%s: experts and weights must be 4-byte aligned", fn);
+  rc = check_workspace(fn, ws, ws_bytes, db_moe_experts_workspace_bytes(m, T, k));
+  if (rc) return rc;
+  dbk::MoeExpertsCall c = experts_call(x, x_stride, experts, weights, *m, y, T, k);
+  dbk::moe_experts_workspace(c, ws);
+  return hip_status(dbk::launch_moe_experts(c, (hipStream_t)stream), fn);
+}
+
+size_t db_moe_layer_workspace_bytes(const db_moe* m, int T, int k) {
+  if (!m || db_moe_experts_workspace_bytes(m, T, k) == 0) return 0;
+  return layer_space(*m, T, k).bytes;
+}
+
+int db_moe_layer(const void* x, long long x_stride, const void* Wr, const db_moe* m, void* y,
+                 int T, int k, int renormalize, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "db_moe_layer";
+  int rc = check_moe(fn, m, x, x_stride, y, T, k);
+  if (!rc) rc = check_route(fn, x, x_stride, Wr, T, m->H, m->E, k, m->dtype);
+  if (rc) return rc;
+  if (T == 0) return ok();
+  rc = check_workspace(fn, ws, ws_bytes, db_moe_layer_workspace_bytes(m, T, k));
+  if (rc) return rc;
+  const LayerSpace s = layer_space(*m, T, k);
+  char* const p = static_cast<char*>(ws);
+  int* const experts = reinterpret_cast<int*>(p + s.experts);
+  float* const weights = reinterpret_cast<float*>(p + s.weights);
+  const size_t logits = db_moe_route_workspace_bytes(T, m->E);
+  const dbk::MoeRouteCall r = {x, Wr, experts, weights, reinterpret_cast<double*>(p + s.rest),
+                               x_stride, T, m->H, m->E, k, renormalize != 0,
+                               m->dtype == DB_DTYPE_BF16};
+  const hipError_t e = dbk::launch_moe_route(r, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_status(e, fn);
+  dbk::MoeExpertsCall c = experts_call(x, x_stride, experts, weights, *m, y, T, k);
+  dbk::moe_experts_workspace(c, p + s.rest + logits);
+  return hip_status(dbk::launch_moe_experts(c, (hipStream_t)stream), fn);
+}
+
+}  // extern "C"

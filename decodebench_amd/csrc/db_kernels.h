@@ -179,6 +179,62 @@ struct PagedCall {
 size_t paged_workspace_bytes(const PagedCall& c, int cu_count, size_t* zeroed);
 hipError_t launch_paged_attention(const PagedCall& c, int cu_count, void* ws, hipStream_t stream);
 
+// Block-scaled e4m3 (quant_blocks.hip, gemm_blocks.hip): the arguments of the
+// entry points as the kernels take them (checked by the caller).
+struct QuantCall {
+  const void* x;      // [T, K], rows x_row elements apart
+  void* q;            // [T, K]
+  float* scale;       // [T, ceil(K / 128)] at the strides below
+  long long x_row, scale_t, scale_b;
+  int T, K;
+  bool bf16;
+};
+hipError_t launch_quantize_blocks(const QuantCall& c, hipStream_t stream);
+
+struct GemmBlocksCall {
+  const void* x;         // [T, K] e4m3, rows x_row apart
+  const float* x_scale;  // [T, ceil(K / 128)] at the strides below
+  const void* W;         // [N, K] e4m3
+  const float* w_scale;  // [ceil(N / 128), ceil(K / 128)]
+  void* y;               // [T, N]
+  long long x_row, xs_t, xs_b;
+  int T, K, N;
+  bool bf16;             // type of y
+};
+hipError_t launch_gemm_blocks(const GemmBlocksCall& c, hipStream_t stream);
+
+// A mixture-of-experts layer (moe_route.hip, moe_experts.hip).
+struct MoeRouteCall {
+  const void* x;       // [T, H], rows x_row elements apart
+  const void* router;  // [E, H]
+  int* experts;        // [T, k]
+  float* weights;      // [T, k]
+  double* logits;      // [T, E] workspace
+  long long x_row;
+  int T, H, E, k;
+  bool renormalize, bf16;
+};
+hipError_t launch_moe_route(const MoeRouteCall& c, hipStream_t stream);
+
+struct MoeExpertsCall {
+  const void* x;         // [T, H], rows x_row elements apart
+  const int* experts;    // [T, k]
+  const float* weights;  // [T, k]
+  void* y;               // [T, H]
+  db_moe w;
+  long long x_row;
+  int T, k;
+  bool bf16;
+  // workspace
+  int* order;    // [T k] pairs sorted by expert
+  int* tiles;    // count, then (expert, first slot, pairs) of each tile
+  void* h;       // [T k, I] by slot
+  float* parts;  // [T k, H] by pair
+};
+// Lays the workspace out from ws on; returns its bytes.
+size_t moe_experts_workspace(MoeExpertsCall& c, void* ws);
+hipError_t launch_moe_experts(const MoeExpertsCall& c, hipStream_t stream);
+
 // Read-only streaming probe (stream_probe.hip): `bytes` (a multiple of
 // kb_per_wave KB, kb_per_wave in {4, 8, 16}) read once, kb_per_wave KB per
 // wave; sink needs bytes / 16 words and is written only when the folded

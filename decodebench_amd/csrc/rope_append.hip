@@ -43,11 +43,6 @@ __device__ __forceinline__ u4 pack8(const float (&x)[8]) {
   return __builtin_bit_cast(u4, r);
 }
 
-// NaN stays NaN, everything else is clamped to the largest finite e4m3.
-__device__ __forceinline__ float clamp448(float x) {
-  return x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x;
-}
-
 __device__ __forceinline__ u2 pack8_e4m3(const float (&x)[8], float scale) {
   u2 r;
 #pragma unroll

@@ -63,6 +63,13 @@ class _PagedCache(C.Structure):
                 ("pages", _i), ("page_size", _i), ("Hkv", _i), ("D", _i), ("dtype", _i)]
 
 
+class _Moe(C.Structure):
+    """``db_moe`` of the C ABI."""
+
+    _fields_ = [("wg", _p), ("wu", _p), ("wd", _p), ("sg", _p), ("su", _p), ("sd", _p),
+                ("E", _i), ("H", _i), ("I", _i), ("dtype", _i), ("w_dtype", _i)]
+
+
 def load_library():
     """Load the HIP library (after torch, so both share one HIP runtime)."""
     global _lib
@@ -105,6 +112,19 @@ def load_library():
             "db_paged_attention": (_i, [_p, _ll, _ll, _p, C.POINTER(_PagedCache), _p, _ll, _i, _p,
                                         _p, _i, _i, _i, _i, C.c_float, _i, _i, _i, _p,
                                         C.c_size_t, _p]),
+            "db_quantize_blocks": (_i, [_p, _ll, _p, _p, _ll, _ll, _i, _i, _i, _p]),
+            "db_gemm_blocks_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i]),
+            "db_gemm_blocks": (_i, [_p, _ll, _p, _ll, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _p,
+                                    C.c_size_t, _p]),
+            "db_moe_route_workspace_bytes": (C.c_size_t, [_i, _i]),
+            "db_moe_route": (_i, [_p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, C.c_size_t,
+                                  _p]),
+            "db_moe_experts_workspace_bytes": (C.c_size_t, [C.POINTER(_Moe), _i, _i]),
+            "db_moe_experts": (_i, [_p, _ll, _p, _p, C.POINTER(_Moe), _p, _i, _i, _p, C.c_size_t,
+                                    _p]),
+            "db_moe_layer_workspace_bytes": (C.c_size_t, [C.POINTER(_Moe), _i, _i]),
+            "db_moe_layer": (_i, [_p, _ll, _p, C.POINTER(_Moe), _p, _i, _i, _i, _p, C.c_size_t,
+                                  _p]),
             "db_stream_read": (_i, [_p, C.c_size_t, _i, C.c_uint, _p, _p]),
             "db_stream_capture_id": (_i, [_p, C.POINTER(C.c_ulonglong)]),
             "db_tune": (_i, [C.c_char_p, _i]),
@@ -883,3 +903,229 @@ def paged_attention(q, K, V, block_table, q_start, kv_len, scale: float | None =
             q_start.data_ptr(), kv_len.data_ptr(), T, R, Hq, most, scale, bool(causal),
             min(int(window or 0), _INT_MAX), dt, ws.data_ptr(), nbytes)
     return o
+
+
+# ------------------------------------- block-scaled e4m3, mixture of experts
+def _workspace(nbytes: int, device):
+    """Memory of one call from torch's allocator, which takes it back in stream
+    order; nothing in it outlives the call."""
+    return _torch.empty(nbytes, dtype=_torch.uint8, device=device) if nbytes else None
+
+
+def _blocks(n: int) -> int:
+    return -(-n // 128)
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def quantize_blocks(x):
+    """e4m3 with one fp32 scale for each 128 elements of a row: ``(q, scale)``,
+    q float8_e4m3fn [T, K] and scale [T, ceil(K / 128)] (a block's tokens side by
+    side in memory, as :func:`gemm_blocks` reads them best).
+
+    x [T, K] fp16 or bf16 (rows may be strided), K a multiple of 16.
+    ``scale[t, b] = max |x[t, 128 b ..]| / 448`` (1 where that is 0) and
+    ``q = e4m3(clamp(x / scale, -448, 448))``, rounded to nearest even; an Inf or
+    NaN makes its block's scale one."""
+    torch = _torch or _torch_mod()
+    idx = _strided(x, "x", None, 2)
+    dt = _activation(x, "x")
+    T, K = x.shape
+    q = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((_blocks(K), T), dtype=torch.float32, device=x.device).t()
+    _launch((_lib or load_library()).db_quantize_blocks, idx, "db_quantize_blocks", x.data_ptr(),
+            _row_stride(x), q.data_ptr(), scale.data_ptr(), 1, T, T, K, dt)
+    return q, scale
+
+
+def _block_scale(s, name: str, shape, idx: int):
+    """The fp32 scales of e4m3 weights, one for each block of 128 x 128."""
+    if s is None:
+        raise ValueError(f"e4m3 weights need {name}, an fp32 tensor of shape {shape}")
+    _one_gpu(idx, (_gpu_tensors((s, name, _torch.float32)), name))
+    if tuple(s.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape} (got {tuple(s.shape)})")
+    return s.data_ptr()
+
+
+def gemm_blocks(x, W, w_scale, x_scale=None, dtype=None, out=None):
+    """Projection ``y = x W^T`` on e4m3 weights with one fp32 scale for each
+    block of 128 x 128, by 8-bit matrix instructions; fp32 sums, rounded once.
+
+    W [N, K] float8_e4m3fn (or its bytes), w_scale [ceil(N/128), ceil(K/128)]
+    (``quant.quantize_e4m3_blocks``), K a multiple of 16.  x [T, K] (or [K]) fp16
+    or bf16 is quantised on the way, as :func:`quantize_blocks` does, and
+    y [T, N] has its type; or x is float8_e4m3fn with x_scale [T, ceil(K/128)],
+    and y is ``dtype`` (torch.float16 if not given).  Rows of x may be strided,
+    and x_scale anyhow."""
+    torch = _torch or _torch_mod()
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    x2, squeeze = _as_2d(x, "x")
+    idx = _strided(x2, "x", None, 2)
+    T, K = x2.shape
+    if x2.dtype == torch.float8_e4m3fn:
+        xdt, dtype = DTYPE_FP8_E4M3, dtype or torch.float16
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be torch.float16 or torch.bfloat16 (got {dtype})")
+        ydt = DTYPE_F16 if dtype == torch.float16 else DTYPE_BF16
+        if x_scale is None:
+            raise ValueError(f"e4m3 activations need x_scale, an fp32 tensor of shape "
+                             f"{(T, _blocks(K))}")
+        if not isinstance(x_scale, torch.Tensor):
+            raise TypeError("x_scale must be a torch.Tensor")
+        xs = x_scale.unsqueeze(0) if squeeze and x_scale.dim() == 1 else x_scale
+        if not xs.is_cuda or xs.dtype != torch.float32 or tuple(xs.shape) != (T, _blocks(K)):
+            raise ValueError(f"x_scale must be an fp32 GPU tensor of shape {(T, _blocks(K))} "
+                             f"(got {xs.dtype} {tuple(xs.shape)} on {xs.device})")
+        _one_gpu(idx, (xs.get_device(), "x_scale"))
+        xsp, (xs_t, xs_b) = xs.data_ptr(), _strides(xs, 2)
+    else:
+        xdt = ydt = _activation(x2, "x")
+        if x_scale is not None:
+            raise ValueError("16-bit activations take no x_scale")
+        if dtype is not None and dtype != x2.dtype:
+            raise TypeError(f"dtype must be {x2.dtype} like x (got {dtype})")
+        dtype, xsp, xs_t, xs_b = x2.dtype, None, 0, 0
+    if not isinstance(W, torch.Tensor) or W.dim() != 2 or W.shape[1] != K:
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)}, "
+                         f"W {tuple(getattr(W, 'shape', ()))}")
+    if W.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        raise TypeError(f"W must be torch.float8_e4m3fn (got {W.dtype})")
+    _one_gpu(idx, (_gpu_tensors((W, "W", None)), "W"))
+    N = W.shape[0]
+    sp = _block_scale(w_scale, "w_scale", (_blocks(N), _blocks(K)), idx)
+    y = _row_output((T, N), dtype, idx, out)
+    lib = _lib or load_library()
+    with _on_device(idx):
+        nbytes = lib.db_gemm_blocks_workspace_bytes(T, K, N, xdt)
+    ws = _workspace(nbytes, x.device)
+    _launch(lib.db_gemm_blocks, idx, "db_gemm_blocks", x2.data_ptr(), _row_stride(x2), xsp, xs_t,
+            xs_b, W.data_ptr(), sp, y.data_ptr(), T, K, N, xdt, ydt,
+            None if ws is None else ws.data_ptr(), nbytes)
+    return y[0] if squeeze else y
+
+
+def _router(x, Wr, top_k):
+    torch = _torch or _torch_mod()
+    idx = _strided(x, "x", None, 2)
+    dt = _activation(x, "x")
+    _one_gpu(idx, (_gpu_tensors((Wr, "Wr", x.dtype)), "Wr"))
+    if Wr.dim() != 2 or Wr.shape[1] != x.shape[1]:
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)}, Wr {tuple(Wr.shape)}")
+    k = int(top_k)
+    if not 1 <= k <= Wr.shape[0]:
+        raise ValueError(f"top_k must be between 1 and the {Wr.shape[0]} experts (got {k})")
+    return idx, dt, k
+
+
+def moe_route(x, Wr, top_k: int, renormalize: bool = True):
+    """The experts of each token and their weights: ``(experts, weights)``,
+    int32 and fp32 [T, top_k], the largest first.
+
+    x [T, H] fp16 or bf16 (rows may be strided), Wr [E, H] of that type, H a
+    multiple of 8, E <= 1024, top_k <= 64.  The logits ``x Wr^T`` are summed in
+    64 bits; equal ones go to the lower index, NaN counts above all numbers.
+    Weights are the softmax over the chosen experts (``renormalize``) or
+    over all of them."""
+    idx, dt, k = _router(x, Wr, top_k)
+    torch = _torch
+    T, H = x.shape
+    E = Wr.shape[0]
+    experts = torch.empty((T, k), dtype=torch.int32, device=x.device)
+    weights = torch.empty((T, k), dtype=torch.float32, device=x.device)
+    lib = _lib or load_library()
+    with _on_device(idx):
+        nbytes = lib.db_moe_route_workspace_bytes(T, E)
+    ws = _workspace(nbytes, x.device)
+    _launch(lib.db_moe_route, idx, "db_moe_route", x.data_ptr(), _row_stride(x), Wr.data_ptr(),
+            experts.data_ptr(), weights.data_ptr(), T, H, E, k, bool(renormalize), dt,
+            None if ws is None else ws.data_ptr(), nbytes)
+    return experts, weights
+
+
+def _experts(x, Wg, Wu, Wd, sg, su, sd, idx: int, dt: int):
+    """The experts' weights as the C ABI takes them: of x's type, or e4m3 with
+    fp32 scales of blocks of 128 x 128."""
+    torch = _torch
+    H = x.shape[1]
+    _one_gpu(idx, (_gpu_tensors((Wg, "Wg", None), (Wu, "Wu", None), (Wd, "Wd", None)), "Wg"))
+    if Wg.dim() != 3 or Wg.shape[2] != H or Wu.shape != Wg.shape or \
+            tuple(Wd.shape) != (Wg.shape[0], H, Wg.shape[1]):
+        raise ValueError(f"expected Wg, Wu [E, I, {H}] and Wd [E, {H}, I]; got "
+                         f"{tuple(Wg.shape)}, {tuple(Wu.shape)}, {tuple(Wd.shape)}")
+    if Wu.dtype != Wg.dtype or Wd.dtype != Wg.dtype:
+        raise TypeError(f"Wg, Wu and Wd must have one type (got {Wg.dtype}, {Wu.dtype}, "
+                        f"{Wd.dtype})")
+    E, I = Wg.shape[:2]
+    m = _Moe(Wg.data_ptr(), Wu.data_ptr(), Wd.data_ptr(), None, None, None, E, H, I, dt, dt)
+    if Wg.dtype in (torch.float8_e4m3fn, torch.uint8):
+        m.w_dtype = DTYPE_FP8_E4M3
+        m.sg = _block_scale(sg, "sg", (E, _blocks(I), _blocks(H)), idx)
+        m.su = _block_scale(su, "su", (E, _blocks(I), _blocks(H)), idx)
+        m.sd = _block_scale(sd, "sd", (E, _blocks(H), _blocks(I)), idx)
+    elif Wg.dtype != x.dtype:
+        raise TypeError(f"the experts' weights must be {x.dtype} like x or "
+                        f"torch.float8_e4m3fn (got {Wg.dtype})")
+    elif sg is not None or su is not None or sd is not None:
+        raise ValueError("16-bit weights take no scales")
+    return m
+
+
+def moe_experts(x, experts, weights, Wg, Wu, Wd, sg=None, su=None, sd=None, out=None):
+    """The experts of a mixture-of-experts layer on tokens that are routed:
+    ``y[t] = sum_j weights[t, j] Wd[e] (silu(Wg[e] x[t]) * (Wu[e] x[t]))``,
+    e = experts[t, j].  Returns [T, H] of x's type.
+
+    x [T, H] fp16 or bf16 (rows may be strided); experts int32 and weights fp32
+    [T, k], as :func:`moe_route` gives them; Wg, Wu [E, I, H] and Wd [E, H, I] of
+    x's type, or float8_e4m3fn (or its bytes) with fp32 scales of blocks of
+    128 x 128 (sg, su [E, ceil(I/128), ceil(H/128)], sd [E, ceil(H/128),
+    ceil(I/128)]).  H and I are multiples of 8, of 16 for e4m3.
+
+    An expert outside [0, E) adds nothing; a token without any gets zeros; an
+    expert named twice counts twice.  Sums are fp32; what the gate gives is
+    rounded to x's type before the down product, and the result once.  Made for
+    the few tokens of a decode step: the weights bound the call."""
+    torch = _torch or _torch_mod()
+    idx = _strided(x, "x", None, 2)
+    dt = _activation(x, "x")
+    _one_gpu(idx, (_gpu_tensors((experts, "experts", torch.int32),
+                                (weights, "weights", torch.float32)), "experts"))
+    T, H = x.shape
+    if experts.dim() != 2 or experts.shape[0] != T or experts.shape != weights.shape:
+        raise ValueError(f"experts {tuple(experts.shape)} and weights {tuple(weights.shape)} "
+                         f"must be [{T}, k]")
+    k = experts.shape[1]
+    m = _experts(x, Wg, Wu, Wd, sg, su, sd, idx, dt)
+    y = _row_output((T, H), x.dtype, idx, out)
+    lib = _lib or load_library()
+    with _on_device(idx):
+        nbytes = lib.db_moe_experts_workspace_bytes(C.byref(m), T, k)
+    ws = _workspace(nbytes, x.device)
+    _launch(lib.db_moe_experts, idx, "db_moe_experts", x.data_ptr(), _row_stride(x),
+            experts.data_ptr(), weights.data_ptr(), C.byref(m), y.data_ptr(), T, k,
+            None if ws is None else ws.data_ptr(), nbytes)
+    return y
+
+
+def moe_layer(x, Wr, Wg, Wu, Wd, top_k: int, renormalize: bool = True, sg=None, su=None, sd=None,
+              out=None):
+    """A whole mixture-of-experts layer: :func:`moe_route` and
+    :func:`moe_experts` in one call, with their arguments.  Returns [T, H]."""
+    idx, dt, k = _router(x, Wr, top_k)
+    m = _experts(x, Wg, Wu, Wd, sg, su, sd, idx, dt)
+    if Wr.shape[0] != m.E:
+        raise ValueError(f"Wr has {Wr.shape[0]} rows for {m.E} experts")
+    T, H = x.shape
+    y = _row_output((T, H), x.dtype, idx, out)
+    lib = _lib or load_library()
+    with _on_device(idx):
+        nbytes = lib.db_moe_layer_workspace_bytes(C.byref(m), T, k)
+    ws = _workspace(nbytes, x.device)
+    _launch(lib.db_moe_layer, idx, "db_moe_layer", x.data_ptr(), _row_stride(x), Wr.data_ptr(),
+            C.byref(m), y.data_ptr(), T, k, bool(renormalize),
+            None if ws is None else ws.data_ptr(), nbytes)
+    return y

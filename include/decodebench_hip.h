@@ -285,6 +285,81 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
                        int causal, int window, int dtype, void* ws, size_t ws_bytes,
                        void* stream);
 
+/* ---- e4m3 with a scale for each block of 128 ------------------------------
+ * Activations [T, K] have one fp32 scale for each 128 elements of a row,
+ * weights [N, K] one for each 128 x 128 elements ([ceil(N / 128), ceil(K / 128)],
+ * dense); the last block of a dimension may be short.  No counterpart in the
+ * reference, whose weights are fp16
+ * (src/decodebench/demos/llama_decode.py:110-116).
+ *
+ * scale[t, b] = max |x[t, 128 b ..]| / 448 in fp32 (1 where that is 0), q =
+ * e4m3(clamp(x / scale, -448, 448)), rounded to nearest even.  A block that holds an Inf or
+ * NaN gets that scale, so it stays visible.
+ * Contract: x [T, K] of dtype DB_DTYPE_F16 or DB_DTYPE_BF16, rows x_stride
+ * elements apart and 16-byte aligned; q [T, K] dense, 16-byte aligned; scale
+ * element (t, b) at t scale_t + b scale_b, no two at one place; K a multiple of
+ * 16; T >= 0; T, K < 2^22. */
+int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
+                       long long scale_t, long long scale_b, int T, int K, int dtype,
+                       void* stream);
+
+/* y[t, n] = sum_b xs[t, b] ws[n / 128, b] sum_{k in b} x[t, k] W[n, k], fp32 sums, one
+ * rounding to y's type.  x is e4m3 with x_scale (element (t, b) at t xs_t + b xs_b), or
+ * of y's type with x_scale NULL: then it is quantised first, as db_quantize_blocks does.
+ * Contract: x_dtype DB_DTYPE_FP8_E4M3 or y_dtype; y_dtype DB_DTYPE_F16 or
+ * DB_DTYPE_BF16; x rows x_stride elements apart and 16-byte aligned; W [N, K] and y
+ * [T, N] dense; K a multiple of 16; T, N, K < 2^22, 64 x_stride < 2^29; W and ws 16-byte
+ * aligned.  ws of db_gemm_blocks_workspace_bytes (NULL if 0) needs no initialisation
+ * and holds nothing after the call; calls that overlap in time need their own. */
+size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype);
+int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long long xs_t,
+                   long long xs_b, const void* W, const float* w_scale, void* y, int T, int K,
+                   int N, int x_dtype, int y_dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- a mixture-of-experts layer for a few tokens --------------------------
+ * No counterpart in the reference, whose feed-forward part is one gated
+ * product (src/decodebench/demos/llama_decode.py:77-87). */
+typedef struct db_moe {
+  const void* wg;   /* [E, I, H] */
+  const void* wu;   /* [E, I, H] */
+  const void* wd;   /* [E, H, I] */
+  const float* sg;  /* e4m3 only: scales of blocks of 128 x 128, [E, ceil(I/128), ceil(H/128)] */
+  const float* su;
+  const float* sd;  /* [E, ceil(H/128), ceil(I/128)] */
+  int E, H, I;
+  int dtype;        /* of x and y: DB_DTYPE_F16 or DB_DTYPE_BF16 */
+  int w_dtype;      /* dtype, or DB_DTYPE_FP8_E4M3 */
+} db_moe;
+
+/* The experts of each token and their weights: logits x . Wr[e] (sums in 64 bits),
+ * experts [T, k] those of the k largest, largest first, ties to the lower index, NaN
+ * above all numbers; weights [T, k] = softmax over the k (renormalize) or over all E.
+ * Contract: x [T, H] rows x_stride elements apart and 16-byte aligned, Wr [E, H] dense,
+ * both of dtype; H a multiple of 8 below 2^22; 1 <= k <= E, k <= 64, E <= 1024; 0 <= T < 2^20;
+ * ws of db_moe_route_workspace_bytes, 256-byte aligned, as that of db_gemm_blocks. */
+size_t db_moe_route_workspace_bytes(int T, int E);
+int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts, float* weights,
+                 int T, int H, int E, int k, int renormalize, int dtype, void* ws,
+                 size_t ws_bytes, void* stream);
+
+/* y[t] = sum_j weights[t, j] Wd[e] h, h = silu(Wg[e] x[t]) * (Wu[e] x[t]) rounded to
+ * x's type, e = experts[t, j]; sums in fp32, one rounding.  An expert outside [0, E)
+ * adds nothing, whatever its weight; a token without any gets zeros.  An expert named
+ * twice counts twice.
+ * Contract: x, experts, weights, T, k as db_moe_route (k need not be below E); H and I
+ * multiples of 8 (16 for e4m3 weights) below 2^22; T x_stride, T k I and T k H below 2^29;
+ * weights 16-byte, scales 4-byte aligned, y [T, H] dense; ws of
+ * db_moe_experts_workspace_bytes, 256-byte aligned, as that of db_gemm_blocks. */
+size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k);
+int db_moe_experts(const void* x, long long x_stride, const int* experts, const float* weights,
+                   const db_moe* m, void* y, int T, int k, void* ws, size_t ws_bytes,
+                   void* stream);
+
+/* db_moe_route and db_moe_experts in one call: the whole layer. */
+size_t db_moe_layer_workspace_bytes(const db_moe* m, int T, int k);
+int db_moe_layer(const void* x, long long x_stride, const void* Wr, const db_moe* m, void* y,
+                 int T, int k, int renormalize, void* ws, size_t ws_bytes, void* stream);
+
 /* Capture state of `stream`: *capture_id is the id of the hipGraph capture
  * the stream is recording into (unique per capture), or 0 when it is not
  * capturing.  Host plumbing with no counterpart in the reference: the
