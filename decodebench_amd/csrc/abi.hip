@@ -842,9 +842,9 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
     return fail(DB_ERR_INVALID, "%s: need T >= 0 and N >= 1 below 2^22 (got %d %d)", fn, T, N);
   if (K < 16 || K % 16 != 0 || K >= kMostSize)
     return fail(DB_ERR_INVALID, "%s: K=%d must be a multiple of 16 below 2^22", fn, K);
-  if (x_stride < K || x_stride % (fp8 ? 16 : 8) != 0 || x_stride >= kMostOffset / 64)
+  if (x_stride < K || x_stride % (fp8 ? 16 : 8) != 0 || x_stride >= kMostSize)
     return fail(DB_ERR_INVALID, "%s: x rows must hold K elements, be 16-byte aligned and less "
-                "than 2^23 elements apart", fn);
+                "than 2^22 elements apart", fn);
   if (fp8 ? !x_scale : x_scale != nullptr)
     return fail(DB_ERR_INVALID, fp8 ? "%s: e4m3 activations need a scale for each block"
                                     : "%s: 16-bit activations take no scales", fn);

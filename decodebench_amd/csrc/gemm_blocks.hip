@@ -99,8 +99,154 @@ __global__ __launch_bounds__(kThreads) void gemm_blocks_rows(GemmBlocksCall c) {
   }
 }
 
+// ------------------------------------------------------------- full tiles
+// A workgroup has BN outputs by BT tokens, its waves WN by WT of them, and goes
+// through K a block at a time: while a block is multiplied from one half of
+// the LDS, the next one is on its way into the other (buffer_load .. lds, no
+// registers).  Rows of 128 bytes lie 16 bytes at a time in the order (chunk ^
+// row % 8), set by which global chunk a lane fetches: the 16 rows that a
+// quarter of a wave reads then lie in different banks.
+template <class E, int BN, int BT, int WN, int WT>
+__global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_tile(
+    GemmBlocksCall c) {
+  constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;
+  constexpr int kLoads = (BN + BT) / 8 / NW;  // of 8 rows, a wave
+  static_assert((BN + BT) % (8 * NW) == 0 && BN % (8 * kLoads) == 0, "whole loads");
+  constexpr int kHalf = (BN + BT) * 128;
+  __shared__ __align__(16) char s_a[kHalf];
+  __shared__ __align__(16) char s_b[kHalf];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int KB = (c.K + 127) / 128;
+
+  // Workgroups i, i + 8, .. run on one XCD: its share of the tiles is a
+  // compact part of the output, strips of eight token tiles wide.
+  const int tn = (c.N + BN - 1) / BN, tt = (c.T + BT - 1) / BT, all = tn * tt;
+  const int xcd = blockIdx.x & 7, each = all >> 3, more = all & 7;
+  const int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+  const int strip = at / (8 * tn), in = at - strip * 8 * tn, wide = min(8, tt - 8 * strip);
+  const int n0 = in / wide * BN, t0 = (8 * strip + in % wide) * BT;
+
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(
+      static_cast<const char*>(c.W) + (size_t)n0 * c.K, min(BN, c.N - n0) * c.K);
+  const __amdgpu_buffer_rsrc_t rx =
+      make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
+                (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
+  // This wave fetches rows 8 kLoads wave .. of the BN + BT.
+  const bool from_w = wave * kLoads * 8 < BN;
+  const int pitch = from_w ? c.K : (int)c.x_row;
+  const int row0 = (from_w ? wave * kLoads * 8 : wave * kLoads * 8 - BN) + (lane >> 3);
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  auto fetch = [&](char* half, int b) {
+    const int k = b * 128 + chunk;
+    const int off = (k < c.K ? k : kOut) + row0 * pitch;
+    char* const to = half + wave * kLoads * 1024;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      typedef __attribute__((address_space(3))) void lds;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(from_w ? rw : rx, (lds*)(to + i * 1024), 16,
+                                               off + i * 8 * pitch, 0, 0, 0);
+    }
+  };
+
+  const int wn = wave % (BN / WN) * WN, wt = wave / (BN / WN) * WT;
+  // scales of this lane's tokens, a block ahead
+  const float* xs[TI];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+    xs[i] = c.x_scale + min(t0 + wt + 16 * i + r16, c.T - 1) * c.xs_t;
+  const float* const ws = c.w_scale + (size_t)min((n0 + wn) / 128, (c.N - 1) / 128) * KB;
+  f4 acc[NI][TI] = {};
+  float scale[TI], ahead[TI], w_ahead;
+  auto load_scales = [&](int b) {
+    const int in = min(b, KB - 1);
+    w_ahead = ws[in];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) ahead[i] = xs[i][in * c.xs_b];
+  };
+  auto take_scales = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i) scale[i] = b < KB ? ahead[i] * w_ahead : 0.0f;
+  };
+  auto multiply = [&](const char* half) {
+    const int s0 = (q ^ (r16 & 7)) * 16, s1 = s0 ^ 64;
+    const char* const pw = half + (wn + r16) * 128;
+    const char* const px = half + (BN + wt + r16) * 128;
+    i8v x[TI];
+#pragma unroll
+    for (int j = 0; j < TI; ++j)
+      x[j] = join(ld16(px + j * 2048 + s0), ld16(px + j * 2048 + s1));
+    i8v w = join(ld16(pw + s0), ld16(pw + s1));
+    f4 p[TI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      // the products of row tile i beside the sums of i - 1 and the reads of i + 1
+      f4 now[TI];
+      i8v next = w;
+      if (i + 1 < NI)
+        next = join(ld16(pw + (i + 1) * 2048 + s0), ld16(pw + (i + 1) * 2048 + s1));
+#pragma unroll
+      for (int j = 0; j < TI; ++j) now[j] = product(w, x[j]);
+      if (i > 0) {
+#pragma unroll
+        for (int j = 0; j < TI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i - 1][j][e] += p[j][e] * scale[j];
+        // (an empty statement that holds the sums here: left free, they all sink
+        // to the end and their operands do not fit the registers)
+#pragma unroll
+        for (int j = 0; j < TI; ++j) asm volatile("" : "+v"(acc[i - 1][j]));
+      }
+#pragma unroll
+      for (int j = 0; j < TI; ++j) p[j] = now[j];
+      w = next;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < TI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[NI - 1][j][e] += p[j][e] * scale[j];
+  };
+  // Two blocks a turn, one from each half; behind the last one zeros are fetched
+  // and scaled by zero.
+  auto step = [&](int b, const char* half, char* other) {
+    __syncthreads();  // the block is there, and nobody reads the other half any more
+    take_scales(b);
+    fetch(other, b + 1);
+    load_scales(b + 1);
+    multiply(half);
+  };
+  fetch(s_a, 0);
+  load_scales(0);
+  for (int b = 0; b < KB; b += 2) {
+    step(b, s_a, s_b);
+    step(b + 1, s_b, s_a);
+  }
+#pragma unroll
+  for (int j = 0; j < TI; ++j) {
+    const int t = t0 + wt + 16 * j + r16;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int n = n0 + wn + 16 * i + 4 * q;
+      if (t < c.T && n < c.N)
+        store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, acc[i][j]);
+    }
+  }
+}
+
 template <class E>
 void launch(const GemmBlocksCall& c, hipStream_t stream) {
+  if (c.T > 64) {
+    const long long large = (long long)((c.N + 255) / 256) * ((c.T + 255) / 256);
+    if (large >= 256) {
+      gemm_blocks_tile<E, 256, 256, 128, 64><<<large, 512, 0, stream>>>(c);
+    } else {
+      const int n = (c.N + 127) / 128 * ((c.T + 127) / 128);
+      gemm_blocks_tile<E, 128, 128, 64, 64><<<n, 256, 0, stream>>>(c);
+    }
+    return;
+  }
   const int TT = c.T <= 16 ? 1 : c.T <= 32 ? 2 : 4;
   const dim3 grid((c.N + 15) / 16, (c.T + 16 * TT - 1) / (16 * TT));
   auto* const fn = TT == 1 ? gemm_blocks_rows<E, 1> : TT == 2 ? gemm_blocks_rows<E, 2>
