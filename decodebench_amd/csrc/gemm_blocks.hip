@@ -100,18 +100,21 @@ __global__ __launch_bounds__(kThreads) void gemm_blocks_rows(GemmBlocksCall c) {
 }
 
 // ------------------------------------------------------------- full tiles
-// A workgroup has BN outputs by BT tokens, its waves WN by WT of them, and goes
-// through K a block at a time: while a block is multiplied from one half of
-// the LDS, the next one is on its way into the other (buffer_load .. lds, no
-// registers).  Rows of 128 bytes lie 16 bytes at a time in the order (chunk ^
-// row % 8), set by which global chunk a lane fetches: the 16 rows that a
-// quarter of a wave reads then lie in different banks.
+// A workgroup has tiles of BN outputs by BT tokens, its waves WN by WT of them,
+// and goes through K a block at a time: while a block is multiplied from one
+// half of the LDS, the next one (behind the last, the first of the workgroup's
+// next tile) is on its way into the other (buffer_load .. lds, no registers).
+// Rows of 128 bytes lie 16 bytes at a time in the order (chunk ^ row % 8), set
+// by which global chunk a lane fetches: the 16 rows that a quarter of a wave
+// reads then lie in different banks.
 template <class E, int BN, int BT, int WN, int WT>
 __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_tile(
     GemmBlocksCall c) {
+  typedef typename E::type elem;
   constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;
   constexpr int kLoads = (BN + BT) / 8 / NW;  // of 8 rows, a wave
   static_assert((BN + BT) % (8 * NW) == 0 && BN % (8 * kLoads) == 0, "whole loads");
+  static_assert(NI % 2 == 0 && 128 % WN == 0, "row tiles in pairs, of one block of the weights");
   constexpr int kHalf = (BN + BT) * 128;
   __shared__ __align__(16) char s_a[kHalf];
   __shared__ __align__(16) char s_b[kHalf];
@@ -119,56 +122,56 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
   const int KB = (c.K + 127) / 128;
+  const int wn = wave % (BN / WN) * WN, wt = wave / (BN / WN) * WT;
 
   // Workgroups i, i + 8, .. run on one XCD: its share of the tiles is a
   // compact part of the output, strips of eight token tiles wide.
   const int tn = (c.N + BN - 1) / BN, tt = (c.T + BT - 1) / BT, all = tn * tt;
-  const int xcd = blockIdx.x & 7, each = all >> 3, more = all & 7;
-  const int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
-  const int strip = at / (8 * tn), in = at - strip * 8 * tn, wide = min(8, tt - 8 * strip);
-  const int n0 = in / wide * BN, t0 = (8 * strip + in % wide) * BT;
+  int n0, t0;
+  auto place = [&](int i) {
+    const int xcd = i & 7, each = all >> 3, more = all & 7;
+    const int at = xcd * each + min(xcd, more) + (i >> 3);
+    const int strip = at / (8 * tn), in = at - strip * 8 * tn, wide = min(8, tt - 8 * strip);
+    n0 = in / wide * BN;
+    t0 = (8 * strip + in % wide) * BT;
+  };
 
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(
-      static_cast<const char*>(c.W) + (size_t)n0 * c.K, min(BN, c.N - n0) * c.K);
-  const __amdgpu_buffer_rsrc_t rx =
-      make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
-                (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
   // This wave fetches rows 8 kLoads wave .. of the BN + BT.
   const bool from_w = wave * kLoads * 8 < BN;
   const int pitch = from_w ? c.K : (int)c.x_row;
-  const int row0 = (from_w ? wave * kLoads * 8 : wave * kLoads * 8 - BN) + (lane >> 3);
+  const int row0 = ((from_w ? wave * kLoads * 8 : wave * kLoads * 8 - BN) + (lane >> 3)) * pitch;
   const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  __amdgpu_buffer_rsrc_t rows_of;
+  // scales of this lane's tokens and of the wave's outputs, loaded a block ahead
+  const float *xs[TI], *ws;
+  float scale[TI], ahead[TI], w_ahead;
+  auto open = [&] {
+    rows_of = from_w ? make_rsrc(static_cast<const char*>(c.W) + (size_t)n0 * c.K,
+                                 min(BN, c.N - n0) * c.K)
+                     : make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
+                                 (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+      xs[i] = c.x_scale + min(t0 + wt + 16 * i + r16, c.T - 1) * c.xs_t;
+    ws = c.w_scale + (size_t)min((n0 + wn) / 128, (c.N - 1) / 128) * KB;
+  };
   auto fetch = [&](char* half, int b) {
     const int k = b * 128 + chunk;
-    const int off = (k < c.K ? k : kOut) + row0 * pitch;
+    const int off = (k < c.K ? k : kOut) + row0;
     char* const to = half + wave * kLoads * 1024;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       typedef __attribute__((address_space(3))) void lds;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(from_w ? rw : rx, (lds*)(to + i * 1024), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows_of, (lds*)(to + i * 1024), 16,
                                                off + i * 8 * pitch, 0, 0, 0);
     }
-  };
-
-  const int wn = wave % (BN / WN) * WN, wt = wave / (BN / WN) * WT;
-  // scales of this lane's tokens, a block ahead
-  const float* xs[TI];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-    xs[i] = c.x_scale + min(t0 + wt + 16 * i + r16, c.T - 1) * c.xs_t;
-  const float* const ws = c.w_scale + (size_t)min((n0 + wn) / 128, (c.N - 1) / 128) * KB;
-  f4 acc[NI][TI] = {};
-  float scale[TI], ahead[TI], w_ahead;
-  auto load_scales = [&](int b) {
     const int in = min(b, KB - 1);
     w_ahead = ws[in];
 #pragma unroll
     for (int i = 0; i < TI; ++i) ahead[i] = xs[i][in * c.xs_b];
   };
-  auto take_scales = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < TI; ++i) scale[i] = b < KB ? ahead[i] * w_ahead : 0.0f;
-  };
+
+  f4 acc[NI][TI];
   auto multiply = [&](const char* half) {
     const int s0 = (q ^ (r16 & 7)) * 16, s1 = s0 ^ 64;
     const char* const pw = half + (wn + r16) * 128;
@@ -177,30 +180,30 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
 #pragma unroll
     for (int j = 0; j < TI; ++j)
       x[j] = join(ld16(px + j * 2048 + s0), ld16(px + j * 2048 + s1));
-    i8v w = join(ld16(pw + s0), ld16(pw + s1));
+    auto rows = [&](int i) { return join(ld16(pw + i * 2048 + s0), ld16(pw + i * 2048 + s1)); };
+    i8v w[3] = {rows(0), rows(1), {}};
     f4 p[TI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      // the products of row tile i beside the sums of i - 1 and the reads of i + 1
+      // the products of row tile i beside the sums of i - 1 and the reads of i + 2
       f4 now[TI];
-      i8v next = w;
-      if (i + 1 < NI)
-        next = join(ld16(pw + (i + 1) * 2048 + s0), ld16(pw + (i + 1) * 2048 + s1));
+      if (i + 2 < NI) w[(i + 2) % 3] = rows(i + 2);
 #pragma unroll
-      for (int j = 0; j < TI; ++j) now[j] = product(w, x[j]);
-      if (i > 0) {
-#pragma unroll
-        for (int j = 0; j < TI; ++j)
+      for (int j = 0; j < TI; ++j) {
+        now[j] = product(w[i % 3], x[j]);
+        if (i > 0) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i - 1][j][e] += p[j][e] * scale[j];
-        // (an empty statement that holds the sums here: left free, they all sink
-        // to the end and their operands do not fit the registers)
-#pragma unroll
-        for (int j = 0; j < TI; ++j) asm volatile("" : "+v"(acc[i - 1][j]));
+          // (an empty statement that holds the sums here: left free, they all sink
+          // to the end and their operands do not fit the registers)
+          asm volatile("" : "+v"(acc[i - 1][j]));
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one product,
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one read,
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // four sums
       }
 #pragma unroll
       for (int j = 0; j < TI; ++j) p[j] = now[j];
-      w = next;
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -208,30 +211,76 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[NI - 1][j][e] += p[j][e] * scale[j];
   };
-  // Two blocks a turn, one from each half; behind the last one zeros are fetched
-  // and scaled by zero.
-  auto step = [&](int b, const char* half, char* other) {
-    __syncthreads();  // the block is there, and nobody reads the other half any more
-    take_scales(b);
-    fetch(other, b + 1);
-    load_scales(b + 1);
-    multiply(half);
+  // The block of `half` is there, and nobody reads the other half any more; behind
+  // the last block lie zeros, scaled by zero.
+  auto ready = [&](int b) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TI; ++i) scale[i] = b < KB ? ahead[i] * w_ahead : 0.0f;
   };
+
+  int tile = blockIdx.x;
+  place(tile);
+  open();
   fetch(s_a, 0);
-  load_scales(0);
-  for (int b = 0; b < KB; b += 2) {
-    step(b, s_a, s_b);
-    step(b + 1, s_b, s_a);
-  }
+  while (true) {
 #pragma unroll
-  for (int j = 0; j < TI; ++j) {
-    const int t = t0 + wt + 16 * j + r16;
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int n = n0 + wn + 16 * i + 4 * q;
-      if (t < c.T && n < c.N)
-        store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, acc[i][j]);
+      for (int j = 0; j < TI; ++j) acc[i][j] = f4{0, 0, 0, 0};
+    const int n_here = n0 + wn, t_here = t0 + wt;
+    for (int b = 0; b < KB; b += 2) {
+      ready(b);
+      fetch(s_b, b + 1);
+      multiply(s_a);
+      ready(b + 1);
+      int next = b + 2;
+      if (next >= KB) {
+        tile += gridDim.x;
+        if (tile < all) {
+          place(tile);
+          open();
+          next = 0;
+        }
+      }
+      fetch(s_a, next);
+      multiply(s_b);
     }
+    // A lane has outputs 4 q .. + 3 of row tile i; two row tiles exchange quarters,
+    // so that it has eight outputs of one of them: 8 (q / 2) .. + 7 of i + q % 2.
+#pragma unroll
+    for (int j = 0; j < TI; ++j) {
+      const int t = t_here + 16 * j + r16;
+      if (t >= c.T) continue;
+#pragma unroll
+      for (int i = 0; i < NI; i += 2) {
+        const int n = n_here + 16 * (i + (q & 1)) + 8 * (q >> 1);
+        u4 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          typename E::vec4 a, b;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] = (elem)acc[i][j][e];
+            b[e] = (elem)acc[i + 1][j][e];
+          }
+          const u2 r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u2, a)[h],
+                                                        __builtin_bit_cast(u2, b)[h], false, false);
+          v[h] = r[0];
+          v[2 + h] = r[1];
+        }
+        elem* const to = static_cast<elem*>(c.y) + (size_t)t * c.N + n;
+        if (c.N % 8 == 0) {
+          if (n < c.N) *reinterpret_cast<u4*>(to) = v;
+        } else {
+          const typename E::vec8 o = __builtin_bit_cast(typename E::vec8, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < c.N) to[e] = o[e];
+        }
+      }
+    }
+    if (tile >= all) break;
   }
 }
 
@@ -240,7 +289,7 @@ void launch(const GemmBlocksCall& c, hipStream_t stream) {
   if (c.T > 64) {
     const long long large = (long long)((c.N + 255) / 256) * ((c.T + 255) / 256);
     if (large >= 256) {
-      gemm_blocks_tile<E, 256, 256, 128, 64><<<large, 512, 0, stream>>>(c);
+      gemm_blocks_tile<E, 256, 256, 128, 64><<<min(large, 256ll), 512, 0, stream>>>(c);
     } else {
       const int n = (c.N + 127) / 128 * ((c.T + 127) / 128);
       gemm_blocks_tile<E, 128, 128, 64, 64><<<n, 256, 0, stream>>>(c);
