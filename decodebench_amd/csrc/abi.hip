@@ -337,6 +337,10 @@ const Knob kKnobs[] = {
      "0 (automatic), 1 or 2", nullptr},
     {"gemv_splits", &dbk::Tuning::gemv_splits, [](int v) { return v >= 0 && v <= 8; },
      "0 (automatic) to 8", nullptr},
+    {"blocks_shape", &dbk::Tuning::blocks_shape, [](int v) { return v >= 0 && v <= 4; },
+     "0 (automatic) to 4", nullptr},
+    {"blocks_parts", &dbk::Tuning::blocks_parts, [](int v) { return v >= 0 && v <= 16; },
+     "0 (automatic) to 16", nullptr},
     {"f4_launch", &dbk::Tuning::f4_launch, [](int v) { return v >= 0 && v <= 2; },
      "0 (both launches), 1 (split kernel only) or 2 (merge only)", nullptr},
 };
@@ -827,7 +831,11 @@ int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
 
 size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype) {
   if (T < 1 || K < 1 || N < 1 || T >= kMostSize || K >= kMostSize || N >= kMostSize) return 0;
-  return is16bit(x_dtype) ? quantized_bytes(T, K) : 0;
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  if (err) return 0;
+  const dbk::GemmBlocksPlan plan = dbk::gemm_blocks_plan(T, K, N, cus);
+  return (is16bit(x_dtype) && !plan.fused ? quantized_bytes(T, K) : 0) + round256(plan.bytes);
 }
 
 int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long long xs_t,
@@ -855,12 +863,18 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
     return fail(DB_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
   if (!aligned4(x_scale) || !aligned4(w_scale))
     return fail(DB_ERR_INVALID, "%s: scales must be 4-byte aligned", fn);
-  const int rc =
-      check_workspace(fn, ws, ws_bytes, db_gemm_blocks_workspace_bytes(T, K, N, x_dtype));
+  int err = 0;
+  const int cus = dbk::device_cu_count(&err);
+  // (without a device the workspace is checked against what x alone needs)
+  dbk::GemmBlocksPlan plan = err ? dbk::GemmBlocksPlan{} : dbk::gemm_blocks_plan(T, K, N, cus);
+  const size_t for_x = fp8 || plan.fused ? 0 : quantized_bytes(T, K);
+  const int rc = check_workspace(fn, ws, ws_bytes, for_x + round256(plan.bytes));
   if (rc) return rc;
+  if (err) return hip_status((hipError_t)err, fn);
+  plan.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + for_x);
   dbk::GemmBlocksCall c = {x, x_scale, W, w_scale, y, x_stride, xs_t, xs_b, T, K, N,
                            y_dtype == DB_DTYPE_BF16};
-  if (!fp8) {
+  if (!fp8 && !plan.fused) {
     char* const q = static_cast<char*>(ws);
     float* const scale = reinterpret_cast<float*>(q + round256((size_t)T * K));
     const dbk::QuantCall quant = {x, q, scale, x_stride, 1, T, T, K, c.bf16};
@@ -872,7 +886,7 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
     c.xs_t = 1;
     c.xs_b = T;
   }
-  return hip_status(dbk::launch_gemm_blocks(c, (hipStream_t)stream), fn);
+  return hip_status(dbk::launch_gemm_blocks(c, plan, (hipStream_t)stream), fn);
 }
 
 size_t db_moe_route_workspace_bytes(int T, int E) {

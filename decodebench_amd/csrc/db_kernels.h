@@ -39,6 +39,9 @@ struct Tuning {
   int gemv_tile = 0;           // batches of 2 rows and more (gemv_mfma_min_batch if set):
                                // 0 automatic, 1 gemv_tile, 2 never gemv_tile
   int gemv_splits = 0;         // K splits of gemv_tile where a workspace is given: 0 auto, 1..8
+  int blocks_shape = 0;        // gemm_blocks: 0 automatic, 1..4 tiles of 256 x 256,
+                               // 256 x 128, 128 x 64, 128 x 32
+  int blocks_parts = 0;        // parts of K of its tiles: 0 automatic, 1..16
   int f4_launch = 0;           // measurement hook for the two-launch F4: 0 both
                                // launches, 1 the split kernel only, 2 the merge only
 };
@@ -192,8 +195,8 @@ struct QuantCall {
 hipError_t launch_quantize_blocks(const QuantCall& c, hipStream_t stream);
 
 struct GemmBlocksCall {
-  const void* x;         // [T, K] e4m3, rows x_row apart
-  const float* x_scale;  // [T, ceil(K / 128)] at the strides below
+  const void* x;         // [T, K] e4m3, rows x_row apart; of y's type where plan.fused
+  const float* x_scale;  // [T, ceil(K / 128)] at the strides below; null where plan.fused
   const void* W;         // [N, K] e4m3
   const float* w_scale;  // [ceil(N / 128), ceil(K / 128)]
   void* y;               // [T, N]
@@ -201,7 +204,18 @@ struct GemmBlocksCall {
   int T, K, N;
   bool bf16;             // type of y
 };
-hipError_t launch_gemm_blocks(const GemmBlocksCall& c, hipStream_t stream);
+// How a product runs: the kernel's shape, K in parts of `each` blocks whose fp32
+// sums a second launch adds, workgroups, bytes of workspace for the sums.
+struct GemmBlocksPlan {
+  int shape, parts, each, grid, pitch;  // few tokens: `each` outputs a workgroup
+  unsigned magic;  // few tokens: 2^32 / blocks of K, rounded up
+  bool fused;      // 16-bit activations are quantised in the same launch
+  size_t bytes;
+  float* sums;  // [parts, T, pitch]
+};
+GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count);
+hipError_t launch_gemm_blocks(const GemmBlocksCall& c, const GemmBlocksPlan& plan,
+                              hipStream_t stream);
 
 // A mixture-of-experts layer (moe_route.hip, moe_experts.hip).
 struct MoeRouteCall {

@@ -7,8 +7,10 @@
 // scaled and added to the fp32 sum with one multiply-add for each of the four
 // outputs of a lane.  Weights are the A operand and tokens the B operand, so a
 // lane's outputs belong to one token and share one scale.
-#include "db_elem.h"
+#include <atomic>
+
 #include "db_kernels.h"
+#include "quant_blocks.h"
 
 namespace dbk {
 
@@ -55,47 +57,163 @@ __device__ __forceinline__ void store4(void* y, size_t at, int left, bool vec, f
   }
 }
 
-// 16 outputs and 16 TT tokens a workgroup, its waves taking blocks of K in turn.
-template <class E, int TT>
-__global__ __launch_bounds__(kThreads) void gemm_blocks_rows(GemmBlocksCall c) {
-  __shared__ f4 s_part[kWaves][TT][kWave];
+// ------------------------------------------------------------- few tokens
+// A workgroup has plan.each outputs (a multiple of 4: even shares of any N) of all
+// T <= 16 tokens, 16 at a time; its waves take blocks of K in turn, and their sums
+// meet in the LDS.  x lies there whole, its scales behind it, copied or quantised
+// by every workgroup for itself while the first weights are on their way.
+//
+// A load instruction has 8 rows of one 128-byte line each, consecutive lanes
+// consecutive chunks (operand order, rows on consecutive lanes, takes the L1 four
+// times as long); a wave's block passes through an LDS tile of its own into operand
+// order, chunk c of row r at place c ^ r % 8.  No barrier: a wave's LDS accesses
+// execute in order.
+constexpr int kAhead = 8;     // blocks of a wave on their way
+constexpr int kFewRounds = 4;  // of 4 blocks of x a wave, asked for before the weights
+constexpr int kFewTiles = 4;  // of 16 outputs, at most, of a workgroup
+
+template <class E, bool QUANT, int NW>
+__global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
+                                                             GemmBlocksPlan plan) {
+  extern __shared__ __align__(16) char s_x[];
+  __shared__ __align__(16) char s_tile[NW][2048];
+  __shared__ f4 s_part[kFewTiles][NW][kWave];
+  constexpr int kThreadsHere = NW * kWave;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT;
-  const int KB = (c.K + 127) / 128;
+  const int KB = (c.K + 127) / 128, KP = (c.K + 1023) / 1024 * 1024;
+  const int n_first = blockIdx.x * plan.each, n_last = min(c.N, n_first + plan.each);
+  const int nb0 = n_first / 128, nbs = (n_last - 1) / 128 - nb0 + 1;
+  float* const s_scale = reinterpret_cast<float*>(s_x + c.T * KP);  // [T, KB]
+  float* const s_w = s_scale + c.T * KB;                            // [nbs, KB]
+
+  // x and all scales are asked for before the first weights, which come in order
+  // behind them; without branches, which would make the waits for them whole.
+  const int items = c.T * KB, w_items = nbs * KB;
+  auto row_of = [&](int i) { return (int)__umulhi(i, plan.magic); };  // i / KB
+  u4 x_raw[kFewRounds];
+  float xs_first = 0.0f;
+  int x_at = threadIdx.x / 16;  // this row of lanes' block of x: every (4 NW)th of them
+  auto ask = [&](int i) {
+    const int in = min(i, items - 1), t = row_of(in), b = in - t * KB;
+    const typename E::type* const row = static_cast<const typename E::type*>(c.x) + t * c.x_row;
+    return ld16(row + min(b * 128 + r16 * 8, c.K - 8));
+  };
+  auto put_x = [&](int i, u4 raw) {
+    const int t = row_of(i), b = i - t * KB;
+    float scale;
+    const u2 v = quantize128<E>(b * 128 + r16 * 8 < c.K ? raw : u4{0, 0, 0, 0}, scale);
+    *reinterpret_cast<u2*>(s_x + t * KP + b * 128 + (((r16 >> 1) ^ (t & 7)) * 16) +
+                           (r16 & 1) * 8) = v;
+    if (r16 == 0) s_scale[i] = scale;
+  };
+  if constexpr (QUANT) {
+    // all but the last rounds go into the LDS at once
+    while (x_at - (int)threadIdx.x / 16 + kFewRounds * NW * 4 < items) {
+#pragma unroll
+      for (int r = 0; r < kFewRounds; ++r) x_raw[r] = ask(x_at + r * NW * 4);
+#pragma unroll
+      for (int r = 0; r < kFewRounds; ++r) put_x(x_at + r * NW * 4, x_raw[r]);
+      x_at += kFewRounds * NW * 4;
+    }
+#pragma unroll
+    for (int r = 0; r < kFewRounds; ++r) x_raw[r] = ask(x_at + r * NW * 4);
+  } else {
+    const __amdgpu_buffer_rsrc_t rx =
+        make_rsrc(c.x, (int)((c.T - 1) * c.x_row) + c.K);
+    for (int t = 0; t < c.T; ++t)
+      for (int at = ((wave + t) & (NW - 1)) * 1024; at < KP; at += NW * 1024) {
+        typedef __attribute__((address_space(3))) void lds;
+        const int k = at + (lane >> 3) * 128 + ((lane & 7) ^ (t & 7)) * 16;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds*)(s_x + t * KP + at), 16,
+                                                 k < c.K ? t * (int)c.x_row + k : kOut, 0, 0, 0);
+      }
+    const int i = min((int)threadIdx.x, items - 1), t = row_of(i);
+    xs_first = c.x_scale[t * c.xs_t + (i - t * KB) * c.xs_b];
+  }
+  const float w_first = c.w_scale[(size_t)nb0 * KB + min((int)threadIdx.x, w_items - 1)];
+  asm volatile("" ::: "memory");
+
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(
-      static_cast<const char*>(c.W) + (size_t)n0 * c.K, min(16, c.N - n0) * c.K);
-  const __amdgpu_buffer_rsrc_t rx =
-      make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
-                (int)((min(16 * TT, c.T - t0) - 1) * c.x_row) + c.K);
-  const float* const ws = c.w_scale + (size_t)(n0 / 128) * KB;
-  f4 acc[TT] = {};
-  for (int b = wave; b < KB; b += kWaves) {
-    const int k0 = b * 128 + q * 16, k1 = k0 + 64;
-    const int wr = r16 * c.K;
-    const i8v w = join(ld_buf(rw, k0 < c.K ? wr + k0 : kOut), ld_buf(rw, k1 < c.K ? wr + k1 : kOut));
-    const float wscale = ws[b];
+      static_cast<const char*>(c.W) + (size_t)n_first * c.K, (n_last - n_first) * c.K);
+  const int turns = (KB - wave + NW - 1) / NW;  // blocks of this wave, of each 16 outputs
+  const int tiles = (n_last - n_first + 15) / 16;
+  const int line = (lane >> 3) * c.K, chunk = (lane & 7) * 16;
+  int at_tile = 0, at_turn = 0;  // the next block to load
+  u4 w[kAhead][2];
+  auto load = [&](int u) {
+    const int k = (wave + at_turn * NW) * 128 + chunk;
+    const int off = at_tile < tiles && k < c.K ? at_tile * 16 * c.K + line + k : kOut;
+    w[u][0] = ld_buf_stream(rw, off);
+    w[u][1] = ld_buf_stream(rw, off + 8 * c.K);
+    const bool wrap = ++at_turn >= turns;
+    at_turn = wrap ? 0 : at_turn;
+    at_tile += wrap ? 1 : 0;
+  };
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      const int t = i * 16 + r16;
-      const int xr = t0 + t < c.T ? t * (int)c.x_row : kOut;
-      const i8v x = join(ld_buf(rx, k0 < c.K ? xr + k0 : kOut), ld_buf(rx, k1 < c.K ? xr + k1 : kOut));
-      const float s = c.x_scale[min(t0 + t, c.T - 1) * c.xs_t + b * c.xs_b] * wscale;
-      const f4 p = product(w, x);
+  for (int u = 0; u < kAhead; ++u) load(u);
+
+  if constexpr (QUANT) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += p[j] * s;
+    for (int r = 0; r < kFewRounds; ++r)
+      if (x_at + r * NW * 4 < items) put_x(x_at + r * NW * 4, x_raw[r]);
+  } else {
+    if (threadIdx.x < items) s_scale[threadIdx.x] = xs_first;
+    for (int i = threadIdx.x + kThreadsHere; i < items; i += kThreadsHere) {
+      const int t = row_of(i);
+      s_scale[i] = c.x_scale[t * c.xs_t + (i - t * KB) * c.xs_b];
+    }
+    // what went straight to the LDS came before the 2 kAhead loads of weights
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kAhead) : "memory");
+  }
+  if (threadIdx.x < w_items) s_w[threadIdx.x] = w_first;
+  for (int i = threadIdx.x + kThreadsHere; i < w_items; i += kThreadsHere)
+    s_w[i] = c.w_scale[(size_t)nb0 * KB + i];
+  __syncthreads();
+
+  const int t = min(r16, c.T - 1);
+  char* const tile = s_tile[wave];
+  char* const put = tile + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) * 16);
+  const char* const get = tile + r16 * 128;
+  const char* const px = s_x + t * KP;
+  const int g0 = (q ^ (r16 & 7)) * 16, g1 = g0 ^ 64;
+  const int x0 = (q ^ (t & 7)) * 16, x1 = x0 ^ 64;
+  int turn = 0, n_tile = 0;
+  f4 acc = {0, 0, 0, 0};
+  const int steps = tiles * turns;
+  for (int s = 0; s < steps; s += kAhead) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s + u >= steps) break;
+      *reinterpret_cast<u4*>(put) = w[u][0];
+      *reinterpret_cast<u4*>(put + 1024) = w[u][1];
+      load(u);
+      wave_lds_order();
+      const int b = wave + turn * NW;
+      const i8v a = join(ld16(get + g0), ld16(get + g1));
+      const i8v x = join(ld16(px + b * 128 + x0), ld16(px + b * 128 + x1));
+      const int n = min(n_first + 16 * n_tile + 4 * q, n_last - 1);
+      const float scale = s_scale[t * KB + b] * s_w[(n / 128 - nb0) * KB + b];
+      wave_lds_order();
+      const f4 p = product(a, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += p[e] * scale;
+      if (++turn == turns) {
+        s_part[n_tile++][wave][lane] = acc;
+        acc = f4{0, 0, 0, 0};
+        turn = 0;
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < TT; ++i) s_part[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int i = wave; i < TT; i += kWaves) {
-    f4 sum = s_part[0][i][lane];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += s_part[w][i][lane];
-    const int t = t0 + i * 16 + r16, n = n0 + 4 * q;
-    if (t < c.T && n < c.N) store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, sum);
+  const int parts = min(NW, KB);
+  for (int i = wave; i < tiles; i += NW) {
+    f4 sum = s_part[i][0][lane];
+    for (int p = 1; p < parts; ++p) sum += s_part[i][p][lane];
+    const int n = n_first + 16 * i + 4 * q;
+    if (r16 < c.T && n < n_last)
+      store4<E>(c.y, (size_t)r16 * c.N + n, n_last - n, c.N % 4 == 0, sum);
   }
 }
 
@@ -107,17 +225,22 @@ __global__ __launch_bounds__(kThreads) void gemm_blocks_rows(GemmBlocksCall c) {
 // Rows of 128 bytes lie 16 bytes at a time in the order (chunk ^ row % 8), set
 // by which global chunk a lane fetches: the 16 rows that a quarter of a wave
 // reads then lie in different banks.
-template <class E, int BN, int BT, int WN, int WT>
+template <class E, int BN, int BT, int WN, int WT, int S>
 __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_tile(
-    GemmBlocksCall c) {
+    GemmBlocksCall c, GemmBlocksPlan plan) {
   typedef typename E::type elem;
   constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;
-  constexpr int kLoads = (BN + BT) / 8 / NW;  // of 8 rows, a wave
-  static_assert((BN + BT) % (8 * NW) == 0 && BN % (8 * kLoads) == 0, "whole loads");
+  constexpr int kLoadsW = BN / 8 / NW, kLoadsX = BT / 8 / NW;  // of 8 rows, a wave
+  constexpr int kLoads = kLoadsW + kLoadsX;
+  static_assert(BN % (8 * NW) == 0 && BT % (8 * NW) == 0, "whole loads");
+  static_assert(S == 2 || S == 3, "two or three stages");
   static_assert(NI % 2 == 0 && 128 % WN == 0, "row tiles in pairs, of one block of the weights");
-  constexpr int kHalf = (BN + BT) * 128;
-  __shared__ __align__(16) char s_a[kHalf];
-  __shared__ __align__(16) char s_b[kHalf];
+  constexpr int kStage = (BN + BT) * 128;
+  // (arrays of their own, so that reads of one need not wait for what is on its
+  // way into another)
+  __shared__ __align__(16) char s_a[kStage];
+  __shared__ __align__(16) char s_b[kStage];
+  __shared__ __align__(16) char s_c[S > 2 ? kStage : 16];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
@@ -126,56 +249,64 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
 
   // Workgroups i, i + 8, .. run on one XCD: its share of the tiles is a
   // compact part of the output, strips of eight token tiles wide.
-  const int tn = (c.N + BN - 1) / BN, tt = (c.T + BT - 1) / BT, all = tn * tt;
-  int n0, t0;
+  const int tn = (c.N + BN - 1) / BN, tt = (c.T + BT - 1) / BT, all = tn * tt * plan.parts;
+  const int steps = (plan.each + S - 1) / S * S;
+  int n0, t0, part, b0, b1;
   auto place = [&](int i) {
     const int xcd = i & 7, each = all >> 3, more = all & 7;
-    const int at = xcd * each + min(xcd, more) + (i >> 3);
+    const int nth = xcd * each + min(xcd, more) + (i >> 3);
+    part = nth / (tn * tt);
+    b0 = part * plan.each;
+    b1 = min(KB, b0 + plan.each);
+    const int at = nth - part * tn * tt;
     const int strip = at / (8 * tn), in = at - strip * 8 * tn, wide = min(8, tt - 8 * strip);
     n0 = in / wide * BN;
     t0 = (8 * strip + in % wide) * BT;
   };
 
-  // This wave fetches rows 8 kLoads wave .. of the BN + BT.
-  const bool from_w = wave * kLoads * 8 < BN;
-  const int pitch = from_w ? c.K : (int)c.x_row;
-  const int row0 = ((from_w ? wave * kLoads * 8 : wave * kLoads * 8 - BN) + (lane >> 3)) * pitch;
-  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-  __amdgpu_buffer_rsrc_t rows_of;
-  // scales of this lane's tokens and of the wave's outputs, loaded a block ahead
+  // Load i of a wave has rows 8 (NW i + wave) .. + 7 of the weights, or of x.
+  const int lane_row = 8 * wave + (lane >> 3), chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  const int w_row = lane_row * c.K, x_row = lane_row * (int)c.x_row;
+  __amdgpu_buffer_rsrc_t rw, rx;
+  // scales of this lane's tokens and of the wave's outputs
   const float *xs[TI], *ws;
-  float scale[TI], ahead[TI], w_ahead;
+  float scale[TI], ahead[S - 1][TI], w_ahead[S - 1];
   auto open = [&] {
-    rows_of = from_w ? make_rsrc(static_cast<const char*>(c.W) + (size_t)n0 * c.K,
-                                 min(BN, c.N - n0) * c.K)
-                     : make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
-                                 (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
+    rw = make_rsrc(static_cast<const char*>(c.W) + (size_t)n0 * c.K, min(BN, c.N - n0) * c.K);
+    rx = make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
+                   (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
 #pragma unroll
     for (int i = 0; i < TI; ++i)
       xs[i] = c.x_scale + min(t0 + wt + 16 * i + r16, c.T - 1) * c.xs_t;
     ws = c.w_scale + (size_t)min((n0 + wn) / 128, (c.N - 1) / 128) * KB;
   };
-  auto fetch = [&](char* half, int b) {
+  // Block b to a stage and its scales to a slot, the scales first: they are there
+  // when kLoads loads are left.  Behind the last block come zeros.
+  auto fetch = [&](char* stage, int slot, int b) {
+    const int in = min(b, b1 - 1);
+    w_ahead[slot] = ws[in];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) ahead[slot][i] = xs[i][in * c.xs_b];
     const int k = b * 128 + chunk;
-    const int off = (k < c.K ? k : kOut) + row0;
-    char* const to = half + wave * kLoads * 1024;
+    const int off = b < b1 && k < c.K ? k : kOut;
+    typedef __attribute__((address_space(3))) void lds;
+    if constexpr (S > 2) asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      typedef __attribute__((address_space(3))) void lds;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rows_of, (lds*)(to + i * 1024), 16,
-                                               off + i * 8 * pitch, 0, 0, 0);
-    }
-    const int in = min(b, KB - 1);
-    w_ahead = ws[in];
+    for (int i = 0; i < kLoadsW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds*)(stage + (i * NW + wave) * 1024), 16,
+                                               off + w_row + i * NW * 8 * c.K, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < TI; ++i) ahead[i] = xs[i][in * c.xs_b];
+    for (int i = 0; i < kLoadsX; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rx, (lds*)(stage + BN * 128 + (i * NW + wave) * 1024), 16,
+          off + x_row + i * NW * 8 * (int)c.x_row, 0, 0, 0);
   };
 
   f4 acc[NI][TI];
-  auto multiply = [&](const char* half) {
+  auto multiply = [&](const char* stage) {
     const int s0 = (q ^ (r16 & 7)) * 16, s1 = s0 ^ 64;
-    const char* const pw = half + (wn + r16) * 128;
-    const char* const px = half + (BN + wt + r16) * 128;
+    const char* const pw = stage + (wn + r16) * 128;
+    const char* const px = stage + (BN + wt + r16) * 128;
     i8v x[TI];
 #pragma unroll
     for (int j = 0; j < TI; ++j)
@@ -211,40 +342,80 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[NI - 1][j][e] += p[j][e] * scale[j];
   };
-  // The block of `half` is there, and nobody reads the other half any more; behind
-  // the last block lie zeros, scaled by zero.
-  auto ready = [&](int b) {
-    __syncthreads();
+  // The oldest block fetched is there, for all waves, and nobody reads the stage
+  // before it any more, which is fetched next.
+  auto ready = [&](int slot, bool exists) {
+    // (a barrier by itself waits for no load into the LDS)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * kLoads) : "memory");
 #pragma unroll
-    for (int i = 0; i < TI; ++i) scale[i] = b < KB ? ahead[i] * w_ahead : 0.0f;
+    for (int i = 0; i < TI; ++i) scale[i] = exists ? ahead[slot][i] * w_ahead[slot] : 0.0f;
   };
-
-  int tile = blockIdx.x;
+  // What comes next: of this tile, then of the workgroup's next one.
+  int tile = blockIdx.x, fetched = 0;
+  auto shift = [&] {
+#pragma unroll
+    for (int i = 0; i < TI; ++i) ahead[0][i] = ahead[S - 2][i];
+    w_ahead[0] = w_ahead[S - 2];
+  };
+  auto fetch_next = [&](char* stage, int slot) {
+    if (fetched == steps) {
+      tile += gridDim.x;
+      fetched = 0;
+      if (tile < all) {
+        place(tile);
+        open();
+      } else {
+        b0 = b1;  // nothing: zeros
+      }
+    }
+    fetch(stage, slot, b0 + fetched++);
+  };
   place(tile);
   open();
-  fetch(s_a, 0);
-  while (true) {
+  fetch_next(s_a, 0);
+  if constexpr (S > 2) fetch_next(s_b, 1);
+  for (int now = tile; now < all; now += gridDim.x) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < TI; ++j) acc[i][j] = f4{0, 0, 0, 0};
-    const int n_here = n0 + wn, t_here = t0 + wt;
-    for (int b = 0; b < KB; b += 2) {
-      ready(b);
-      fetch(s_b, b + 1);
-      multiply(s_a);
-      ready(b + 1);
-      int next = b + 2;
-      if (next >= KB) {
-        tile += gridDim.x;
-        if (tile < all) {
-          place(tile);
-          open();
-          next = 0;
+    const int n_here = n0 + wn, t_here = t0 + wt, part_here = part, blocks = b1 - b0;
+    for (int s = 0; s < steps; s += S) {
+      if constexpr (S == 2) {
+        ready(0, s < blocks);
+        fetch_next(s_b, 0);
+        multiply(s_a);
+        ready(0, s + 1 < blocks);
+        fetch_next(s_a, 0);
+        multiply(s_b);
+      } else {
+        ready(0, s < blocks);
+        shift();
+        fetch_next(s_c, 1);
+        multiply(s_a);
+        ready(0, s + 1 < blocks);
+        shift();
+        fetch_next(s_a, 1);
+        multiply(s_b);
+        ready(0, s + 2 < blocks);
+        shift();
+        fetch_next(s_b, 1);
+        multiply(s_c);
+      }
+    }
+    if (plan.parts > 1) {
+      float* const to = plan.sums + (size_t)part_here * c.T * plan.pitch;
+#pragma unroll
+      for (int j = 0; j < TI; ++j) {
+        const int t = t_here + 16 * j + r16;
+        if (t >= c.T) continue;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int n = n_here + 16 * i + 4 * q;
+          if (n < c.N) *reinterpret_cast<f4*>(to + (size_t)t * plan.pitch + n) = acc[i][j];
         }
       }
-      fetch(s_a, next);
-      multiply(s_b);
+      continue;
     }
     // A lane has outputs 4 q .. + 3 of row tile i; two row tiles exchange quarters,
     // so that it has eight outputs of one of them: 8 (q / 2) .. + 7 of i + q % 2.
@@ -280,37 +451,140 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
         }
       }
     }
-    if (tile >= all) break;
   }
+  // what is still on its way into the LDS (zeros) arrives before that is given back
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// The sums of the parts of K, in order.
+template <class E>
+__global__ __launch_bounds__(kThreads) void gemm_blocks_join(GemmBlocksCall c,
+                                                             GemmBlocksPlan plan) {
+  const int quads = plan.pitch / 4;
+  const size_t at = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  const int t = (int)(at / quads), n = (int)(at - (size_t)t * quads) * 4;
+  if (t >= c.T) return;
+  const float* from = plan.sums + (size_t)t * plan.pitch + n;
+  f4 sum = *reinterpret_cast<const f4*>(from);
+  for (int p = 1; p < plan.parts; ++p)
+    sum += *reinterpret_cast<const f4*>(from + (size_t)p * c.T * plan.pitch);
+  store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, sum);
+}
+
+// Shapes of the tile kernel; kFew: the kernel of few tokens.
+enum Shape { kFew, k256x256, k256x128, k128x64, k128x32, kShapes };
+struct ShapeSize {
+  int n, t, threads, slots;  // slots: workgroups a CU
+  double step, step2;        // us of a block of K, with one and with two workgroups a CU
+};
+constexpr ShapeSize kShape[kShapes] = {{16, 16, 512, 1, 0.0, 0.0},
+                                       {256, 256, 512, 1, 1.95, 1.95},
+                                       {256, 128, 512, 1, 1.15, 1.15},
+                                       {128, 64, 256, 2, 0.45, 0.72},
+                                       {128, 32, 256, 2, 0.38, 0.55}};
+
+constexpr int kFewWaves = 8;
+constexpr size_t kFewLds = 100 * 1024;  // dynamic, next to 48 KB of partial sums and tiles
+
+size_t few_lds(int T, int K, int each) {
+  const int KB = (K + 127) / 128;
+  return (size_t)T * ((K + 1023) / 1024 * 1024 + KB * 4) + (size_t)(each / 128 + 2) * KB * 4;
+}
+
+template <class F>
+hipError_t launch_few(F* fn, const GemmBlocksCall& c, const GemmBlocksPlan& plan,
+                      hipStream_t stream) {
+  // (once per kernel and device; a second call asks for the same)
+  static std::atomic<unsigned long long> asked{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev >= 64 || !(asked.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)kFewLds);
+    if (e != hipSuccess) return e;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+  }
+  fn<<<plan.grid, kFewWaves * kWave, few_lds(c.T, c.K, plan.each), stream>>>(c, plan);
+  return hipGetLastError();
 }
 
 template <class E>
-void launch(const GemmBlocksCall& c, hipStream_t stream) {
-  if (c.T > 64) {
-    const long long large = (long long)((c.N + 255) / 256) * ((c.T + 255) / 256);
-    if (large >= 256) {
-      gemm_blocks_tile<E, 256, 256, 128, 64><<<min(large, 256ll), 512, 0, stream>>>(c);
-    } else {
-      const int n = (c.N + 127) / 128 * ((c.T + 127) / 128);
-      gemm_blocks_tile<E, 128, 128, 64, 64><<<n, 256, 0, stream>>>(c);
+hipError_t launch(const GemmBlocksCall& c, const GemmBlocksPlan& plan, hipStream_t stream) {
+  if (plan.shape == kFew) {
+    if (!c.x_scale) {
+      static const auto fn = gemm_blocks_few<E, true, kFewWaves>;
+      return launch_few(fn, c, plan, stream);
     }
-    return;
+    static const auto fn = gemm_blocks_few<E, false, kFewWaves>;
+    return launch_few(fn, c, plan, stream);
   }
-  const int TT = c.T <= 16 ? 1 : c.T <= 32 ? 2 : 4;
-  const dim3 grid((c.N + 15) / 16, (c.T + 16 * TT - 1) / (16 * TT));
-  auto* const fn = TT == 1 ? gemm_blocks_rows<E, 1> : TT == 2 ? gemm_blocks_rows<E, 2>
-                                                              : gemm_blocks_rows<E, 4>;
-  fn<<<grid, kThreads, 0, stream>>>(c);
+  auto* const fn = plan.shape == k256x256   ? gemm_blocks_tile<E, 256, 256, 128, 64, 2>
+                   : plan.shape == k256x128 ? gemm_blocks_tile<E, 256, 128, 64, 64, 3>
+                   : plan.shape == k128x64  ? gemm_blocks_tile<E, 128, 64, 64, 32, 3>
+                                            : gemm_blocks_tile<E, 128, 32, 32, 32, 3>;
+  fn<<<plan.grid, kShape[plan.shape].threads, 0, stream>>>(c, plan);
+  if (plan.parts > 1) {
+    const size_t quads = (size_t)c.T * plan.pitch / 4;
+    gemm_blocks_join<E><<<(quads + kThreads - 1) / kThreads, kThreads, 0, stream>>>(c, plan);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_gemm_blocks(const GemmBlocksCall& c, hipStream_t stream) {
-  if (c.bf16)
-    launch<ElemBF16>(c, stream);
-  else
-    launch<ElemF16>(c, stream);
-  return hipGetLastError();
+GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count) {
+  const int KB = (K + 127) / 128;
+  GemmBlocksPlan p = {};
+  p.parts = 1;
+  p.pitch = (N + 3) / 4 * 4;
+  if (T <= 16 && !tuning().blocks_shape) {
+    const int rounds = (N + 64 * cu_count - 1) / (64 * cu_count);
+    p.each = ((N + rounds * cu_count - 1) / (rounds * cu_count) + 3) / 4 * 4;
+    p.grid = (N + p.each - 1) / p.each;
+    p.magic = KB > 1 ? 0xFFFFFFFFu / KB + 1 : 0;
+    // Every workgroup quantises all of x: 8 tokens of 4096 16.7 us and 18.9 with a
+    // launch for it ([14336, 4096]), 16 of them 21.2 and 19.7.
+    p.fused = T * KB <= 320;
+    if (few_lds(T, K, p.each) <= kFewLds) return p;
+    p.fused = false;
+  }
+  // The shape and the parts of K whose rounds of workgroups are estimated to take
+  // the least time.
+  double best = 0.0;
+  for (int shape = k256x256; shape < kShapes; ++shape) {
+    if (tuning().blocks_shape && shape != tuning().blocks_shape) continue;
+    const ShapeSize& s = kShape[shape];
+    const long long tiles = (long long)((N + s.n - 1) / s.n) * ((T + s.t - 1) / s.t);
+    for (int parts = 1; parts <= 16 && parts <= KB; ++parts) {
+      if (tuning().blocks_parts && parts != tuning().blocks_parts &&
+          parts < min(KB, tuning().blocks_parts))
+        continue;
+      const int each = (KB + parts - 1) / parts, have = (KB + each - 1) / each;
+      const long long work = tiles * have;
+      // workgroups of 128 outputs run two to a CU, a step of two takes longer
+      const long long rounds = (work + s.slots * cu_count - 1) / (s.slots * cu_count);
+      const bool crowded = s.slots > 1 && work > cu_count;
+      const double sums = have > 1 ? (double)have * T * p.pitch * sizeof(float) : 0.0;
+      const double us = rounds * (each + 2) * (crowded ? s.step2 : s.step) +
+                        (have > 1 ? 2.5 + sums * 2 / 6e6 : 0.0);
+      if (best == 0.0 || us < best) {
+        best = us;
+        p.shape = shape;
+        p.each = each;
+        p.parts = have;
+        p.grid = (int)min(work, (long long)cu_count * s.slots);
+        p.bytes = have > 1 ? (size_t)have * T * p.pitch * sizeof(float) : 0;
+      }
+    }
+  }
+  return p;
+}
+
+hipError_t launch_gemm_blocks(const GemmBlocksCall& c, const GemmBlocksPlan& plan,
+                              hipStream_t stream) {
+  return c.bf16 ? launch<ElemBF16>(c, plan, stream) : launch<ElemF16>(c, plan, stream);
 }
 
 }  // namespace dbk

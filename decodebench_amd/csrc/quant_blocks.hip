@@ -10,8 +10,8 @@
 // stay visible in the scale.  A workgroup has 16 tokens and four blocks of each:
 // the scales of a block's tokens lie side by side in memory (the product's
 // lanes read them so), and each row is read 1 KB at a time.
-#include "db_elem.h"
 #include "db_kernels.h"
+#include "quant_blocks.h"
 
 namespace dbk {
 
@@ -20,27 +20,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTokens = kThreads / 16;  // of a workgroup
 constexpr int kBlocks = 4;              // of each of its tokens
-
-template <int CTRL>
-__device__ __forceinline__ unsigned dpp_max(unsigned v) {
-  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
-}
-
-// The largest magnitude's bits of the 128 elements that a DPP row holds.
-__device__ __forceinline__ unsigned row_magnitude(u4 w) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-  m = dpp_max<kQuadSwap1>(m);
-  m = dpp_max<kQuadSwap2>(m);
-  m = dpp_max<kRowHalfMirror>(m);
-  return dpp_max<kRowMirror>(m);
-}
-
-template <class E>
-__device__ __forceinline__ float to_float(unsigned bits) {
-  return (float)__builtin_bit_cast(typename E::type, (unsigned short)bits);
-}
 
 template <class E>
 __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(QuantCall c) {
@@ -59,19 +38,8 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(QuantCall c) 
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) {
     const int b = blockIdx.y * kBlocks + i, k = b * 128 + lane * 8;
-    float scale = to_float<E>(row_magnitude(w[i])) / 448.0f;
-    if (scale == 0.0f) scale = 1.0f;
-    u2 r;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[j] = clamp448(to_float<E>(w[i][2 * h + j / 2] >> (16 * (j & 1))) / scale);
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-      p = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], p, true);
-      r[h] = (unsigned)p;
-    }
+    float scale;
+    const u2 r = quantize128<E>(w[i], scale);
     if (k < c.K) *reinterpret_cast<u2*>(out + k) = r;
     if (lane == 0 && b < KB) c.scale[t * c.scale_t + b * c.scale_b] = scale;
   }
