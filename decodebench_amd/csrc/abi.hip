@@ -933,6 +933,10 @@ int db_moe_experts(const void* x, long long x_stride, const int* experts, const 
   if (rc) return rc;
   dbk::MoeExpertsCall c = experts_call(x, x_stride, experts, weights, *m, y, T, k);
   dbk::moe_experts_workspace(c, ws);
+  if (dbk::moe_few(*m, T, k)) {
+    const dbk::MoeFewCall f = {c, nullptr, nullptr, nullptr, false};
+    return hip_status(dbk::launch_moe_few(f, (hipStream_t)stream), fn);
+  }
   return hip_status(dbk::launch_moe_experts(c, (hipStream_t)stream), fn);
 }
 
@@ -958,10 +962,16 @@ int db_moe_layer(const void* x, long long x_stride, const void* Wr, const db_moe
   const dbk::MoeRouteCall r = {x, Wr, experts, weights, reinterpret_cast<double*>(p + s.rest),
                                x_stride, T, m->H, m->E, k, renormalize != 0,
                                m->dtype == DB_DTYPE_BF16};
-  const hipError_t e = dbk::launch_moe_route(r, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_status(e, fn);
   dbk::MoeExpertsCall c = experts_call(x, x_stride, experts, weights, *m, y, T, k);
   dbk::moe_experts_workspace(c, p + s.rest + logits);
+  const bool few = dbk::moe_few(*m, T, k);
+  const hipError_t e = few ? dbk::launch_moe_logits(r, (hipStream_t)stream)
+                           : dbk::launch_moe_route(r, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_status(e, fn);
+  if (few) {
+    const dbk::MoeFewCall f = {c, r.logits, experts, weights, r.renormalize};
+    return hip_status(dbk::launch_moe_few(f, (hipStream_t)stream), fn);
+  }
   return hip_status(dbk::launch_moe_experts(c, (hipStream_t)stream), fn);
 }
 

@@ -229,6 +229,7 @@ struct MoeRouteCall {
   bool renormalize, bf16;
 };
 hipError_t launch_moe_route(const MoeRouteCall& c, hipStream_t stream);
+hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream);  // its first half
 
 struct MoeExpertsCall {
   const void* x;         // [T, H], rows x_row elements apart
@@ -245,6 +246,18 @@ struct MoeExpertsCall {
   void* h;       // [T k, I] by slot
   float* parts;  // [T k, H] by pair
 };
+// The experts of a few tokens (moe_few.hip), whose pairs each read their expert's
+// weights: with `route` the choice among c.logits is theirs too, and c.experts and
+// c.weights are written.
+struct MoeFewCall {
+  MoeExpertsCall c;
+  const double* logits;  // [T, E], or null: experts and weights are given
+  int* experts;
+  float* weights;
+  bool renormalize;
+};
+bool moe_few(const db_moe& m, int T, int k);
+hipError_t launch_moe_few(const MoeFewCall& f, hipStream_t stream);
 // Lays the workspace out from ws on; returns its bytes.
 size_t moe_experts_workspace(MoeExpertsCall& c, void* ws);
 hipError_t launch_moe_experts(const MoeExpertsCall& c, hipStream_t stream);

@@ -14,8 +14,8 @@
 // g, u, silu and the product are fp32; h is rounded once to the activations'
 // type, which the second product takes; what the pairs of a token add up to is
 // fp32 again, in the order of its experts, and rounded once.
-#include "db_elem.h"
 #include "db_kernels.h"
+#include "moe_select.h"
 
 namespace dbk {
 
@@ -24,7 +24,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kOut = 1 << 30;  // an offset behind every buffer: loads give zero
-constexpr int kMostExperts = 1024;
 
 // Sorts the pairs by expert and cuts them into tiles of `most`.
 //   order[slot]   = pair

@@ -1,0 +1,312 @@
+// moe_few.hip -- the experts of a mixture-of-experts layer for a token or a few:
+// two launches, and none to sort, choose or add up.
+//
+//   moe_few_gate   h[p, i] = silu(Wg[e] x[t]) * (Wu[e] x[t])   for each pair p = (t, j)
+//   moe_few_down   y[t, n] = sum_j w[t, j] Wd[e] h[p]
+//
+// Each pair reads its expert's weights itself: with few tokens hardly any expert is
+// asked twice, and then its second reader finds the rows in the L2 or behind it.
+// The bytes of the weights bound it.  A wave has a row (of gate and up, or of down
+// for all of a token's experts): a load instruction takes 1 KB of it, the next
+// kAhead items of the wave are on their way to registers, products are two 16-bit
+// elements at a time (e4m3 is widened first, exactly) with fp32 sums, and a row's
+// sum over the lanes comes once, at its end.  The scale of a block multiplies the
+// lane's sum of its 16 elements of the block.
+//
+// With the router's logits given, every workgroup of the first launch chooses its
+// token's experts for itself (1 us, and no launch between): the second launch gets
+// the choice from the workgroups of the first rows.
+#include "db_kernels.h"
+#include "moe_select.h"
+
+namespace dbk {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kOut = 1 << 30;  // an offset behind every buffer: loads give zero
+
+__device__ __forceinline__ float dot2(h2 a, h2 b, float c) {
+  return __builtin_amdgcn_fdot2(a, b, c, false);
+}
+__device__ __forceinline__ float dot2(b2 a, b2 b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(a, b, c, false);
+}
+// (by value: a bit cast of a vector's element takes the vector's first bytes)
+template <class V>
+__device__ __forceinline__ V as2(unsigned v) {
+  return __builtin_bit_cast(V, v);
+}
+template <class V>
+__device__ __forceinline__ float dot8v(u4 a, u4 b, float c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = dot2(as2<V>(a[i]), as2<V>(b[i]), c);
+  return c;
+}
+
+template <class E>
+struct Pair2;
+template <>
+struct Pair2<ElemF16> {
+  typedef h2 type;
+};
+template <>
+struct Pair2<ElemBF16> {
+  typedef b2 type;
+};
+
+// A lane's 16 bytes of a row times the same columns of x in the LDS.
+template <class E, bool FP8>
+__device__ __forceinline__ float dot_chunk(u4 w, const char* x) {
+  typedef typename Pair2<E>::type V;
+  if constexpr (!FP8) {
+    return dot8v<V>(w, ld16(x), 0.0f);
+  } else {
+    const u2 a = E::widen(w[0]), b = E::widen(w[1]), c = E::widen(w[2]), d = E::widen(w[3]);
+    const float lo = dot8v<V>(u4{a[0], a[1], b[0], b[1]}, ld16(x), 0.0f);
+    return dot8v<V>(u4{c[0], c[1], d[0], d[1]}, ld16(x + 16), lo);
+  }
+}
+
+// Copies a row of K elements to the LDS, with zeros up to a whole number of chunks.
+__device__ __forceinline__ void row_to_lds(char* to, const void* from, int K, int padded) {
+  for (int k = threadIdx.x * 8; k < padded; k += kThreads * 8)
+    *reinterpret_cast<u4*>(to + k * 2) =
+        k < K ? ld16(static_cast<const unsigned short*>(from) + k) : u4{0, 0, 0, 0};
+}
+
+struct FewArgs {
+  MoeFewCall f;
+  int slices;    // workgroups of a pair, or of a token
+  int padded;    // K in whole chunks
+};
+
+// A workgroup has every (slices)th group of kWaves rows of one pair.
+template <class E, bool FP8>
+__global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
+  typedef typename E::type elem;
+  constexpr int CE = FP8 ? 1024 : 512;  // elements of a row a load instruction takes
+  constexpr int CH = FP8 ? 2 : 4;       // of each matrix in an item
+  constexpr int kAhead = 2;
+  extern __shared__ __align__(16) char s_x[];
+  __shared__ MoeChoice s_choice;
+  const MoeExpertsCall& c = a.f.c;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int pair = blockIdx.x / a.slices, slice = blockIdx.x - pair * a.slices;
+  const int t = pair / c.k, j = pair - t * c.k;
+  const int H = c.w.H, I = c.w.I;
+  row_to_lds(s_x, static_cast<const elem*>(c.x) + t * c.x_row, H, a.padded);
+  int expert;
+  if (a.f.logits) {
+    moe_choose<kThreads>(s_choice, a.f.logits + (size_t)t * c.w.E, c.w.E, c.k, a.f.renormalize);
+    expert = s_choice.expert[j];
+    if (slice == 0 && threadIdx.x == 0) {
+      a.f.experts[pair] = expert;
+      a.f.weights[pair] = s_choice.p[j] / s_choice.total;
+    }
+  } else {
+    expert = c.experts[pair];
+    __syncthreads();
+  }
+  expert = __builtin_amdgcn_readfirstlane(expert);
+  if ((unsigned)expert >= (unsigned)c.w.E) return;
+
+  const int KB = (H + 127) / 128, NB = (I + 127) / 128;
+  constexpr int CB = FP8 ? 1 : 2;
+  const size_t row_bytes = (size_t)H * CB;
+  const char* const wg = static_cast<const char*>(c.w.wg) + (size_t)expert * I * row_bytes;
+  const char* const wu = static_cast<const char*>(c.w.wu) + (size_t)expert * I * row_bytes;
+  const int items = (a.padded / CE + CH - 1) / CH;  // of a row
+  const int stride = a.slices * kWaves;
+  int at_row = slice * kWaves + wave, at_item = 0;
+  u4 w[kAhead][2][CH];
+  float scale[kAhead][2][CH];
+  auto load = [&](int u) {
+    // (behind the last row nothing is read)
+    const int row = min(at_row, I - 1), bytes = at_row < I ? (int)row_bytes : 0;
+    const __amdgpu_buffer_rsrc_t rg = make_rsrc(wg + row * row_bytes, bytes);
+    const __amdgpu_buffer_rsrc_t ru = make_rsrc(wu + row * row_bytes, bytes);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int off = ((at_item * CH + i) * kWave + lane) * 16;
+      w[u][0][i] = ld_buf_stream(rg, off);
+      w[u][1][i] = ld_buf_stream(ru, off);
+      if constexpr (FP8) {
+        const size_t at = ((size_t)expert * NB + row / 128) * KB + min(off / 128, KB - 1);
+        scale[u][0][i] = off < H ? c.w.sg[at] : 0.0f;
+        scale[u][1][i] = off < H ? c.w.su[at] : 0.0f;
+      }
+    }
+    const bool wrap = ++at_item >= items;
+    at_item = wrap ? 0 : at_item;
+    at_row += wrap ? stride : 0;
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) load(u);
+  int row = slice * kWaves + wave, item = 0;
+  float g = 0.0f, up = 0.0f;
+  while (row < I) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (row >= I) break;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const char* const x = s_x + ((item * CH + i) * kWave + lane) * (FP8 ? 32 : 16);
+        if ((item * CH + i) * CE >= a.padded) break;
+        const float pg = dot_chunk<E, FP8>(w[u][0][i], x), pu = dot_chunk<E, FP8>(w[u][1][i], x);
+        g += FP8 ? pg * scale[u][0][i] : pg;
+        up += FP8 ? pu * scale[u][1][i] : pu;
+      }
+      load(u);
+      if (++item == items) {
+        g = wave_sum(g);
+        up = wave_sum(up);
+        if (lane == 0)
+          static_cast<elem*>(c.h)[(size_t)pair * I + row] = (elem)(g / (1.0f + expf(-g)) * up);
+        g = up = 0.0f;
+        item = 0;
+        row += stride;
+      }
+    }
+  }
+}
+
+// A workgroup has every (slices)th group of kWaves rows of one token.
+template <class E, bool FP8>
+__global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
+  typedef typename E::type elem;
+  constexpr int CE = FP8 ? 1024 : 512;
+  constexpr int CH = 2;
+  constexpr int kAhead = 4;
+  extern __shared__ __align__(16) char s_h[];
+  __shared__ int s_expert[kMostChoices];
+  __shared__ float s_weight[kMostChoices];
+  const MoeExpertsCall& c = a.f.c;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int t = blockIdx.x / a.slices, slice = blockIdx.x - t * a.slices;
+  const int H = c.w.H, I = c.w.I, k = c.k;
+  if (threadIdx.x < k) {
+    const int e = c.experts[t * k + threadIdx.x];
+    s_expert[threadIdx.x] = e;
+    s_weight[threadIdx.x] = (unsigned)e < (unsigned)c.w.E ? c.weights[t * k + threadIdx.x] : 0.0f;
+  }
+  for (int j = 0; j < k; ++j) {
+    // h of an expert that does not exist was not written
+    const bool exists = (unsigned)c.experts[t * k + j] < (unsigned)c.w.E;
+    row_to_lds(s_h + (size_t)j * a.padded * 2,
+               static_cast<const elem*>(c.h) + (size_t)(t * k + j) * I, exists ? I : 0, a.padded);
+  }
+  __syncthreads();
+
+  const int KB = (I + 127) / 128, NB = (H + 127) / 128;
+  constexpr int CB = FP8 ? 1 : 2;
+  const size_t row_bytes = (size_t)I * CB;
+  const int items = (a.padded / CE + CH - 1) / CH;  // of a row of one expert
+  const int stride = a.slices * kWaves;
+  int at_row = slice * kWaves + wave, at_j = 0, at_item = 0;
+  u4 w[kAhead][CH];
+  float scale[kAhead][CH];
+  auto load = [&](int u) {
+    const int e = __builtin_amdgcn_readfirstlane(s_expert[at_j]);
+    const bool exists = at_row < H && (unsigned)e < (unsigned)c.w.E;
+    const size_t row = exists ? (size_t)e * H + at_row : 0;
+    const __amdgpu_buffer_rsrc_t rd = make_rsrc(
+        static_cast<const char*>(c.w.wd) + row * row_bytes, exists ? (int)row_bytes : 0);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int off = ((at_item * CH + i) * kWave + lane) * 16;
+      w[u][i] = ld_buf_stream(rd, off);
+      if constexpr (FP8) {
+        const size_t nb = exists ? (size_t)e * NB + at_row / 128 : 0;
+        scale[u][i] = off < I ? c.w.sd[nb * KB + min(off / 128, KB - 1)] : 0.0f;
+      }
+    }
+    const bool wrap = ++at_item >= items;
+    at_item = wrap ? 0 : at_item;
+    at_j += wrap ? 1 : 0;
+    const bool next = at_j >= k;
+    at_j = next ? 0 : at_j;
+    at_row += next ? stride : 0;
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) load(u);
+  int row = slice * kWaves + wave, j = 0, item = 0;
+  float sum = 0.0f, part = 0.0f;
+  while (row < H) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (row >= H) break;
+      const char* const h = s_h + (size_t)j * a.padded * 2;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        if ((item * CH + i) * CE >= a.padded) break;
+        const float p = dot_chunk<E, FP8>(
+            w[u][i], h + ((item * CH + i) * kWave + lane) * (FP8 ? 32 : 16));
+        part += FP8 ? p * scale[u][i] : p;
+      }
+      load(u);
+      if (++item == items) {
+        // (a pair without an expert adds nothing, whatever its weight was)
+        if ((unsigned)s_expert[j] < (unsigned)c.w.E) sum += part * s_weight[j];
+        part = 0.0f;
+        item = 0;
+        if (++j == k) {
+          sum = wave_sum(sum);
+          if (lane == 0) static_cast<elem*>(c.y)[(size_t)t * H + row] = (elem)sum;
+          sum = 0.0f;
+          j = 0;
+          row += stride;
+        }
+      }
+    }
+  }
+}
+
+int chunks(int K, bool fp8) {
+  const int CE = fp8 ? 1024 : 512;
+  return (K + CE - 1) / CE * CE;
+}
+
+template <class E, bool FP8>
+hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
+  const MoeExpertsCall& c = f.c;
+  int err = 0;
+  const int cus = device_cu_count(&err);
+  if (err) return (hipError_t)err;
+  // waves for each CU, and no more than rows
+  auto slices = [&](int groups, int rows) {
+    const int want = (8 * cus / kWaves + groups - 1) / groups;
+    return max(1, min(want, (rows + kWaves - 1) / kWaves));
+  };
+  const int P = c.T * c.k;
+  FewArgs g = {f, slices(P, c.w.I), chunks(c.w.H, FP8)};
+  moe_few_gate<E, FP8><<<P * g.slices, kThreads, (size_t)g.padded * 2, stream>>>(g);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  FewArgs d = {f, slices(c.T, c.w.H), chunks(c.w.I, FP8)};
+  moe_few_down<E, FP8><<<c.T * d.slices, kThreads, (size_t)d.padded * 2 * c.k, stream>>>(d);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Few pairs, whose rows of x and h fit the LDS that a launch has without asking.
+bool moe_few(const db_moe& m, int T, int k) {
+  const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
+  constexpr size_t kLds = 64 * 1024;
+  return T <= 4 && T * k <= 32 &&
+         (size_t)chunks(m.H, fp8) * 2 + sizeof(MoeChoice) + 1024 <= kLds &&
+         (size_t)chunks(m.I, fp8) * 2 * k + 1024 <= kLds;
+}
+
+hipError_t launch_moe_few(const MoeFewCall& f, hipStream_t stream) {
+  const bool fp8 = f.c.w.w_dtype == DB_DTYPE_FP8_E4M3;
+  if (f.c.bf16)
+    return fp8 ? launch<ElemBF16, true>(f, stream) : launch<ElemBF16, false>(f, stream);
+  return fp8 ? launch<ElemF16, true>(f, stream) : launch<ElemF16, false>(f, stream);
+}
+
+}  // namespace dbk

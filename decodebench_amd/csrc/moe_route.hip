@@ -9,8 +9,8 @@
 // summed in 64 bits (v_mfma_f64_16x16x4, products of 16-bit numbers are exact):
 // they do not depend on the order of the sum where that could be seen, and a
 // token's experts not on the batch it comes in.
-#include "db_elem.h"
 #include "db_kernels.h"
+#include "moe_select.h"
 
 namespace dbk {
 
@@ -63,89 +63,72 @@ __global__ __launch_bounds__(kWaves* kWave) void moe_logits(MoeRouteCall c) {
   }
 }
 
-__device__ __forceinline__ double shfl_xor(double v, int mask) {
-  return __shfl_xor(v, mask, kWave);
+// Few tokens: a wave has an expert and all of them.  Eight elements of a row a
+// lane and step, their products (exact in fp32) added up in 64 bits.
+constexpr int kFewTokens = 4;
+
+template <class E>
+__global__ __launch_bounds__(4 * kWave) void moe_logits_few(MoeRouteCall c) {
+  typedef typename E::type elem;
+  typedef typename E::vec8 vec8;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int e = blockIdx.x * 4 + threadIdx.x / kWave;
+  if (e >= c.E) return;
+  const elem* const wr = static_cast<const elem*>(c.router) + (size_t)e * c.H;
+  double acc[kFewTokens] = {};
+  for (int h = lane * 8; h < c.H; h += kWave * 8) {
+    const vec8 w = __builtin_bit_cast(vec8, ld16(wr + h));
+#pragma unroll
+    for (int t = 0; t < kFewTokens; ++t) {
+      if (t >= c.T) break;
+      const vec8 x = __builtin_bit_cast(vec8, ld16(static_cast<const elem*>(c.x) + t * c.x_row + h));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[t] += (double)((float)w[j] * (float)x[j]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kFewTokens; ++t) {
+    if (t >= c.T) break;
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) acc[t] += __shfl_xor(acc[t], m, kWave);
+    if (lane == 0) c.logits[(size_t)t * c.E + e] = acc[t];
+  }
 }
 
-// Whether logit a of expert i comes before logit b of expert j.
-__device__ __forceinline__ bool before(double a, int i, double b, int j) {
-  const bool an = a != a, bn = b != b;
-  if (an != bn) return an;
-  if (an || a == b) return i < j;
-  return a > b;
-}
-
-// A wave has a token; lane l its experts l, l + 64, ...
-template <int N>
-__global__ __launch_bounds__(kWave) void moe_select(MoeRouteCall c) {
-  const int t = blockIdx.x, lane = threadIdx.x;
-  double l[N];
-  bool left[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = lane + 64 * i;
-    left[i] = e < c.E;
-    l[i] = left[i] ? c.logits[(size_t)t * c.E + e] : 0.0;
-  }
-  double top = 0.0;
-  float total = 0.0f, mine = 0.0f;  // mine: exp of choice `lane`
-  int chosen = 0;
-  for (int j = 0; j < c.k; ++j) {
-    double best = 0.0;
-    int at = 1 << 30;  // none left in this lane
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (left[i] && (at == 1 << 30 || before(l[i], lane + 64 * i, best, at))) {
-        best = l[i];
-        at = lane + 64 * i;
-      }
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) {
-      const double ob = shfl_xor(best, m);
-      const int oa = __shfl_xor(at, m, kWave);
-      if (oa != 1 << 30 && (at == 1 << 30 || before(ob, oa, best, at))) {
-        best = ob;
-        at = oa;
-      }
-    }
-    if (j == 0) top = best;
-    const float p = expf((float)(best - top));
-    total += p;
-    if (lane == j) {
-      mine = p;
-      chosen = at;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) left[i] = left[i] && lane + 64 * i != at;
-  }
-  if (!c.renormalize) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 64 * i < c.E) sum += expf((float)(l[i] - top));
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) sum += __shfl_xor(sum, m, kWave);
-    total = sum;
-  }
-  if (lane < c.k) {
-    c.experts[(size_t)t * c.k + lane] = chosen;
-    c.weights[(size_t)t * c.k + lane] = mine / total;
+// A workgroup has a token.
+__global__ __launch_bounds__(256) void moe_select(MoeRouteCall c) {
+  __shared__ MoeChoice s;
+  const size_t t = blockIdx.x;
+  moe_choose<256>(s, c.logits + t * c.E, c.E, c.k, c.renormalize);
+  if (threadIdx.x < c.k) {
+    c.experts[t * c.k + threadIdx.x] = s.expert[threadIdx.x];
+    c.weights[t * c.k + threadIdx.x] = s.p[threadIdx.x] / s.total;
   }
 }
 
 }  // namespace
 
-hipError_t launch_moe_route(const MoeRouteCall& c, hipStream_t stream) {
+hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream) {
+  if (c.T <= kFewTokens) {
+    const int grid = (c.E + 3) / 4;
+    if (c.bf16)
+      moe_logits_few<ElemBF16><<<grid, 4 * kWave, 0, stream>>>(c);
+    else
+      moe_logits_few<ElemF16><<<grid, 4 * kWave, 0, stream>>>(c);
+    return hipGetLastError();
+  }
   const dim3 grid((c.E + 15) / 16, (c.T + 15) / 16);
   if (c.bf16)
     moe_logits<ElemBF16><<<grid, kWaves * kWave, 0, stream>>>(c);
   else
     moe_logits<ElemF16><<<grid, kWaves * kWave, 0, stream>>>(c);
-  const hipError_t e = hipGetLastError();
+  return hipGetLastError();
+}
+
+hipError_t launch_moe_route(const MoeRouteCall& c, hipStream_t stream) {
+  const hipError_t e = launch_moe_logits(c, stream);
   if (e != hipSuccess) return e;
-  auto* const fn = c.E <= 64 ? moe_select<1> : c.E <= 128 ? moe_select<2> : c.E <= 256
-                   ? moe_select<4> : moe_select<16>;
-  fn<<<c.T, kWave, 0, stream>>>(c);
+  moe_select<<<c.T, 256, 0, stream>>>(c);
   return hipGetLastError();
 }
 

@@ -1,0 +1,77 @@
+// moe_select.h -- the k experts of one token and their weights, from its E logits,
+// by the threads of a workgroup.  Shared by the router's own kernel and by the
+// expert kernel of few tokens, which chooses for itself: both give the same bits.
+#pragma once
+
+#include "db_elem.h"
+
+namespace dbk {
+
+constexpr int kMostExperts = 1024;
+constexpr int kMostChoices = 64;
+
+struct MoeChoice {
+  double logit[kMostExperts];
+  int rank[kMostExperts];
+  int expert[kMostChoices];
+  float p[kMostChoices];
+  float total;
+};
+
+// A logit's place in the order: NaN above Inf above all numbers (sums of products of
+// 16-bit numbers stay far below the largest double).
+__device__ __forceinline__ double logit_key(double l) {
+  return l != l ? __builtin_huge_val() : l == __builtin_huge_val() ? 0x1.fffffffffffffp1023 : l;
+}
+
+// Fills s.expert and s.p (exp of each choice against the largest) and s.total (of
+// the choices, or of all experts).  Ranks are counted: an expert comes after those
+// of larger logits, and of equal ones with a lower index.  NT threads, barriers
+// within; E and k are uniform.
+template <int NT>
+__device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, int E, int k,
+                                           bool renormalize) {
+  const int tid = threadIdx.x;
+  for (int e = tid; e < E; e += NT) {
+    s.logit[e] = logits[e];
+    s.rank[e] = 0;
+  }
+  __syncthreads();
+  // experts by the threads, what they are compared with in `parts` parts
+  int lanes = 64;
+  while (lanes < E && lanes < NT) lanes *= 2;
+  const int parts = NT / lanes, mine = tid & (lanes - 1), part = tid / lanes;
+  const int each = (E + parts - 1) / parts, begin = part * each, end = min(E, begin + each);
+  for (int e = mine; e < E; e += lanes) {
+    const double l = logit_key(s.logit[e]);
+    int before = 0;
+#pragma unroll 4
+    for (int o = begin; o < end; ++o) {
+      const double v = logit_key(s.logit[o]);
+      before += (v > l || (v == l && o < e)) ? 1 : 0;
+    }
+    atomicAdd(&s.rank[e], before);
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += NT)
+    if (s.rank[e] < k) s.expert[s.rank[e]] = e;
+  __syncthreads();
+  const double top = s.logit[s.expert[0]];
+  if (tid < k) s.p[tid] = expf((float)(s.logit[s.expert[tid]] - top));
+  if (!renormalize && tid < kWave) {
+    float sum = 0.0f;
+    for (int e = tid; e < E; e += kWave) sum += expf((float)(s.logit[e] - top));
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) sum += __shfl_xor(sum, m, kWave);
+    if (tid == 0) s.total = sum;
+  }
+  __syncthreads();
+  if (renormalize && tid == 0) {
+    float sum = 0.0f;
+    for (int j = 0; j < k; ++j) sum += s.p[j];
+    s.total = sum;
+  }
+  __syncthreads();
+}
+
+}  // namespace dbk
