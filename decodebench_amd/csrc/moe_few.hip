@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;  // elements of a row a load instruction takes
   constexpr int CH = FP8 ? 2 : 4;       // of each matrix in an item
-  constexpr int kAhead = 2;
+  constexpr int kAhead = FP8 ? 4 : 2;   // items on their way: 16 KB a wave
   extern __shared__ __align__(16) char s_x[];
   __shared__ MoeChoice s_choice;
   const MoeExpertsCall& c = a.f.c;
@@ -178,8 +178,8 @@ template <class E, bool FP8>
 __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;
-  constexpr int CH = 2;
-  constexpr int kAhead = 4;
+  constexpr int CH = FP8 ? 1 : 2;
+  constexpr int kAhead = 8;  // items on their way: 8 or 16 KB a wave
   extern __shared__ __align__(16) char s_h[];
   __shared__ int s_expert[kMostChoices];
   __shared__ float s_weight[kMostChoices];
@@ -193,12 +193,18 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
     s_expert[threadIdx.x] = e;
     s_weight[threadIdx.x] = (unsigned)e < (unsigned)c.w.E ? c.weights[t * k + threadIdx.x] : 0.0f;
   }
-  for (int j = 0; j < k; ++j) {
-    // h of an expert that does not exist was not written
-    const bool exists = (unsigned)c.experts[t * k + j] < (unsigned)c.w.E;
-    row_to_lds(s_h + (size_t)j * a.padded * 2,
-               static_cast<const elem*>(c.h) + (size_t)(t * k + j) * I, exists ? I : 0, a.padded);
-  }
+  // The first pieces of h are asked for before the weights, which come in order
+  // behind them.  (What h holds of a pair without an expert does not count.)
+  const int row_pieces = a.padded / 8, pieces = k * row_pieces;
+  const elem* const h_from = static_cast<const elem*>(c.h) + (size_t)t * k * I;
+  auto piece = [&](int i) {
+    const int j = i / row_pieces, at = (i - j * row_pieces) * 8;
+    return at < I && j < k ? ld16(h_from + (size_t)j * I + at) : u4{0, 0, 0, 0};
+  };
+  constexpr int kFirst = 4;
+  u4 first[kFirst];
+#pragma unroll
+  for (int r = 0; r < kFirst; ++r) first[r] = piece(threadIdx.x + r * kThreads);
   __syncthreads();
 
   const int KB = (I + 127) / 128, NB = (H + 127) / 128;
@@ -233,6 +239,14 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   };
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) load(u);
+#pragma unroll
+  for (int r = 0; r < kFirst; ++r) {
+    const int i = threadIdx.x + r * kThreads;
+    if (i < pieces) *reinterpret_cast<u4*>(s_h + (size_t)i * 16) = first[r];
+  }
+  for (int i = threadIdx.x + kFirst * kThreads; i < pieces; i += kThreads)
+    *reinterpret_cast<u4*>(s_h + (size_t)i * 16) = piece(i);
+  __syncthreads();
   int row = slice * kWaves + wave, j = 0, item = 0;
   float sum = 0.0f, part = 0.0f;
   while (row < H) {

@@ -76,14 +76,31 @@ __global__ __launch_bounds__(4 * kWave) void moe_logits_few(MoeRouteCall c) {
   if (e >= c.E) return;
   const elem* const wr = static_cast<const elem*>(c.router) + (size_t)e * c.H;
   double acc[kFewTokens] = {};
-  for (int h = lane * 8; h < c.H; h += kWave * 8) {
-    const vec8 w = __builtin_bit_cast(vec8, ld16(wr + h));
+  // four steps' loads at once
+  constexpr int kSteps = 4;
+  for (int h0 = lane * 8; h0 < c.H; h0 += kWave * 8 * kSteps) {
+    u4 w[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int h = h0 + i * kWave * 8;
+      w[i] = h < c.H ? ld16(wr + h) : u4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int t = 0; t < kFewTokens; ++t) {
       if (t >= c.T) break;
-      const vec8 x = __builtin_bit_cast(vec8, ld16(static_cast<const elem*>(c.x) + t * c.x_row + h));
+      const elem* const row = static_cast<const elem*>(c.x) + t * c.x_row;
+      u4 x[kSteps];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[t] += (double)((float)w[j] * (float)x[j]);
+      for (int i = 0; i < kSteps; ++i) {
+        const int h = h0 + i * kWave * 8;
+        x[i] = h < c.H ? ld16(row + h) : u4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const vec8 wv = __builtin_bit_cast(vec8, w[i]), xv = __builtin_bit_cast(vec8, x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[t] += (double)((float)wv[j] * (float)xv[j]);
+      }
     }
   }
 #pragma unroll

@@ -12,6 +12,7 @@ constexpr int kMostChoices = 64;
 
 struct MoeChoice {
   double logit[kMostExperts];
+  __align__(16) double key[kMostExperts + 2];
   int rank[kMostExperts];
   int expert[kMostChoices];
   float p[kMostChoices];
@@ -32,23 +33,30 @@ template <int NT>
 __device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, int E, int k,
                                            bool renormalize) {
   const int tid = threadIdx.x;
-  for (int e = tid; e < E; e += NT) {
-    s.logit[e] = logits[e];
-    s.rank[e] = 0;
+  for (int e = tid; e < E + 2; e += NT) {
+    const double l = e < E ? logits[e] : 0.0;
+    // (behind the last one stands what comes before nothing)
+    s.key[e] = e < E ? logit_key(l) : -__builtin_huge_val();
+    if (e < E) {
+      s.logit[e] = l;
+      s.rank[e] = 0;
+    }
   }
   __syncthreads();
   // experts by the threads, what they are compared with in `parts` parts
   int lanes = 64;
   while (lanes < E && lanes < NT) lanes *= 2;
   const int parts = NT / lanes, mine = tid & (lanes - 1), part = tid / lanes;
-  const int each = (E + parts - 1) / parts, begin = part * each, end = min(E, begin + each);
+  const int each = ((E + parts - 1) / parts + 1) & ~1, begin = part * each;
+  const int end = min(E, begin + each);
   for (int e = mine; e < E; e += lanes) {
-    const double l = logit_key(s.logit[e]);
+    const double l = s.key[e];
     int before = 0;
-#pragma unroll 4
-    for (int o = begin; o < end; ++o) {
-      const double v = logit_key(s.logit[o]);
-      before += (v > l || (v == l && o < e)) ? 1 : 0;
+#pragma unroll 8
+    for (int o = begin; o < end; o += 2) {
+      const double a = s.key[o], b = s.key[o + 1];
+      before += (a > l) | ((a == l) & (o < e)) ? 1 : 0;
+      before += (b > l) | ((b == l) & (o + 1 < e)) ? 1 : 0;
     }
     atomicAdd(&s.rank[e], before);
   }
