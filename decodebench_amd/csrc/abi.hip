@@ -695,6 +695,7 @@ namespace {
 
 constexpr int kMostSize = 1 << 22;   // of the tokens, rows and columns of a product
 constexpr int kMostTokens = 1 << 20; // of a mixture-of-experts layer
+constexpr int kMostWidth = 1 << 20;  // of its rows
 constexpr long long kMostOffset = 1ll << 29;  // elements that a kernel's 32-bit offsets reach
 
 size_t blocks128(int n) { return ((size_t)n + 127) / 128; }
@@ -747,9 +748,9 @@ int check_moe(const char* fn, const db_moe* m, const void* x, long long x_stride
   if (m->E < 1 || m->E > 1024)
     return fail(DB_ERR_INVALID, "%s: E=%d outside [1, 1024]", fn, m->E);
   const int step = fp8 ? 16 : 8;
-  if (m->H < step || m->I < step || m->H % step || m->I % step || m->H >= kMostSize ||
-      m->I >= kMostSize)
-    return fail(DB_ERR_INVALID, "%s: H=%d and I=%d must be multiples of %d below 2^22", fn, m->H,
+  if (m->H < step || m->I < step || m->H % step || m->I % step || m->H >= kMostWidth ||
+      m->I >= kMostWidth)
+    return fail(DB_ERR_INVALID, "%s: H=%d and I=%d must be multiples of %d below 2^20", fn, m->H,
                 m->I, step);
   if (k < 1 || k > 64) return fail(DB_ERR_INVALID, "%s: k=%d outside [1, 64]", fn, k);
   if (T < 0 || T >= kMostTokens)
@@ -913,7 +914,7 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
 
 size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k) {
   if (!m || T < 1 || T >= kMostTokens || k < 1 || k > 64 || m->E < 1 || m->E > 1024 || m->H < 1 ||
-      m->I < 1 || m->H >= kMostSize || m->I >= kMostSize)
+      m->I < 1 || m->H >= kMostWidth || m->I >= kMostWidth)
     return 0;
   dbk::MoeExpertsCall c = experts_call(nullptr, 0, nullptr, nullptr, *m, nullptr, T, k);
   return dbk::moe_experts_workspace(c, nullptr);

@@ -15,6 +15,7 @@
 // type, which the second product takes; what the pairs of a token add up to is
 // fp32 again, in the order of its experts, and rounded once.
 #include "db_kernels.h"
+#include "lds_dma.h"
 #include "moe_select.h"
 
 namespace dbk {
@@ -75,144 +76,182 @@ __global__ __launch_bounds__(1024) void moe_sort(MoeExpertsCall c, int most) {
   }
 }
 
-__device__ __forceinline__ u4 ld_buf(__amdgpu_buffer_rsrc_t r, int offset) {
-  return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
-}
-
-// A block of 128 columns of 16 weight rows, as a lane (row r16, quarter q) holds
-// it: 16-bit load j has columns 32 j + 8 q .. + 7, e4m3 load j columns
-// 64 j + 16 q .. + 15.
-template <bool FP8>
-struct Weights {
-  static constexpr int kLoads = FP8 ? 2 : 4;
-  u4 w[kLoads];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row, int b, int q, int K) {
-    constexpr int CB = FP8 ? 1 : 2, VE = 16 / CB;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int k = b * 128 + j * (128 / kLoads) + q * VE;
-      w[j] = ld_buf(r, k < K ? (row * K + k) * CB : kOut);
-    }
-  }
-  // Operand s of four: columns col(s, q) .. + 7.
-  template <class E>
-  __device__ __forceinline__ typename E::vec8 operand(int s) const {
-    if constexpr (!FP8) {
-      return __builtin_bit_cast(typename E::vec8, w[s]);
-    } else {
-      const u2 lo = E::widen(w[s / 2][2 * (s % 2)]), hi = E::widen(w[s / 2][2 * (s % 2) + 1]);
-      return __builtin_bit_cast(typename E::vec8, u4{lo[0], lo[1], hi[0], hi[1]});
-    }
-  }
-  __device__ __forceinline__ static int col(int s, int q) {
-    return FP8 ? 64 * (s / 2) + 16 * q + 8 * (s % 2) : 32 * s + 8 * q;
-  }
-};
-
-// GATED: gate and up rows of the experts on the tokens, h to the workspace;
-// otherwise the down rows on h, each pair's sums to the workspace in fp32.
-template <class E, bool FP8, int TT, bool GATED>
-__global__ __launch_bounds__(kThreads) void moe_product(MoeExpertsCall c) {
+// GATED: 64 gate rows and the 64 up rows of the same channels on the tokens of a
+// tile, h to the workspace; otherwise 128 down rows on h, each pair's sums to the
+// workspace in fp32.  K goes in steps of 128 bytes of a weight row; S stages lie in
+// the LDS, S - 1 of them on their way while one is multiplied.  A row's 16-byte
+// chunk c lies at place c ^ row % 8, set by which chunk a lane fetches: the rows
+// that a quarter of a wave reads then lie in different banks.
+template <class E, bool FP8, int BT, bool GATED, int S>
+__global__ __launch_bounds__(kThreads, 2) void moe_product(MoeExpertsCall c) {
   typedef typename E::type elem;
   typedef typename E::vec8 vec8;
-  constexpr int NW = GATED ? 2 : 1, CB = FP8 ? 1 : 2;
-  __shared__ f4 s_part[kWaves][NW * TT][kWave];
-  const int slices = ((GATED ? c.w.I : c.w.H) + 15) / 16;
+  constexpr int CB = FP8 ? 1 : 2, KE = 128 / CB, XB = KE * 2;  // XB: bytes of a token's step
+  constexpr int TT = BT / 16;
+  constexpr int kLoadsW = 16 / kWaves, kLoadsX = BT * XB / 1024 / kWaves;
+  static_assert(kLoadsX >= 1 && BT * XB % (1024 * kWaves) == 0, "whole loads");
+  constexpr int kLoads = kLoadsW + kLoadsX;
+  constexpr int kRowsX = 1024 / XB;  // tokens of a load instruction
+  constexpr int kStage = 128 * 128 + BT * XB;
+  __shared__ __align__(16) char s_stage[S * kStage];
+  const int slices = GATED ? (c.w.I + 63) / 64 : (c.w.H + 127) / 128;
   const int tile = blockIdx.x / slices, slice = blockIdx.x - tile * slices;
-  if (tile >= c.tiles[0]) return;
-  const int expert = c.tiles[1 + 3 * tile], first = c.tiles[2 + 3 * tile],
-            pairs = c.tiles[3 + 3 * tile];
+  if (tile >= scalar_load(c.tiles)) return;
+  const int expert = scalar_load(c.tiles + 1 + 3 * tile),
+            first = scalar_load(c.tiles + 2 + 3 * tile),
+            pairs = scalar_load(c.tiles + 3 + 3 * tile);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
   const int K = GATED ? c.w.H : c.w.I, N = GATED ? c.w.I : c.w.H;
-  const int n0 = slice * 16, KB = (K + 127) / 128, NB = (N + 127) / 128;
+  const int n0 = slice * (GATED ? 64 : 128), KB = (K + 127) / 128, NB = (N + 127) / 128;
+  const int rows = min(GATED ? 64 : 128, N - n0);
   const size_t w_at = ((size_t)expert * N + n0) * K * CB;
-  const int w_bytes = min(16, N - n0) * K * CB;
-  __amdgpu_buffer_rsrc_t rw[NW];
-  const float* ws[NW] = {};
+
+  // Load i of a wave has weight rows 8 (4 i + wave) .. + 7: of gate (or down) in the
+  // first half of the loads, of up in the second.
+  const u4 rw[2] = {
+      dma_rsrc(static_cast<const char*>(GATED ? c.w.wg : c.w.wd) + w_at, rows * K * CB),
+      dma_rsrc(static_cast<const char*>(GATED ? c.w.wu : c.w.wd) + w_at, rows * K * CB)};
+  const int w_row = (8 * wave + (lane >> 3)) * K * CB;
+  const int w_chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  // The tokens of x (or slots of h): kRowsX of a load, 1024 / kRowsX bytes of each.
+  const u4 rx = GATED ? dma_rsrc(c.x, ((c.T - 1) * (int)c.x_row + K) * 2)
+                      : dma_rsrc(c.h, c.T * c.k * K * 2);
+  constexpr int kLanesX = 64 / kRowsX;
+  int x_row[kLoadsX];
 #pragma unroll
-  for (int m = 0; m < NW; ++m) {
-    const void* base = GATED ? (m ? c.w.wu : c.w.wg) : c.w.wd;
-    rw[m] = make_rsrc(static_cast<const char*>(base) + w_at, w_bytes);
-    if constexpr (FP8)
-      ws[m] = (GATED ? (m ? c.w.su : c.w.sg) : c.w.sd) + ((size_t)expert * NB + n0 / 128) * KB;
+  for (int i = 0; i < kLoadsX; ++i) {
+    const int p = (i * kWaves + wave) * kRowsX + lane / kLanesX;
+    x_row[i] = p >= pairs ? kOut
+               : GATED    ? c.order[first + p] / c.k * (int)c.x_row * 2
+                          : (first + p) * K * 2;
   }
-  // rows of the other operand: tokens of x, or slots of h
-  const __amdgpu_buffer_rsrc_t rx = GATED ? make_rsrc(c.x, (c.T - 1) * (int)c.x_row * 2 + K * 2)
-                                          : make_rsrc(c.h, c.T * c.k * K * 2);
-  int xr[TT];
+  const int x_place = lane % kLanesX;
+  const unsigned lds = lds_address(s_stage);
+  auto fetch = [&](int stage, int step) {
+    const unsigned to = lds + stage * kStage;
+    // behind the row's end, and behind the last step, come zeros
+    const int kw = step * 128 + w_chunk;
+    const int ow = kw < K * CB ? kw : kOut;
 #pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    const int p = i * 16 + r16;
-    xr[i] = p >= pairs ? kOut
-            : GATED    ? c.order[first + p] / c.k * (int)c.x_row * 2
-                       : (first + p) * K * 2;
+    for (int i = 0; i < kLoadsW; ++i) {
+      const int half = GATED && i >= kLoadsW / 2 ? 1 : 0, group = i - half * (kLoadsW / 2);
+      dma16(to + (i * kWaves + wave) * 1024, rw[half], ow + w_row + group * kWaves * 8 * K * CB);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoadsX; ++i) {
+      const int row = (i * kWaves + wave) * kRowsX + lane / kLanesX;
+      const int kx = step * XB + (x_place ^ (row & 7)) * 16;
+      dma16(to + 128 * 128 + (i * kWaves + wave) * 1024, rx,
+            kx < K * 2 ? x_row[i] + kx : kOut);
+    }
+  };
+
+  // Two row tiles of a wave: gate and up of the same channels, or two of down.
+  const int tile_row[2] = {GATED ? 16 * wave : 32 * wave, GATED ? 64 + 16 * wave : 32 * wave + 16};
+  const float* ws[2] = {};
+  if constexpr (FP8) {
+    const size_t at = ((size_t)expert * NB + n0 / 128) * KB;
+    ws[0] = (GATED ? c.w.sg : c.w.sd) + at;
+    ws[1] = (GATED ? c.w.su : c.w.sd) + at;
   }
-  f4 acc[NW][TT] = {};
-  for (int b = wave; b < KB; b += kWaves) {
-    Weights<FP8> w[NW];
+  f4 acc[2][TT] = {};
+  auto multiply = [&](int stage, int step) {
+    const char* const pw = s_stage + stage * kStage;
+    const char* const px = pw + 128 * 128;
+    const int sw = r16 & 7;
+    f4 part[2][TT] = {};
+    vec8 a[2][4];
+    constexpr int kOps = FP8 ? 4 : 2;  // products of 32 columns a step
 #pragma unroll
-    for (int m = 0; m < NW; ++m) w[m].load(rw[m], r16, b, q, K);
-    f4 part[NW][TT] = {};
+    for (int m = 0; m < 2; ++m) {
+      const char* const row = pw + (tile_row[m] + r16) * 128;
+      if constexpr (FP8) {
+        // 16-byte chunks q and 4 + q: columns 16 q .. + 15 of each half, two operands each
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      vec8 a[NW];
+        for (int h = 0; h < 2; ++h) {
+          const u4 v = ld16(row + ((4 * h + q) ^ sw) * 16);
+          const u2 b0 = E::widen(v[0]), b1 = E::widen(v[1]), b2 = E::widen(v[2]),
+                   b3 = E::widen(v[3]);
+          a[m][2 * h] = __builtin_bit_cast(vec8, u4{b0[0], b0[1], b1[0], b1[1]});
+          a[m][2 * h + 1] = __builtin_bit_cast(vec8, u4{b2[0], b2[1], b3[0], b3[1]});
+        }
+      } else {
 #pragma unroll
-      for (int m = 0; m < NW; ++m) a[m] = w[m].template operand<E>(s);
-      const int k = b * 128 + Weights<FP8>::col(s, q);
+        for (int h = 0; h < 2; ++h)
+          a[m][h] = __builtin_bit_cast(vec8, ld16(row + ((4 * h + q) ^ sw) * 16));
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < TT; ++i) {
-        const vec8 x = __builtin_bit_cast(vec8, ld_buf(rx, k < K ? xr[i] + k * 2 : kOut));
+    for (int j = 0; j < TT; ++j) {
+      if (16 * j >= pairs) break;
+      const char* const row = px + (16 * j + r16) * XB;
 #pragma unroll
-        for (int m = 0; m < NW; ++m) {
+      for (int s = 0; s < kOps; ++s) {
+        // the same columns: e4m3 64 (s / 2) + 16 q + 8 (s % 2), 16-bit 32 s + 8 q
+        const int place = FP8 ? 8 * (s / 2) + 2 * q + s % 2 : 4 * s + q;
+        const vec8 x = __builtin_bit_cast(vec8, ld16(row + (place ^ sw) * 16));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
           if constexpr (FP8)
-            part[m][i] = E::mfma16(a[m], x, part[m][i]);
+            part[m][j] = E::mfma16(a[m][s], x, part[m][j]);
           else
-            acc[m][i] = E::mfma16(a[m], x, acc[m][i]);
+            acc[m][j] = E::mfma16(a[m][s], x, acc[m][j]);
         }
       }
     }
     if constexpr (FP8) {
 #pragma unroll
-      for (int m = 0; m < NW; ++m) {
-        const float scale = ws[m][b];
+      for (int m = 0; m < 2; ++m) {
+        const float scale = scalar_load(ws[m] + step);
 #pragma unroll
-        for (int i = 0; i < TT; ++i)
+        for (int j = 0; j < TT; ++j) {
+          if (16 * j >= pairs) break;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[m][i][j] += part[m][i][j] * scale;
+          for (int e = 0; e < 4; ++e) acc[m][j][e] += part[m][j][e] * scale;
+        }
       }
     }
+  };
+  const int steps = (K + KE - 1) / KE;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s, s);
+  int stage = 0, free_stage = S - 1;
+  for (int s = 0; s < steps; ++s) {
+    dma_barrier<(S - 2) * kLoads>();
+    fetch(free_stage, s + S - 1);
+    multiply(stage, s);
+    stage = stage + 1 == S ? 0 : stage + 1;
+    free_stage = free_stage + 1 == S ? 0 : free_stage + 1;
   }
+  // register i of a lane is row 4 q + i of a row tile, column r16: a pair
 #pragma unroll
-  for (int m = 0; m < NW; ++m)
-#pragma unroll
-    for (int i = 0; i < TT; ++i) s_part[wave][m * TT + i][lane] = acc[m][i];
-  __syncthreads();
-  for (int i = wave; i < TT; i += kWaves) {
-    f4 sum[NW];
-#pragma unroll
-    for (int m = 0; m < NW; ++m) {
-      sum[m] = s_part[0][m * TT + i][lane];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) sum[m] += s_part[w][m * TT + i][lane];
-    }
-    // register j of a lane is row 4 q + j, column r16
-    const int p = i * 16 + r16, n = n0 + 4 * q;
-    if (p >= pairs || n >= N) continue;
+  for (int j = 0; j < TT; ++j) {
+    const int p = 16 * j + r16;
+    if (p >= pairs) continue;
     if constexpr (GATED) {
-      typename E::vec4 h;
+      const int n = n0 + 16 * wave + 4 * q;
+      if (n < N) {
+        typename E::vec4 h;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float g = sum[0][j];
-        h[j] = (elem)(g / (1.0f + expf(-g)) * sum[1][j]);
+        for (int e = 0; e < 4; ++e) {
+          const float g = acc[0][j][e];
+          h[e] = (elem)(g / (1.0f + expf(-g)) * acc[1][j][e]);
+        }
+        *reinterpret_cast<typename E::vec4*>(static_cast<elem*>(c.h) + (size_t)(first + p) * N +
+                                             n) = h;
       }
-      *reinterpret_cast<typename E::vec4*>(static_cast<elem*>(c.h) + (size_t)(first + p) * N + n) =
-          h;
     } else {
-      *reinterpret_cast<f4*>(c.parts + (size_t)c.order[first + p] * N + n) = sum[0];
+      float* const to = c.parts + (size_t)c.order[first + p] * N;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int n = n0 + tile_row[m] + 4 * q;
+        if (n < N) *reinterpret_cast<f4*>(to + n) = acc[m][j];
+      }
     }
   }
+  dma_drain();  // what is still on its way into the LDS (zeros), before that is given back
 }
 
 template <class E>
@@ -236,13 +275,13 @@ __global__ __launch_bounds__(kThreads) void moe_combine(MoeExpertsCall c) {
   *reinterpret_cast<typename E::vec4*>(static_cast<elem*>(c.y) + (size_t)t * c.w.H + n) = r;
 }
 
-template <class E, bool FP8, int TT>
+template <class E, bool FP8, int BT, int S>
 void launch(const MoeExpertsCall& c, hipStream_t stream) {
   const int P = c.T * c.k;
-  const int tiles = min(P, c.w.E) + P / (16 * TT);  // at most
-  moe_sort<<<1, 1024, 0, stream>>>(c, 16 * TT);
-  moe_product<E, FP8, TT, true><<<(c.w.I + 15) / 16 * tiles, kThreads, 0, stream>>>(c);
-  moe_product<E, FP8, TT, false><<<(c.w.H + 15) / 16 * tiles, kThreads, 0, stream>>>(c);
+  const int tiles = min(P, c.w.E) + P / BT;  // at most
+  moe_sort<<<1, 1024, 0, stream>>>(c, BT);
+  moe_product<E, FP8, BT, true, S><<<(c.w.I + 63) / 64 * tiles, kThreads, 0, stream>>>(c);
+  moe_product<E, FP8, BT, false, S><<<(c.w.H + 127) / 128 * tiles, kThreads, 0, stream>>>(c);
   const size_t quads = (size_t)c.T * c.w.H / 4;
   moe_combine<E><<<(quads + kThreads - 1) / kThreads, kThreads, 0, stream>>>(c);
 }
@@ -251,12 +290,12 @@ template <class E, bool FP8>
 void pick(const MoeExpertsCall& c, hipStream_t stream) {
   // tokens that an expert has on average
   const int mean = c.T * c.k / c.w.E;
-  if (mean <= 8)
-    launch<E, FP8, 1>(c, stream);
-  else if (mean <= 24)
-    launch<E, FP8, 2>(c, stream);
+  if (mean <= 12)
+    launch<E, FP8, 32, FP8 ? 3 : 4>(c, stream);
+  else if (mean <= 36)
+    launch<E, FP8, 64, FP8 ? 2 : 3>(c, stream);
   else
-    launch<E, FP8, 4>(c, stream);
+    launch<E, FP8, 128, FP8 ? 3 : 2>(c, stream);
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }

@@ -347,7 +347,7 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
  * adds nothing, whatever its weight; a token without any gets zeros.  An expert named
  * twice counts twice.
  * Contract: x, experts, weights, T, k as db_moe_route (k need not be below E); H and I
- * multiples of 8 (16 for e4m3 weights) below 2^22; T x_stride, T k I and T k H below 2^29;
+ * multiples of 8 (16 for e4m3 weights) below 2^20; T x_stride, T k I and T k H below 2^29;
  * weights 16-byte, scales 4-byte aligned, y [T, H] dense; ws of
  * db_moe_experts_workspace_bytes, 256-byte aligned, as that of db_gemm_blocks. */
 size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k);
