@@ -800,7 +800,7 @@ LayerSpace layer_space(const db_moe& m, int T, int k) {
   s.experts = 0;
   s.weights = round256(pairs * sizeof(int));
   s.rest = s.weights + round256(pairs * sizeof(float));
-  s.bytes = s.rest + db_moe_route_workspace_bytes(T, m.E) + db_moe_experts_workspace_bytes(&m, T, k);
+  s.bytes = s.rest + db_moe_route_workspace_bytes(T, m.H, m.E) + db_moe_experts_workspace_bytes(&m, T, k);
   return s;
 }
 
@@ -890,9 +890,9 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
   return hip_status(dbk::launch_gemm_blocks(c, plan, (hipStream_t)stream), fn);
 }
 
-size_t db_moe_route_workspace_bytes(int T, int E) {
-  if (T < 1 || T >= kMostTokens || E < 1 || E > 1024) return 0;
-  return round256((size_t)T * E * sizeof(double));
+size_t db_moe_route_workspace_bytes(int T, int H, int E) {
+  if (T < 1 || T >= kMostTokens || E < 1 || E > 1024 || H < 1 || H >= kMostSize) return 0;
+  return round256((size_t)dbk::moe_logit_parts(T, H, E) * T * E * sizeof(double));
 }
 
 int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts, float* weights,
@@ -905,10 +905,11 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
   if (!experts || !weights) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
   if (!aligned4(experts) || !aligned4(weights))
     return fail(DB_ERR_INVALID, "%s: experts and weights must be 4-byte aligned", fn);
-  rc = check_workspace(fn, ws, ws_bytes, db_moe_route_workspace_bytes(T, E));
+  rc = check_workspace(fn, ws, ws_bytes, db_moe_route_workspace_bytes(T, H, E));
   if (rc) return rc;
   const dbk::MoeRouteCall c = {x, Wr, experts, weights, static_cast<double*>(ws), x_stride, T, H,
-                               E, k, renormalize != 0, dtype == DB_DTYPE_BF16};
+                               E, k, dbk::moe_logit_parts(T, H, E), renormalize != 0,
+                               dtype == DB_DTYPE_BF16};
   return hip_status(dbk::launch_moe_route(c, (hipStream_t)stream), fn);
 }
 
@@ -959,9 +960,10 @@ int db_moe_layer(const void* x, long long x_stride, const void* Wr, const db_moe
   char* const p = static_cast<char*>(ws);
   int* const experts = reinterpret_cast<int*>(p + s.experts);
   float* const weights = reinterpret_cast<float*>(p + s.weights);
-  const size_t logits = db_moe_route_workspace_bytes(T, m->E);
+  const size_t logits = db_moe_route_workspace_bytes(T, m->H, m->E);
   const dbk::MoeRouteCall r = {x, Wr, experts, weights, reinterpret_cast<double*>(p + s.rest),
-                               x_stride, T, m->H, m->E, k, renormalize != 0,
+                               x_stride, T, m->H, m->E, k,
+                               dbk::moe_logit_parts(T, m->H, m->E), renormalize != 0,
                                m->dtype == DB_DTYPE_BF16};
   dbk::MoeExpertsCall c = experts_call(x, x_stride, experts, weights, *m, y, T, k);
   dbk::moe_experts_workspace(c, p + s.rest + logits);

@@ -223,12 +223,13 @@ struct MoeRouteCall {
   const void* router;  // [E, H]
   int* experts;        // [T, k]
   float* weights;      // [T, k]
-  double* logits;      // [T, E] workspace
+  double* logits;      // [parts, T, E] workspace: sums over parts of H
   long long x_row;
-  int T, H, E, k;
+  int T, H, E, k, parts;
   bool renormalize, bf16;
 };
 hipError_t launch_moe_route(const MoeRouteCall& c, hipStream_t stream);
+int moe_logit_parts(int T, int H, int E);
 hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream);  // its first half
 
 struct MoeExpertsCall {

@@ -23,7 +23,6 @@ namespace dbk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kOut = 1 << 30;  // an offset behind every buffer: loads give zero
 
 // Sorts the pairs by expert and cuts them into tiles of `most`.
@@ -76,25 +75,27 @@ __global__ __launch_bounds__(1024) void moe_sort(MoeExpertsCall c, int most) {
   }
 }
 
-// GATED: 64 gate rows and the 64 up rows of the same channels on the tokens of a
-// tile, h to the workspace; otherwise 128 down rows on h, each pair's sums to the
+// GATED: 16 NW gate rows and the up rows of the same channels on the tokens of a
+// tile, h to the workspace; otherwise 32 NW down rows on h, each pair's sums to the
 // workspace in fp32.  K goes in steps of 128 bytes of a weight row; S stages lie in
 // the LDS, S - 1 of them on their way while one is multiplied.  A row's 16-byte
 // chunk c lies at place c ^ row % 8, set by which chunk a lane fetches: the rows
 // that a quarter of a wave reads then lie in different banks.
-template <class E, bool FP8, int BT, bool GATED, int S>
-__global__ __launch_bounds__(kThreads, 2) void moe_product(MoeExpertsCall c) {
+template <class E, bool FP8, int BT, bool GATED, int S, int NW>
+__global__ __launch_bounds__(NW* kWave, 2) void moe_product(MoeExpertsCall c) {
   typedef typename E::type elem;
   typedef typename E::vec8 vec8;
   constexpr int CB = FP8 ? 1 : 2, KE = 128 / CB, XB = KE * 2;  // XB: bytes of a token's step
   constexpr int TT = BT / 16;
-  constexpr int kLoadsW = 16 / kWaves, kLoadsX = BT * XB / 1024 / kWaves;
-  static_assert(kLoadsX >= 1 && BT * XB % (1024 * kWaves) == 0, "whole loads");
+  constexpr int BN = 32 * NW;  // weight rows: 32 a wave
+  constexpr int kLoadsW = 4, kLoadsX = BT * XB / 1024 / NW;
+  static_assert(kLoadsX >= 1 && BT * XB % (1024 * NW) == 0, "whole loads");
   constexpr int kLoads = kLoadsW + kLoadsX;
   constexpr int kRowsX = 1024 / XB;  // tokens of a load instruction
-  constexpr int kStage = 128 * 128 + BT * XB;
+  constexpr int kStage = BN * 128 + BT * XB;
+  constexpr int kOutputs = GATED ? BN / 2 : BN;
   __shared__ __align__(16) char s_stage[S * kStage];
-  const int slices = GATED ? (c.w.I + 63) / 64 : (c.w.H + 127) / 128;
+  const int slices = ((GATED ? c.w.I : c.w.H) + kOutputs - 1) / kOutputs;
   const int tile = blockIdx.x / slices, slice = blockIdx.x - tile * slices;
   if (tile >= scalar_load(c.tiles)) return;
   const int expert = scalar_load(c.tiles + 1 + 3 * tile),
@@ -104,11 +105,11 @@ __global__ __launch_bounds__(kThreads, 2) void moe_product(MoeExpertsCall c) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
   const int K = GATED ? c.w.H : c.w.I, N = GATED ? c.w.I : c.w.H;
-  const int n0 = slice * (GATED ? 64 : 128), KB = (K + 127) / 128, NB = (N + 127) / 128;
-  const int rows = min(GATED ? 64 : 128, N - n0);
+  const int n0 = slice * kOutputs, KB = (K + 127) / 128, NB = (N + 127) / 128;
+  const int rows = min(kOutputs, N - n0);
   const size_t w_at = ((size_t)expert * N + n0) * K * CB;
 
-  // Load i of a wave has weight rows 8 (4 i + wave) .. + 7: of gate (or down) in the
+  // Load i of a wave has weight rows 8 (NW i + wave) .. + 7: of gate (or down) in the
   // first half of the loads, of up in the second.
   const u4 rw[2] = {
       dma_rsrc(static_cast<const char*>(GATED ? c.w.wg : c.w.wd) + w_at, rows * K * CB),
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(kThreads, 2) void moe_product(MoeExpertsCall c) {
   int x_row[kLoadsX];
 #pragma unroll
   for (int i = 0; i < kLoadsX; ++i) {
-    const int p = (i * kWaves + wave) * kRowsX + lane / kLanesX;
+    const int p = (i * NW + wave) * kRowsX + lane / kLanesX;
     x_row[i] = p >= pairs ? kOut
                : GATED    ? c.order[first + p] / c.k * (int)c.x_row * 2
                           : (first + p) * K * 2;
@@ -137,29 +138,30 @@ __global__ __launch_bounds__(kThreads, 2) void moe_product(MoeExpertsCall c) {
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i) {
       const int half = GATED && i >= kLoadsW / 2 ? 1 : 0, group = i - half * (kLoadsW / 2);
-      dma16(to + (i * kWaves + wave) * 1024, rw[half], ow + w_row + group * kWaves * 8 * K * CB);
+      dma16(to + (i * NW + wave) * 1024, rw[half], ow + w_row + group * NW * 8 * K * CB);
     }
 #pragma unroll
     for (int i = 0; i < kLoadsX; ++i) {
-      const int row = (i * kWaves + wave) * kRowsX + lane / kLanesX;
+      const int row = (i * NW + wave) * kRowsX + lane / kLanesX;
       const int kx = step * XB + (x_place ^ (row & 7)) * 16;
-      dma16(to + 128 * 128 + (i * kWaves + wave) * 1024, rx,
+      dma16(to + BN * 128 + (i * NW + wave) * 1024, rx,
             kx < K * 2 ? x_row[i] + kx : kOut);
     }
   };
 
   // Two row tiles of a wave: gate and up of the same channels, or two of down.
-  const int tile_row[2] = {GATED ? 16 * wave : 32 * wave, GATED ? 64 + 16 * wave : 32 * wave + 16};
+  const int tile_row[2] = {GATED ? 16 * wave : 32 * wave, GATED ? BN / 2 + 16 * wave : 32 * wave + 16};
   const float* ws[2] = {};
   if constexpr (FP8) {
-    const size_t at = ((size_t)expert * NB + n0 / 128) * KB;
+    static_assert(kOutputs <= 128 || 128 % 32 == 0, "a wave's rows lie in one block");
+    const size_t at = ((size_t)expert * NB + min((n0 + tile_row[0] % kOutputs) / 128, NB - 1)) * KB;
     ws[0] = (GATED ? c.w.sg : c.w.sd) + at;
     ws[1] = (GATED ? c.w.su : c.w.sd) + at;
   }
   f4 acc[2][TT] = {};
   auto multiply = [&](int stage, int step) {
     const char* const pw = s_stage + stage * kStage;
-    const char* const px = pw + 128 * 128;
+    const char* const px = pw + BN * 128;
     const int sw = r16 & 7;
     f4 part[2][TT] = {};
     vec8 a[2][4];
@@ -261,13 +263,24 @@ __global__ __launch_bounds__(kThreads) void moe_combine(MoeExpertsCall c) {
   const int t = at / c.w.H, n = at - (size_t)t * c.w.H;
   if (t >= c.T) return;
   f4 sum = {0, 0, 0, 0};
-  for (int j = 0; j < c.k; ++j) {
-    const int p = t * c.k + j;
-    if ((unsigned)c.experts[p] >= (unsigned)c.w.E) continue;
-    const f4 v = *reinterpret_cast<const f4*>(c.parts + (size_t)p * c.w.H + n);
-    const float w = c.weights[p];
+  // eight pairs' loads at once, added in order; what lies there for a pair without
+  // an expert does not count
+  for (int j0 = 0; j0 < c.k; j0 += 8) {
+    f4 v[8];
+    float w[8];
+    bool exists[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += w * v[i];
+    for (int i = 0; i < 8; ++i) {
+      const int p = t * c.k + min(j0 + i, c.k - 1);
+      exists[i] = j0 + i < c.k && (unsigned)c.experts[p] < (unsigned)c.w.E;
+      v[i] = *reinterpret_cast<const f4*>(c.parts + (size_t)p * c.w.H + n);
+      w[i] = c.weights[p];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (exists[i])
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += w[i] * v[i][e];
   }
   typename E::vec4 r;
 #pragma unroll
@@ -275,27 +288,48 @@ __global__ __launch_bounds__(kThreads) void moe_combine(MoeExpertsCall c) {
   *reinterpret_cast<typename E::vec4*>(static_cast<elem*>(c.y) + (size_t)t * c.w.H + n) = r;
 }
 
-template <class E, bool FP8, int BT, int S>
+template <class E, bool FP8, int BT, int S, int NW>
 void launch(const MoeExpertsCall& c, hipStream_t stream) {
   const int P = c.T * c.k;
   const int tiles = min(P, c.w.E) + P / BT;  // at most
+  const int gate = (c.w.I + 16 * NW - 1) / (16 * NW), down = (c.w.H + 32 * NW - 1) / (32 * NW);
   moe_sort<<<1, 1024, 0, stream>>>(c, BT);
-  moe_product<E, FP8, BT, true, S><<<(c.w.I + 63) / 64 * tiles, kThreads, 0, stream>>>(c);
-  moe_product<E, FP8, BT, false, S><<<(c.w.H + 127) / 128 * tiles, kThreads, 0, stream>>>(c);
+  moe_product<E, FP8, BT, true, S, NW><<<gate * tiles, NW * kWave, 0, stream>>>(c);
+  moe_product<E, FP8, BT, false, S, NW><<<down * tiles, NW * kWave, 0, stream>>>(c);
   const size_t quads = (size_t)c.T * c.w.H / 4;
   moe_combine<E><<<(quads + kThreads - 1) / kThreads, kThreads, 0, stream>>>(c);
 }
 
+// The tile's tokens go by how many an expert has on average, the stages by what
+// two workgroups a CU leave room for; us, others beside it:
+//   e4m3  33 tokens, 6 of 64 experts of 1392 x 2048 (3): 16 tokens, 3 stages 116;
+//         16, 4 stages 118; 32, 3 stages 117
+//         201 tokens, 2 of 8 of 14336 x 4096 (50): 64, 2 stages 362; 64, 4 stages (one
+//         workgroup a CU) 399; 128 526
+//         512 of these (128): 64 and eight waves 662, four 892; 128, eight waves 702
+//   16-bit  33 tokens (3): 32, 4 stages 221, 64, 3 stages 206; 16 tokens, 8 of 128
+//         of 768 x 2048 (1): 160 and 161; 201 tokens (50): 64, 3 stages 549, 128 579
+//         512 (128): 128 and eight waves 719, 64 and four 973
 template <class E, bool FP8>
 void pick(const MoeExpertsCall& c, hipStream_t stream) {
-  // tokens that an expert has on average
   const int mean = c.T * c.k / c.w.E;
-  if (mean <= 12)
-    launch<E, FP8, 32, FP8 ? 3 : 4>(c, stream);
-  else if (mean <= 36)
-    launch<E, FP8, 64, FP8 ? 2 : 3>(c, stream);
-  else
-    launch<E, FP8, 128, FP8 ? 3 : 2>(c, stream);
+  if constexpr (FP8) {
+    if (mean <= 5)
+      launch<E, FP8, 16, 3, 4>(c, stream);
+    else if (mean <= 12)
+      launch<E, FP8, 32, 3, 4>(c, stream);
+    else if (mean <= 64)
+      launch<E, FP8, 64, 2, 4>(c, stream);
+    else
+      launch<E, FP8, 64, 3, 8>(c, stream);
+  } else {
+    if (mean <= 2)
+      launch<E, FP8, 32, 4, 4>(c, stream);
+    else if (mean <= 64)
+      launch<E, FP8, 64, 3, 4>(c, stream);
+    else
+      launch<E, FP8, 128, 3, 8>(c, stream);
+  }
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }

@@ -100,7 +100,8 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   row_to_lds(s_x, static_cast<const elem*>(c.x) + t * c.x_row, H, a.padded);
   int expert;
   if (a.f.logits) {
-    moe_choose<kThreads>(s_choice, a.f.logits + (size_t)t * c.w.E, c.w.E, c.k, a.f.renormalize);
+    moe_choose<kThreads>(s_choice, a.f.logits + (size_t)t * c.w.E, 1, 0, c.w.E, c.k,
+                         a.f.renormalize);
     expert = s_choice.expert[j];
     if (slice == 0 && threadIdx.x == 0) {
       a.f.experts[pair] = expert;
@@ -307,13 +308,21 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
 
 }  // namespace
 
-// Few pairs, whose rows of x and h fit the LDS that a launch has without asking.
+// Few pairs, whose rows of x and h fit the LDS that a launch has without asking, and
+// that read hardly more together than the experts they name among equally likely
+// ones: the tile kernels read an expert once for all its tokens, but take 15 us more
+// for sorting and adding up (80 MB at the rate of the weights).
 bool moe_few(const db_moe& m, int T, int k) {
   const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
   constexpr size_t kLds = 64 * 1024;
-  return T <= 4 && T * k <= 32 &&
-         (size_t)chunks(m.H, fp8) * 2 + sizeof(MoeChoice) + 1024 <= kLds &&
-         (size_t)chunks(m.I, fp8) * 2 * k + 1024 <= kLds;
+  const int P = T * k;
+  if (T > 4 || P > 32 || (size_t)chunks(m.H, fp8) * 2 + sizeof(MoeChoice) + 1024 > kLds ||
+      (size_t)chunks(m.I, fp8) * 2 * k + 1024 > kLds)
+    return false;
+  double missed = 1.0;  // chance that an expert is not named
+  for (int t = 0; t < T; ++t) missed *= 1.0 - (double)min(k, m.E) / m.E;
+  const double bytes = 3.0 * m.H * m.I * (fp8 ? 1 : 2);
+  return (P - 1.06 * m.E * (1.0 - missed)) * bytes <= 80e6;
 }
 
 hipError_t launch_moe_few(const MoeFewCall& f, hipStream_t stream) {

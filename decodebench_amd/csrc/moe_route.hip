@@ -18,7 +18,16 @@ namespace {
 
 typedef double d4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 16;  // of a logits workgroup: each has a part of H
+constexpr int kWaves = 4;       // of a logits workgroup: each has a part of its columns
+constexpr int kMostParts = 16;  // of H
+
+// Workgroups of the logits: 16 tokens, 16 experts and one of the parts of H that make
+// enough of them (201 tokens, 8 experts of 4096: 13 us in one part, XXX so).
+int logit_parts(int T, int H, int E) {
+  const long long tiles = (long long)((T + 15) / 16) * ((E + 15) / 16);
+  const long long want = (1024 + tiles - 1) / tiles;
+  return (int)max(1ll, min(want, (long long)min(kMostParts, H / 256)));
+}
 
 // Logits of 16 tokens and 16 experts: experts are the rows of A, tokens the
 // columns of B.  A lane loads eight elements of a row at a time, the elements
@@ -32,35 +41,43 @@ __global__ __launch_bounds__(kWaves* kWave) void moe_logits(MoeRouteCall c) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r16 = lane & 15, q = lane >> 4;
   const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+  const int steps = (c.H + 31) / 32, each = (steps + c.parts - 1) / c.parts;
+  const int begin = blockIdx.z * each, end = min(steps, begin + each);
   const elem* const wr = static_cast<const elem*>(c.router) +
                          (size_t)min(e0 + r16, c.E - 1) * c.H;
   const elem* const xr = static_cast<const elem*>(c.x) + min(t0 + r16, c.T - 1) * c.x_row;
   d4 acc = {0, 0, 0, 0};
-  for (int s = wave; 32 * s < c.H; s += kWaves) {
-    const int h = 32 * s + 8 * q;
-    u4 w = {0, 0, 0, 0}, x = {0, 0, 0, 0};
-    if (h < c.H) {
-      w = ld16(wr + h);
-      x = ld16(xr + h);
-    }
-    const vec8 wv = __builtin_bit_cast(vec8, w), xv = __builtin_bit_cast(vec8, x);
+  // four steps' loads at once
+  constexpr int kSteps = 4;
+  for (int s0 = begin + wave; s0 < end; s0 += kWaves * kSteps) {
+    u4 w[kSteps], x[kSteps];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)wv[j], (double)(float)xv[j], acc,
-                                                 0, 0, 0);
+    for (int i = 0; i < kSteps; ++i) {
+      const int s = s0 + i * kWaves, h = 32 * s + 8 * q;
+      const bool in = s < end && h < c.H;
+      w[i] = in ? ld16(wr + h) : u4{0, 0, 0, 0};
+      x[i] = in ? ld16(xr + h) : u4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (s0 + i * kWaves >= end) break;
+      const vec8 wv = __builtin_bit_cast(vec8, w[i]), xv = __builtin_bit_cast(vec8, x[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)wv[j], (double)(float)xv[j], acc,
+                                                   0, 0, 0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) s_part[wave][i][lane] = acc[i];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    const int i = threadIdx.x >> 6;
-    double sum = s_part[0][i][lane];
+  const int i = wave;
+  double sum = s_part[0][i][lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += s_part[w][i][lane];
-    // register i of a lane is row 4 i + lane / 16, column lane % 16
-    const int e = e0 + 4 * i + q, t = t0 + r16;
-    if (e < c.E && t < c.T) c.logits[(size_t)t * c.E + e] = sum;
-  }
+  for (int w = 1; w < kWaves; ++w) sum += s_part[w][i][lane];
+  // register i of a lane is row 4 i + lane / 16, column lane % 16
+  const int e = e0 + 4 * i + q, t = t0 + r16;
+  if (e < c.E && t < c.T) c.logits[((size_t)blockIdx.z * c.T + t) * c.E + e] = sum;
 }
 
 // Few tokens: a wave has an expert and all of them.  Eight elements of a row a
@@ -116,7 +133,7 @@ __global__ __launch_bounds__(4 * kWave) void moe_logits_few(MoeRouteCall c) {
 __global__ __launch_bounds__(256) void moe_select(MoeRouteCall c) {
   __shared__ MoeChoice s;
   const size_t t = blockIdx.x;
-  moe_choose<256>(s, c.logits + t * c.E, c.E, c.k, c.renormalize);
+  moe_choose<256>(s, c.logits + t * c.E, c.parts, (size_t)c.T * c.E, c.E, c.k, c.renormalize);
   if (threadIdx.x < c.k) {
     c.experts[t * c.k + threadIdx.x] = s.expert[threadIdx.x];
     c.weights[t * c.k + threadIdx.x] = s.p[threadIdx.x] / s.total;
@@ -124,6 +141,10 @@ __global__ __launch_bounds__(256) void moe_select(MoeRouteCall c) {
 }
 
 }  // namespace
+
+int moe_logit_parts(int T, int H, int E) {
+  return T <= kFewTokens ? 1 : logit_parts(T, H, E);
+}
 
 hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream) {
   if (c.T <= kFewTokens) {
@@ -134,7 +155,7 @@ hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream) {
       moe_logits_few<ElemF16><<<grid, 4 * kWave, 0, stream>>>(c);
     return hipGetLastError();
   }
-  const dim3 grid((c.E + 15) / 16, (c.T + 15) / 16);
+  const dim3 grid((c.E + 15) / 16, (c.T + 15) / 16, c.parts);
   if (c.bf16)
     moe_logits<ElemBF16><<<grid, kWaves * kWave, 0, stream>>>(c);
   else

@@ -25,16 +25,17 @@ __device__ __forceinline__ double logit_key(double l) {
   return l != l ? __builtin_huge_val() : l == __builtin_huge_val() ? 0x1.fffffffffffffp1023 : l;
 }
 
-// Fills s.expert and s.p (exp of each choice against the largest) and s.total (of
+// A logit is the sum of `sums` parts, each `apart` from the one before.  Fills s.expert and s.p (exp of each choice against the largest) and s.total (of
 // the choices, or of all experts).  Ranks are counted: an expert comes after those
 // of larger logits, and of equal ones with a lower index.  NT threads, barriers
 // within; E and k are uniform.
 template <int NT>
-__device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, int E, int k,
-                                           bool renormalize) {
+__device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, int sums,
+                                           size_t apart, int E, int k, bool renormalize) {
   const int tid = threadIdx.x;
   for (int e = tid; e < E + 2; e += NT) {
-    const double l = e < E ? logits[e] : 0.0;
+    double l = e < E ? logits[e] : 0.0;
+    for (int i = 1; i < sums && e < E; ++i) l += logits[i * apart + e];
     // (behind the last one stands what comes before nothing)
     s.key[e] = e < E ? logit_key(l) : -__builtin_huge_val();
     if (e < E) {

@@ -116,7 +116,7 @@ def load_library():
             "db_gemm_blocks_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i]),
             "db_gemm_blocks": (_i, [_p, _ll, _p, _ll, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _p,
                                     C.c_size_t, _p]),
-            "db_moe_route_workspace_bytes": (C.c_size_t, [_i, _i]),
+            "db_moe_route_workspace_bytes": (C.c_size_t, [_i, _i, _i]),
             "db_moe_route": (_i, [_p, _ll, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, C.c_size_t,
                                   _p]),
             "db_moe_experts_workspace_bytes": (C.c_size_t, [C.POINTER(_Moe), _i, _i]),
@@ -1038,7 +1038,7 @@ def moe_route(x, Wr, top_k: int, renormalize: bool = True):
     weights = torch.empty((T, k), dtype=torch.float32, device=x.device)
     lib = _lib or load_library()
     with _on_device(idx):
-        nbytes = lib.db_moe_route_workspace_bytes(T, E)
+        nbytes = lib.db_moe_route_workspace_bytes(T, H, E)
     ws = _workspace(nbytes, x.device)
     _launch(lib.db_moe_route, idx, "db_moe_route", x.data_ptr(), _row_stride(x), Wr.data_ptr(),
             experts.data_ptr(), weights.data_ptr(), T, H, E, k, bool(renormalize), dt,

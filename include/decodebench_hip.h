@@ -337,7 +337,7 @@ typedef struct db_moe {
  * Contract: x [T, H] rows x_stride elements apart and 16-byte aligned, Wr [E, H] dense,
  * both of dtype; H a multiple of 8 below 2^22; 1 <= k <= E, k <= 64, E <= 1024; 0 <= T < 2^20;
  * ws of db_moe_route_workspace_bytes, 256-byte aligned, as that of db_gemm_blocks. */
-size_t db_moe_route_workspace_bytes(int T, int E);
+size_t db_moe_route_workspace_bytes(int T, int H, int E);
 int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts, float* weights,
                  int T, int H, int E, int k, int renormalize, int dtype, void* ws,
                  size_t ws_bytes, void* stream);
