@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -45,6 +46,15 @@ struct Abi {
   decltype(&db_rope_append) rope_append;
   decltype(&db_paged_attention_workspace_bytes) paged_workspace_bytes;
   decltype(&db_paged_attention) paged_attention;
+  decltype(&db_quantize_blocks) quantize_blocks;
+  decltype(&db_gemm_blocks_workspace_bytes) gemm_blocks_workspace_bytes;
+  decltype(&db_gemm_blocks) gemm_blocks;
+  decltype(&db_moe_route_workspace_bytes) moe_route_workspace_bytes;
+  decltype(&db_moe_route) moe_route;
+  decltype(&db_moe_experts_workspace_bytes) moe_experts_workspace_bytes;
+  decltype(&db_moe_experts) moe_experts;
+  decltype(&db_moe_layer_workspace_bytes) moe_layer_workspace_bytes;
+  decltype(&db_moe_layer) moe_layer;
 } abi;
 
 PyObject* raw_stream = nullptr;  // device index -> current stream's handle
@@ -532,29 +542,294 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (entry point addresses, raw_stream, get_device, workspaces, cu_counts)
-PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long p[14];
-  PyObject *rs, *gd, *ws, *cu;
-  if (!PyArg_ParseTuple(args, "(KKKKKKKKKKKKKK)OOO!O!", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5],
-                        &p[6], &p[7], &p[8], &p[9], &p[10], &p[11], &p[12], &p[13], &rs, &gd,
-                        &PyDict_Type, &ws, &PyDict_Type, &cu))
+// ------------------------------------- block-scaled e4m3, mixture of experts
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+
+long long row_stride(const at::Tensor* t) { return t->size(0) > 1 ? t->stride(0) : t->size(1); }
+
+bool codes(const at::Tensor* t, int idx) {
+  return plain(t, at::kFloat8_e4m3fn, idx) || plain(t, at::kByte, idx);
+}
+
+// Rows of 16-bit activations [T, K].
+const at::Tensor* rows16(PyObject* o, int* idx) {
+  const at::Tensor* x = tensor(o);
+  if (!x || activation(x->scalar_type()) < 0 || !strided(x, x->scalar_type(), 2, -1) || !ints(x))
     return nullptr;
-  abi.f1 = reinterpret_cast<decltype(abi.f1)>((uintptr_t)p[0]);
-  abi.f2 = reinterpret_cast<decltype(abi.f2)>((uintptr_t)p[1]);
-  abi.f2n = reinterpret_cast<decltype(abi.f2n)>((uintptr_t)p[2]);
-  abi.gemv = reinterpret_cast<decltype(abi.gemv)>((uintptr_t)p[3]);
-  abi.f4_default_splits = reinterpret_cast<decltype(abi.f4_default_splits)>((uintptr_t)p[4]);
-  abi.f4_workspace_bytes = reinterpret_cast<decltype(abi.f4_workspace_bytes)>((uintptr_t)p[5]);
-  abi.f4 = reinterpret_cast<decltype(abi.f4)>((uintptr_t)p[6]);
-  abi.capture_id = reinterpret_cast<decltype(abi.capture_id)>((uintptr_t)p[7]);
-  abi.gemv_workspace_bytes = reinterpret_cast<decltype(abi.gemv_workspace_bytes)>((uintptr_t)p[8]);
-  abi.gemv_ws = reinterpret_cast<decltype(abi.gemv_ws)>((uintptr_t)p[9]);
-  abi.paged_plan = reinterpret_cast<decltype(abi.paged_plan)>((uintptr_t)p[10]);
-  abi.rope_append = reinterpret_cast<decltype(abi.rope_append)>((uintptr_t)p[11]);
-  abi.paged_workspace_bytes =
-      reinterpret_cast<decltype(abi.paged_workspace_bytes)>((uintptr_t)p[12]);
-  abi.paged_attention = reinterpret_cast<decltype(abi.paged_attention)>((uintptr_t)p[13]);
+  *idx = x->get_device();
+  return x;
+}
+
+// (x): (q, scale)
+PyObject* quantize_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int idx = -1;
+  const at::Tensor* x = n == 1 ? rows16(a[0], &idx) : nullptr;
+  if (!x) Py_RETURN_NONE;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  const int64_t T = x->size(0), K = x->size(1);
+  at::Tensor q = empty_on({T, K}, at::kFloat8_e4m3fn, idx);
+  at::Tensor scale = empty_on({blocks128(K), T}, at::kFloat, idx).t();
+  const void* xp = x->data_ptr();
+  const long long row = row_stride(x);
+  const int dtype = activation(x->scalar_type());
+  void* qp = q.data_ptr();
+  float* sp = static_cast<float*>(scale.data_ptr());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.quantize_blocks(xp, row, qp, sp, 1, T, (int)T, (int)K, dtype, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(2);
+  if (!result) return nullptr;
+  PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(q));
+  PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(scale));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, W, w_scale, x_scale or None, dtype or None): x [T, K]
+PyObject* gemm_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) Py_RETURN_NONE;
+  const at::Tensor *x = tensor(a[0]), *w = tensor(a[1]), *ws = tensor(a[2]);
+  if (!x || x->dim() != 2 || !x->is_cuda() || !ints(x)) Py_RETURN_NONE;
+  const at::ScalarType type = x->scalar_type();
+  const int idx = x->get_device();
+  const bool fp8 = type == at::kFloat8_e4m3fn;
+  if (!strided(x, type, 2, idx) || (!fp8 && activation(type) < 0)) Py_RETURN_NONE;
+  const int64_t T = x->size(0), K = x->size(1);
+  at::ScalarType out = fp8 ? at::kHalf : type;
+  if (a[4] != Py_None) {
+    if (!THPDtype_Check(a[4])) Py_RETURN_NONE;
+    const at::ScalarType want = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    if (activation(want) < 0 || (!fp8 && want != type)) Py_RETURN_NONE;
+    out = want;
+  }
+  const float* xs = nullptr;
+  long long xs_t = 0, xs_b = 0;
+  if (fp8) {
+    const at::Tensor* s = tensor(a[3]);
+    if (!s || !s->is_cuda() || s->get_device() != idx || s->scalar_type() != at::kFloat ||
+        s->dim() != 2 || s->size(0) != T || s->size(1) != blocks128(K))
+      Py_RETURN_NONE;
+    xs = static_cast<const float*>(s->data_ptr());
+    xs_t = stride_of(s, 0);
+    xs_b = stride_of(s, 1);
+  } else if (a[3] != Py_None) {
+    Py_RETURN_NONE;
+  }
+  if (!codes(w, idx) || w->dim() != 2 || w->size(1) != K || !ints(w)) Py_RETURN_NONE;
+  const int64_t N = w->size(0);
+  if (!plain(ws, at::kFloat, idx) || ws->dim() != 2 || ws->size(0) != blocks128(N) ||
+      ws->size(1) != blocks128(K))
+    Py_RETURN_NONE;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  const int xdt = fp8 ? DB_DTYPE_FP8_E4M3 : activation(type), ydt = activation(out);
+  at::Tensor y = empty_on({T, N}, out, idx);
+  const size_t bytes = abi.gemm_blocks_workspace_bytes((int)T, (int)K, (int)N, xdt);
+  at::Tensor work;
+  if (bytes > 0) work = empty_here((int64_t)bytes, at::kByte, idx);
+  const void *xp = x->data_ptr(), *wp = w->data_ptr();
+  const float* wsp = static_cast<const float*>(ws->data_ptr());
+  const long long row = row_stride(x);
+  void *yp = y.data_ptr(), *kp = bytes > 0 ? work.data_ptr() : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.gemm_blocks(xp, row, xs, xs_t, xs_b, wp, wsp, yp, (int)T, (int)K, (int)N, xdt, ydt, kp,
+                       bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, Wr, top_k, renormalize): (experts, weights)
+PyObject* moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int idx = -1;
+  long k = 0;
+  const at::Tensor* x = n == 4 ? rows16(a[0], &idx) : nullptr;
+  if (!x || !integer(a[2], &k) || !PyBool_Check(a[3])) Py_RETURN_NONE;
+  const at::Tensor* wr = tensor(a[1]);
+  const int64_t T = x->size(0), H = x->size(1);
+  if (!plain(wr, x->scalar_type(), idx) || wr->dim() != 2 || wr->size(1) != H || !ints(wr))
+    Py_RETURN_NONE;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  const int E = (int)wr->size(0);
+  if (k < 1 || k > E) Py_RETURN_NONE;
+  at::Tensor experts = empty_on({T, k}, at::kInt, idx), weights = empty_on({T, k}, at::kFloat, idx);
+  const size_t bytes = abi.moe_route_workspace_bytes((int)T, (int)H, E);
+  at::Tensor work;
+  if (bytes > 0) work = empty_here((int64_t)bytes, at::kByte, idx);
+  const void *xp = x->data_ptr(), *wp = wr->data_ptr();
+  const long long row = row_stride(x);
+  int* ep = static_cast<int*>(experts.data_ptr());
+  float* sp = static_cast<float*>(weights.data_ptr());
+  void* kp = bytes > 0 ? work.data_ptr() : nullptr;
+  const int renormalize = a[3] == Py_True, dtype = activation(x->scalar_type());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.moe_route(xp, row, wp, ep, sp, (int)T, (int)H, E, (int)k, renormalize, dtype, kp, bytes,
+                     stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(2);
+  if (!result) return nullptr;
+  PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(experts));
+  PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(weights));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// The experts' weights (Wg, Wu, Wd) and scales (sg, su, sd) for activations of x's
+// type and width.
+bool experts_of(PyObject* const* w, PyObject* const* s, const at::Tensor* x, int idx, db_moe* m) {
+  const at::Tensor *wg = tensor(w[0]), *wu = tensor(w[1]), *wd = tensor(w[2]);
+  if (!wg) return false;
+  const at::ScalarType type = wg->scalar_type();
+  const int64_t H = x->size(1);
+  if (!plain(wg, type, idx) || !plain(wu, type, idx) || !plain(wd, type, idx) || wg->dim() != 3 ||
+      wg->size(2) != H || wu->sizes() != wg->sizes() || wd->dim() != 3 || !ints(wg))
+    return false;
+  const int64_t E = wg->size(0), I = wg->size(1);
+  if (wd->size(0) != E || wd->size(1) != H || wd->size(2) != I) return false;
+  *m = {};
+  m->dtype = m->w_dtype = activation(x->scalar_type());
+  if (type == at::kFloat8_e4m3fn || type == at::kByte) {
+    m->w_dtype = DB_DTYPE_FP8_E4M3;
+    const float** to[3] = {&m->sg, &m->su, &m->sd};
+    for (int i = 0; i < 3; ++i) {
+      const at::Tensor* t = tensor(s[i]);
+      if (!plain(t, at::kFloat, idx) || t->dim() != 3 || t->size(0) != E ||
+          t->size(1) != blocks128(i < 2 ? I : H) || t->size(2) != blocks128(i < 2 ? H : I))
+        return false;
+      *to[i] = static_cast<const float*>(t->data_ptr());
+    }
+  } else if (type != x->scalar_type() || s[0] != Py_None || s[1] != Py_None || s[2] != Py_None) {
+    return false;
+  }
+  m->wg = wg->data_ptr();
+  m->wu = wu->data_ptr();
+  m->wd = wd->data_ptr();
+  m->E = (int)E;
+  m->H = (int)H;
+  m->I = (int)I;
+  return true;
+}
+
+// (x, experts, weights, Wg, Wu, Wd, sg, su, sd)
+PyObject* moe_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int idx = -1;
+  const at::Tensor* x = n == 9 ? rows16(a[0], &idx) : nullptr;
+  if (!x) Py_RETURN_NONE;
+  const at::Tensor *e = tensor(a[1]), *w = tensor(a[2]);
+  const int64_t T = x->size(0);
+  if (!plain(e, at::kInt, idx) || !plain(w, at::kFloat, idx) || e->dim() != 2 || e->size(0) != T ||
+      w->sizes() != e->sizes() || !ints(e))
+    Py_RETURN_NONE;
+  db_moe m;
+  if (!experts_of(a + 3, a + 6, x, idx, &m)) Py_RETURN_NONE;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  const int k = (int)e->size(1);
+  const size_t bytes = abi.moe_experts_workspace_bytes(&m, (int)T, k);
+  if (bytes == 0) Py_RETURN_NONE;
+  at::Tensor y = empty_on({T, x->size(1)}, x->scalar_type(), idx);
+  at::Tensor work = empty_here((int64_t)bytes, at::kByte, idx);
+  const void* xp = x->data_ptr();
+  const long long row = row_stride(x);
+  const int* ep = static_cast<const int*>(e->data_ptr());
+  const float* sp = static_cast<const float*>(w->data_ptr());
+  void *yp = y.data_ptr(), *kp = work.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.moe_experts(xp, row, ep, sp, &m, yp, (int)T, k, kp, bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, Wr, Wg, Wu, Wd, top_k, renormalize, sg, su, sd)
+PyObject* moe_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int idx = -1;
+  long k = 0;
+  const at::Tensor* x = n == 10 ? rows16(a[0], &idx) : nullptr;
+  if (!x || !integer(a[5], &k) || k < 1 || !PyBool_Check(a[6])) Py_RETURN_NONE;
+  const at::Tensor* wr = tensor(a[1]);
+  const int64_t T = x->size(0);
+  db_moe m;
+  if (!experts_of(a + 2, a + 7, x, idx, &m) || !plain(wr, x->scalar_type(), idx) ||
+      wr->dim() != 2 || wr->size(0) != m.E || wr->size(1) != m.H || k > m.E)
+    Py_RETURN_NONE;
+  void* stream = nullptr;
+  const int found = stream_of(idx, &stream);
+  if (found < 0) return nullptr;
+  if (found == 0) Py_RETURN_NONE;
+  const size_t bytes = abi.moe_layer_workspace_bytes(&m, (int)T, (int)k);
+  if (bytes == 0) Py_RETURN_NONE;
+  at::Tensor y = empty_on({T, x->size(1)}, x->scalar_type(), idx);
+  at::Tensor work = empty_here((int64_t)bytes, at::kByte, idx);
+  const void *xp = x->data_ptr(), *wp = wr->data_ptr();
+  const long long row = row_stride(x);
+  const int renormalize = a[6] == Py_True;
+  void *yp = y.data_ptr(), *kp = work.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = abi.moe_layer(xp, row, wp, &m, yp, (int)T, (int)k, renormalize, kp, bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != DB_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// Entry point i of the list that init is given.
+template <class F>
+bool entry(PyObject* list, Py_ssize_t i, F* to) {
+  const unsigned long long p = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(list, i));
+  if (p == (unsigned long long)-1 && PyErr_Occurred()) return false;
+  *to = reinterpret_cast<F>((uintptr_t)p);
+  return true;
+}
+
+// (entry point addresses in the order of Abi, raw_stream, get_device, workspaces, cu_counts)
+PyObject* init(PyObject*, PyObject* args) {
+  PyObject *list, *rs, *gd, *ws, *cu;
+  if (!PyArg_ParseTuple(args, "O!OOO!O!", &PyTuple_Type, &list, &rs, &gd, &PyDict_Type, &ws,
+                        &PyDict_Type, &cu))
+    return nullptr;
+  if (PyTuple_GET_SIZE(list) != 23) {
+    PyErr_SetString(PyExc_ValueError, "init takes 23 entry points");
+    return nullptr;
+  }
+  Abi e;
+  if (!entry(list, 0, &e.f1) || !entry(list, 1, &e.f2) || !entry(list, 2, &e.f2n) ||
+      !entry(list, 3, &e.gemv) || !entry(list, 4, &e.f4_default_splits) ||
+      !entry(list, 5, &e.f4_workspace_bytes) || !entry(list, 6, &e.f4) ||
+      !entry(list, 7, &e.capture_id) || !entry(list, 8, &e.gemv_workspace_bytes) ||
+      !entry(list, 9, &e.gemv_ws) || !entry(list, 10, &e.paged_plan) ||
+      !entry(list, 11, &e.rope_append) || !entry(list, 12, &e.paged_workspace_bytes) ||
+      !entry(list, 13, &e.paged_attention) || !entry(list, 14, &e.quantize_blocks) ||
+      !entry(list, 15, &e.gemm_blocks_workspace_bytes) || !entry(list, 16, &e.gemm_blocks) ||
+      !entry(list, 17, &e.moe_route_workspace_bytes) || !entry(list, 18, &e.moe_route) ||
+      !entry(list, 19, &e.moe_experts_workspace_bytes) || !entry(list, 20, &e.moe_experts) ||
+      !entry(list, 21, &e.moe_layer_workspace_bytes) || !entry(list, 22, &e.moe_layer))
+    return nullptr;
+  abi = e;
   Py_INCREF(rs);
   Py_INCREF(gd);
   Py_INCREF(ws);
@@ -581,6 +856,11 @@ PyMethodDef methods[] = {
     {"plan", fast<plan>(), METH_FASTCALL, nullptr},
     {"rope", fast<rope>(), METH_FASTCALL, nullptr},
     {"paged", fast<paged>(), METH_FASTCALL, nullptr},
+    {"quantize_blocks", fast<quantize_blocks>(), METH_FASTCALL, nullptr},
+    {"gemm_blocks", fast<gemm_blocks>(), METH_FASTCALL, nullptr},
+    {"moe_route", fast<moe_route>(), METH_FASTCALL, nullptr},
+    {"moe_experts", fast<moe_experts>(), METH_FASTCALL, nullptr},
+    {"moe_layer", fast<moe_layer>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;  // elements of a row a load instruction takes
   constexpr int CH = FP8 ? 2 : 4;       // of each matrix in an item
-  constexpr int kAhead = FP8 ? 4 : 2;   // items on their way: 16 KB a wave
+  constexpr int kAhead = 2;               // items on their way: 8 or 16 KB a wave
   extern __shared__ __align__(16) char s_x[];
   __shared__ MoeChoice s_choice;
   const MoeExpertsCall& c = a.f.c;
@@ -179,8 +179,8 @@ template <class E, bool FP8>
 __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;
-  constexpr int CH = FP8 ? 1 : 2;
-  constexpr int kAhead = 8;  // items on their way: 8 or 16 KB a wave
+  constexpr int CH = 2;
+  constexpr int kAhead = 4;  // items on their way: 8 KB a wave
   extern __shared__ __align__(16) char s_h[];
   __shared__ int s_expert[kMostChoices];
   __shared__ float s_weight[kMostChoices];
@@ -311,7 +311,8 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
 // Few pairs, whose rows of x and h fit the LDS that a launch has without asking, and
 // that read hardly more together than the experts they name among equally likely
 // ones: the tile kernels read an expert once for all its tokens, but take 15 us more
-// for sorting and adding up (80 MB at the rate of the weights).
+// for sorting and adding up (80 MB at the rate of the weights; two tokens, 2 of 8 experts of
+// 14336 x 4096: 231 us here, 260 there, four 409 and 374).
 bool moe_few(const db_moe& m, int T, int k) {
   const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
   constexpr size_t kLds = 64 * 1024;
@@ -322,7 +323,7 @@ bool moe_few(const db_moe& m, int T, int k) {
   double missed = 1.0;  // chance that an expert is not named
   for (int t = 0; t < T; ++t) missed *= 1.0 - (double)min(k, m.E) / m.E;
   const double bytes = 3.0 * m.H * m.I * (fp8 ? 1 : 2);
-  return (P - 1.06 * m.E * (1.0 - missed)) * bytes <= 80e6;
+  return (P - 1.06 * m.E * (1.0 - missed)) * bytes <= 130e6;
 }
 
 hipError_t launch_moe_few(const MoeFewCall& f, hipStream_t stream) {

@@ -173,7 +173,10 @@ def _load_fast(lib) -> None:
         "db_f1_rmsnorm_gemv", "db_f2_gateup_swiglu", "db_f2_rmsnorm_gateup_swiglu", "db_gemv",
         "db_f4_default_splits", "db_f4_workspace_bytes", "db_f4_splitkv",
         "db_stream_capture_id", "db_gemv_workspace_bytes", "db_gemv_ws", "db_paged_plan",
-        "db_rope_append", "db_paged_attention_workspace_bytes", "db_paged_attention"))
+        "db_rope_append", "db_paged_attention_workspace_bytes", "db_paged_attention",
+        "db_quantize_blocks", "db_gemm_blocks_workspace_bytes", "db_gemm_blocks",
+        "db_moe_route_workspace_bytes", "db_moe_route", "db_moe_experts_workspace_bytes",
+        "db_moe_experts", "db_moe_layer_workspace_bytes", "db_moe_layer"))
     mod.init(entry, _raw_stream, get_device, _ws_cache, _cu_cache)
     _fast = mod
 
@@ -929,6 +932,10 @@ def quantize_blocks(x):
     ``scale[t, b] = max |x[t, 128 b ..]| / 448`` (1 where that is 0) and
     ``q = e4m3(clamp(x / scale, -448, 448))``, rounded to nearest even; an Inf or
     NaN makes its block's scale one."""
+    if _fast is not None:
+        r = _fast.quantize_blocks(x)
+        if r is not None:
+            return r
     torch = _torch or _torch_mod()
     idx = _strided(x, "x", None, 2)
     dt = _activation(x, "x")
@@ -960,6 +967,10 @@ def gemm_blocks(x, W, w_scale, x_scale=None, dtype=None, out=None):
     y [T, N] has its type; or x is float8_e4m3fn with x_scale [T, ceil(K/128)],
     and y is ``dtype`` (torch.float16 if not given).  Rows of x may be strided,
     and x_scale anyhow."""
+    if out is None and _fast is not None:
+        y = _fast.gemm_blocks(x, W, w_scale, x_scale, dtype)
+        if y is not None:
+            return y
     torch = _torch or _torch_mod()
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
@@ -1030,6 +1041,10 @@ def moe_route(x, Wr, top_k: int, renormalize: bool = True):
     64 bits; equal ones go to the lower index, NaN counts above all numbers.
     Weights are the softmax over the chosen experts (``renormalize``) or
     over all of them."""
+    if _fast is not None:
+        r = _fast.moe_route(x, Wr, top_k, renormalize)
+        if r is not None:
+            return r
     idx, dt, k = _router(x, Wr, top_k)
     torch = _torch
     T, H = x.shape
@@ -1089,6 +1104,10 @@ def moe_experts(x, experts, weights, Wg, Wu, Wd, sg=None, su=None, sd=None, out=
     expert named twice counts twice.  Sums are fp32; what the gate gives is
     rounded to x's type before the down product, and the result once.  Made for
     the few tokens of a decode step: the weights bound the call."""
+    if out is None and _fast is not None:
+        y = _fast.moe_experts(x, experts, weights, Wg, Wu, Wd, sg, su, sd)
+        if y is not None:
+            return y
     torch = _torch or _torch_mod()
     idx = _strided(x, "x", None, 2)
     dt = _activation(x, "x")
@@ -1115,6 +1134,10 @@ def moe_layer(x, Wr, Wg, Wu, Wd, top_k: int, renormalize: bool = True, sg=None, 
               out=None):
     """A whole mixture-of-experts layer: :func:`moe_route` and
     :func:`moe_experts` in one call, with their arguments.  Returns [T, H]."""
+    if out is None and _fast is not None:
+        y = _fast.moe_layer(x, Wr, Wg, Wu, Wd, top_k, renormalize, sg, su, sd)
+        if y is not None:
+            return y
     idx, dt, k = _router(x, Wr, top_k)
     m = _experts(x, Wg, Wu, Wd, sg, su, sd, idx, dt)
     if Wr.shape[0] != m.E:

@@ -417,3 +417,23 @@ def test_the_oracle_sees_a_wrong_block():
 
 def test_prototypes_take_their_arguments(lib):
     assert lib.db_gemm_blocks.argtypes[-2] is C.c_size_t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 20, 100])
+def test_native_call_path_and_python_steps_agree(T, monkeypatch):
+    W, ws = (t.to(DEV) for t in weights(200, 528, 1))
+    x = torch.randn(T, 528, generator=generator(5)).bfloat16().to(DEV)
+
+    def calls():
+        q, xs = ops.quantize_blocks(x)
+        return (q.float(), xs, ops.gemm_blocks(x, W, ws), ops.gemm_blocks(q, W, ws, x_scale=xs),
+                ops.gemm_blocks(q, W, ws, x_scale=xs, dtype=torch.bfloat16))
+
+    ops.load_library()
+    assert ops._fast is not None
+    native = calls()
+    monkeypatch.setattr(ops, "_fast", None)
+    for a, b in zip(native, calls()):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+        assert a.stride() == b.stride()

@@ -499,3 +499,24 @@ def test_refusals():
             ops.moe_experts(*args, **more)
     with pytest.raises(ValueError):
         ops.moe_layer(x, torch.randn(E + 1, H).half().to(DEV), Wg, Wu, Wd, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_native_call_path_and_python_steps_agree(T, fp8, monkeypatch):
+    E, H, I = 8, 272, 144
+    on_gpu, _ = layer(E, H, I, torch.float16, fp8, 1)
+    x = torch.randn(T, H, generator=generator(2)).half().to(DEV)
+    Wr = torch.randn(E, H, generator=generator(3)).half().to(DEV)
+
+    def calls():
+        e, w = ops.moe_route(x, Wr, 2, renormalize=False)
+        return e, w, ops.moe_experts(x, e, w, **on_gpu), ops.moe_layer(x, Wr, top_k=2, **on_gpu)
+
+    ops.load_library()
+    assert ops._fast is not None
+    native = calls()
+    monkeypatch.setattr(ops, "_fast", None)
+    for a, b in zip(native, calls()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
