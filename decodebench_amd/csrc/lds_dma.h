@@ -31,6 +31,13 @@ __device__ __forceinline__ void dma16(unsigned lds, u4 rsrc, int offset) {
                "v"(offset), "s"(rsrc)
                : "memory");
 }
+// The same for data that is read once: not kept in the caches.
+__device__ __forceinline__ void dma16_stream(unsigned lds, u4 rsrc, int offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds),
+      "v"(offset), "s"(rsrc)
+      : "memory");
+}
 
 // Waits until at most LEFT of the wave's loads are on their way, then for the
 // workgroup's other waves.

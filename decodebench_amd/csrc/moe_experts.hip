@@ -138,7 +138,7 @@ __global__ __launch_bounds__(NW* kWave, 2) void moe_product(MoeExpertsCall c) {
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i) {
       const int half = GATED && i >= kLoadsW / 2 ? 1 : 0, group = i - half * (kLoadsW / 2);
-      dma16(to + (i * NW + wave) * 1024, rw[half], ow + w_row + group * NW * 8 * K * CB);
+      dma16_stream(to + (i * NW + wave) * 1024, rw[half], ow + w_row + group * NW * 8 * K * CB);
     }
 #pragma unroll
     for (int i = 0; i < kLoadsX; ++i) {
@@ -323,7 +323,7 @@ void pick(const MoeExpertsCall& c, hipStream_t stream) {
     else
       launch<E, FP8, 64, 3, 8>(c, stream);
   } else {
-    if (mean <= 2)
+    if (mean <= 12)
       launch<E, FP8, 32, 4, 4>(c, stream);
     else if (mean <= 64)
       launch<E, FP8, 64, 3, 4>(c, stream);
