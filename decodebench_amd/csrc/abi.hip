@@ -857,7 +857,9 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
   if (fp8 ? !x_scale : x_scale != nullptr)
     return fail(DB_ERR_INVALID, fp8 ? "%s: e4m3 activations need a scale for each block"
                                     : "%s: 16-bit activations take no scales", fn);
-  if (xs_t < 0 || xs_b < 0) return fail(DB_ERR_INVALID, "%s: strides must be >= 0", fn);
+  if (xs_t < 0 || xs_b < 0 || xs_t >= kMostSize)
+    return fail(DB_ERR_INVALID, "%s: strides of the scales must be >= 0, that of a token below 2^22",
+                fn);
   if (T == 0) return ok();
   if (!x || !W || !w_scale || !y) return fail(DB_ERR_INVALID, "%s: null tensor pointer", fn);
   if (!aligned16(x) || !aligned16(W) || !aligned16(y))

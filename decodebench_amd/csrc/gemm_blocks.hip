@@ -10,6 +10,7 @@
 #include <atomic>
 
 #include "db_kernels.h"
+#include "lds_dma.h"
 #include "quant_blocks.h"
 
 namespace dbk {
@@ -218,29 +219,25 @@ __global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
 }
 
 // ------------------------------------------------------------- full tiles
-// A workgroup has tiles of BN outputs by BT tokens, its waves WN by WT of them,
-// and goes through K a block at a time: while a block is multiplied from one
-// half of the LDS, the next one (behind the last, the first of the workgroup's
-// next tile) is on its way into the other (buffer_load .. lds, no registers).
-// Rows of 128 bytes lie 16 bytes at a time in the order (chunk ^ row % 8), set
-// by which global chunk a lane fetches: the 16 rows that a quarter of a wave
-// reads then lie in different banks.
+// A workgroup has tiles of BN outputs by BT tokens, its waves WN by WT of them, and
+// goes through K a block at a time: S stages lie in the LDS, S - 1 of them on their
+// way (behind a tile's last blocks, the first ones of the workgroup's next tile)
+// while one is multiplied.  Rows of 128 bytes lie 16 bytes at a time in the order
+// (chunk ^ row % 8), set by which global chunk a lane fetches: the 16 rows that a
+// quarter of a wave reads then lie in different banks.  Each wave fetches the scales
+// of its own tokens along with them.
 template <class E, int BN, int BT, int WN, int WT, int S>
 __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_tile(
     GemmBlocksCall c, GemmBlocksPlan plan) {
   typedef typename E::type elem;
   constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;
   constexpr int kLoadsW = BN / 8 / NW, kLoadsX = BT / 8 / NW;  // of 8 rows, a wave
-  constexpr int kLoads = kLoadsW + kLoadsX;
+  constexpr int kLoads = kLoadsW + kLoadsX + 1;                // and one of scales
   static_assert(BN % (8 * NW) == 0 && BT % (8 * NW) == 0, "whole loads");
-  static_assert(S == 2 || S == 3, "two or three stages");
   static_assert(NI % 2 == 0 && 128 % WN == 0, "row tiles in pairs, of one block of the weights");
-  constexpr int kStage = (BN + BT) * 128;
-  // (arrays of their own, so that reads of one need not wait for what is on its
-  // way into another)
-  __shared__ __align__(16) char s_a[kStage];
-  __shared__ __align__(16) char s_b[kStage];
-  __shared__ __align__(16) char s_c[S > 2 ? kStage : 16];
+  static_assert(WT <= kWave, "a lane for each token's scale");
+  constexpr int kScales = (BN + BT) * 128, kStage = kScales + NW * kWave * 4;
+  __shared__ __align__(16) char s_stage[S * kStage];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r16 = lane & 15, q = lane >> 4;
@@ -250,60 +247,60 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
   // Workgroups i, i + 8, .. run on one XCD: its share of the tiles is a
   // compact part of the output, strips of eight token tiles wide.
   const int tn = (c.N + BN - 1) / BN, tt = (c.T + BT - 1) / BT, all = tn * tt * plan.parts;
-  const int steps = (plan.each + S - 1) / S * S;
-  int n0, t0, part, b0, b1;
+  struct Place {
+    int n0, t0, part, b0, b1;  // blocks b0 .. b1 - 1 of K
+  };
   auto place = [&](int i) {
     const int xcd = i & 7, each = all >> 3, more = all & 7;
     const int nth = xcd * each + min(xcd, more) + (i >> 3);
-    part = nth / (tn * tt);
-    b0 = part * plan.each;
-    b1 = min(KB, b0 + plan.each);
-    const int at = nth - part * tn * tt;
+    const int part = nth / (tn * tt), at = nth - part * tn * tt;
     const int strip = at / (8 * tn), in = at - strip * 8 * tn, wide = min(8, tt - 8 * strip);
-    n0 = in / wide * BN;
-    t0 = (8 * strip + in % wide) * BT;
+    return Place{in / wide * BN, (8 * strip + in % wide) * BT, part, part * plan.each,
+                 min(KB, (part + 1) * plan.each)};
   };
 
   // Load i of a wave has rows 8 (NW i + wave) .. + 7 of the weights, or of x.
   const int lane_row = 8 * wave + (lane >> 3), chunk = ((lane & 7) ^ (lane >> 3)) * 16;
   const int w_row = lane_row * c.K, x_row = lane_row * (int)c.x_row;
-  __amdgpu_buffer_rsrc_t rw, rx;
-  // scales of this lane's tokens and of the wave's outputs
-  const float *xs[TI], *ws;
-  float scale[TI], ahead[S - 1][TI], w_ahead[S - 1];
+  // What is fetched: the next block of a tile, then of the workgroup's next one.
+  int tile = blockIdx.x, next, last;
+  u4 rw, rx;
+  const float* xs;  // of the wave's first token
+  int xs_lane;
   auto open = [&] {
-    rw = make_rsrc(static_cast<const char*>(c.W) + (size_t)n0 * c.K, min(BN, c.N - n0) * c.K);
-    rx = make_rsrc(static_cast<const char*>(c.x) + t0 * c.x_row,
-                   (int)((min(BT, c.T - t0) - 1) * c.x_row) + c.K);
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-      xs[i] = c.x_scale + min(t0 + wt + 16 * i + r16, c.T - 1) * c.xs_t;
-    ws = c.w_scale + (size_t)min((n0 + wn) / 128, (c.N - 1) / 128) * KB;
+    const Place f = place(tile);
+    next = f.b0;
+    last = f.b1;
+    rw = dma_rsrc(static_cast<const char*>(c.W) + (size_t)f.n0 * c.K, min(BN, c.N - f.n0) * c.K);
+    rx = dma_rsrc(static_cast<const char*>(c.x) + f.t0 * c.x_row,
+                  (int)((min(BT, c.T - f.t0) - 1) * c.x_row) + c.K);
+    const int t = min(f.t0 + wt, c.T - 1);
+    xs = c.x_scale + t * c.xs_t;
+    xs_lane = min(min(lane, WT - 1), c.T - 1 - t) * (int)c.xs_t * 4;
   };
-  // Block b to a stage and its scales to a slot, the scales first: they are there
-  // when kLoads loads are left.  Behind the last block come zeros.
-  auto fetch = [&](char* stage, int slot, int b) {
-    const int in = min(b, b1 - 1);
-    w_ahead[slot] = ws[in];
-#pragma unroll
-    for (int i = 0; i < TI; ++i) ahead[slot][i] = xs[i][in * c.xs_b];
-    const int k = b * 128 + chunk;
-    const int off = b < b1 && k < c.K ? k : kOut;
-    typedef __attribute__((address_space(3))) void lds;
-    if constexpr (S > 2) asm volatile("" ::: "memory");
+  const unsigned lds = lds_address(s_stage);
+  auto fetch = [&](int stage) {
+    if (next == last && tile < all) {
+      tile += gridDim.x;
+      if (tile < all) open();
+    }
+    const unsigned to = lds + stage * kStage;
+    const int b = min(next, last - 1), k = next * 128 + chunk;
+    const int off = next < last && k < c.K ? k : kOut;  // behind the last tile come zeros
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds*)(stage + (i * NW + wave) * 1024), 16,
-                                               off + w_row + i * NW * 8 * c.K, 0, 0, 0);
+      dma16(to + (i * NW + wave) * 1024, rw, off + w_row + i * NW * 8 * c.K);
 #pragma unroll
     for (int i = 0; i < kLoadsX; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rx, (lds*)(stage + BN * 128 + (i * NW + wave) * 1024), 16,
-          off + x_row + i * NW * 8 * (int)c.x_row, 0, 0, 0);
+      dma16(to + BN * 128 + (i * NW + wave) * 1024, rx, off + x_row + i * NW * 8 * (int)c.x_row);
+    dma4(to + kScales + wave * kWave * 4, dma_rsrc(xs + b * c.xs_b, 0x7FFFFFFF), xs_lane);
+    next = min(next + 1, last);
   };
 
   f4 acc[NI][TI];
-  auto multiply = [&](const char* stage) {
+  // (the next stage is asked for behind the first reads, whose wait that fills)
+  auto multiply = [&](int at, float w_scale, int ask) {
+    const char* const stage = s_stage + at * kStage;
     const int s0 = (q ^ (r16 & 7)) * 16, s1 = s0 ^ 64;
     const char* const pw = stage + (wn + r16) * 128;
     const char* const px = stage + (BN + wt + r16) * 128;
@@ -313,7 +310,13 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
       x[j] = join(ld16(px + j * 2048 + s0), ld16(px + j * 2048 + s1));
     auto rows = [&](int i) { return join(ld16(pw + i * 2048 + s0), ld16(pw + i * 2048 + s1)); };
     i8v w[3] = {rows(0), rows(1), {}};
+    fetch(ask);
     f4 p[TI];
+    float scale[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+      scale[i] = *reinterpret_cast<const float*>(stage + kScales + (wave * kWave + 16 * i + r16) * 4) *
+                 w_scale;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       // the products of row tile i beside the sums of i - 1 and the reads of i + 2
@@ -342,69 +345,33 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[NI - 1][j][e] += p[j][e] * scale[j];
   };
-  // The oldest block fetched is there, for all waves, and nobody reads the stage
-  // before it any more, which is fetched next.
-  auto ready = [&](int slot, bool exists) {
-    // (a barrier by itself waits for no load into the LDS)
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * kLoads) : "memory");
-#pragma unroll
-    for (int i = 0; i < TI; ++i) scale[i] = exists ? ahead[slot][i] * w_ahead[slot] : 0.0f;
-  };
-  // What comes next: of this tile, then of the workgroup's next one.
-  int tile = blockIdx.x, fetched = 0;
-  auto shift = [&] {
-#pragma unroll
-    for (int i = 0; i < TI; ++i) ahead[0][i] = ahead[S - 2][i];
-    w_ahead[0] = w_ahead[S - 2];
-  };
-  auto fetch_next = [&](char* stage, int slot) {
-    if (fetched == steps) {
-      tile += gridDim.x;
-      fetched = 0;
-      if (tile < all) {
-        place(tile);
-        open();
-      } else {
-        b0 = b1;  // nothing: zeros
-      }
-    }
-    fetch(stage, slot, b0 + fetched++);
-  };
-  place(tile);
   open();
-  fetch_next(s_a, 0);
-  if constexpr (S > 2) fetch_next(s_b, 1);
-  for (int now = tile; now < all; now += gridDim.x) {
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i);
+  int stage = 0, free_stage = S - 1;
+  for (int now = blockIdx.x; now < all; now += gridDim.x) {
+    const Place here = place(now);
+    const float* const ws =
+        c.w_scale + (size_t)min((here.n0 + wn) / 128, (c.N - 1) / 128) * KB;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < TI; ++j) acc[i][j] = f4{0, 0, 0, 0};
-    const int n_here = n0 + wn, t_here = t0 + wt, part_here = part, blocks = b1 - b0;
-    for (int s = 0; s < steps; s += S) {
-      if constexpr (S == 2) {
-        ready(0, s < blocks);
-        fetch_next(s_b, 0);
-        multiply(s_a);
-        ready(0, s + 1 < blocks);
-        fetch_next(s_a, 0);
-        multiply(s_b);
-      } else {
-        ready(0, s < blocks);
-        shift();
-        fetch_next(s_c, 1);
-        multiply(s_a);
-        ready(0, s + 1 < blocks);
-        shift();
-        fetch_next(s_a, 1);
-        multiply(s_b);
-        ready(0, s + 2 < blocks);
-        shift();
-        fetch_next(s_b, 1);
-        multiply(s_c);
-      }
+    float w_scale = scalar_load(ws + here.b0);
+    for (int b = here.b0; b < here.b1; ++b) {
+      // the oldest stage is there, for all waves, and nobody reads the one before it
+      dma_barrier<(S - 2) * kLoads>();
+      // (the block's scale is waited for here, before the next one is asked for)
+      asm volatile("" : "+s"(w_scale));
+      const float w_next = scalar_load(ws + min(b + 1, here.b1 - 1));
+      multiply(stage, w_scale, free_stage);
+      w_scale = w_next;
+      stage = stage + 1 == S ? 0 : stage + 1;
+      free_stage = free_stage + 1 == S ? 0 : free_stage + 1;
     }
+    const int n_here = here.n0 + wn, t_here = here.t0 + wt;
     if (plan.parts > 1) {
-      float* const to = plan.sums + (size_t)part_here * c.T * plan.pitch;
+      float* const to = plan.sums + (size_t)here.part * c.T * plan.pitch;
 #pragma unroll
       for (int j = 0; j < TI; ++j) {
         const int t = t_here + 16 * j + r16;
@@ -452,8 +419,7 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
       }
     }
   }
-  // what is still on its way into the LDS (zeros) arrives before that is given back
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  dma_drain();  // what is still on its way into the LDS (zeros), before that is given back
 }
 
 // The sums of the parts of K, in order.
@@ -471,6 +437,7 @@ __global__ __launch_bounds__(kThreads) void gemm_blocks_join(GemmBlocksCall c,
   store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, sum);
 }
 
+
 // Shapes of the tile kernel; kFew: the kernel of few tokens.
 enum Shape { kFew, k256x256, k256x128, k128x64, k128x32, kShapes };
 struct ShapeSize {
@@ -480,8 +447,8 @@ struct ShapeSize {
 constexpr ShapeSize kShape[kShapes] = {{16, 16, 512, 1, 0.0, 0.0},
                                        {256, 256, 512, 1, 1.95, 1.95},
                                        {256, 128, 512, 1, 1.15, 1.15},
-                                       {128, 64, 256, 2, 0.45, 0.72},
-                                       {128, 32, 256, 2, 0.38, 0.55}};
+                                       {128, 64, 256, 2, 0.47, 0.82},
+                                       {128, 32, 256, 2, 0.42, 0.62}};
 
 constexpr int kFewWaves = 8;
 constexpr size_t kFewLds = 100 * 1024;  // dynamic, next to 48 KB of partial sums and tiles
@@ -558,9 +525,7 @@ GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count) {
     const ShapeSize& s = kShape[shape];
     const long long tiles = (long long)((N + s.n - 1) / s.n) * ((T + s.t - 1) / s.t);
     for (int parts = 1; parts <= 16 && parts <= KB; ++parts) {
-      if (tuning().blocks_parts && parts != tuning().blocks_parts &&
-          parts < min(KB, tuning().blocks_parts))
-        continue;
+      if (tuning().blocks_parts && parts != min(KB, tuning().blocks_parts)) continue;
       const int each = (KB + parts - 1) / parts, have = (KB + each - 1) / each;
       const long long work = tiles * have;
       // workgroups of 128 outputs run two to a CU, a step of two takes longer

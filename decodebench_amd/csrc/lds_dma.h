@@ -39,6 +39,13 @@ __device__ __forceinline__ void dma16_stream(unsigned lds, u4 rsrc, int offset) 
       : "memory");
 }
 
+// 4 bytes a lane, to lds + 4 l.
+__device__ __forceinline__ void dma4(unsigned lds, u4 rsrc, int offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds),
+               "v"(offset), "s"(rsrc)
+               : "memory");
+}
+
 // Waits until at most LEFT of the wave's loads are on their way, then for the
 // workgroup's other waves.
 template <int LEFT>
