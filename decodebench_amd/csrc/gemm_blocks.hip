@@ -121,14 +121,11 @@ __global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
 #pragma unroll
     for (int r = 0; r < kFewRounds; ++r) x_raw[r] = ask(x_at + r * NW * 4);
   } else {
-    const __amdgpu_buffer_rsrc_t rx =
-        make_rsrc(c.x, (int)((c.T - 1) * c.x_row) + c.K);
+    const u4 rx = dma_rsrc(c.x, (int)((c.T - 1) * c.x_row) + c.K);
     for (int t = 0; t < c.T; ++t)
       for (int at = ((wave + t) & (NW - 1)) * 1024; at < KP; at += NW * 1024) {
-        typedef __attribute__((address_space(3))) void lds;
         const int k = at + (lane >> 3) * 128 + ((lane & 7) ^ (t & 7)) * 16;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds*)(s_x + t * KP + at), 16,
-                                                 k < c.K ? t * (int)c.x_row + k : kOut, 0, 0, 0);
+        dma16(lds_address(s_x) + t * KP + at, rx, k < c.K ? t * (int)c.x_row + k : kOut);
       }
     const int i = min((int)threadIdx.x, items - 1), t = row_of(i);
     xs_first = c.x_scale[t * c.xs_t + (i - t * KB) * c.xs_b];
@@ -458,16 +455,16 @@ size_t few_lds(int T, int K, int each) {
   return (size_t)T * ((K + 1023) / 1024 * 1024 + KB * 4) + (size_t)(each / 128 + 2) * KB * 4;
 }
 
-template <class F>
-hipError_t launch_few(F* fn, const GemmBlocksCall& c, const GemmBlocksPlan& plan,
-                      hipStream_t stream) {
-  // (once per kernel and device; a second call asks for the same)
-  static std::atomic<unsigned long long> asked{0};
+// The kernel of few tokens may take more dynamic LDS than a launch has unasked.
+template <class E, bool QUANT>
+hipError_t launch_few(const GemmBlocksCall& c, const GemmBlocksPlan& plan, hipStream_t stream) {
+  auto* const fn = gemm_blocks_few<E, QUANT, kFewWaves>;
+  static std::atomic<unsigned long long> asked{0};  // devices this kernel was asked for
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (dev >= 64 || !(asked.load(std::memory_order_relaxed) & bit)) {
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (!(asked.load(std::memory_order_relaxed) & bit)) {
     e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)kFewLds);
     if (e != hipSuccess) return e;
@@ -479,14 +476,8 @@ hipError_t launch_few(F* fn, const GemmBlocksCall& c, const GemmBlocksPlan& plan
 
 template <class E>
 hipError_t launch(const GemmBlocksCall& c, const GemmBlocksPlan& plan, hipStream_t stream) {
-  if (plan.shape == kFew) {
-    if (!c.x_scale) {
-      static const auto fn = gemm_blocks_few<E, true, kFewWaves>;
-      return launch_few(fn, c, plan, stream);
-    }
-    static const auto fn = gemm_blocks_few<E, false, kFewWaves>;
-    return launch_few(fn, c, plan, stream);
-  }
+  if (plan.shape == kFew)
+    return c.x_scale ? launch_few<E, false>(c, plan, stream) : launch_few<E, true>(c, plan, stream);
   auto* const fn = plan.shape == k256x256   ? gemm_blocks_tile<E, 256, 256, 128, 64, 2>
                    : plan.shape == k256x128 ? gemm_blocks_tile<E, 256, 128, 64, 64, 3>
                    : plan.shape == k128x64  ? gemm_blocks_tile<E, 128, 64, 64, 32, 3>

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kWaves* kWave) void moe_logits(MoeRouteCall c) {
   __shared__ double s_part[kWaves][4][kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r16 = lane & 15, q = lane >> 4;
-  const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+  const int e0 = blockIdx.y * 16, t0 = blockIdx.x * 16;
   const int steps = (c.H + 31) / 32, each = (steps + c.parts - 1) / c.parts;
   const int begin = blockIdx.z * each, end = min(steps, begin + each);
   const elem* const wr = static_cast<const elem*>(c.router) +
@@ -155,7 +155,7 @@ hipError_t launch_moe_logits(const MoeRouteCall& c, hipStream_t stream) {
       moe_logits_few<ElemF16><<<grid, 4 * kWave, 0, stream>>>(c);
     return hipGetLastError();
   }
-  const dim3 grid((c.E + 15) / 16, (c.T + 15) / 16, c.parts);
+  const dim3 grid((c.T + 15) / 16, (c.E + 15) / 16, c.parts);
   if (c.bf16)
     moe_logits<ElemBF16><<<grid, kWaves * kWave, 0, stream>>>(c);
   else

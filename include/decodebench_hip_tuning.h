@@ -62,6 +62,9 @@ extern "C" {
  *                         K = 2048 and 4096 off the tile kernel
  *  "gemv_splits"         (K splits of a db_gemv_ws call: 1 to 8 where its shape
  *                         allows them; 0 automatic)
+ *  "blocks_shape"        (tiles of db_gemm_blocks, outputs by tokens: 1 256 x 256,
+ *                         2 256 x 128, 3 128 x 64, 4 128 x 32; 0 automatic)
+ *  "blocks_parts"        (parts of K of its tiles, 1 to 16; 0 automatic)
  *  "f4_launch"           (a call of F4 whose split merge runs in a second
  *                         launch makes only one of its two launches: 1 the
  *                         split kernel, 2 the merge, which then reads whatever

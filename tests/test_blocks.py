@@ -194,6 +194,63 @@ def test_gemm_quantizes_on_the_way(dtype, T, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K", [(16, 4096), (16, 5120), (9, 8192), (4, 14336), (1, 16384),
+                                 (16, 14336)])
+def test_gemm_of_few_tokens_and_long_rows(dtype, T, K):
+    """Rows that fill most of a CU's LDS, and those that do not fit it."""
+    N = 200
+    W, ws = weights(N, K, K)
+    x = torch.randn(T, K, generator=generator(T)).to(dtype)
+    q, xs = quantized(x)
+    want, S = reference(q, xs, W, ws)
+    near(ops.gemm_blocks(x.to(DEV), W.to(DEV), ws.to(DEV)), want, S, K)
+    near(ops.gemm_blocks(q.to(DEV), W.to(DEV), ws.to(DEV), x_scale=xs.to(DEV), dtype=dtype), want,
+         S, K)
+
+
+@pytest.fixture
+def tuned():
+    yield ops.tune
+    ops.tune("blocks_shape", 0)
+    ops.tune("blocks_parts", 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [1, 2, 3, 4])
+@pytest.mark.parametrize("T,N,K", [(1, 16, 16), (5, 77, 2064), (33, 1000, 272), (200, 1031, 2048),
+                                   (300, 2048, 1536), (513, 700, 656), (1100, 3000, 400)])
+def test_gemm_of_every_tile_shape(tuned, shape, T, N, K):
+    """Each shape of the tile kernel, whole rows and parts of them, also where another
+    would be taken: tiles behind the ends, several tiles a workgroup, odd parts."""
+    W, ws = weights(N, K, 3)
+    q, xs = quantized(torch.randn(T, K, generator=generator(1)))
+    want, S = reference(q, xs, W, ws)
+    args = [t.to(DEV) for t in (q, W, ws)]
+    tuned("blocks_shape", shape)
+    for parts in (1, 2, 3, 5, 16):
+        tuned("blocks_parts", parts)
+        near(ops.gemm_blocks(*args, x_scale=xs.to(DEV)), want, S, K)
+
+
+@pytest.mark.gpu
+def test_gemm_of_more_tiles_than_workgroups(tuned):
+    """A workgroup of 256 x 256 goes from one tile to the next: 300 of them."""
+    T, N, K = 256 * 15 - 100, 256 * 20 - 60, 400
+    W, ws = weights(N, K, 8)
+    q, xs = quantized(torch.randn(T, K, generator=generator(2)))
+    tuned("blocks_shape", 1)
+    y = ops.gemm_blocks(q.to(DEV), W.to(DEV), ws.to(DEV), x_scale=xs.to(DEV))
+    # some rows and columns of every tile
+    rows, cols = torch.arange(0, T, 37), torch.arange(0, N, 41)
+    want, S = reference(q[rows], xs[rows], W, ws)
+    near(y.cpu()[rows][:, cols], want[:, cols], S[:, cols], K)
+    tuned("blocks_shape", 0)
+    near(ops.gemm_blocks(q.to(DEV), W.to(DEV), ws.to(DEV), x_scale=xs.to(DEV)).cpu()[rows], want,
+         S, K)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 24, 300])
 def test_gemm_rows_do_not_touch_each_other(T):
     """Inf, NaN and zeros of one token stay with it; those of a weight row with its output."""
@@ -344,7 +401,7 @@ def test_gemm_contract(lib):
                 dict(T=1 << 22), dict(stride=240), dict(stride=264), dict(stride=1 << 23),
                 dict(xdt=0), dict(xdt=2), dict(xdt=2, xs=None), dict(ydt=1), dict(ydt=9),
                 dict(x=P + 8), dict(W=P + 8), dict(y=P + 4), dict(xs=P + 2), dict(ws=P + 1),
-                dict(st=-1), dict(sb=-4), dict(xdt=0, xs=None), dict(xdt=0, xs=None, work=P),
+                dict(st=-1), dict(sb=-4), dict(st=1 << 22), dict(xdt=0, xs=None), dict(xdt=0, xs=None, work=P),
                 dict(xdt=0, xs=None, work=P + 128, nbytes=1 << 20)):
         assert call(**bad) == ops.DB_ERR_INVALID, bad
         assert b"db_gemm_blocks" in lib.db_last_error()
