@@ -80,6 +80,7 @@ struct FewArgs {
   MoeFewCall f;
   int slices;    // workgroups of a pair, or of a token
   int padded;    // K in whole chunks
+  unsigned magic;  // 2^32 / (padded / 8), rounded up
 };
 
 // A workgroup has every (slices)th group of kWaves rows of one pair.
@@ -97,16 +98,14 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   const int pair = blockIdx.x / a.slices, slice = blockIdx.x - pair * a.slices;
   const int t = pair / c.k, j = pair - t * c.k;
   const int H = c.w.H, I = c.w.I;
+  const bool chooses = a.f.logits != nullptr;
+  MoeLogits<kThreads> logits;
+  if (chooses) logits.load(a.f.logits + (size_t)t * c.w.E, 1, 0, c.w.E);
   row_to_lds(s_x, static_cast<const elem*>(c.x) + t * c.x_row, H, a.padded);
   int expert;
-  if (a.f.logits) {
-    moe_choose<kThreads>(s_choice, a.f.logits + (size_t)t * c.w.E, 1, 0, c.w.E, c.k,
-                         a.f.renormalize);
+  if (chooses) {
+    moe_rank(s_choice, logits, c.w.E, c.k);
     expert = s_choice.expert[j];
-    if (slice == 0 && threadIdx.x == 0) {
-      a.f.experts[pair] = expert;
-      a.f.weights[pair] = s_choice.p[j] / s_choice.total;
-    }
   } else {
     expert = c.experts[pair];
     __syncthreads();
@@ -146,6 +145,13 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   };
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) load(u);
+  if (chooses && slice == 0) {
+    moe_weigh(s_choice, c.w.E, c.k, a.f.renormalize);
+    if (threadIdx.x == 0) {
+      a.f.experts[pair] = expert;
+      a.f.weights[pair] = s_choice.p[j] / s_choice.total;
+    }
+  }
   int row = slice * kWaves + wave, item = 0;
   float g = 0.0f, up = 0.0f;
   while (row < I) {
@@ -199,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   const int row_pieces = a.padded / 8, pieces = k * row_pieces;
   const elem* const h_from = static_cast<const elem*>(c.h) + (size_t)t * k * I;
   auto piece = [&](int i) {
-    const int j = i / row_pieces, at = (i - j * row_pieces) * 8;
+    const int j = (int)__umulhi(i, a.magic), at = (i - j * row_pieces) * 8;
     return at < I && j < k ? ld16(h_from + (size_t)j * I + at) : u4{0, 0, 0, 0};
   };
   constexpr int kFirst = 4;
@@ -297,11 +303,12 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
     return max(1, min(want, (rows + kWaves - 1) / kWaves));
   };
   const int P = c.T * c.k;
-  FewArgs g = {f, slices(P, c.w.I), chunks(c.w.H, FP8)};
+  FewArgs g = {f, slices(P, c.w.I), chunks(c.w.H, FP8), 0};
   moe_few_gate<E, FP8><<<P * g.slices, kThreads, (size_t)g.padded * 2, stream>>>(g);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  FewArgs d = {f, slices(c.T, c.w.H), chunks(c.w.I, FP8)};
+  FewArgs d = {f, slices(c.T, c.w.H), chunks(c.w.I, FP8), 0};
+  d.magic = 0xFFFFFFFFu / (d.padded / 8) + 1;
   moe_few_down<E, FP8><<<c.T * d.slices, kThreads, (size_t)d.padded * 2 * c.k, stream>>>(d);
   return hipGetLastError();
 }

@@ -133,7 +133,10 @@ __global__ __launch_bounds__(4 * kWave) void moe_logits_few(MoeRouteCall c) {
 __global__ __launch_bounds__(256) void moe_select(MoeRouteCall c) {
   __shared__ MoeChoice s;
   const size_t t = blockIdx.x;
-  moe_choose<256>(s, c.logits + t * c.E, c.parts, (size_t)c.T * c.E, c.E, c.k, c.renormalize);
+  MoeLogits<256> logits;
+  logits.load(c.logits + t * c.E, c.parts, (size_t)c.T * c.E, c.E);
+  moe_rank(s, logits, c.E, c.k);
+  moe_weigh(s, c.E, c.k, c.renormalize);
   if (threadIdx.x < c.k) {
     c.experts[t * c.k + threadIdx.x] = s.expert[threadIdx.x];
     c.weights[t * c.k + threadIdx.x] = s.p[threadIdx.x] / s.total;

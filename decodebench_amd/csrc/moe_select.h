@@ -25,24 +25,40 @@ __device__ __forceinline__ double logit_key(double l) {
   return l != l ? __builtin_huge_val() : l == __builtin_huge_val() ? 0x1.fffffffffffffp1023 : l;
 }
 
-// A logit is the sum of `sums` parts, each `apart` from the one before.  Fills s.expert and s.p (exp of each choice against the largest) and s.total (of
-// the choices, or of all experts).  Ranks are counted: an expert comes after those
-// of larger logits, and of equal ones with a lower index.  NT threads, barriers
-// within; E and k are uniform.
+// A token's logits as the threads of a workgroup load them: expert tid + i NT's is l[i],
+// the sum of `sums` parts, each `apart` from the one before.
 template <int NT>
-__device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, int sums,
-                                           size_t apart, int E, int k, bool renormalize) {
+struct MoeLogits {
+  double l[kMostExperts / NT];
+  __device__ __forceinline__ void load(const double* logits, int sums, size_t apart, int E) {
+#pragma unroll
+    for (int i = 0; i < kMostExperts / NT; ++i) {
+      const int e = threadIdx.x + i * NT;
+      if (i * NT >= E) break;
+      l[i] = e < E ? logits[e] : 0.0;
+      for (int j = 1; j < sums; ++j) l[i] += e < E ? logits[j * apart + e] : 0.0;
+    }
+  }
+};
+
+// Fills s.logit and s.expert, the k largest in order.  Ranks are counted: an expert
+// comes after those of larger logits, and of equal ones with a lower index.  NT
+// threads, barriers within (the last one behind all of it); E and k are uniform.
+template <int NT>
+__device__ __forceinline__ void moe_rank(MoeChoice& s, const MoeLogits<NT>& in, int E, int k) {
   const int tid = threadIdx.x;
-  for (int e = tid; e < E + 2; e += NT) {
-    double l = e < E ? logits[e] : 0.0;
-    for (int i = 1; i < sums && e < E; ++i) l += logits[i * apart + e];
-    // (behind the last one stands what comes before nothing)
-    s.key[e] = e < E ? logit_key(l) : -__builtin_huge_val();
+#pragma unroll
+  for (int i = 0; i < kMostExperts / NT; ++i) {
+    const int e = tid + i * NT;
+    if (i * NT >= E) break;
     if (e < E) {
-      s.logit[e] = l;
+      s.logit[e] = in.l[i];
+      s.key[e] = logit_key(in.l[i]);
       s.rank[e] = 0;
     }
   }
+  // (behind the last one stands what comes before nothing)
+  if (tid < 2) s.key[E + tid] = -__builtin_huge_val();
   __syncthreads();
   // experts by the threads, what they are compared with in `parts` parts
   int lanes = 64;
@@ -65,6 +81,12 @@ __device__ __forceinline__ void moe_choose(MoeChoice& s, const double* logits, i
   for (int e = tid; e < E; e += NT)
     if (s.rank[e] < k) s.expert[s.rank[e]] = e;
   __syncthreads();
+}
+
+// After moe_rank: s.p (exp of each choice against the largest) and s.total (of the
+// choices, or of all experts).
+__device__ __forceinline__ void moe_weigh(MoeChoice& s, int E, int k, bool renormalize) {
+  const int tid = threadIdx.x;
   const double top = s.logit[s.expert[0]];
   if (tid < k) s.p[tid] = expf((float)(s.logit[s.expert[tid]] - top));
   if (!renormalize && tid < kWave) {
