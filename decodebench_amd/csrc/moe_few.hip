@@ -69,6 +69,11 @@ __device__ __forceinline__ float dot_chunk(u4 w, const char* x) {
   }
 }
 
+// The scale of the block of the lane's bytes from `off` on (zero behind the last one).
+__device__ __forceinline__ float ld_scale(__amdgpu_buffer_rsrc_t r, int off) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off / 128 * 4, 0, 0));
+}
+
 // Copies a row of K elements to the LDS, with zeros up to a whole number of chunks.
 __device__ __forceinline__ void row_to_lds(char* to, const void* from, int K, int padded) {
   for (int k = threadIdx.x * 8; k < padded; k += kThreads * 8)
@@ -128,15 +133,17 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
     const int row = min(at_row, I - 1), bytes = at_row < I ? (int)row_bytes : 0;
     const __amdgpu_buffer_rsrc_t rg = make_rsrc(wg + row * row_bytes, bytes);
     const __amdgpu_buffer_rsrc_t ru = make_rsrc(wu + row * row_bytes, bytes);
+    const size_t scales = ((size_t)expert * NB + row / 128) * KB;
+    const __amdgpu_buffer_rsrc_t sg = make_rsrc(c.w.sg + scales, KB * 4);
+    const __amdgpu_buffer_rsrc_t su = make_rsrc(c.w.su + scales, KB * 4);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int off = ((at_item * CH + i) * kWave + lane) * 16;
       w[u][0][i] = ld_buf_stream(rg, off);
       w[u][1][i] = ld_buf_stream(ru, off);
       if constexpr (FP8) {
-        const size_t at = ((size_t)expert * NB + row / 128) * KB + min(off / 128, KB - 1);
-        scale[u][0][i] = off < H ? c.w.sg[at] : 0.0f;
-        scale[u][1][i] = off < H ? c.w.su[at] : 0.0f;
+        scale[u][0][i] = ld_scale(sg, off);
+        scale[u][1][i] = ld_scale(su, off);
       }
     }
     const bool wrap = ++at_item >= items;
@@ -181,25 +188,21 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
 }
 
 // A workgroup has every (slices)th group of kWaves rows of one token.
-template <class E, bool FP8>
+template <class E, bool FP8, int CH>
 __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;
-  constexpr int CH = 2;
-  constexpr int kAhead = 4;  // items on their way: 8 KB a wave
+  constexpr int kAhead = 8 / CH;  // items on their way: 8 KB a wave
   extern __shared__ __align__(16) char s_h[];
-  __shared__ int s_expert[kMostChoices];
-  __shared__ float s_weight[kMostChoices];
   const MoeExpertsCall& c = a.f.c;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int t = blockIdx.x / a.slices, slice = blockIdx.x - t * a.slices;
   const int H = c.w.H, I = c.w.I, k = c.k;
-  if (threadIdx.x < k) {
-    const int e = c.experts[t * k + threadIdx.x];
-    s_expert[threadIdx.x] = e;
-    s_weight[threadIdx.x] = (unsigned)e < (unsigned)c.w.E ? c.weights[t * k + threadIdx.x] : 0.0f;
-  }
+  // Lane j holds the token's expert j and its weight.
+  static_assert(kMostChoices <= kWave, "a lane for each");
+  const int my_expert = c.experts[t * k + min(lane, k - 1)];
+  const float my_weight = c.weights[t * k + min(lane, k - 1)];
   // The first pieces of h are asked for before the weights, which come in order
   // behind them.  (What h holds of a pair without an expert does not count.)
   const int row_pieces = a.padded / 8, pieces = k * row_pieces;
@@ -212,7 +215,6 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   u4 first[kFirst];
 #pragma unroll
   for (int r = 0; r < kFirst; ++r) first[r] = piece(threadIdx.x + r * kThreads);
-  __syncthreads();
 
   const int KB = (I + 127) / 128, NB = (H + 127) / 128;
   constexpr int CB = FP8 ? 1 : 2;
@@ -223,19 +225,18 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   u4 w[kAhead][CH];
   float scale[kAhead][CH];
   auto load = [&](int u) {
-    const int e = __builtin_amdgcn_readfirstlane(s_expert[at_j]);
+    const int e = __builtin_amdgcn_readlane(my_expert, at_j);
     const bool exists = at_row < H && (unsigned)e < (unsigned)c.w.E;
     const size_t row = exists ? (size_t)e * H + at_row : 0;
     const __amdgpu_buffer_rsrc_t rd = make_rsrc(
         static_cast<const char*>(c.w.wd) + row * row_bytes, exists ? (int)row_bytes : 0);
+    const size_t nb = exists ? (size_t)e * NB + at_row / 128 : 0;
+    const __amdgpu_buffer_rsrc_t sd = make_rsrc(c.w.sd + nb * KB, KB * 4);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int off = ((at_item * CH + i) * kWave + lane) * 16;
       w[u][i] = ld_buf_stream(rd, off);
-      if constexpr (FP8) {
-        const size_t nb = exists ? (size_t)e * NB + at_row / 128 : 0;
-        scale[u][i] = off < I ? c.w.sd[nb * KB + min(off / 128, KB - 1)] : 0.0f;
-      }
+      if constexpr (FP8) scale[u][i] = ld_scale(sd, off);
     }
     const bool wrap = ++at_item >= items;
     at_item = wrap ? 0 : at_item;
@@ -271,7 +272,8 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
       load(u);
       if (++item == items) {
         // (a pair without an expert adds nothing, whatever its weight was)
-        if ((unsigned)s_expert[j] < (unsigned)c.w.E) sum += part * s_weight[j];
+        if ((unsigned)__builtin_amdgcn_readlane(my_expert, j) < (unsigned)c.w.E)
+          sum += part * lane_value(my_weight, j);
         part = 0.0f;
         item = 0;
         if (++j == k) {
@@ -309,7 +311,9 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
   if (e != hipSuccess) return e;
   FewArgs d = {f, slices(c.T, c.w.H), chunks(c.w.I, FP8), 0};
   d.magic = 0xFFFFFFFFu / (d.padded / 8) + 1;
-  moe_few_down<E, FP8><<<c.T * d.slices, kThreads, (size_t)d.padded * 2 * c.k, stream>>>(d);
+  // (rows of one load have items of one)
+  auto* const down = d.padded == chunks(1, FP8) ? moe_few_down<E, FP8, 1> : moe_few_down<E, FP8, 2>;
+  down<<<c.T * d.slices, kThreads, (size_t)d.padded * 2 * c.k, stream>>>(d);
   return hipGetLastError();
 }
 
