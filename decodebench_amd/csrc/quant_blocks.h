@@ -1,5 +1,7 @@
 // quant_blocks.h -- 128 elements to e4m3 and their scale, by the 16 lanes of a DPP row:
-//   scale = max |x| / 448 (1 where that is 0), q = e4m3(clamp(x / scale, -448, 448)).
+//   scale = max |x| * fp32(1 / 448) (1 where that is 0), q = e4m3(clamp(x / scale, -448, 448)).
+// The product, not the quotient: it is what a tensor divided by a number gives on the
+// GPU in torch, so a plain form there has the same codes.
 #pragma once
 
 #include "db_elem.h"
@@ -34,11 +36,12 @@ __device__ __forceinline__ float float_of(unsigned bits) {
 // p = x r is at most two steps off, p + (x - p scale) r rounds the exact quotient
 // but for errors of 2^-46 of it (Markstein's correction of a quotient), and one that fp32
 // holds exactly, as a tie between two codes is, comes out as it is.  Three
-// operations an element instead of ten: 8191 x 14336 elements XXX.
+// operations an element instead of ten: 8191 x 14336 elements 67.7 us, 76.5 with the
+// division.
 // Scales near the ends of fp32's range, Inf and NaN among them, take the division.
 template <class E>
 __device__ __forceinline__ u2 quantize128(u4 w, float& scale) {
-  scale = float_of<E>(row_magnitude(w)) / 448.0f;
+  scale = float_of<E>(row_magnitude(w)) * (1.0f / 448.0f);
   if (scale == 0.0f) scale = 1.0f;
   float v[8];
 #pragma unroll

@@ -1,7 +1,7 @@
 // quant_blocks.hip -- activations to OCP e4m3 with one fp32 scale for each 128
 // elements of a row.
 //
-//   scale[t, b] = max |x[t, 128 b ..]| / 448  (1 where that is 0)
+//   scale[t, b] = max |x[t, 128 b ..]| * fp32(1 / 448)  (1 where that is 0)
 //   q[t, k]     = e4m3(clamp(x[t, k] / scale[t, k / 128], -448, 448))
 //
 // Bound by HBM: three bytes an element.  Sixteen lanes have a block, eight

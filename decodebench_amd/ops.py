@@ -929,7 +929,7 @@ def quantize_blocks(x):
     side in memory, as :func:`gemm_blocks` reads them best).
 
     x [T, K] fp16 or bf16 (rows may be strided), K a multiple of 16.
-    ``scale[t, b] = max |x[t, 128 b ..]| / 448`` (1 where that is 0) and
+    ``scale[t, b] = max |x[t, 128 b ..]| * (1 / 448)`` in fp32 (1 where that is 0) and
     ``q = e4m3(clamp(x / scale, -448, 448))``, rounded to nearest even; an Inf or
     NaN makes its block's scale one."""
     if _fast is not None:

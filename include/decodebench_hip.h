@@ -292,8 +292,8 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
  * reference, whose weights are fp16
  * (src/decodebench/demos/llama_decode.py:110-116).
  *
- * scale[t, b] = max |x[t, 128 b ..]| / 448 in fp32 (1 where that is 0), q =
- * e4m3(clamp(x / scale, -448, 448)), rounded to nearest even.  A block that holds an Inf or
+ * scale[t, b] = max |x[t, 128 b ..]| * (1 / 448), both in fp32 (1 where that is 0),
+ * q = e4m3(clamp(x / scale, -448, 448)), rounded to nearest even.  A block that holds an Inf or
  * NaN gets that scale, so it stays visible.
  * Contract: x [T, K] of dtype DB_DTYPE_F16 or DB_DTYPE_BF16, rows x_stride
  * elements apart and 16-byte aligned; q [T, K] dense, 16-byte aligned; scale

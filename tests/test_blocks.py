@@ -4,8 +4,9 @@ implementations in 64 bits, their refusals, and a product after a quantisation.
 Tolerances count roundings: u is half a step of the output's type (fp16 2^-11,
 bf16 2^-8).
 
-* quantize_blocks: none.  The scale is an fp32 quotient, the codes are e4m3 of an
-  fp32 quotient; a quotient in 64 bits rounded to 32 is the same number.
+* quantize_blocks: none.  The scale is an fp32 product of a 16-bit magnitude and the
+  rounded 1 / 448, which 64 bits hold exactly; the codes are e4m3 of an fp32
+  quotient, and a quotient in 64 bits rounded to 32 is the same number.
 * gemm_blocks: products of e4m3 are exact; with S = sum_k |x_k W_k| (scales
   included) K fp32 additions are off by at most 2^-23 S each, also where they cut
   instead of rounding, the scales and their products by 2^-22 S in all, the
@@ -42,7 +43,7 @@ def quantized(x):
     scale = torch.empty(T, blocks(K), dtype=torch.float32)
     for b in range(blocks(K)):
         part = x[:, 128 * b:128 * b + 128].double()
-        s = (part.abs().amax(1) / 448.0).float()
+        s = (part.abs().amax(1) * torch.tensor(1.0 / 448.0).double()).float()
         s[s == 0] = 1.0
         v = (part / s.double()[:, None]).float().clamp(-448.0, 448.0)
         q[:, 128 * b:128 * b + 128] = v.to(FP8)
