@@ -22,7 +22,7 @@ constexpr int kWaves = 4;       // of a logits workgroup: each has a part of its
 constexpr int kMostParts = 16;  // of H
 
 // Workgroups of the logits: 16 tokens, 16 experts and one of the parts of H that make
-// enough of them (201 tokens, 8 experts of 4096: 13 us in one part, XXX so).
+// enough of them (201 tokens, 8 experts of 4096: the router 15.7 us in one part, 8 so).
 int logit_parts(int T, int H, int E) {
   const long long tiles = (long long)((T + 15) / 16) * ((E + 15) / 16);
   const long long want = (1024 + tiles - 1) / tiles;

@@ -36,7 +36,15 @@ struct MoeLogits {
       const int e = threadIdx.x + i * NT;
       if (i * NT >= E) break;
       l[i] = e < E ? logits[e] : 0.0;
-      for (int j = 1; j < sums; ++j) l[i] += e < E ? logits[j * apart + e] : 0.0;
+      // four parts' loads at once
+      for (int j0 = 1; j0 < sums; j0 += 4) {
+        double v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = e < E && j0 + j < sums ? logits[(j0 + j) * apart + e] : 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[i] += v[j];
+      }
     }
   }
 };
