@@ -147,11 +147,24 @@ def reference(q, xs, W, ws):
     return x @ w.t(), x.abs() @ w.abs().t()
 
 
-def near(y, want, S, K):
+def near(y, want, S, K, cut=0.0):
     y = y.cpu()
-    tol = HALF_STEP[y.dtype] * want.abs() + (K + 2) * 2.0 ** -23 * S
+    tol = HALF_STEP[y.dtype] * want.abs() + (K + 2) * 2.0 ** -23 * S + cut
     off = (y.double() - want).abs()
     assert (off <= tol).all(), f"{(off / tol).max()} of the tolerance at {(off / tol).argmax()}"
+
+
+def instruction_cut(q, xs, W, ws):
+    """What the matrix instruction's own sum may lose.  It adds eight products of
+    consecutive k at a time, cut off (towards zero) 13 binary places below the leading
+    one of the largest: seven of them lose less than 2^-13 of it each, the largest, a
+    product of two numbers of 4 bits, nothing.  It is at most the largest |x| of the
+    eight times the largest |w|.  (Over long rows the bound of the fp32 sums, which is
+    K steps of all magnitudes together, is wider than this one.)"""
+    x = q.double() * xs.double().repeat_interleave(128, 1)[:, :q.shape[1]]
+    w = W.double() * spread(ws, *W.shape)
+    x, w = (v.abs().view(v.shape[0], -1, 8).amax(2) for v in (x, w))
+    return 7 * 2.0 ** -13 * (x @ w.t())
 
 
 SIZES = [
@@ -208,6 +221,26 @@ def test_gemm_of_few_tokens_and_long_rows(dtype, T, K):
     near(ops.gemm_blocks(x.to(DEV), W.to(DEV), ws.to(DEV)), want, S, K)
     near(ops.gemm_blocks(q.to(DEV), W.to(DEV), ws.to(DEV), x_scale=xs.to(DEV), dtype=dtype), want,
          S, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K", [(2, 16), (2, 128), (7, 112), (16, 16), (16, 128), (3, 144),
+                                 (16, 256)])
+def test_gemm_of_few_tokens_and_one_block(dtype, T, K):
+    """Rows of one block, and of little more: a token's scales, whatever their strides."""
+    N = 150
+    W, ws = weights(N, K, K)
+    x = torch.randn(T, K, generator=generator(T)).to(dtype)
+    q, xs = quantized(x)
+    want, S = reference(q, xs, W, ws)
+    cut = instruction_cut(q, xs, W, ws)
+    near(ops.gemm_blocks(x.to(DEV), W.to(DEV), ws.to(DEV)), want, S, K, cut)
+    column = torch.full((T, 3 + blocks(K)), float("nan"))
+    column[:, 3:] = xs
+    for scale in (xs.to(DEV), xs.t().contiguous().to(DEV).t(), column.to(DEV)[:, 3:]):
+        near(ops.gemm_blocks(q.to(DEV), W.to(DEV), ws.to(DEV), x_scale=scale, dtype=dtype), want,
+             S, K, cut)
 
 
 @pytest.fixture
