@@ -314,6 +314,25 @@ def test_layer(dtype, fp8, renormalize, T, E, k, H, I):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T,E,k", [(1, 1024, 64), (4, 1024, 8), (5, 1024, 64), (513, 1, 1),
+                                   (700, 1000, 33)])
+def test_layer_of_many_experts_and_of_one(fp8, T, E, k):
+    H, I = 64, 32
+    on_gpu, plain = layer(E, H, I, torch.bfloat16, fp8, T + E)
+    gen = generator(T)
+    x = torch.randn(T, H, generator=gen).bfloat16()
+    Wr = (torch.randn(E, H, generator=gen) / H ** 0.5).bfloat16()
+    y = ops.moe_layer(x.to(DEV), Wr.to(DEV), top_k=k, **on_gpu)
+    e, w = ops.moe_route(x.to(DEV), Wr.to(DEV), k)
+    assert torch.equal(e.cpu(), route_reference(x, Wr, k, True)[0])
+    some = torch.arange(0, T, 37)
+    want, tol = experts_reference(x[some], e.cpu()[some], w.cpu()[some], plain)
+    assert ((y.cpu()[some].double() - want).abs() <= tol).all()
+    assert torch.equal(ops.moe_experts(x.to(DEV), e, w, **on_gpu), y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 5, 40])
 def test_layer_in_graphs_and_on_two_streams(T):
     E, k, H, I = 16, 4, 512, 256
