@@ -337,8 +337,8 @@ const Knob kKnobs[] = {
      "0 (automatic), 1 or 2", nullptr},
     {"gemv_splits", &dbk::Tuning::gemv_splits, [](int v) { return v >= 0 && v <= 8; },
      "0 (automatic) to 8", nullptr},
-    {"blocks_shape", &dbk::Tuning::blocks_shape, [](int v) { return v >= 0 && v <= 4; },
-     "0 (automatic) to 4", nullptr},
+    {"blocks_shape", &dbk::Tuning::blocks_shape, [](int v) { return v >= 0 && v <= 7; },
+     "0 (automatic) to 7", nullptr},
     {"blocks_parts", &dbk::Tuning::blocks_parts, [](int v) { return v >= 0 && v <= 16; },
      "0 (automatic) to 16", nullptr},
     {"f4_launch", &dbk::Tuning::f4_launch, [](int v) { return v >= 0 && v <= 2; },

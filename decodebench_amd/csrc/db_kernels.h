@@ -39,8 +39,8 @@ struct Tuning {
   int gemv_tile = 0;           // batches of 2 rows and more (gemv_mfma_min_batch if set):
                                // 0 automatic, 1 gemv_tile, 2 never gemv_tile
   int gemv_splits = 0;         // K splits of gemv_tile where a workspace is given: 0 auto, 1..8
-  int blocks_shape = 0;        // gemm_blocks: 0 automatic, 1..4 tiles of 256 x 256,
-                               // 256 x 128, 128 x 64, 128 x 32
+  int blocks_shape = 0;        // gemm_blocks: 0 automatic, 1..7 tiles of 256 x 256,
+                               // 256 x 128, 128 x 64, 128 x 32, 64 x 64, 64 x 32, 32 x 32
   int blocks_parts = 0;        // parts of K of its tiles: 0 automatic, 1..16
   int f4_launch = 0;           // measurement hook for the two-launch F4: 0 both
                                // launches, 1 the split kernel only, 2 the merge only

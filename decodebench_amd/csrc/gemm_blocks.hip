@@ -14,6 +14,7 @@
 // eight meet in fp32.  Eight products so lose less than 7 * 2^-13 of the largest of
 // them, where rounding x to e4m3 has cost each up to 2^-4.  Sums that keep all places
 // would take the 16-bit instructions, at half the rate.
+#include <algorithm>
 #include <atomic>
 
 #include "db_kernels.h"
@@ -70,6 +71,9 @@ __device__ __forceinline__ void store4(void* y, size_t at, int left, bool vec, f
 // T <= 16 tokens, 16 at a time; its waves take blocks of K in turn, and their sums
 // meet in the LDS.  x lies there whole, its scales behind it, copied or quantised
 // by every workgroup for itself while the first weights are on their way.
+//
+// Bound by the weights' bytes: one token of [14336, 4096] 12.2 us, 4.8 TB/s, where a
+// kernel that only reads them takes 9.7; the difference is the start, x before weights.
 //
 // A load instruction has 8 rows of one 128-byte line each, consecutive lanes
 // consecutive chunks (operand order, rows on consecutive lanes, takes the L1 four
@@ -231,20 +235,34 @@ __global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
 // (chunk ^ row % 8), set by which global chunk a lane fetches: the 16 rows that a
 // quarter of a wave reads then lie in different banks.  Each wave fetches the scales
 // of its own tokens along with them.
-template <class E, int BN, int BT, int WN, int WT, int S>
-__global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_tile(
+//
+// Small tiles, of few tokens, have G groups of waves that take the blocks of K in turn,
+// each with stages of its own: a barrier then has G blocks, and a step of small tiles
+// is the latency of barrier, reads and products (0.3 us), whatever they are.  The
+// groups' sums meet in the LDS in order.  48 tokens of [6144, 4096], quantised: 12.3 us
+// in 128 x 64 with K in five parts, 13.5 in 32 x 64 with ten stages, 9.2 in 64 x 32 with four
+// groups; such workgroups have one tile each.
+//
+// Large tiles keep the matrix cores busy: 8192 x 14336 x 4096 418 us, 2.3 PFLOP/s (2.48 in a
+// library product with one scale), where the scaled sums take 14%.  256 x 128 reads
+// more of the LDS for a product and is for outputs that 256 x 256 would leave half the
+// CUs without: 2047 x 4096 x 4096 39 us, 52 in 256 x 256.
+template <class E, int BN, int BT, int WN, int WT, int S, int G = 1>
+__global__ __launch_bounds__(G*(BN / WN) * (BT / WT) * kWave, G > 2 ? 1 : 2) void gemm_blocks_tile(
     GemmBlocksCall c, GemmBlocksPlan plan) {
   typedef typename E::type elem;
-  constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;
+  constexpr int NW = (BN / WN) * (BT / WT), NI = WN / 16, TI = WT / 16;  // NW: of a group
   constexpr int kLoadsW = BN / 8 / NW, kLoadsX = BT / 8 / NW;  // of 8 rows, a wave
   constexpr int kLoads = kLoadsW + kLoadsX + 1;                // and one of scales
   static_assert(BN % (8 * NW) == 0 && BT % (8 * NW) == 0, "whole loads");
   static_assert(NI % 2 == 0 && 128 % WN == 0, "row tiles in pairs, of one block of the weights");
   static_assert(WT <= kWave, "a lane for each token's scale");
   constexpr int kScales = (BN + BT) * 128, kStage = kScales + NW * kWave * 4;
-  __shared__ __align__(16) char s_stage[S * kStage];
+  static_assert(G == 1 || S * kStage >= NW * kWave * NI * TI * 16, "room to join the groups' sums");
+  __shared__ __align__(16) char s_stage[G * S * kStage];
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int all_wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int group = G > 1 ? all_wave / NW : 0, wave = G > 1 ? all_wave % NW : all_wave;
   const int r16 = lane & 15, q = lane >> 4;
   const int KB = (c.K + 127) / 128;
   const int wn = wave % (BN / WN) * WN, wt = wave / (BN / WN) * WT;
@@ -274,7 +292,7 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
   int xs_lane;
   auto open = [&] {
     const Place f = place(tile);
-    next = f.b0;
+    next = f.b0 + group;
     last = f.b1;
     rw = dma_rsrc(static_cast<const char*>(c.W) + (size_t)f.n0 * c.K, min(BN, c.N - f.n0) * c.K);
     rx = dma_rsrc(static_cast<const char*>(c.x) + f.t0 * c.x_row,
@@ -283,9 +301,10 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
     xs = c.x_scale + t * c.xs_t;
     xs_lane = min(min(lane, WT - 1), c.T - 1 - t) * (int)c.xs_t * 4;
   };
-  const unsigned lds = lds_address(s_stage);
+  char* const my_stages = s_stage + group * S * kStage;
+  const unsigned lds = lds_address(my_stages);
   auto fetch = [&](int stage) {
-    if (next == last && tile < all) {
+    if (G == 1 && next == last && tile < all) {
       tile += gridDim.x;
       if (tile < all) open();
     }
@@ -299,13 +318,13 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
     for (int i = 0; i < kLoadsX; ++i)
       dma16(to + BN * 128 + (i * NW + wave) * 1024, rx, off + x_row + i * NW * 8 * (int)c.x_row);
     dma4(to + kScales + wave * kWave * 4, dma_rsrc(xs + b * c.xs_b, 0x7FFFFFFF), xs_lane);
-    next = min(next + 1, last);
+    next = G > 1 ? next + G : min(next + 1, last);
   };
 
   f4 acc[NI][TI];
   // (the next stage is asked for behind the first reads, whose wait that fills)
   auto multiply = [&](int at, float w_scale, int ask) {
-    const char* const stage = s_stage + at * kStage;
+    const char* const stage = my_stages + at * kStage;
     const int s0 = (q ^ (r16 & 7)) * 16, s1 = s0 ^ 64;
     const char* const pw = stage + (wn + r16) * 128;
     const char* const px = stage + (BN + wt + r16) * 128;
@@ -362,17 +381,35 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < TI; ++j) acc[i][j] = f4{0, 0, 0, 0};
-    float w_scale = scalar_load(ws + here.b0);
-    for (int b = here.b0; b < here.b1; ++b) {
+    float w_scale = scalar_load(ws + min(here.b0 + group, here.b1 - 1));
+    for (int b = here.b0; b < here.b1; b += G) {
       // the oldest stage is there, for all waves, and nobody reads the one before it
       dma_barrier<(S - 2) * kLoads>();
       // (the block's scale is waited for here, before the next one is asked for)
       asm volatile("" : "+s"(w_scale));
-      const float w_next = scalar_load(ws + min(b + 1, here.b1 - 1));
-      multiply(stage, w_scale, free_stage);
+      const float w_next = scalar_load(ws + min(b + group + G, here.b1 - 1));
+      // (a group without a block is at its end, where nothing more is fetched)
+      if (G == 1 || b + group < here.b1) multiply(stage, w_scale, free_stage);
       w_scale = w_next;
       stage = stage + 1 == S ? 0 : stage + 1;
       free_stage = free_stage + 1 == S ? 0 : free_stage + 1;
+    }
+    if constexpr (G > 1) {
+      // the groups' sums, in order; the stages have no other use left (what is
+      // on its way into them are zeros, waited for first)
+      f4* const sums = reinterpret_cast<f4*>(s_stage) + (wave * NI * TI) * kWave + lane;
+#pragma unroll
+      for (int g = 1; g < G; ++g) {
+        dma_barrier<0>();
+        if (group == g)
+#pragma unroll
+          for (int i = 0; i < NI * TI; ++i) sums[i * kWave] = acc[i / TI][i % TI];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+          for (int i = 0; i < NI * TI; ++i) acc[i / TI][i % TI] += sums[i * kWave];
+      }
+      if (group > 0) return;
     }
     const int n_here = here.n0 + wn, t_here = here.t0 + wt;
     if (plan.parts > 1) {
@@ -427,7 +464,7 @@ __global__ __launch_bounds__((BN / WN) * (BT / WT) * kWave, 2) void gemm_blocks_
   dma_drain();  // what is still on its way into the LDS (zeros), before that is given back
 }
 
-// The sums of the parts of K, in order.
+// The sums of the parts of K, in order.  (A launch of its own: 3 to 5 us in all.)
 template <class E>
 __global__ __launch_bounds__(kThreads) void gemm_blocks_join(GemmBlocksCall c,
                                                              GemmBlocksPlan plan) {
@@ -437,23 +474,36 @@ __global__ __launch_bounds__(kThreads) void gemm_blocks_join(GemmBlocksCall c,
   if (t >= c.T) return;
   const float* from = plan.sums + (size_t)t * plan.pitch + n;
   f4 sum = *reinterpret_cast<const f4*>(from);
-  for (int p = 1; p < plan.parts; ++p)
-    sum += *reinterpret_cast<const f4*>(from + (size_t)p * c.T * plan.pitch);
+  // five parts' loads at once, added in order
+  constexpr int kLoads = 5;
+  for (int p0 = 1; p0 < plan.parts; p0 += kLoads) {
+    f4 v[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      v[i] = *reinterpret_cast<const f4*>(
+          from + (size_t)min(p0 + i, plan.parts - 1) * c.T * plan.pitch);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      if (p0 + i < plan.parts) sum += v[i];
+  }
   store4<E>(c.y, (size_t)t * c.N + n, c.N - n, c.N % 4 == 0, sum);
 }
 
-
 // Shapes of the tile kernel; kFew: the kernel of few tokens.
-enum Shape { kFew, k256x256, k256x128, k128x64, k128x32, kShapes };
+enum Shape { kFew, k256x256, k256x128, k128x64, k128x32, k64x64, k64x32, k32x32, kShapes };
 struct ShapeSize {
   int n, t, threads, slots;  // slots: workgroups a CU
-  double step, step2;        // us of a block of K, with one and with two workgroups a CU
+  int groups;                // of waves, with a block of K each
+  double step, step2;        // us of a block of K for each group, with one and with two workgroups a CU
 };
-constexpr ShapeSize kShape[kShapes] = {{16, 16, 512, 1, 0.0, 0.0},
-                                       {256, 256, 512, 1, 1.95, 1.95},
-                                       {256, 128, 512, 1, 1.15, 1.15},
-                                       {128, 64, 256, 2, 0.47, 0.82},
-                                       {128, 32, 256, 2, 0.42, 0.62}};
+constexpr ShapeSize kShape[kShapes] = {{16, 16, 512, 1, 1, 0.0, 0.0},
+                                       {256, 256, 512, 1, 1, 1.95, 1.95},
+                                       {256, 128, 512, 1, 1, 1.15, 1.15},
+                                       {128, 64, 256, 2, 1, 0.47, 0.82},
+                                       {128, 32, 256, 2, 1, 0.42, 0.62},
+                                       {64, 64, 512, 1, 2, 0.58, 0.58},
+                                       {64, 32, 512, 1, 4, 0.82, 0.82},
+                                       {32, 32, 512, 1, 4, 0.59, 0.59}};
 
 constexpr int kFewWaves = 8;
 constexpr size_t kFewLds = 100 * 1024;  // dynamic, next to 48 KB of partial sums and tiles
@@ -489,7 +539,10 @@ hipError_t launch(const GemmBlocksCall& c, const GemmBlocksPlan& plan, hipStream
   auto* const fn = plan.shape == k256x256   ? gemm_blocks_tile<E, 256, 256, 128, 64, 2>
                    : plan.shape == k256x128 ? gemm_blocks_tile<E, 256, 128, 64, 64, 3>
                    : plan.shape == k128x64  ? gemm_blocks_tile<E, 128, 64, 64, 32, 3>
-                                            : gemm_blocks_tile<E, 128, 32, 32, 32, 3>;
+                   : plan.shape == k128x32  ? gemm_blocks_tile<E, 128, 32, 32, 32, 3>
+                   : plan.shape == k64x64   ? gemm_blocks_tile<E, 64, 64, 32, 32, 4, 2>
+                   : plan.shape == k64x32   ? gemm_blocks_tile<E, 64, 32, 32, 32, 3, 4>
+                                            : gemm_blocks_tile<E, 32, 32, 32, 16, 4, 4>;
   fn<<<plan.grid, kShape[plan.shape].threads, 0, stream>>>(c, plan);
   if (plan.parts > 1) {
     const size_t quads = (size_t)c.T * plan.pitch / 4;
@@ -517,7 +570,9 @@ GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count) {
     p.fused = false;
   }
   // The shape and the parts of K whose rounds of workgroups are estimated to take
-  // the least time.
+  // the least time, by the steps that each shape measured.  27 sizes from 16 to 8192
+  // tokens: within 4% of the best of all forced ones on 22 of them, 20% on the worst
+  // (64 x 1024 x 8192, 10.6 for 8.7 us).
   double best = 0.0;
   for (int shape = k256x256; shape < kShapes; ++shape) {
     if (tuning().blocks_shape && shape != tuning().blocks_shape) continue;
@@ -531,14 +586,21 @@ GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count) {
       const long long rounds = (work + s.slots * cu_count - 1) / (s.slots * cu_count);
       const bool crowded = s.slots > 1 && work > cu_count;
       const double sums = have > 1 ? (double)have * T * p.pitch * sizeof(float) : 0.0;
-      const double us = rounds * (each + 2) * (crowded ? s.step2 : s.step) +
-                        (have > 1 ? 2.5 + sums * 2 / 6e6 : 0.0);
+      const int steps = (each + s.groups - 1) / s.groups;
+      // a first tile starts cold, a workgroup's next ones cost two steps more
+      const double step = crowded ? s.step2 : s.step, cold = 2.4;
+      const double start = s.groups > 1 ? rounds * cold : std::max(cold, rounds * 2 * step);
+      const double busy = rounds * steps * step + start;
+      // The weights come at 5.5 TB/s to all CUs together; neither hides all of the other.
+      const double stream = (double)K * N / 5.5e6 * std::max(1.0, (double)cu_count / work);
+      const double us = std::max(busy, stream) + 0.1 * std::min(busy, stream) +
+                        (have > 1 ? 4.2 + 0.1 * have + sums * 1.2 / 6e6 : 0.0);
       if (best == 0.0 || us < best) {
         best = us;
         p.shape = shape;
         p.each = each;
         p.parts = have;
-        p.grid = (int)min(work, (long long)cu_count * s.slots);
+        p.grid = (int)(s.groups > 1 ? work : min(work, (long long)cu_count * s.slots));
         p.bytes = have > 1 ? (size_t)have * T * p.pitch * sizeof(float) : 0;
       }
     }

@@ -5,11 +5,16 @@
 //
 // The weights of the experts that are asked are read once for all their tokens,
 // and are what bounds the call: a batch of few tokens reads megabytes for each
-// of them.  Pairs are sorted by expert, 16 TT of one expert make a tile, and
-// each product is 16 rows of the weights (A) by the tile's tokens (B) on
-// v_mfma_f32_16x16x32, the waves of a workgroup taking blocks of 128 columns in
-// turn.  e4m3 weights are widened to the activations' type (exact), each block's
+// of them.  Pairs are sorted by expert and cut into tiles of 16 to 128 of one expert;
+// a workgroup has 64 or 128 gate rows and the up rows beside them (or twice as many
+// down rows) of a tile, a wave 32 of the weight rows (A) by all of the tile's tokens (B)
+// on v_mfma_f32_16x16x32.  Both operands come straight into the LDS, several stages
+// ahead.  e4m3 weights are widened to the activations' type (exact), each block's
 // sum scaled in fp32; the activations keep their 16 bits.
+//
+// 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 535 to 555 us, 5.2 TB/s; 33
+// tokens, 6 of 64 of 1392 x 2048, e4m3 (530 MB): 104 us, of which the gate takes 54
+// and the down product 41 (4.7 TB/s), the other launches the rest.
 //
 // g, u, silu and the product are fp32; h is rounded once to the activations'
 // type, which the second product takes; what the pairs of a token add up to is

@@ -9,6 +9,10 @@
 // summed in 64 bits (v_mfma_f64_16x16x4, products of 16-bit numbers are exact):
 // they do not depend on the order of the sum where that could be seen, and a
 // token's experts not on the batch it comes in.
+//
+// Bound by latency: two launches, each a few dependent reads long.  One token, 128
+// experts of 4096: 8.3 us; 509 tokens, 64 experts of 2048: 10.3 (the matrix cores would
+// need 1.7 at their 64-bit rate).
 #include "db_kernels.h"
 #include "moe_select.h"
 

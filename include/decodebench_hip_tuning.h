@@ -63,7 +63,8 @@ extern "C" {
  *  "gemv_splits"         (K splits of a db_gemv_ws call: 1 to 8 where its shape
  *                         allows them; 0 automatic)
  *  "blocks_shape"        (tiles of db_gemm_blocks, outputs by tokens: 1 256 x 256,
- *                         2 256 x 128, 3 128 x 64, 4 128 x 32; 0 automatic)
+ *                         2 256 x 128, 3 128 x 64, 4 128 x 32, 5 64 x 64,
+ *                         6 64 x 32, 7 32 x 32; 0 automatic)
  *  "blocks_parts"        (parts of K of its tiles, 1 to 16; 0 automatic)
  *  "f4_launch"           (a call of F4 whose split merge runs in a second
  *                         launch makes only one of its two launches: 1 the

@@ -268,6 +268,47 @@ def test_gemm_of_every_tile_shape(tuned, shape, T, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [5, 6, 7])
+@pytest.mark.parametrize("T,N,K", [(1, 16, 16), (5, 77, 2064), (33, 1000, 272), (33, 30, 128),
+                                   (200, 1031, 2048), (70, 2048, 1536), (513, 700, 656),
+                                   (1100, 3000, 400), (20, 100, 144)])
+def test_gemm_of_every_tile_shape_with_groups(tuned, shape, T, N, K):
+    """The shapes whose waves have blocks of K in turn: blocks fewer than groups, odd
+    ones, more workgroups than CUs; the groups add up in order."""
+    W, ws = weights(N, K, 3)
+    q, xs = quantized(torch.randn(T, K, generator=generator(1)))
+    want, S = reference(q, xs, W, ws)
+    cut = instruction_cut(q, xs, W, ws)
+    args = [t.to(DEV) for t in (q, W, ws)]
+    tuned("blocks_shape", shape)
+    for parts in (1, 2, 3, 5, 16):
+        tuned("blocks_parts", parts)
+        y = ops.gemm_blocks(*args, x_scale=xs.to(DEV))
+        near(y, want, S, K, cut)
+        assert torch.equal(y, ops.gemm_blocks(*args, x_scale=xs.to(DEV)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [5, 6, 7])
+def test_gemm_groups_without_a_block_add_nothing(tuned, shape):
+    """The last block's scale is infinite, for one token and one block of outputs: the
+    groups behind the end of K must not multiply it by zeros for anybody else."""
+    T, N, K = 20, 160, 128 * 5
+    W, ws = weights(N, K, 4)
+    q, xs = quantized(torch.randn(T, K, generator=generator(1)))
+    args = [t.to(DEV) for t in (q, W, ws)]
+    tuned("blocks_shape", shape)
+    clean = ops.gemm_blocks(*args, x_scale=xs.to(DEV)).cpu()
+    xs[3, 4] = float("inf")
+    got = ops.gemm_blocks(*args, x_scale=xs.to(DEV)).cpu()
+    keep = [t for t in range(T) if t != 3]
+    assert torch.equal(got[keep], clean[keep])
+    # the sum of that block decides, whose sign is known
+    part = (q[3, 512:].double() @ W[:, 512:].double().t())
+    assert torch.equal(got[3], torch.where(part > 0, float("inf"), -float("inf")).half())
+
+
+@pytest.mark.gpu
 def test_gemm_of_more_tiles_than_workgroups(tuned):
     """A workgroup of 256 x 256 goes from one tile to the next: 300 of them."""
     T, N, K = 256 * 15 - 100, 256 * 20 - 60, 400
