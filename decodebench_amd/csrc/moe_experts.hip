@@ -13,8 +13,8 @@
 // sum scaled in fp32; the activations keep their 16 bits.
 //
 // 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 535 to 555 us, 5.2 TB/s; 33
-// tokens, 6 of 64 of 1392 x 2048, e4m3 (530 MB): 104 us, of which the gate takes 54
-// and the down product 41 (4.7 TB/s), the other launches the rest.
+// tokens, 6 of 64 of 1392 x 2048, e4m3 (530 MB): 103 us, of which the gate takes 48
+// (7.2 TB/s) and the down product 40, whose rows are 11 steps long and mostly start.
 //
 // g, u, silu and the product are fp32; h is rounded once to the activations'
 // type, which the second product takes; what the pairs of a token add up to is

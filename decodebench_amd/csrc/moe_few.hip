@@ -18,7 +18,7 @@
 // the choice from the workgroups of the first rows.
 //
 // One token, 8 of 128 experts of 768 x 2048, bf16 (75.5 MB): the layer 21.8 us, of which
-// the gate takes 10.4 (4.8 TB/s), the down product 6.9 and the logits 1.9.  A launch
+// the gate takes 11 to 13 (4.2 TB/s), the down product 6.7 and the logits 2 to 3.  A launch
 // pays about 3 us before its stream runs at its rate: x, the choice, the first rows.
 #include "db_kernels.h"
 #include "moe_select.h"
@@ -326,8 +326,9 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
 // Few pairs, whose rows of x and h fit the LDS that a launch has without asking, and
 // that read hardly more together than the experts they name among equally likely
 // ones: the tile kernels read an expert once for all its tokens, but take 15 us more
-// for sorting and adding up (80 MB at the rate of the weights; two tokens, 2 of 8 experts of
-// 14336 x 4096: 231 us here, 260 there, four 409 and 374).
+// for sorting and adding up (80 MB at the rate of the weights, and 50 more for what the
+// L2 holds of a second reading).  Two tokens, 2 of 8 experts of 14336 x 4096, e4m3: 231
+// us here, 260 there; four tokens 409 and 374.
 bool moe_few(const db_moe& m, int T, int k) {
   const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
   constexpr size_t kLds = 64 * 1024;
