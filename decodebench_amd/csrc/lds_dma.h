@@ -29,21 +29,21 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 __device__ __forceinline__ void dma16(unsigned lds, u4 rsrc, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds),
                "v"(offset), "s"(rsrc)
-               : "memory");
+               : "m0", "memory");
 }
 // The same for data that is read once: not kept in the caches.
 __device__ __forceinline__ void dma16_stream(unsigned lds, u4 rsrc, int offset) {
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds),
       "v"(offset), "s"(rsrc)
-      : "memory");
+      : "m0", "memory");
 }
 
 // 4 bytes a lane, to lds + 4 l.
 __device__ __forceinline__ void dma4(unsigned lds, u4 rsrc, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds),
                "v"(offset), "s"(rsrc)
-               : "memory");
+               : "m0", "memory");
 }
 
 // Waits until at most LEFT of the wave's loads are on their way, then for the
