@@ -28,7 +28,6 @@ namespace {
 typedef int i8v __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kOut = 1 << 30;  // an offset behind every buffer: loads give zero
 
 __device__ __forceinline__ i8v join(u4 lo, u4 hi) {
@@ -244,9 +243,10 @@ __global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
 // groups; such workgroups have one tile each.
 //
 // Large tiles keep the matrix cores busy: 8192 x 14336 x 4096 418 us, 2.3 PFLOP/s (2.48 in a
-// library product with one scale), where the scaled sums take 14%.  256 x 128 reads
-// more of the LDS for a product and is for outputs that 256 x 256 would leave half the
-// CUs without: 2047 x 4096 x 4096 39 us, 52 in 256 x 256.
+// library product with one scale), where the scaled sums take 14%.  256 x 128 fetches
+// and reads more for a product (1.15 us a block of K, of which the LDS is busy 0.6 and the
+// matrix cores 0.43) and is for outputs that 256 x 256 would leave half the CUs without:
+// 2047 x 4096 x 4096 39 us, 52 in 256 x 256.
 template <class E, int BN, int BT, int WN, int WT, int S, int G = 1>
 __global__ __launch_bounds__(G*(BN / WN) * (BT / WT) * kWave, G > 2 ? 1 : 2) void gemm_blocks_tile(
     GemmBlocksCall c, GemmBlocksPlan plan) {
