@@ -6,9 +6,10 @@
 //   weights[t, j] = exp(l_j - max) / sum of the same over the k, or over all E
 //
 // The choice is a comparison of sums that may be nearly alike, so the logits are
-// summed in 64 bits (v_mfma_f64_16x16x4, products of 16-bit numbers are exact):
-// they do not depend on the order of the sum where that could be seen, and a
-// token's experts not on the batch it comes in.
+// multiplied and summed in 64 bits (v_mfma_f64_16x16x4, products of 16-bit numbers
+// are exact).  The order of a sum goes by the number of tokens: where the 64-bit sums
+// are exact, a token's experts do not depend on the batch it comes in; elsewhere two
+// logits that are as near to each other as the roundings of 64 bits may change places.
 //
 // Bound by latency: two launches, each a few dependent reads long.  One token, 128
 // experts of 4096: 8.3 us; 509 tokens, 64 experts of 2048: 10.3 (the matrix cores would
@@ -85,7 +86,8 @@ __global__ __launch_bounds__(kWaves* kWave) void moe_logits(MoeRouteCall c) {
 }
 
 // Few tokens: a wave has an expert and all of them.  Eight elements of a row a
-// lane and step, their products (exact in fp32) added up in 64 bits.
+// lane and step, multiplied and added up in 64 bits: bf16 products leave the range
+// of 32 at both ends.
 constexpr int kFewTokens = 4;
 
 template <class E>
@@ -120,7 +122,8 @@ __global__ __launch_bounds__(4 * kWave) void moe_logits_few(MoeRouteCall c) {
       for (int i = 0; i < kSteps; ++i) {
         const vec8 wv = __builtin_bit_cast(vec8, w[i]), xv = __builtin_bit_cast(vec8, x[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[t] += (double)((float)wv[j] * (float)xv[j]);
+        for (int j = 0; j < 8; ++j)
+          acc[t] = __builtin_fma((double)(float)wv[j], (double)(float)xv[j], acc[t]);
       }
     }
   }

@@ -331,7 +331,7 @@ typedef struct db_moe {
   int w_dtype;      /* dtype, or DB_DTYPE_FP8_E4M3 */
 } db_moe;
 
-/* The experts of each token and their weights: logits x . Wr[e] (sums in 64 bits),
+/* The experts of each token and their weights: logits x . Wr[e] (products and sums in 64 bits),
  * experts [T, k] those of the k largest, largest first, ties to the lower index, NaN
  * above all numbers; weights [T, k] = softmax over the k (renormalize) or over all E.
  * Contract: x [T, H] rows x_stride elements apart and 16-byte aligned, Wr [E, H] dense,

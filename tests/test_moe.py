@@ -135,6 +135,29 @@ def test_route_does_not_depend_on_the_batch():
     assert e0.shape == (0, 8) and w0.shape == (0, 8)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 4, 5, 40])
+def test_route_products_beyond_the_range_of_32_bits(T):
+    """bf16 products reach from 2^-266 to 2^256.  Exact sums: two products of 2^140
+    cancel beside small terms; all products are near 2^-160."""
+    H, E, k = 64, 20, 6
+    score = (torch.randperm(E, generator=generator(T)) + 1).float()   # differ by 1 and more
+    want = score.argsort(descending=True)[:k].int()
+    Wr = torch.zeros(E, H)
+    Wr[:, 0], Wr[:, 1], Wr[:, 32] = 2.0 ** 40, -2.0 ** 40, score
+    x = torch.zeros(T, H)
+    x[:, 0], x[:, 1], x[:, 32] = 2.0 ** 100, 2.0 ** 100, 1.0
+    experts, w = ops.moe_route(x.bfloat16().to(DEV), Wr.bfloat16().to(DEV), k)
+    assert torch.equal(experts.cpu(), want.expand(T, k))
+    share = torch.softmax(score[want.long()].double(), 0)
+    assert ((w.cpu().double() - share).abs() <= (2 * E + 16) * 2.0 ** -23 * share).all()
+    Wr[:, :2], Wr[:, 32] = 0.0, score * 2.0 ** -80
+    x[:, 32] = 2.0 ** -80
+    experts, w = ops.moe_route(x.bfloat16().to(DEV), Wr.bfloat16().to(DEV), k)
+    assert torch.equal(experts.cpu(), want.expand(T, k))
+    assert (w == w[0, 0]).all() and (w.cpu().double() - 1 / k).abs().max() <= 2.0 ** -23 / k
+
+
 # ----------------------------------------------------------------- moe_experts
 def layer(E, H, I, dtype, fp8, seed):
     """(weights on the GPU as keywords, the same in 64 bits on the CPU)."""
