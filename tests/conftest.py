@@ -30,8 +30,18 @@ def _has_gpu() -> bool:
         return False
 
 
+# Tests of refusals by addresses that nobody owns, some of whose calls a host with a GPU
+# takes: four tokens of 256 elements need a workspace only where no GPU is found, so
+# there the kernel would be launched and fault.
+_ONLY_WITHOUT_GPU = {"test_gemm_contract"}
+
+
 def pytest_collection_modifyitems(config, items):
     if _has_gpu():
+        skip = pytest.mark.skip(reason="passes addresses that a GPU would follow")
+        for item in items:
+            if item.name in _ONLY_WITHOUT_GPU:
+                item.add_marker(skip)
         return
     skip = pytest.mark.skip(reason="no GPU visible")
     for item in items:
