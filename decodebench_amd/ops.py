@@ -273,6 +273,20 @@ def _output(shape, idx: int, out, name: str = "out"):
     return out
 
 
+def _apart(out, *named) -> None:
+    """Refuse an ``out`` that shares memory with an input, from its first element
+    to its last: some workgroups write it while others still read."""
+    begin = out.data_ptr()
+    end = begin + out.numel() * out.element_size()
+    for t, name in named:
+        if t is None or t.numel() == 0:
+            continue
+        first = t.data_ptr()
+        last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+        if first < end and begin < first + (last + 1) * t.element_size():
+            raise ValueError(f"out must not share memory with {name}")
+
+
 def cu_count(device=None) -> int:
     """Compute units of a GPU (index, torch.device or None for the current one)."""
     if isinstance(device, int) and device in _cu_cache:
@@ -966,7 +980,7 @@ def gemm_blocks(x, W, w_scale, x_scale=None, dtype=None, out=None):
     or bf16 is quantised on the way, as :func:`quantize_blocks` does, and
     y [T, N] has its type; or x is float8_e4m3fn with x_scale [T, ceil(K/128)],
     and y is ``dtype`` (torch.float16 if not given).  Rows of x may be strided,
-    and x_scale anyhow."""
+    and x_scale anyhow; ``out`` shares no memory with an input."""
     if out is None and _fast is not None:
         y = _fast.gemm_blocks(x, W, w_scale, x_scale, dtype)
         if y is not None:
@@ -1009,6 +1023,8 @@ def gemm_blocks(x, W, w_scale, x_scale=None, dtype=None, out=None):
     N = W.shape[0]
     sp = _block_scale(w_scale, "w_scale", (_blocks(N), _blocks(K)), idx)
     y = _row_output((T, N), dtype, idx, out)
+    if out is not None:
+        _apart(out, (x2, "x"), (W, "W"), (w_scale, "w_scale"), (x_scale, "x_scale"))
     lib = _lib or load_library()
     with _on_device(idx):
         nbytes = lib.db_gemm_blocks_workspace_bytes(T, K, N, xdt)
@@ -1103,7 +1119,8 @@ def moe_experts(x, experts, weights, Wg, Wu, Wd, sg=None, su=None, sd=None, out=
     An expert outside [0, E) adds nothing; a token without any gets zeros; an
     expert named twice counts twice.  Sums are fp32; what the gate gives is
     rounded to x's type before the down product, and the result once.  Made for
-    the few tokens of a decode step: the weights bound the call."""
+    the few tokens of a decode step: the weights bound the call.  ``out`` may be x
+    itself and shares no memory with another input."""
     if out is None and _fast is not None:
         y = _fast.moe_experts(x, experts, weights, Wg, Wu, Wd, sg, su, sd)
         if y is not None:
@@ -1120,6 +1137,9 @@ def moe_experts(x, experts, weights, Wg, Wu, Wd, sg=None, su=None, sd=None, out=
     k = experts.shape[1]
     m = _experts(x, Wg, Wu, Wd, sg, su, sd, idx, dt)
     y = _row_output((T, H), x.dtype, idx, out)
+    if out is not None:
+        _apart(out, (experts, "experts"), (weights, "weights"), (Wg, "Wg"), (Wu, "Wu"),
+               (Wd, "Wd"), (sg, "sg"), (su, "su"), (sd, "sd"))
     lib = _lib or load_library()
     with _on_device(idx):
         nbytes = lib.db_moe_experts_workspace_bytes(C.byref(m), T, k)
@@ -1144,6 +1164,9 @@ def moe_layer(x, Wr, Wg, Wu, Wd, top_k: int, renormalize: bool = True, sg=None, 
         raise ValueError(f"Wr has {Wr.shape[0]} rows for {m.E} experts")
     T, H = x.shape
     y = _row_output((T, H), x.dtype, idx, out)
+    if out is not None:
+        _apart(out, (Wr, "Wr"), (Wg, "Wg"), (Wu, "Wu"), (Wd, "Wd"), (sg, "sg"), (su, "su"),
+               (sd, "sd"))
     lib = _lib or load_library()
     with _on_device(idx):
         nbytes = lib.db_moe_layer_workspace_bytes(C.byref(m), T, k)

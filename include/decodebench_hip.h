@@ -298,7 +298,7 @@ int db_paged_attention(const void* q, long long q_token_stride, long long q_head
  * Contract: x [T, K] of dtype DB_DTYPE_F16 or DB_DTYPE_BF16, rows x_stride
  * elements apart and 16-byte aligned; q [T, K] dense, 16-byte aligned; scale
  * element (t, b) at t scale_t + b scale_b, no two at one place; K a multiple of
- * 16; T >= 0; T, K < 2^22. */
+ * 16; T >= 0; T, K < 2^22; q and scale overlap no input. */
 int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
                        long long scale_t, long long scale_b, int T, int K, int dtype,
                        void* stream);
@@ -309,7 +309,7 @@ int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
  * Contract: x_dtype DB_DTYPE_FP8_E4M3 or y_dtype; y_dtype DB_DTYPE_F16 or
  * DB_DTYPE_BF16; x rows x_stride elements apart and 16-byte aligned; W [N, K] and y
  * [T, N] dense; K a multiple of 16; T, N, K, x_stride, xs_t < 2^22; W 16-byte
- * aligned.  ws of db_gemm_blocks_workspace_bytes (NULL if 0) needs no initialisation
+ * aligned; y overlaps no input.  ws of db_gemm_blocks_workspace_bytes (NULL if 0) needs no initialisation
  * and holds nothing after the call; calls that overlap in time need their own. */
 size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype);
 int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long long xs_t,
@@ -348,7 +348,8 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
  * twice counts twice.
  * Contract: x, experts, weights, T, k as db_moe_route (k need not be below E); H and I
  * multiples of 8 (16 for e4m3 weights) below 2^20; T x_stride, T k I and T k H below 2^29;
- * weights 16-byte, scales 4-byte aligned, y [T, H] dense; ws of
+ * weights 16-byte, scales 4-byte aligned, y [T, H] dense (it may be x, and overlaps
+ * no other input); ws of
  * db_moe_experts_workspace_bytes, 256-byte aligned, as that of db_gemm_blocks. */
 size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k);
 int db_moe_experts(const void* x, long long x_stride, const int* experts, const float* weights,

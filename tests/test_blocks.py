@@ -535,6 +535,42 @@ def test_gemm_refusals():
         ops.quantize_blocks(x[0])
 
 
+def test_shared_memory_is_seen():
+    """From the first element to the last, whatever the strides; neighbours are apart."""
+    buf = torch.zeros(64, 32, dtype=torch.float16)
+    out = buf[10:20]
+    for other in (buf, out, buf[19:21], buf[::2], buf[0:11], buf[5:30, 8:16], out.view(torch.uint8)):
+        with pytest.raises(ValueError, match="share memory with x"):
+            ops._apart(out, (None, "none"), (other, "x"))
+    ops._apart(out, (buf[:10], "before"), (buf[20:], "behind"), (buf[10:10], "nothing"),
+               (buf.clone(), "another"), (buf[0:9:2], "rows before"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 8, 16, 40, 300])
+def test_gemm_does_not_write_over_its_inputs(T):
+    N = K = 256
+    W, ws = (t.to(DEV) for t in weights(N, K, 1))
+    buf = torch.randn(T + 8, K, generator=generator(2)).half().to(DEV)
+    x, before = buf[4:T + 4], buf.clone()
+    want = ops.gemm_blocks(x, W, ws)
+    for out in (x, buf[3:T + 3], buf[5:T + 5])[:3 if T > 1 else 1]:
+        with pytest.raises(ValueError, match="share memory"):
+            ops.gemm_blocks(x, W, ws, out=out)
+    with pytest.raises(ValueError, match="share memory"):   # one token from the middle of its row
+        ops.gemm_blocks(x[0], W, ws, out=buf.view(-1)[4 * K + 8:5 * K + 8].view(1, N))
+    q, xs = ops.quantize_blocks(x)
+    codes = torch.empty(T * K * 2, dtype=torch.uint8, device=DEV)
+    codes[:T * K] = q.view(torch.uint8).view(-1)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.gemm_blocks(codes[:T * K].view(FP8).view(T, K), W, ws, x_scale=xs,
+                        out=codes.view(torch.float16).view(T, N))
+    assert torch.equal(buf, before)
+    two = torch.empty(2 * T, N, dtype=torch.float16, device=DEV)
+    two[:T] = x
+    assert torch.equal(ops.gemm_blocks(two[:T], W, ws, out=two[T:]), want)
+
+
 def test_the_oracle_sees_a_wrong_block():
     """The tolerance of a product is far below what one left-out block changes."""
     W, ws = weights(64, 512, 2)

@@ -309,6 +309,34 @@ def test_experts_do_not_depend_on_strides_or_neighbours(T):
     assert ops.moe_experts(x[:0], experts[:0], weights[:0], **on_gpu).shape == (0, H)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [1, 4, 5, 60])
+def test_layers_may_write_over_x_and_nothing_else(T, fp8):
+    E, H, I, k = 8, 528, 400, 3
+    on_gpu, _ = layer(E, H, I, torch.float16, fp8, 3)
+    Wr = (torch.randn(E, H, generator=generator(1)) / 20).half().to(DEV)
+    buf = torch.randn(T + 8, H, generator=generator(2)).half().to(DEV)
+    experts, weights = (t.to(DEV) for t in routed(T, E, k, 2))
+    start = buf.clone()
+    x = start[4:T + 4]
+    want = ops.moe_experts(x, experts, weights, **on_gpu), ops.moe_layer(x, Wr, top_k=k, **on_gpu)
+    for begin in (4, 0, 7):   # in place, and moved by some rows
+        rows = slice(begin, T + begin)
+        buf.copy_(start)
+        ops.moe_experts(buf[4:T + 4], experts, weights, out=buf[rows], **on_gpu)
+        assert torch.equal(buf[rows], want[0])
+        buf.copy_(start)
+        ops.moe_layer(buf[4:T + 4], Wr, top_k=k, out=buf[rows], **on_gpu)
+        assert torch.equal(buf[rows], want[1])
+    with pytest.raises(ValueError, match="share memory with Wr"):
+        ops.moe_layer(x[:1], Wr, top_k=k, out=Wr[2:3], **on_gpu)
+    shared = torch.zeros(T * max(H, 2 * k), dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError, match="share memory with weights"):
+        ops.moe_experts(x, experts, shared[:2 * T * k].view(torch.float32).view(T, k),
+                        out=shared[:T * H].view(T, H), **on_gpu)
+
+
 # ------------------------------------------------------------------- moe_layer
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
