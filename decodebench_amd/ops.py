@@ -420,6 +420,8 @@ def f1_rmsnorm_gemv(x, g, W, eps: float = 1e-6, w_scale=None, out=None):
     dt, sp, sc = _weights(W, w_scale, "W", N, K)
     idx = _gpu_tensors((x, "x", torch.float16), (g, "g", torch.float16), (W, "W", None), *sc)
     y = _output((B, N), idx, out)
+    if out is not None:
+        _apart(out, (x2, "x"))
     if not _split_launch(out, x2.data_ptr(), g.data_ptr(), W.data_ptr(), None, sp, None, y, B, K,
                          N, float(eps), dt, idx):
         _launch((_lib or load_library()).db_f1_rmsnorm_gemv, idx, "db_f1_rmsnorm_gemv",
@@ -447,6 +449,8 @@ def f2_gateup_swiglu(x, Wg, Wu, sg=None, su=None, out=None):
     _, sup, suc = _weights(Wu, su, "Wu", N, K)
     idx = _gpu_tensors((x, "x", torch.float16), (Wg, "Wg", None), (Wu, "Wu", None), *sgc, *suc)
     y = _output((B, N), idx, out)
+    if out is not None:
+        _apart(out, (x2, "x"))
     if not _split_launch(out, x2.data_ptr(), None, Wg.data_ptr(), Wu.data_ptr(), sgp, sup, y, B,
                          K, N, 0.0, dt, idx):
         _launch((_lib or load_library()).db_f2_gateup_swiglu, idx, "db_f2_gateup_swiglu",
@@ -478,6 +482,8 @@ def f2_rmsnorm_gateup_swiglu(x, g, Wg, Wu, eps: float = 1e-6, sg=None, su=None, 
     idx = _gpu_tensors((x, "x", torch.float16), (g, "g", torch.float16), (Wg, "Wg", None),
                        (Wu, "Wu", None), *sgc, *suc)
     y = _output((B, N), idx, out)
+    if out is not None:
+        _apart(out, (x2, "x"))
     if not _split_launch(out, x2.data_ptr(), g.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), sgp, sup,
                          y, B, K, N, float(eps), dt, idx):
         _launch((_lib or load_library()).db_f2_rmsnorm_gateup_swiglu, idx,
@@ -501,6 +507,8 @@ def gemv(x, W, w_scale=None, out=None):
     dt, sp, sc = _weights(W, w_scale, "W", N, K)
     idx = _gpu_tensors((x, "x", torch.float16), (W, "W", None), *sc)
     y = _output((B, N), idx, out)
+    if out is not None:
+        _apart(out, (x2, "x"))
     if not _split_launch(out, x2.data_ptr(), None, W.data_ptr(), None, sp, None, y, B, K, N, 0.0,
                          dt, idx):
         _launch((_lib or load_library()).db_gemv, idx, "db_gemv",

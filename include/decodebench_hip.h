@@ -69,7 +69,8 @@ int db_device_cu_count(int* cu_count);
  * y [B,N] fp16.  w_dtype must be DB_DTYPE_F16 (w_scale NULL) or
  * DB_DTYPE_FP8_E4M3: W then holds N*K OCP e4m3fn bytes, K % 16 == 0, and
  * w_scale [N] fp32 (4-byte aligned) multiplies each row's fp32 dot product
- * before its fp16 rounding: y = fp16(w_scale[n] * sum_k e4m3(W[n,k]) xh[k]). */
+ * before its fp16 rounding: y = fp16(w_scale[n] * sum_k e4m3(W[n,k]) xh[k]).
+ * y overlaps no input. */
 int db_f1_rmsnorm_gemv(const void* x, const void* g, const void* W,
                        const float* w_scale, void* y, int B, int K, int N,
                        float eps, int w_dtype, void* stream);

@@ -44,3 +44,25 @@ def test_gemm_needs_its_workspace(lib):
     for bad in (dict(work=None), dict(work=P + 128), dict(nbytes=256), dict(xs=P)):
         assert call(**bad) == ops.DB_ERR_INVALID, bad
         assert b"db_gemm_blocks" in lib.db_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 4, 40])
+def test_projections_do_not_write_over_x(B):
+    """Every workgroup reads all of x, some after others have written their outputs."""
+    K = 256
+    gen = torch.Generator().manual_seed(B)
+    buf = torch.randn(2 * B, K, generator=gen).half().cuda()
+    x, g = buf[:B], torch.ones(K).half().cuda()
+    W, W2 = ((torch.randn(K, K, generator=gen) / 16).half().cuda() for _ in range(2))
+    before = buf.clone()
+    for call in (lambda out: ops.gemv(x, W, out=out), lambda out: ops.f1_rmsnorm_gemv(x, g, W, out=out),
+                 lambda out: ops.f2_gateup_swiglu(x, W, W2, out=out),
+                 lambda out: ops.f2_rmsnorm_gateup_swiglu(x, g, W, W2, out=out)):
+        with pytest.raises(ValueError, match="share memory with x"):
+            call(x)
+        assert torch.equal(buf, before)
+        beside = torch.empty_like(x)
+        want = call(beside).clone()
+        assert torch.equal(call(buf[B:]), want)
+        buf.copy_(before)
