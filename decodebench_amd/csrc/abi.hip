@@ -737,6 +737,12 @@ int check_route(const char* fn, const void* x, long long x_stride, const void* r
   return DB_OK;
 }
 
+// Whether the pairs of a call are more than a kernel's 32-bit offsets reach.
+bool too_many_pairs(const db_moe& m, int T, int k) {
+  const long long pairs = (long long)T * k;
+  return pairs * m.I >= kMostOffset || pairs * m.H >= kMostOffset;
+}
+
 int check_moe(const char* fn, const db_moe* m, const void* x, long long x_stride, const void* y,
               int T, int k) {
   if (!m) return fail(DB_ERR_INVALID, "%s: null weights", fn);
@@ -757,9 +763,7 @@ int check_moe(const char* fn, const db_moe* m, const void* x, long long x_stride
     return fail(DB_ERR_INVALID, "%s: T=%d must be >= 0 and below 2^20", fn, T);
   if (x_stride < m->H || x_stride % 8 != 0)
     return fail(DB_ERR_INVALID, "%s: x rows must hold H elements and be 16-byte aligned", fn);
-  const long long pairs = (long long)T * k;
-  if (x_stride >= kMostOffset || T * x_stride >= kMostOffset || pairs * m->I >= kMostOffset ||
-      pairs * m->H >= kMostOffset)
+  if (x_stride >= kMostOffset || T * x_stride >= kMostOffset || too_many_pairs(*m, T, k))
     return fail(DB_ERR_INVALID, "%s: T=%d tokens are too many for one call", fn, T);
   if (fp8 ? !m->sg || !m->su || !m->sd : m->sg || m->su || m->sd)
     return fail(DB_ERR_INVALID, fp8 ? "%s: e4m3 weights need a scale for each block"
@@ -831,7 +835,9 @@ int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
 }
 
 size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype) {
-  if (T < 1 || K < 1 || N < 1 || T >= kMostSize || K >= kMostSize || N >= kMostSize) return 0;
+  if (T < 1 || K < 16 || K % 16 != 0 || N < 1 || T >= kMostSize || K >= kMostSize ||
+      N >= kMostSize || !(is16bit(x_dtype) || x_dtype == DB_DTYPE_FP8_E4M3))
+    return 0;
   int err = 0;
   const int cus = dbk::device_cu_count(&err);
   if (err) return 0;
@@ -893,7 +899,8 @@ int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long
 }
 
 size_t db_moe_route_workspace_bytes(int T, int H, int E) {
-  if (T < 1 || T >= kMostTokens || E < 1 || E > 1024 || H < 1 || H >= kMostSize) return 0;
+  if (T < 1 || T >= kMostTokens || E < 1 || E > 1024 || H < 8 || H % 8 != 0 || H >= kMostSize)
+    return 0;
   return round256((size_t)dbk::moe_logit_parts(T, H, E) * T * E * sizeof(double));
 }
 
@@ -916,8 +923,14 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
 }
 
 size_t db_moe_experts_workspace_bytes(const db_moe* m, int T, int k) {
-  if (!m || T < 1 || T >= kMostTokens || k < 1 || k > 64 || m->E < 1 || m->E > 1024 || m->H < 1 ||
-      m->I < 1 || m->H >= kMostWidth || m->I >= kMostWidth)
+  // what check_moe refuses for its sizes gets none
+  if (!m || !is16bit(m->dtype) || T < 1 || T >= kMostTokens || k < 1 || k > 64 || m->E < 1 ||
+      m->E > 1024)
+    return 0;
+  const bool fp8 = m->w_dtype == DB_DTYPE_FP8_E4M3;
+  const int step = fp8 ? 16 : 8;
+  if ((!fp8 && m->w_dtype != m->dtype) || m->H < step || m->I < step || m->H % step ||
+      m->I % step || m->H >= kMostWidth || m->I >= kMostWidth || too_many_pairs(*m, T, k))
     return 0;
   dbk::MoeExpertsCall c = experts_call(nullptr, 0, nullptr, nullptr, *m, nullptr, T, k);
   return dbk::moe_experts_workspace(c, nullptr);
@@ -945,7 +958,7 @@ int db_moe_experts(const void* x, long long x_stride, const int* experts, const 
 }
 
 size_t db_moe_layer_workspace_bytes(const db_moe* m, int T, int k) {
-  if (!m || db_moe_experts_workspace_bytes(m, T, k) == 0) return 0;
+  if (!m || k > m->E || db_moe_experts_workspace_bytes(m, T, k) == 0) return 0;
   return layer_space(*m, T, k).bytes;
 }
 

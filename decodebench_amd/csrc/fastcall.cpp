@@ -666,7 +666,7 @@ PyObject* moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (found < 0) return nullptr;
   if (found == 0) Py_RETURN_NONE;
   const int E = (int)wr->size(0);
-  if (k < 1 || k > E) Py_RETURN_NONE;
+  if (k < 1 || k > E || k > 64) Py_RETURN_NONE;
   at::Tensor experts = empty_on({T, k}, at::kInt, idx), weights = empty_on({T, k}, at::kFloat, idx);
   const size_t bytes = abi.moe_route_workspace_bytes((int)T, (int)H, E);
   at::Tensor work;

@@ -1051,8 +1051,9 @@ def _router(x, Wr, top_k):
     if Wr.dim() != 2 or Wr.shape[1] != x.shape[1]:
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, Wr {tuple(Wr.shape)}")
     k = int(top_k)
-    if not 1 <= k <= Wr.shape[0]:
-        raise ValueError(f"top_k must be between 1 and the {Wr.shape[0]} experts (got {k})")
+    if not 1 <= k <= min(Wr.shape[0], 64):
+        raise ValueError(f"top_k must be between 1 and the {Wr.shape[0]} experts, at most 64 "
+                         f"(got {k})")
     return idx, dt, k
 
 

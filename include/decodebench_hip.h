@@ -310,8 +310,9 @@ int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
  * Contract: x_dtype DB_DTYPE_FP8_E4M3 or y_dtype; y_dtype DB_DTYPE_F16 or
  * DB_DTYPE_BF16; x rows x_stride elements apart and 16-byte aligned; W [N, K] and y
  * [T, N] dense; K a multiple of 16; T, N, K, x_stride, xs_t < 2^22; W 16-byte
- * aligned; y overlaps no input.  ws of db_gemm_blocks_workspace_bytes (NULL if 0) needs no initialisation
- * and holds nothing after the call; calls that overlap in time need their own. */
+ * aligned; y overlaps no input.  ws of db_gemm_blocks_workspace_bytes (NULL if 0; 0 as
+ * well for sizes that the call refuses) needs no initialisation and holds nothing after
+ * the call; calls that overlap in time need their own. */
 size_t db_gemm_blocks_workspace_bytes(int T, int K, int N, int x_dtype);
 int db_gemm_blocks(const void* x, long long x_stride, const float* x_scale, long long xs_t,
                    long long xs_b, const void* W, const float* w_scale, void* y, int T, int K,
