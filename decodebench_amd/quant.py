@@ -45,7 +45,8 @@ def quantize_e4m3_blocks(W):
     last of a dimension may be short).
 
     ``scale = max |W| / 448`` over the block (1 for an all-zero one), and
-    ``Wq = e4m3(clamp(W / scale, -448, 448))``."""
+    ``Wq = e4m3(clamp(W / scale, -448, 448))``.  An Inf or NaN makes its block's
+    scale one, and so the whole block NaN."""
     import torch
 
     if W.dim() < 2:
@@ -55,7 +56,7 @@ def quantize_e4m3_blocks(W):
     Wf = torch.nn.functional.pad(W.float(), (0, kb * 128 - K, 0, nb * 128 - N))
     Wf = Wf.view(*W.shape[:-2], nb, 128, kb, 128)
     amax = Wf.abs().amax(dim=(-3, -1))
-    scale = torch.where(amax > 0, amax / E4M3_MAX, torch.ones_like(amax))
+    scale = torch.where(amax == 0, torch.ones_like(amax), amax / E4M3_MAX)
     q = (Wf / scale[..., :, None, :, None]).clamp_(-E4M3_MAX, E4M3_MAX)
     q = q.view(*W.shape[:-2], nb * 128, kb * 128)[..., :N, :K].to(torch.float8_e4m3fn)
     return q.contiguous(), scale.contiguous()

@@ -439,6 +439,22 @@ def test_block_weights_on_the_cpu():
         quant.quantize_e4m3_blocks(W[0, 0])
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_block_weights_that_are_not_finite_stay_visible(bad):
+    """In their own block, whose numbers no scale holds beside them; no other changes."""
+    W = torch.randn(256, 256, generator=generator(2)) / 50
+    q0, s0 = quant.quantize_e4m3_blocks(W)
+    W[3, 130] = bad
+    q, s = quant.quantize_e4m3_blocks(W)
+    back = quant.dequantize_e4m3_blocks(q, s)
+    assert not s[0, 1].isfinite() and back[:128, 128:].isnan().all()
+    s[0, 1] = s0[0, 1]
+    assert torch.equal(s, s0)
+    codes, codes0 = q.float(), q0.float()
+    codes[:128, 128:] = codes0[:128, 128:] = 0
+    assert torch.equal(codes, codes0)
+
+
 # -------------------------------------------------------------------- refusals
 P = 0x10000  # a fake, 256-byte aligned device address: never dereferenced
 
