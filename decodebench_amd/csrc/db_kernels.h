@@ -248,8 +248,8 @@ struct MoeExpertsCall {
   float* parts;  // [T k, H] by pair
 };
 // The experts of a few tokens (moe_few.hip), whose pairs each read their expert's
-// weights: with `route` the choice among c.logits is theirs too, and c.experts and
-// c.weights are written.
+// weights: with `logits` the choice among them is theirs too, and `experts` and
+// `weights` (which c has as well) are written.
 struct MoeFewCall {
   MoeExpertsCall c;
   const double* logits;  // [T, E], or null: experts and weights are given

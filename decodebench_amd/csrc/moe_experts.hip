@@ -158,7 +158,8 @@ __global__ __launch_bounds__(NW* kWave, 2) void moe_product(MoeExpertsCall c) {
   const int tile_row[2] = {GATED ? 16 * wave : 32 * wave, GATED ? BN / 2 + 16 * wave : 32 * wave + 16};
   const float* ws[2] = {};
   if constexpr (FP8) {
-    static_assert(kOutputs <= 128 || 128 % 32 == 0, "a wave's rows lie in one block");
+    constexpr int kRows = kOutputs / NW;  // of a wave, of each matrix
+    static_assert(kOutputs % NW == 0 && 128 % kRows == 0, "a wave's rows lie in one block");
     const size_t at = ((size_t)expert * NB + min((n0 + tile_row[0] % kOutputs) / 128, NB - 1)) * KB;
     ws[0] = (GATED ? c.w.sg : c.w.sd) + at;
     ws[1] = (GATED ? c.w.su : c.w.sd) + at;
