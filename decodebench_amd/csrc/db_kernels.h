@@ -244,7 +244,7 @@ struct MoeExpertsCall {
   // workspace
   int* order;    // [T k] pairs sorted by expert
   int* tiles;    // count, then (expert, first slot, pairs) of each tile
-  void* h;       // [T k, I] by slot
+  void* h;       // [T k, I] by slot, of x's type; of few tokens by pair, fp32
   float* parts;  // [T k, H] by pair
 };
 // The experts of a few tokens (moe_few.hip), whose pairs each read their expert's

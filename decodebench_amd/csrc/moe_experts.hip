@@ -17,8 +17,10 @@
 // (7.2 TB/s) and the down product 40, whose rows are 11 steps long and mostly start.
 //
 // g, u, silu and the product are fp32; h is rounded once to the activations'
-// type, which the second product takes; what the pairs of a token add up to is
-// fp32 again, in the order of its experts, and rounded once.
+// type, which the second product's matrix instructions take (two 16-bit parts of it
+// would double that product and the LDS that its operand fills), so that in fp16 an h
+// above 65504 becomes Inf; what the pairs of a token add up to is fp32 again, in the
+// order of its experts, and rounded once.
 #include "db_kernels.h"
 #include "lds_dma.h"
 #include "moe_select.h"
@@ -352,7 +354,7 @@ size_t moe_experts_workspace(MoeExpertsCall& c, void* ws) {
   };
   c.order = reinterpret_cast<int*>(take(P * 4));
   c.tiles = reinterpret_cast<int*>(take((1 + 3 * (P + (size_t)c.w.E)) * 4));
-  c.h = take(P * c.w.I * 2);
+  c.h = take(P * c.w.I * (moe_few(c.w, c.T, c.k) ? 4 : 2));
   c.parts = reinterpret_cast<float*>(take(P * c.w.H * 4));
   return p - static_cast<char*>(ws);
 }

@@ -11,7 +11,10 @@
 // kAhead items of the wave are on their way to registers, products are two 16-bit
 // elements at a time (e4m3 is widened first, exactly) with fp32 sums, and a row's
 // sum over the lanes comes once, at its end.  The scale of a block multiplies the
-// lane's sum of its 16 elements of the block.
+// lane's sum of its 16 elements of the block.  h stays in fp32, which the down product
+// takes with fp32 multiply-adds: a layer is 1.4 times nearer to 64 bits than with h of
+// 16 (bf16), and costs up to 3% more (one token, 8 of 128 experts of 768 x 2048: 23.0
+// us for 22.7, e4m3 20.4 for 19.8; 2 of 8 of 14336 x 4096: the same).
 //
 // With the router's logits given, every workgroup of the first launch chooses its
 // token's experts for itself (1 us, and no launch between): the second launch gets
@@ -20,6 +23,8 @@
 // One token, 8 of 128 experts of 768 x 2048, bf16 (75.5 MB): the layer 21.8 us, of which
 // the gate takes 11 to 13 (4.2 TB/s), the down product 6.7 and the logits 2 to 3.  A launch
 // pays about 3 us before its stream runs at its rate: x, the choice, the first rows.
+#include <atomic>
+
 #include "db_kernels.h"
 #include "moe_select.h"
 
@@ -72,6 +77,36 @@ __device__ __forceinline__ float dot_chunk(u4 w, const char* x) {
   }
 }
 
+// The same with h in fp32: element 4 p + i of the lane's 8 (16 of e4m3) lies 1 KB * p
+// behind the first one, so that lanes side by side read places side by side.
+template <class E, bool FP8>
+__device__ __forceinline__ float dot_chunk32(u4 w, const char* h) {
+  float even = 0.0f, odd = 0.0f;
+  auto add = [&](f4 v, float a, float b, float c, float d) {
+    even = __builtin_fmaf(a, v[0], even);
+    odd = __builtin_fmaf(b, v[1], odd);
+    even = __builtin_fmaf(c, v[2], even);
+    odd = __builtin_fmaf(d, v[3], odd);
+  };
+  constexpr int kPlane = kWave * 16;
+  if constexpr (FP8) {
+    typedef float v2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const v2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[p], false);
+      const v2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[p], true);
+      add(*reinterpret_cast<const f4*>(h + p * kPlane), lo[0], lo[1], hi[0], hi[1]);
+    }
+  } else {
+    const typename E::vec8 v = __builtin_bit_cast(typename E::vec8, w);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      add(*reinterpret_cast<const f4*>(h + p * kPlane), (float)v[4 * p], (float)v[4 * p + 1],
+          (float)v[4 * p + 2], (float)v[4 * p + 3]);
+  }
+  return even + odd;
+}
+
 // The scale of the block of the lane's bytes from `off` on (zero behind the last one).
 __device__ __forceinline__ float ld_scale(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off / 128 * 4, 0, 0));
@@ -88,13 +123,12 @@ struct FewArgs {
   MoeFewCall f;
   int slices;    // workgroups of a pair, or of a token
   int padded;    // K in whole chunks
-  unsigned magic;  // 2^32 / (padded / 8), rounded up
+  unsigned magic;  // 2^32 / (padded / 4), rounded up
 };
 
 // A workgroup has every (slices)th group of kWaves rows of one pair.
 template <class E, bool FP8>
 __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
-  typedef typename E::type elem;
   constexpr int CE = FP8 ? 1024 : 512;  // elements of a row a load instruction takes
   constexpr int CH = FP8 ? 2 : 4;       // of each matrix in an item
   constexpr int kAhead = 2;               // items on their way: 8 or 16 KB a wave
@@ -109,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   const bool chooses = a.f.logits != nullptr;
   MoeLogits<kThreads> logits;
   if (chooses) logits.load(a.f.logits + (size_t)t * c.w.E, 1, 0, c.w.E);
-  row_to_lds(s_x, static_cast<const elem*>(c.x) + t * c.x_row, H, a.padded);
+  row_to_lds(s_x, static_cast<const typename E::type*>(c.x) + t * c.x_row, H, a.padded);
   int expert;
   if (chooses) {
     moe_rank(s_choice, logits, c.w.E, c.k);
@@ -181,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
         g = wave_sum(g);
         up = wave_sum(up);
         if (lane == 0)
-          static_cast<elem*>(c.h)[(size_t)pair * I + row] = (elem)(g / (1.0f + expf(-g)) * up);
+          static_cast<float*>(c.h)[(size_t)pair * I + row] = g / (1.0f + expf(-g)) * up;
         g = up = 0.0f;
         item = 0;
         row += stride;
@@ -190,10 +224,11 @@ __global__ __launch_bounds__(kThreads) void moe_few_gate(FewArgs a) {
   }
 }
 
-// A workgroup has every (slices)th group of kWaves rows of one token.
-template <class E, bool FP8, int CH>
-__global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
+// A workgroup of NW waves has every (slices)th group of NW rows of one token.
+template <class E, bool FP8, int CH, int NW>
+__global__ __launch_bounds__(NW* kWave) void moe_few_down(FewArgs a) {
   typedef typename E::type elem;
+  constexpr int kThreads = NW * kWave;
   constexpr int CE = FP8 ? 1024 : 512;
   constexpr int kAhead = 8 / CH;  // items on their way: 8 KB a wave
   extern __shared__ __align__(16) char s_h[];
@@ -208,13 +243,19 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   const float my_weight = c.weights[t * k + min(lane, k - 1)];
   // The first pieces of h are asked for before the weights, which come in order
   // behind them.  (What h holds of a pair without an expert does not count.)
-  const int row_pieces = a.padded / 8, pieces = k * row_pieces;
-  const elem* const h_from = static_cast<const elem*>(c.h) + (size_t)t * k * I;
+  const int row_pieces = a.padded / 4, pieces = k * row_pieces;
+  const float* const h_from = static_cast<const float*>(c.h) + (size_t)t * k * I;
   auto piece = [&](int i) {
-    const int j = (int)__umulhi(i, a.magic), at = (i - j * row_pieces) * 8;
+    const int j = (int)__umulhi(i, a.magic), at = (i - j * row_pieces) * 4;
     return at < I && j < k ? ld16(h_from + (size_t)j * I + at) : u4{0, 0, 0, 0};
   };
-  constexpr int kFirst = 4;
+  // Piece i goes to plane i % kPlanes, place i / kPlanes, of its chunk of the row.
+  constexpr int kPlanes = CE / kWave / 4;
+  auto put = [&](int i, u4 v) {
+    const int in = i & (CE / 4 - 1);
+    *reinterpret_cast<u4*>(s_h + (size_t)(i - in + in % kPlanes * kWave + in / kPlanes) * 16) = v;
+  };
+  constexpr int kFirst = 8;
   u4 first[kFirst];
 #pragma unroll
   for (int r = 0; r < kFirst; ++r) first[r] = piece(threadIdx.x + r * kThreads);
@@ -223,8 +264,8 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
   constexpr int CB = FP8 ? 1 : 2;
   const size_t row_bytes = (size_t)I * CB;
   const int items = (a.padded / CE + CH - 1) / CH;  // of a row of one expert
-  const int stride = a.slices * kWaves;
-  int at_row = slice * kWaves + wave, at_j = 0, at_item = 0;
+  const int stride = a.slices * NW;
+  int at_row = slice * NW + wave, at_j = 0, at_item = 0;
   u4 w[kAhead][CH];
   float scale[kAhead][CH];
   auto load = [&](int u) {
@@ -253,23 +294,21 @@ __global__ __launch_bounds__(kThreads) void moe_few_down(FewArgs a) {
 #pragma unroll
   for (int r = 0; r < kFirst; ++r) {
     const int i = threadIdx.x + r * kThreads;
-    if (i < pieces) *reinterpret_cast<u4*>(s_h + (size_t)i * 16) = first[r];
+    if (i < pieces) put(i, first[r]);
   }
-  for (int i = threadIdx.x + kFirst * kThreads; i < pieces; i += kThreads)
-    *reinterpret_cast<u4*>(s_h + (size_t)i * 16) = piece(i);
+  for (int i = threadIdx.x + kFirst * kThreads; i < pieces; i += kThreads) put(i, piece(i));
   __syncthreads();
-  int row = slice * kWaves + wave, j = 0, item = 0;
+  int row = slice * NW + wave, j = 0, item = 0;
   float sum = 0.0f, part = 0.0f;
   while (row < H) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (row >= H) break;
-      const char* const h = s_h + (size_t)j * a.padded * 2;
+      const char* const h = s_h + (size_t)j * a.padded * 4;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         if ((item * CH + i) * CE >= a.padded) break;
-        const float p = dot_chunk<E, FP8>(
-            w[u][i], h + ((item * CH + i) * kWave + lane) * (FP8 ? 32 : 16));
+        const float p = dot_chunk32<E, FP8>(w[u][i], h + (item * CH + i) * CE * 4 + lane * 16);
         part += FP8 ? p * scale[u][i] : p;
       }
       load(u);
@@ -296,6 +335,27 @@ int chunks(int K, bool fp8) {
   return (K + CE - 1) / CE * CE;
 }
 
+constexpr size_t kLds = 156 * 1024;  // of a CU, for h
+
+// The down kernel may take more dynamic LDS than a launch has unasked.
+template <class E, bool FP8, int CH, int NW>
+hipError_t launch_down(const FewArgs& d, size_t bytes, hipStream_t stream) {
+  auto* const fn = moe_few_down<E, FP8, CH, NW>;
+  static std::atomic<unsigned long long> asked{0};  // devices this kernel was asked for
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (!(asked.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
+    if (e != hipSuccess) return e;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+  }
+  fn<<<d.f.c.T * d.slices, NW * kWave, bytes, stream>>>(d);
+  return hipGetLastError();
+}
+
 template <class E, bool FP8>
 hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
   const MoeExpertsCall& c = f.c;
@@ -303,37 +363,41 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
   const int cus = device_cu_count(&err);
   if (err) return (hipError_t)err;
   // waves for each CU, and no more than rows
-  auto slices = [&](int groups, int rows) {
-    const int want = (8 * cus / kWaves + groups - 1) / groups;
-    return max(1, min(want, (rows + kWaves - 1) / kWaves));
+  auto slices = [&](int groups, int rows, int waves) {
+    const int want = (8 * cus / waves + groups - 1) / groups;
+    return max(1, min(want, (rows + waves - 1) / waves));
   };
   const int P = c.T * c.k;
-  FewArgs g = {f, slices(P, c.w.I), chunks(c.w.H, FP8), 0};
+  FewArgs g = {f, slices(P, c.w.I, kWaves), chunks(c.w.H, FP8), 0};
   moe_few_gate<E, FP8><<<P * g.slices, kThreads, (size_t)g.padded * 2, stream>>>(g);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  FewArgs d = {f, slices(c.T, c.w.H), chunks(c.w.I, FP8), 0};
-  d.magic = 0xFFFFFFFFu / (d.padded / 8) + 1;
+  // h in fp32 may fill most of a CU's LDS: one workgroup with the waves of two
+  const size_t h_bytes = (size_t)chunks(c.w.I, FP8) * 4 * c.k;
+  const int waves = h_bytes <= kLds / 2 ? kWaves : 2 * kWaves;
+  FewArgs d = {f, slices(c.T, c.w.H, waves), chunks(c.w.I, FP8), 0};
+  d.magic = 0xFFFFFFFFu / (d.padded / 4) + 1;
   // (rows of one load have items of one)
-  auto* const down = d.padded == chunks(1, FP8) ? moe_few_down<E, FP8, 1> : moe_few_down<E, FP8, 2>;
-  down<<<c.T * d.slices, kThreads, (size_t)d.padded * 2 * c.k, stream>>>(d);
-  return hipGetLastError();
+  const bool one = d.padded == chunks(1, FP8);
+  return waves == kWaves ? (one ? launch_down<E, FP8, 1, kWaves>(d, h_bytes, stream)
+                                : launch_down<E, FP8, 2, kWaves>(d, h_bytes, stream))
+                         : (one ? launch_down<E, FP8, 1, 2 * kWaves>(d, h_bytes, stream)
+                                : launch_down<E, FP8, 2, 2 * kWaves>(d, h_bytes, stream));
 }
 
 }  // namespace
 
-// Few pairs, whose rows of x and h fit the LDS that a launch has without asking, and
-// that read hardly more together than the experts they name among equally likely
+// Few pairs, whose row of x fits the LDS that a launch has without asking and whose rows
+// of h fit a CU's, and that read hardly more together than the experts they name among equally likely
 // ones: the tile kernels read an expert once for all its tokens, but take 15 us more
 // for sorting and adding up (80 MB at the rate of the weights, and 50 more for what the
 // L2 holds of a second reading).  Two tokens, 2 of 8 experts of 14336 x 4096, e4m3: 231
 // us here, 260 there; four tokens 409 and 374.
 bool moe_few(const db_moe& m, int T, int k) {
   const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
-  constexpr size_t kLds = 64 * 1024;
   const int P = T * k;
-  if (T > 4 || P > 32 || (size_t)chunks(m.H, fp8) * 2 + sizeof(MoeChoice) + 1024 > kLds ||
-      (size_t)chunks(m.I, fp8) * 2 * k + 1024 > kLds)
+  if (T > 4 || P > 32 || (size_t)chunks(m.H, fp8) * 2 + sizeof(MoeChoice) + 1024 > 64 * 1024 ||
+      (size_t)chunks(m.I, fp8) * 4 * k > 126 * 1024)
     return false;
   double missed = 1.0;  // chance that an expert is not named
   for (int t = 0; t < T; ++t) missed *= 1.0 - (double)min(k, m.E) / m.E;

@@ -1126,8 +1126,9 @@ def moe_experts(x, experts, weights, Wg, Wu, Wd, sg=None, su=None, sd=None, out=
     ceil(I/128)]).  H and I are multiples of 8, of 16 for e4m3.
 
     An expert outside [0, E) adds nothing; a token without any gets zeros; an
-    expert named twice counts twice.  Sums are fp32; what the gate gives is
-    rounded to x's type before the down product, and the result once.  Made for
+    expert named twice counts twice.  Sums are fp32, the result is rounded once.
+    What the gate gives stays in fp32 for a token or a few; beyond that it is rounded
+    to x's type before the down product (in fp16, above 65504 it becomes Inf).  Made for
     the few tokens of a decode step: the weights bound the call.  ``out`` may be x
     itself and shares no memory with another input."""
     if out is None and _fast is not None:

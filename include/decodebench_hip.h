@@ -344,8 +344,10 @@ int db_moe_route(const void* x, long long x_stride, const void* Wr, int* experts
                  int T, int H, int E, int k, int renormalize, int dtype, void* ws,
                  size_t ws_bytes, void* stream);
 
-/* y[t] = sum_j weights[t, j] Wd[e] h, h = silu(Wg[e] x[t]) * (Wu[e] x[t]) rounded to
- * x's type, e = experts[t, j]; sums in fp32, one rounding.  An expert outside [0, E)
+/* y[t] = sum_j weights[t, j] Wd[e] h, h = silu(Wg[e] x[t]) * (Wu[e] x[t]), e =
+ * experts[t, j]; sums in fp32, one rounding.  h is kept in fp32 in calls of a token or
+ * a few; otherwise it is rounded to x's type, for the matrix instructions (in fp16 an
+ * |h| above 65504 so becomes Inf).  An expert outside [0, E)
  * adds nothing, whatever its weight; a token without any gets zeros.  An expert named
  * twice counts twice.
  * Contract: x, experts, weights, T, k as db_moe_route (k need not be below E); H and I

@@ -53,8 +53,8 @@ def layer(E, H, I, dtype, fp8, seed, std=(None, None)):
     return on_gpu, plain
 
 
-def reference(x, experts, weights, plain):
-    """(y, tolerance) in 64 bits, an expert's tokens at a time."""
+def reference(x, experts, weights, plain, rounded=True):
+    """(y, tolerance) in 64 bits, an expert's tokens at a time; ``rounded``: with that of h."""
     u, low = HALF_STEP[x.dtype], LOWEST[x.dtype]
     x, k = x.double(), experts.shape[1]
     E, I, H = plain["Wg"].shape
@@ -72,7 +72,8 @@ def reference(x, experts, weights, plain):
         h = silu * up
         es = 1.1 * eg + 2.0 ** -21 * silu.abs()
         eh = es * up.abs() + silu.abs() * eu + es * eu
-        eh = eh + u * (h.abs() + eh) + low
+        if rounded:
+            eh = eh + u * (h.abs() + eh) + low
         size = h.abs() @ Wd.abs().t()
         y.index_add_(0, t, share * (h @ Wd.t()))
         tol.index_add_(0, t, share.abs() * (eh @ Wd.abs().t() * 1.01
@@ -145,6 +146,43 @@ def test_experts_at_the_ends_of_the_range(dtype, what, fp8, T):
     assert x.isfinite().all()
     experts, weights = routed(T, E, k, 3)
     near(ops.moe_experts(x, experts, weights, **on_gpu), *reference(x, experts, weights, plain))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 4, 2, 512, 272), (4, 4, 2, 272, 528), (1, 2, 2, 256, 14336),
+                                       (2, 4, 4, 256, 6160)])
+def test_few_tokens_keep_h_in_32_bits(dtype, fp8, T, E, k, H, I):
+    """h is near 2^18, which fp16 does not hold, and a layer is off by less than a rounding
+    of h alone would cost: the steps of all other roundings are counted, that one not."""
+    on_gpu, plain = layer(E, H, I, dtype, fp8, T, (2.0 ** 9 / H ** 0.5, 2.0 ** -17 / I ** 0.5))
+    x = normal((T, H), 7).to(dtype)
+    experts, weights = routed(T, E, k, 3)
+    weights += 0.5
+    y = ops.moe_experts(x, experts, weights, **on_gpu)
+    want, tol = reference(x, experts, weights, plain, rounded=False)
+    near(y, want, tol)
+    # The output's rounding is off by up to u 2^e, u 2^e / sqrt(3) in the root mean square:
+    # 0.41 u of normally distributed outputs.  One of h as well would make that 0.58 u.
+    off = (y.double() - want).square().mean().sqrt() / want.square().mean().sqrt()
+    assert off <= 0.5 * HALF_STEP[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 24, 200])
+def test_tokens_whose_h_leaves_fp16_stay_alone(T):
+    """In calls of more than a few tokens, whose h is rounded to fp16."""
+    E, k, H, I = 3, 2, 512, 272
+    on_gpu, _ = layer(E, H, I, torch.float16, False, T, (2.0 ** 3 / H ** 0.5, 2.0 ** -8 / I ** 0.5))
+    x = normal((T, H), 7).half()
+    experts, weights = routed(T, E, k, 3)
+    clean = ops.moe_experts(x, experts, weights, **on_gpu)
+    assert clean.isfinite().all()
+    x[T // 2] *= 2.0 ** 8
+    y = ops.moe_experts(x, experts, weights, **on_gpu)
+    keep = torch.arange(T, device=DEV) != T // 2
+    assert torch.equal(y[keep], clean[keep]) and not y[T // 2].isfinite().any()
 
 
 @pytest.mark.gpu
