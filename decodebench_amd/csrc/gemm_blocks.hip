@@ -563,8 +563,13 @@ GemmBlocksPlan gemm_blocks_plan(int T, int K, int N, int cu_count) {
     p.each = ((N + rounds * cu_count - 1) / (rounds * cu_count) + 3) / 4 * 4;
     p.grid = (N + p.each - 1) / p.each;
     p.magic = KB > 1 ? 0xFFFFFFFFu / KB + 1 : 0;
-    // Every workgroup quantises all of x: 8 tokens of 4096 16.7 us and 18.9 with a
-    // launch for it ([14336, 4096]), 16 of them 21.2 and 19.7.
+    // Every workgroup quantises all of x, whatever N.  us, and with a launch for it:
+    //   K = 4096, tokens   2          8          12         16
+    //   N = 14336       13.0 16.4  15.6 17.0  17.8 17.6  19.5 18.1
+    //   N = 4096         6.9  9.8   9.7 10.2  11.4 10.5  14.7 11.0
+    //   N = 1024         6.0  8.6   8.6  8.9  10.9  9.3  13.6  9.7
+    // [4096, 14336], 2 tokens 14.4 and 16.1, 4 tokens 18.2 and 16.2; [2048, 2048], 16
+    // tokens 8.3 and 8.7.
     p.fused = T * KB <= 320;
     if (few_lds(T, K, p.each) <= kFewLds) return p;
     p.fused = false;

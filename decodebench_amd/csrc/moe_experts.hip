@@ -308,23 +308,33 @@ void launch(const MoeExpertsCall& c, hipStream_t stream) {
   moe_combine<E><<<(quads + kThreads - 1) / kThreads, kThreads, 0, stream>>>(c);
 }
 
-// The tile's tokens go by how many an expert has on average, the stages by what
-// two workgroups a CU leave room for; us, others beside it:
-//   e4m3  33 tokens, 6 of 64 experts of 1392 x 2048 (3): 16 tokens, 3 stages 116;
-//         16, 4 stages 118; 32, 3 stages 117
-//         201 tokens, 2 of 8 of 14336 x 4096 (50): 64, 2 stages 362; 64, 4 stages (one
-//         workgroup a CU) 399; 128 526
-//         512 of these (128): 64 and eight waves 662, four 892; 128, eight waves 702
-//   16-bit  33 tokens (3): 32, 4 stages 221, 64, 3 stages 206; 16 tokens, 8 of 128
-//         of 768 x 2048 (1): 160 and 161; 201 tokens (50): 64, 3 stages 549, 128 579
-//         512 (128): 128 and eight waves 719, 64 and four 973
+// The tile's tokens go by how many an expert has on average (the fullest has more), the
+// stages by what two workgroups a CU leave room for.  us of a layer with tiles of, in
+// brackets the tokens an expert has:
+//   e4m3                                     16   32   64   64 and eight waves
+//     33 tokens, 6 of 64 of 1392 x 2048 (3)  100  102  115  113
+//     32 tokens, 2 of 8 of 14336 x 4096 (8)  235  235  288  277
+//     64 of these (16)                       328  234  278  284
+//     128 (32)                               501  358  315  343
+//     256 (64)                               872  583  454  446
+//     512 (128)                                   993  769  756
+//   16-bit                                   32   64   128 and eight waves
+//     33 tokens, 6 of 64 of 1392 x 2048 (3)  177  180  194
+//     32 tokens, 2 of 8 of 14336 x 4096 (8)  467  464  526
+//     64 of these (16)                       467  468  514
+//     128 (32)                               673  485  552
+//     201 (50)                               884  604  606
+//     256 (64)                              1129  752  627
+//     512 (128)                             1882 1193  818
+// With other stages or waves: e4m3 16 tokens in four stages the same, 64 in four (one
+// workgroup a CU) 331 at 128 tokens, 128 tokens and eight waves 708 at 512.
 template <class E, bool FP8>
 void pick(const MoeExpertsCall& c, hipStream_t stream) {
   const int mean = c.T * c.k / c.w.E;
   if constexpr (FP8) {
     if (mean <= 5)
       launch<E, FP8, 16, 3, 4>(c, stream);
-    else if (mean <= 12)
+    else if (mean <= 20)
       launch<E, FP8, 32, 3, 4>(c, stream);
     else if (mean <= 64)
       launch<E, FP8, 64, 2, 4>(c, stream);
@@ -333,7 +343,7 @@ void pick(const MoeExpertsCall& c, hipStream_t stream) {
   } else {
     if (mean <= 12)
       launch<E, FP8, 32, 4, 4>(c, stream);
-    else if (mean <= 64)
+    else if (mean <= 50)
       launch<E, FP8, 64, 3, 4>(c, stream);
     else
       launch<E, FP8, 128, 3, 8>(c, stream);

@@ -391,8 +391,12 @@ hipError_t launch(const MoeFewCall& f, hipStream_t stream) {
 // of h fit a CU's, and that read hardly more together than the experts they name among equally likely
 // ones: the tile kernels read an expert once for all its tokens, but take 15 us more
 // for sorting and adding up (80 MB at the rate of the weights, and 50 more for what the
-// L2 holds of a second reading).  Two tokens, 2 of 8 experts of 14336 x 4096, e4m3: 231
-// us here, 260 there; four tokens 409 and 374.
+// L2 holds of a second reading).  us here and there, at one to four tokens:
+//   2 of 8 experts of 14336 x 4096, e4m3   67 103  121 142  237 184  211 204
+//   the same, 16-bit                      117 165  222 263  414 344  397 374
+//   8 of 128 of 768 x 2048, e4m3           21  32   29  33   39  40   43  44
+//   6 of 64 of 1408 x 2048, e4m3           23  31   34  37   44  43   54  48
+// The rule takes the slower one in the last two only.
 bool moe_few(const db_moe& m, int T, int k) {
   const bool fp8 = m.w_dtype == DB_DTYPE_FP8_E4M3;
   const int P = T * k;
