@@ -242,11 +242,11 @@ __global__ __launch_bounds__(NW* kWave) void gemm_blocks_few(GemmBlocksCall c,
 // in 128 x 64 with K in five parts, 13.5 in 32 x 64 with ten stages, 9.2 in 64 x 32 with four
 // groups; such workgroups have one tile each.
 //
-// Large tiles keep the matrix cores busy: 8192 x 14336 x 4096 418 us, 2.3 PFLOP/s (2.48 in a
-// library product with one scale), where the scaled sums take 14%.  256 x 128 fetches
+// Large tiles keep the matrix cores busy: 8192 x 14336 x 4096 418 to 440 us by card, 2.2 to
+// 2.3 PFLOP/s (2.36 to 2.48 in a library product with one scale), where the scaled sums take 14%.  256 x 128 fetches
 // and reads more for a product (1.15 us a block of K, of which the LDS is busy 0.6 and the
 // matrix cores 0.43) and is for outputs that 256 x 256 would leave half the CUs without:
-// 2047 x 4096 x 4096 39 us, 52 in 256 x 256.
+// 2047 x 4096 x 4096 40 us, 52 in 256 x 256.
 template <class E, int BN, int BT, int WN, int WT, int S, int G = 1>
 __global__ __launch_bounds__(G*(BN / WN) * (BT / WT) * kWave, G > 2 ? 1 : 2) void gemm_blocks_tile(
     GemmBlocksCall c, GemmBlocksPlan plan) {

@@ -12,9 +12,11 @@
 // ahead.  e4m3 weights are widened to the activations' type (exact), each block's
 // sum scaled in fp32; the activations keep their 16 bits.
 //
-// 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 535 to 555 us, 5.2 TB/s; 33
-// tokens, 6 of 64 of 1392 x 2048, e4m3 (530 MB): 103 us, of which the gate takes 48
-// (7.2 TB/s) and the down product 40, whose rows are 11 steps long and mostly start.
+// 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 577 to 593 us on several
+// cards, 4.8 TB/s (gate and up 363 us, 5.2; down 231, 4.1, in 290 workgroups on 256 CUs);
+// 33 tokens, 6 of 64 of 1392 x 2048, e4m3 (about 54 of the experts asked, 465 MB): 103
+// us, of which the gate takes 48 (6.5 TB/s) and the down product 40 (3.9), whose rows are
+// 11 steps long and mostly start.
 //
 // g, u, silu and the product are fp32; h is rounded once to the activations'
 // type, which the second product's matrix instructions take (two 16-bit parts of it

@@ -20,8 +20,10 @@
 // token's experts for itself (1 us, and no launch between): the second launch gets
 // the choice from the workgroups of the first rows.
 //
-// One token, 8 of 128 experts of 768 x 2048, bf16 (75.5 MB): the layer 21.8 us, of which
-// the gate takes 11 to 13 (4.2 TB/s), the down product 6.7 and the logits 2 to 3.  A launch
+// One token, 8 of 128 experts of 768 x 2048, bf16 (75.5 MB): the layer 22.2 us, of which
+// the gate takes 11 to 13 (4.2 TB/s), the down product 6.9 and the logits 2 to 3; 2 of 8
+// of 14336 x 4096 116 us (6.1 TB/s), e4m3 66 (5.3; half the bytes on their way, and a
+// load of scales with each KB).  A launch
 // pays about 3 us before its stream runs at its rate: x, the choice, the first rows.
 #include <atomic>
 
