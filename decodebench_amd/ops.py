@@ -276,6 +276,8 @@ def _output(shape, idx: int, out, name: str = "out"):
 def _apart(out, *named) -> None:
     """Refuse an ``out`` that shares memory with an input, from its first element
     to its last: some workgroups write it while others still read."""
+    if out.numel() == 0:
+        return
     begin = out.data_ptr()
     end = begin + out.numel() * out.element_size()
     for t, name in named:

@@ -558,6 +558,7 @@ def test_shared_memory_is_seen():
     for other in (buf, out, buf[19:21], buf[::2], buf[0:11], buf[5:30, 8:16], out.view(torch.uint8)):
         with pytest.raises(ValueError, match="share memory with x"):
             ops._apart(out, (None, "none"), (other, "x"))
+    ops._apart(buf[10:10], (buf, "around nothing"))
     ops._apart(out, (buf[:10], "before"), (buf[20:], "behind"), (buf[10:10], "nothing"),
                (buf.clone(), "another"), (buf[0:9:2], "rows before"))
 
