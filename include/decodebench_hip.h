@@ -306,8 +306,9 @@ int db_quantize_blocks(const void* x, long long x_stride, void* q, float* scale,
 
 /* y[t, n] = sum_b xs[t, b] ws[n / 128, b] sum_{k in b} x[t, k] W[n, k], fp32 sums, one
  * rounding to y's type (xs ws is formed first, in fp32: scales whose product leaves its
- * range lose what the sum might have kept).  x is e4m3 with x_scale (element (t, b) at t xs_t + b xs_b), or
- * of y's type with x_scale NULL: then it is quantised first, as db_quantize_blocks does.
+ * range lose what the sum might have kept).  x is e4m3 with x_scale (element (t, b) at
+ * t xs_t + b xs_b), or of y's type with x_scale NULL: then it is quantised first, as
+ * db_quantize_blocks does.
  * Contract: x_dtype DB_DTYPE_FP8_E4M3 or y_dtype; y_dtype DB_DTYPE_F16 or
  * DB_DTYPE_BF16; x rows x_stride elements apart and 16-byte aligned; W [N, K] and y
  * [T, N] dense; K a multiple of 16; T, N, K, x_stride, xs_t < 2^22; W 16-byte
