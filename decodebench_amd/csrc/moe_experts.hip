@@ -12,8 +12,9 @@
 // ahead.  e4m3 weights are widened to the activations' type (exact), each block's
 // sum scaled in fp32; the activations keep their 16 bits.
 //
-// 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 577 to 593 us on several
-// cards, 4.8 TB/s (gate and up 363 us, 5.2; down 231, 4.1, in 290 workgroups on 256 CUs);
+// 201 tokens, 2 of 8 experts of 14336 x 4096, fp16 (2.8 GB): 504 to 593 us by
+// card, 4.8 to 5.6 TB/s (traced on one: gate and up 363 us, 5.2 TB/s; down 231, 4.1, in
+// 290 workgroups on 256 CUs);
 // 33 tokens, 6 of 64 of 1392 x 2048, e4m3 (about 54 of the experts asked, 465 MB): 103
 // us, of which the gate takes 48 (6.5 TB/s) and the down product 40 (3.9), whose rows are
 // 11 steps long and mostly start.
